@@ -463,7 +463,7 @@ def run(s):
     from loquetier_amd.kernel_utils import qk_norm_rope
     from loquetier_amd.ops import _kernels as K
     if case["op"] == "attention":
-        plan = K.AttentionPlan(s["q_indptr"], s["kv_len"], s["table"], s["rows"], case["q_heads"], case["kv_heads"])
+        plan = K.AttentionPlan(s["q_indptr"], s["kv_len"], s["table"], s["rows"], case["q_heads"], case["kv_heads"], case["page"])
         out = torch.empty_like(s["q"])
         K.paged_attention(out, s["q"], s["k_cache"], s["v_cache"], plan)
         return out
