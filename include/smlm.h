@@ -455,6 +455,126 @@ SMLM_API int smlm_segment_scales(const int32_t* seg_adapter, int S, const float*
                                  float* part_out, void* stream);
 
 /*
+ * Heads of a batch's rows: [rows, heads, head_dim] of 16-bit elements at data[row * row_stride + head * head_stride], strides in
+ * elements and multiples of 8, the dimensions of a head next to each other, data 16-byte aligned.
+ */
+typedef struct smlm_heads {
+  void* data;
+  int64_t row_stride;
+  int64_t head_stride;
+} smlm_heads;
+
+/*
+ * Norms of queries and keys by head, and their rotation by position, in one pass (the model's q_norm / k_norm and
+ * apply_rotary_pos_emb, which the reference leaves to tensor expressions: src/loquetier_src/models/mixed_llama.py:93-195):
+ *   y = x * w / sqrt(mean_j x_j^2 + eps) by head, or y = x where the weight is NULL
+ *   out[j] = y[j] c_j - y[j + h] s_j,  out[j + h] = y[j + h] c_j + y[j] s_j  for j < h = rot_dim / 2, the rest is y
+ * in float, rounded once.  table: float [table_rows, rot_dim], by position h cosines and then h sines; positions: int32 [rows].
+ * A row of a position below 0 is padding (its outputs are zero, it has no gradient and it is not cached); a position past the
+ * table gives NaN.  head_dim and rot_dim multiples of 16, rot_dim <= head_dim <= 512.  q_out may be q, k_out may be k.
+ *
+ * With k_cache the rotated keys, and v, also go to a cache's pages: row t to place slots[t] % page_size of page
+ * slots[t] / page_size, at data[page * page_stride + head * head_stride + place * slot_stride] (elements, multiples of 8) of both caches; a slot
+ * outside [0, n_pages * page_size) (-1: rows that are not cached) is not written.  k_out's data may then be NULL.  Two rows of one
+ * slot leave either.
+ */
+typedef struct smlm_qk_rope {
+  smlm_heads q, k, v;         /* v: with k_cache only */
+  smlm_heads q_out, k_out;
+  const void* q_weight;       /* [head_dim] or NULL */
+  const void* k_weight;
+  const float* table;
+  const int32_t* positions;
+  void* k_cache;              /* NULL: no cache */
+  void* v_cache;
+  const int64_t* slots;
+  int64_t page_stride, head_stride, slot_stride;
+  int rows, q_heads, kv_heads, head_dim, rot_dim, table_rows;
+  int n_pages, page_size;
+  int dtype;
+  float eps;
+} smlm_qk_rope;
+SMLM_API int smlm_qk_norm_rope_fwd(const smlm_qk_rope* args, void* stream);
+
+/*
+ * Its backward: q and k as in the forward, gq and gk the gradients of q_out and k_out; dq, dk, and where the weight is not NULL
+ * dq_weight / dk_weight ([head_dim], summed over rows and heads in a fixed order).  The root mean squares are computed
+ * again.  Reads of args: q, k, weights, table, positions and sizes.  Without a weight q (or k) is not read.  dq may be gq, dk gk.
+ */
+SMLM_API int smlm_qk_norm_rope_bwd_workspace_size(int rows, int q_heads, int kv_heads, int head_dim, size_t* bytes);
+SMLM_API int smlm_qk_norm_rope_bwd(const smlm_qk_rope* args, const smlm_heads* gq, const smlm_heads* gk, const smlm_heads* dq,
+                                   const smlm_heads* dk, void* dq_weight, void* dk_weight, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
+/*
+ * Pages of a cache, kept on the device (the reference keeps them in Python lists: kernel_src/src/loquetier/utils/kvcache.py).  State, all
+ * int32: table [R, M] (the pages of request r in order, -1 past the last), length [R] (its tokens), refs [N] (requests that
+ * hold page n, 0: free); the requests' rows start with tables of -1 and lengths of 0.  Free pages are taken lowest number first.  A
+ * request's last page, where it is part-filled, is its own.
+ * A call does all it is asked or, where it cannot, nothing, and then adds SMLM_KV_* bits to *status (int32 on the device; may be NULL).
+ */
+#define SMLM_KV_BAD_REQUEST 1 /* past R, named twice, a child that is not empty, a count below 0 */
+#define SMLM_KV_TOO_LONG 2    /* more pages than a row of the table holds          */
+#define SMLM_KV_ROWS 4        /* more new tokens than rows                          */
+#define SMLM_KV_NO_PAGES 8    /* the pool has not enough free pages                 */
+
+/*
+ * Room for counts[s] more tokens of requests[s] (int32 [S]; below 0: skipped), and the step's tables: q_indptr int32 [S + 1] (running sum of
+ * the counts), kv_len int32 [S] (tokens with the new ones), and for each of `rows` rows (at least the counts' sum) positions int32 and
+ * slots int64 (page * page_size + place); rows past the sum get -1.  A refused step has zeros in q_indptr and kv_len, and -1.
+ */
+SMLM_API int smlm_kv_workspace_size(int R, int N, int S, size_t* bytes);
+SMLM_API int smlm_kv_extend(int32_t* table, int32_t* length, int32_t* refs, const int32_t* requests, const int32_t* counts,
+                            int32_t* q_indptr, int32_t* kv_len, int32_t* positions, int64_t* slots, void* workspace,
+                            size_t workspace_bytes, int R, int M, int N, int S, int rows, int page_size, int32_t* status,
+                            void* stream);
+
+/* The requests' pages lose a holder, their rows become -1 and their lengths 0.  One named twice is freed once; below 0 is skipped. */
+SMLM_API int smlm_kv_free(int32_t* table, int32_t* length, int32_t* refs, const int32_t* requests, int R, int M, int N, int K,
+                          int page_size, int32_t* status, void* stream);
+
+/*
+ * children[i], empty so far, becomes a second parents[i] (int32 [K]; a parent may be named often, a child below 0 is skipped; parents count as they were before the call): full pages
+ * are shared, of a part-filled last page the filled places are copied to a page of the child's own.
+ * pool: [N, blocks, page_size, place_bytes], contiguous and 16-byte aligned, place_bytes a multiple of 16 (blocks: layers x keys and
+ * values x kv heads, say).
+ */
+SMLM_API int smlm_kv_fork(void* pool, int32_t* table, int32_t* length, int32_t* refs, const int32_t* parents,
+                          const int32_t* children, void* workspace, size_t workspace_bytes, int R, int M, int N, int K,
+                          int blocks, int page_size, int place_bytes, int32_t* status, void* stream);
+
+/* The pages in use become pages 0, 1, ... : those past their number move to the free ones below it, in order; table and refs follow. */
+SMLM_API int smlm_kv_compact(void* pool, int32_t* table, int32_t* refs, void* workspace, size_t workspace_bytes, int R, int M,
+                             int N, int blocks, int page_size, int place_bytes, void* stream);
+
+/* Page dst[i] becomes a copy of page src[i] (int32 [K]; pairs with a number outside the pool are skipped).  No page may be dst twice, or src and dst. */
+SMLM_API int smlm_kv_copy_pages(void* pool, const int32_t* src, const int32_t* dst, int K, int N, int blocks, int page_size,
+                                int place_bytes, void* stream);
+
+/*
+ * Causal attention of a batch's new rows over a paged cache, prompts and decoding requests in one call (the reference's batch_prefill and
+ * batch_decode, kernel_src/csrc/loquetier_ops.cc:90-273).  Sequence s has the rows [q_indptr[s], q_indptr[s + 1]) of q, the last of
+ * its kv_len[s] tokens, all of which are in the cache: token j lies in place j % page_size of page table[requests[s]][j / page_size]
+ * (requests NULL: row s of the table), at k_cache[page * page_stride + kv head * head_stride + place * slot_stride].
+ *   out[t, h] = sum_j softmax_j(scale q[t, h] . k[j]) v[j],  j up to the row's own token, kv head h / (q_heads / kv_heads)
+ * Rows that see no token are zero; rows of no sequence are left alone.  Pages outside the pool, requests outside the table and
+ * tokens past a row of the table do not count.  head_dim 64 or 128; any page size; scale > 0; strides multiples of 8 elements.
+ *
+ * The plan depends on q_indptr, kv_len and requests alone: one for all the layers of a step.  q_indptr must not decrease.
+ */
+SMLM_API int smlm_attn_plan_size(int T, int S, int q_heads, int kv_heads, size_t* bytes);
+SMLM_API int smlm_attn_plan_build(void* plan, size_t plan_bytes, const int32_t* q_indptr, const int32_t* kv_len,
+                                  const int32_t* requests, int T, int S, int R, int M, int page_size, int q_heads,
+                                  int kv_heads, void* stream);
+SMLM_API int smlm_paged_attn_workspace_size(int T, int S, int M, int page_size, int q_heads, int kv_heads, int head_dim,
+                                            size_t* bytes);
+SMLM_API int smlm_paged_attn(const smlm_heads* out, const smlm_heads* q, const void* k_cache, const void* v_cache,
+                             int64_t page_stride, int64_t head_stride, int64_t slot_stride, const int32_t* table,
+                             const void* plan, size_t plan_bytes, void* workspace, size_t workspace_bytes, int T, int S, int R,
+                             int M, int n_pages, int page_size, int q_heads, int kv_heads, int head_dim, int dtype, float scale,
+                             void* stream);
+
+/*
  * Copies `bytes` (a multiple of 4) of host memory to device memory (4-byte aligned) in the
  * arguments of launches on `stream`, 3584 bytes each: src has been read when the call
  * returns, and the host waits for nothing.  For the small tables a call needs (row

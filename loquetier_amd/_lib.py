@@ -20,6 +20,7 @@ SMLM_ERR_SCRATCH = -7
 SMLM_STATIC_SCRATCH_BYTES = 8 << 20
 SMLM_STAGE_SHRINK, SMLM_STAGE_EXPAND = 1, 2
 SMLM_BWD_PRODUCTS, SMLM_BWD_DX, SMLM_BWD_WGRAD = 1, 2, 4
+SMLM_KV_BAD_REQUEST, SMLM_KV_TOO_LONG, SMLM_KV_ROWS, SMLM_KV_NO_PAGES = 1, 2, 4, 8
 
 _vp, _i, _sz, _f = C.c_void_p, C.c_int, C.c_size_t, C.c_float
 _psz = C.POINTER(C.c_size_t)
@@ -40,6 +41,24 @@ class LoraOpts(C.Structure):
 
 
 _popts = C.POINTER(LoraOpts)
+
+
+class Heads(C.Structure):
+    """struct smlm_heads of include/smlm.h."""
+    _fields_ = [("data", C.c_void_p), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class QkRope(C.Structure):
+    """struct smlm_qk_rope of include/smlm.h."""
+    _fields_ = [("q", Heads), ("k", Heads), ("v", Heads), ("q_out", Heads), ("k_out", Heads),
+                ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("table", C.c_void_p), ("positions", C.c_void_p),
+                ("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("slots", C.c_void_p),
+                ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("slot_stride", C.c_int64),
+                *[(n, C.c_int) for n in ("rows", "q_heads", "kv_heads", "head_dim", "rot_dim", "table_rows", "n_pages",
+                                         "page_size", "dtype")], ("eps", C.c_float)]
+
+
+_pheads, _prope, _i64 = C.POINTER(Heads), C.POINTER(QkRope), C.c_int64
 
 # name -> (restype, argtypes); must list every symbol include/smlm.h declares
 SIGNATURES = {
@@ -75,6 +94,19 @@ SIGNATURES = {
     "smlm_rms_norm_bwd": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i, _i, _i, _vp]),
     "smlm_segments_build": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp]),
     "smlm_segment_scales": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp]),
+    "smlm_qk_norm_rope_fwd": (_i, [_prope, _vp]),
+    "smlm_qk_norm_rope_bwd_workspace_size": (_i, [_i, _i, _i, _i, _psz]),
+    "smlm_qk_norm_rope_bwd": (_i, [_prope, _pheads, _pheads, _pheads, _pheads, _vp, _vp, _vp, _sz, _vp]),
+    "smlm_kv_workspace_size": (_i, [_i, _i, _i, _psz]),
+    "smlm_kv_extend": (_i, [_vp] * 10 + [_sz] + [_i] * 6 + [_vp, _vp]),
+    "smlm_kv_free": (_i, [_vp] * 4 + [_i] * 5 + [_vp, _vp]),
+    "smlm_kv_fork": (_i, [_vp] * 7 + [_sz] + [_i] * 7 + [_vp, _vp]),
+    "smlm_kv_compact": (_i, [_vp] * 4 + [_sz] + [_i] * 6 + [_vp]),
+    "smlm_kv_copy_pages": (_i, [_vp] * 3 + [_i] * 5 + [_vp]),
+    "smlm_attn_plan_size": (_i, [_i] * 4 + [_psz]),
+    "smlm_attn_plan_build": (_i, [_vp, _sz, _vp, _vp, _vp] + [_i] * 7 + [_vp]),
+    "smlm_paged_attn_workspace_size": (_i, [_i] * 7 + [_psz]),
+    "smlm_paged_attn": (_i, [_pheads, _pheads, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _sz, _vp, _sz] + [_i] * 10 + [_f, _vp]),
     "smlm_put_words": (_i, [_vp, _vp, _sz, _vp]),
 }
 

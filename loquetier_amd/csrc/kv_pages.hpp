@@ -1,0 +1,419 @@
+// The life of a paged cache's pages, on the device: alloting them to growing requests, sharing them between the
+// answers to one prompt, giving them back, packing the pool to its front, copying.
+//
+// State, all int32 on the device: table [R, M] (page ids of request r, -1 past its last page), length [R] (tokens cached),
+// refs [N] (requests that hold page n; 0: free).  Free pages are taken lowest number first, so that every result is a
+// function of the inputs alone; the counts are changed by integer atomics, whose order does not show.  A request's
+// part-filled last page belongs to it alone (a fork copies it), so growing never has to copy.
+//
+// A call changes all it should or nothing: what it needs is counted and checked first, and a call that cannot be done
+// sets bits of `status`.
+//
+// The bookkeeping is a few kilobytes of integers, bound by latency: one workgroup of 1024 threads counts and takes the
+// pages (scans and a pass over refs, sixteen pages a thread at a time, ended as soon as enough are found); what
+// grows with tokens or page contents runs in a second launch that has the card.
+#pragma once
+#include "smlm_common.hpp"
+
+namespace smlm {
+
+constexpr int kKvThreads = 1024;
+
+// inclusive sum over the workgroup's 1024 threads; `total` gets the sum of all
+__device__ __forceinline__ int kv_scan(int v, int* wave_tot, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int d = 1; d < kWaveSize; d *= 2) {
+    const int u = __shfl_up(v, d, kWaveSize);
+    if (lane >= d) v += u;
+  }
+  __syncthreads();  // earlier readers of wave_tot are done
+  if (lane == 63) wave_tot[wave] = v;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kKvThreads / kWaveSize; ++w) {
+    const int t = wave_tot[w];
+    before += w < wave ? t : 0;
+    total += t;
+  }
+  return v + before;
+}
+
+// Atomics reach memory past the CU's own cache, so what they wrote is read the same way.
+__device__ __forceinline__ int kv_load(const int* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void kv_store(int* p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// The `want` lowest pages without holders into out[0, want); returns how many there are (at most want).
+__device__ __forceinline__ int kv_take_free(const int* refs, int N, int want, int* out, int* wave_tot) {
+  int found = 0;
+  for (int base = 0; base < N && found < want; base += kKvThreads * 16) {
+    const int first = base + (int)threadIdx.x * 16;
+    uint32_t mask = 0;
+    if (first + 16 <= N) {
+      i32x4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) __builtin_memcpy(&v[j], refs + first + 4 * j, 16);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) mask |= (v[j >> 2][j & 3] == 0 ? 1u : 0u) << j;
+    } else {
+      for (int j = 0; j < 16 && first + j < N; ++j) mask |= (refs[first + j] == 0 ? 1u : 0u) << j;
+    }
+    const int n = __popc(mask);
+    int total;
+    int at = found + kv_scan(n, wave_tot, total) - n;
+    while (mask && at < want) {
+      out[at++] = first + __ffs(mask) - 1;
+      mask &= mask - 1;
+    }
+    found += total;
+  }
+  return found < want ? found : want;
+}
+
+struct KvExtendArgs {
+  int *table, *length, *refs, *status;
+  const int *requests, *counts;  // [S]; a request below 0 is skipped
+  int *q_indptr, *kv_len;        // [S + 1], [S]
+  int* positions;                // [rows]
+  int64_t* slots;                // [rows]
+  int *owner, *start, *fresh;    // scratch: [R], [S + 1] running sum of new pages, [N]
+  int R, M, N, S, rows, P;
+};
+
+// One workgroup: counts, checks, takes the pages and writes the step's tables.  q_indptr doubles as the counts' running sum.
+__global__ __launch_bounds__(kKvThreads) void kv_extend_kernel(KvExtendArgs a) {
+  __shared__ int wave_tot[16];
+  __shared__ int bad;
+  const int tid = threadIdx.x;
+  if (tid == 0) bad = 0;
+  for (int i = tid; i < a.S; i += kKvThreads) {
+    const int r = a.requests[i];
+    if (r >= 0 && r < a.R) kv_store(a.owner + r, 0x7fffffff);
+  }
+  __threadfence();
+  __syncthreads();
+  for (int i = tid; i < a.S; i += kKvThreads) {
+    const int r = a.requests[i];
+    if (r >= 0 && r < a.R) atomicMin(a.owner + r, i);
+  }
+  __threadfence();
+  __syncthreads();
+  int rows = 0, pages = 0;
+  for (int base = 0; base < a.S; base += kKvThreads) {
+    const int i = base + tid;
+    int r = -1, n = 0, need = 0, err = 0;
+    if (i < a.S) {
+      r = a.requests[i];
+      n = r < 0 ? 0 : a.counts[i];
+      if (r >= a.R || n < 0) {
+        err = SMLM_KV_BAD_REQUEST;
+      } else if (r >= 0) {
+        if (kv_load(a.owner + r) != i) err = SMLM_KV_BAD_REQUEST;
+        const int64_t old = a.length[r], now = old + n;
+        const int64_t had = (old + a.P - 1) / a.P, has = (now + a.P - 1) / a.P;
+        if (has > a.M || old < 0) err |= SMLM_KV_TOO_LONG;
+        else need = (int)(has - had);
+      }
+      if (err) n = 0, need = 0;
+    }
+    if (n > a.rows) err |= SMLM_KV_ROWS, n = 0;  // (and so the sum stays small)
+    if (err) atomicOr(&bad, err);
+    int total;
+    const int upto = kv_scan(n, wave_tot, total);
+    if (i < a.S) a.q_indptr[i + 1] = rows + upto;
+    if (rows <= a.rows) rows += total;
+    int total_pages;
+    const int pages_upto = kv_scan(need, wave_tot, total_pages);
+    if (i < a.S) a.start[i + 1] = pages + pages_upto;
+    if (pages <= a.N) pages += total_pages;
+  }
+  if (tid == 0) {
+    a.q_indptr[0] = a.start[0] = 0;
+    if (rows > a.rows) atomicOr(&bad, SMLM_KV_ROWS);
+    if (pages > a.N) atomicOr(&bad, SMLM_KV_NO_PAGES);
+  }
+  __syncthreads();
+  if (!bad) {
+    const int found = kv_take_free(a.refs, a.N, pages, a.fresh, wave_tot);
+    if (tid == 0 && found < pages) bad = SMLM_KV_NO_PAGES;
+  }
+  __threadfence_block();
+  __syncthreads();
+  const int err = bad;
+  if (err) {
+    for (int i = tid; i <= a.S; i += kKvThreads) {
+      a.q_indptr[i] = 0;
+      if (i < a.S) a.kv_len[i] = 0;
+    }
+    if (tid == 0 && a.status) atomicOr(a.status, err);
+    return;
+  }
+  // (flat over the pages: one prompt may take most of them)
+  for (int p = tid; p < pages; p += kKvThreads) {
+    int lo = 0, hi = a.S;
+    while (hi - lo > 1) {  // last i with start[i] <= p; start[i + 1] > p there
+      const int mid = (lo + hi) >> 1;
+      if (a.start[mid] <= p) lo = mid;
+      else hi = mid;
+    }
+    const int r = a.requests[lo], id = a.fresh[p];
+    a.table[(int64_t)r * a.M + (a.length[r] + a.P - 1) / a.P + (p - a.start[lo])] = id;
+    a.refs[id] = 1;
+  }
+  __syncthreads();  // (the lengths are read above)
+  for (int i = tid; i < a.S; i += kKvThreads) {
+    const int r = a.requests[i];
+    const int now = r < 0 ? 0 : a.length[r] + (a.q_indptr[i + 1] - a.q_indptr[i]);
+    if (r >= 0) a.length[r] = now;
+    a.kv_len[i] = now;
+  }
+}
+
+// Positions and slots of the step's rows; rows past the last request's, and all of them where the step was refused, get -1.
+__global__ __launch_bounds__(256) void kv_rows_kernel(KvExtendArgs a) {
+  const int row = (int)blockIdx.x * 256 + (int)threadIdx.x;
+  if (row >= a.rows) return;
+  int pos = -1;
+  int64_t slot = -1;
+  if (a.S > 0 && row < a.q_indptr[a.S]) {
+    int lo = 0, hi = a.S;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (a.q_indptr[mid] <= row) lo = mid;
+      else hi = mid;
+    }
+    const int r = a.requests[lo];
+    pos = a.kv_len[lo] - (a.q_indptr[lo + 1] - row);
+    const int j = pos / a.P;
+    slot = (int64_t)a.table[(int64_t)r * a.M + j] * a.P + (pos - j * a.P);
+  }
+  a.positions[row] = pos;
+  a.slots[row] = slot;
+}
+
+struct KvFreeArgs {
+  int *table, *length, *refs, *status;
+  const int* requests;  // [K]
+  int R, M, N, K, P;
+};
+
+// A workgroup a request; who takes its length away gives its pages back, so a request named twice is freed once.
+__global__ __launch_bounds__(256) void kv_free_kernel(KvFreeArgs a) {
+  __shared__ int had;
+  const int r = a.requests[blockIdx.x];
+  if (r < 0) return;
+  if (r >= a.R) {
+    if (threadIdx.x == 0 && a.status) atomicOr(a.status, SMLM_KV_BAD_REQUEST);
+    return;
+  }
+  if (threadIdx.x == 0) had = atomicExch(a.length + r, 0);
+  __syncthreads();
+  const int64_t pages = ((int64_t)had + a.P - 1) / a.P;
+  int* row = a.table + (int64_t)r * a.M;
+  for (int i = threadIdx.x; i < pages && i < a.M; i += 256) {
+    const int id = row[i];
+    if (id >= 0 && id < a.N) atomicSub(a.refs + id, 1);
+    row[i] = -1;
+  }
+}
+
+// ---- copies of pages --------------------------------------------------------------------------------------
+// A page holds C blocks of P places of `place` 16-byte pieces (layers x keys and values x heads, tokens, dimensions);
+// of each block the first `filled` places are copied.
+struct KvCopy {
+  int src, dst, filled;
+};
+struct KvPool {
+  uint16_t* data;
+  int64_t page;    // elements of a page
+  int N, C, P, place;
+  int group, groups;  // blocks a workgroup copies, workgroups a page
+};
+
+__device__ __forceinline__ void kv_copy_part(const KvPool& pool, int src, int dst, int filled, int part) {
+  if (src < 0 || src >= pool.N || dst < 0 || dst >= pool.N || src == dst) return;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int n = filled * pool.place, block = pool.P * pool.place * 8;
+  const int last = (part + 1) * pool.group < pool.C ? (part + 1) * pool.group : pool.C;
+  for (int c = part * pool.group + wave; c < last; c += 4) {
+    const uint16_t* from = pool.data + src * pool.page + (int64_t)c * block;
+    uint16_t* to = pool.data + dst * pool.page + (int64_t)c * block;
+    int i = lane;
+    for (; i + 3 * kWaveSize < n; i += 4 * kWaveSize) {
+      u32x4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = ldg16_nt(from + (int64_t)(i + j * kWaveSize) * 8);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) stg16_nt(to + (int64_t)(i + j * kWaveSize) * 8, v[j]);
+    }
+    for (; i < n; i += kWaveSize) stg16_nt(to + (int64_t)i * 8, ldg16_nt(from + (int64_t)i * 8));
+  }
+}
+
+struct KvCopyArgs {
+  KvPool pool;
+  const int *src, *dst;  // [K] pages
+  int K;
+};
+__global__ __launch_bounds__(256) void kv_copy_kernel(KvCopyArgs a) {
+  for (int64_t w = blockIdx.x; w < (int64_t)a.K * a.pool.groups; w += gridDim.x) {
+    const int k = (int)(w / a.pool.groups);
+    kv_copy_part(a.pool, a.src[k], a.dst[k], a.pool.P, (int)(w - (int64_t)k * a.pool.groups));
+  }
+}
+
+struct KvForkArgs {
+  KvPool pool;
+  int *table, *length, *refs, *status;
+  const int *parents, *children;  // [K]
+  int *owner, *start, *fresh;     // scratch: [R], [K + 1] running sum of copied pages (0 everywhere: refused), [N]
+  int* forked;                    // scratch: [K] tokens of the children, -1 where there is nothing to do
+  int R, M, K;
+};
+
+__global__ __launch_bounds__(kKvThreads) void kv_fork_kernel(KvForkArgs a) {
+  __shared__ int wave_tot[16];
+  __shared__ int bad;
+  const int tid = threadIdx.x, P = a.pool.P;
+  if (tid == 0) bad = 0;
+  for (int i = tid; i < a.K; i += kKvThreads) {
+    const int c = a.children[i];
+    if (c >= 0 && c < a.R) kv_store(a.owner + c, 0x7fffffff);
+  }
+  __threadfence();
+  __syncthreads();
+  for (int i = tid; i < a.K; i += kKvThreads) {
+    const int c = a.children[i];
+    if (c >= 0 && c < a.R) atomicMin(a.owner + c, i);
+  }
+  __threadfence();
+  __syncthreads();
+  int pages = 0;
+  for (int base = 0; base < a.K; base += kKvThreads) {
+    const int i = base + tid;
+    int need = 0, err = 0, n = -1;
+    if (i < a.K) {
+      const int p = a.parents[i], c = a.children[i];
+      if (c >= 0) {
+        if (p < 0 || p >= a.R || c >= a.R || kv_load(a.owner + c) != i || a.length[c] != 0) {
+          err = SMLM_KV_BAD_REQUEST;
+        } else {
+          n = a.length[p];
+          if (n < 0 || n > (int64_t)a.M * P) err = SMLM_KV_TOO_LONG;
+          else need = n % P != 0;
+        }
+      }
+      a.forked[i] = n;
+    }
+    if (err) atomicOr(&bad, err);
+    int total;
+    const int upto = kv_scan(need, wave_tot, total);
+    if (i < a.K) a.start[i + 1] = pages + upto;
+    pages += total;
+  }
+  if (tid == 0) {
+    a.start[0] = 0;
+    if (pages > a.pool.N) atomicOr(&bad, SMLM_KV_NO_PAGES);
+  }
+  __syncthreads();
+  if (!bad) {
+    const int found = kv_take_free(a.refs, a.pool.N, pages, a.fresh, wave_tot);
+    if (tid == 0 && found < pages) bad = SMLM_KV_NO_PAGES;
+  }
+  __threadfence_block();
+  __syncthreads();
+  const int err = bad;
+  for (int i = tid; i < a.K; i += kKvThreads) {
+    if (err) {
+      a.forked[i] = -1;
+      continue;
+    }
+    const int n = a.forked[i];
+    if (n < 0) continue;
+    const int c = a.children[i];
+    a.length[c] = n;
+    if (n % P != 0) {
+      const int id = a.fresh[a.start[i]];
+      a.table[(int64_t)c * a.M + n / P] = id;
+      a.refs[id] = 1;
+    }
+  }
+  if (tid == 0 && err && a.status) atomicOr(a.status, err);
+}
+
+// A workgroup a child and part of a page: the full pages' ids and counts (part 0), and its share of the last page's copy.
+__global__ __launch_bounds__(256) void kv_fork_copy_kernel(KvForkArgs a) {
+  const int k = (int)blockIdx.x / a.pool.groups, part = (int)blockIdx.x % a.pool.groups, P = a.pool.P;
+  const int n = a.forked[k];
+  if (n < 0) return;
+  const int* from = a.table + (int64_t)a.parents[k] * a.M;
+  int* to = a.table + (int64_t)a.children[k] * a.M;
+  if (part == 0)
+    for (int i = threadIdx.x; i < n / P; i += 256) {
+      const int id = from[i];
+      to[i] = id;
+      if (id >= 0 && id < a.pool.N) atomicAdd(a.refs + id, 1);
+    }
+  if (n % P) kv_copy_part(a.pool, from[n / P], to[n / P], n % P, part);
+}
+
+struct KvCompactArgs {
+  KvPool pool;
+  int *table, *refs;
+  int *src, *dst, *moved;  // scratch: [N] pages that move, [N] where to, [N] where a page from `live` on went
+  int* head;               // scratch: [2] pages in use, pages that move
+  int64_t entries;         // of the table
+  int table_blocks;
+};
+
+// Pages in use from number `live` (their count) on move into the free ones below it, both in ascending order.
+__global__ __launch_bounds__(kKvThreads) void kv_compact_kernel(KvCompactArgs a) {
+  __shared__ int wave_tot[16];
+  const int tid = threadIdx.x, N = a.pool.N;
+  int mine = 0, live;
+  for (int i = tid; i < N; i += kKvThreads) mine += a.refs[i] > 0;
+  kv_scan(mine, wave_tot, live);
+  int holes = 0, movers = 0;
+  for (int base = 0; base < N; base += kKvThreads) {
+    const int i = base + tid;
+    const bool used = i < N && a.refs[i] > 0;
+    const int hole = i < live && !used, mover = i >= live && used;
+    int total;
+    const int upto = kv_scan(hole | (mover << 16), wave_tot, total);
+    if (hole) a.dst[holes + (upto & 0xffff) - 1] = i;
+    if (mover) a.src[movers + (upto >> 16) - 1] = i;
+    if (i >= live && i < N && !used) a.moved[i] = i;  // (a table may still name it)
+    holes += total & 0xffff;
+    movers += total >> 16;
+  }
+  __threadfence_block();
+  __syncthreads();
+  for (int k = tid; k < movers; k += kKvThreads) {
+    const int from = a.src[k], to = a.dst[k];
+    a.moved[from] = to;
+    a.refs[to] = a.refs[from];
+    a.refs[from] = 0;
+  }
+  if (tid == 0) a.head[0] = live, a.head[1] = movers;
+}
+
+// The first workgroups rewrite the table, the others copy.
+__global__ __launch_bounds__(256) void kv_compact_copy_kernel(KvCompactArgs a) {
+  if ((int)blockIdx.x < a.table_blocks) {
+    const int live = a.head[0];
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.entries; i += (int64_t)a.table_blocks * 256) {
+      const int id = a.table[i];
+      if (id >= live && id < a.pool.N) a.table[i] = a.moved[id];
+    }
+    return;
+  }
+  const int movers = a.head[1], blocks = (int)gridDim.x - a.table_blocks;
+  for (int64_t w = (int)blockIdx.x - a.table_blocks; w < (int64_t)movers * a.pool.groups; w += blocks) {
+    const int k = (int)(w / a.pool.groups);
+    kv_copy_part(a.pool, a.src[k], a.dst[k], a.pool.P, (int)(w - (int64_t)k * a.pool.groups));
+  }
+}
+
+}  // namespace smlm

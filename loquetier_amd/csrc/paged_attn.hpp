@@ -1,0 +1,692 @@
+// Causal attention of the new rows of a batch over a paged cache.
+//
+//   o[t, h] = sum_j p_j v[j, h / g],  p = softmax_j(scale q[t, h] . k[j, h / g]),  j <= len - n + (t - first row)
+// for every sequence of the batch: n new rows (one when it decodes, a chunk when a prompt comes in), len tokens in the cache
+// with the new ones, g = q heads a kv head.  A row that sees no key is zero.
+//
+// The g query heads of a kv head read the same keys, so they are rows of one tile: row p of a sequence's tiles is token p / g,
+// head p % g.  Both products run on the matrix cores with the keys' product transposed, S^T = K Q^T: a lane then
+// holds one query row and some keys of it, the softmax's maximum and sum cross lanes once or twice, and the probabilities lie in
+// the registers as the next product, O^T = V^T P^T, reads them (the keys of a step may come in any order, as long as P and V
+// agree).  V is read from LDS through the transposing load.  One pass over the keys with the running maximum and sum; statistics
+// and accumulators in float.  The probabilities are rounded to the element type for the second product: relative errors of half
+// a step each, of random sign, so about as much as the rounding of the result itself.
+//
+// Sequences of up to 32 tile rows (decoding, short chunks) are bound by HBM: the four waves of a workgroup take 32 keys in turn,
+// K straight to registers, V through a part of LDS of the wave's own, no barrier until the end.  Others take 128 tile rows
+// a workgroup, 32 a wave, over K and V tiles of 64 keys that the four waves share.  A long axis is cut into parts where there are few
+// tiles (the plan decides, by the batch's total of keys); the parts' results are joined by a second launch, in order.
+//
+// Keys past a sequence's end and keys of pages that the pool does not hold read as zeros from a constant and get no weight.
+// Keys of later rows of a chunk are in the cache already; their weight is zero, but zero times an infinity or NaN is
+// not, so the tiles that some rows see in part look whether their V has such a value and then add key by key to the rows that see it.
+#pragma once
+#include "smlm_common.hpp"
+
+namespace smlm {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <int DT>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  if (DT == SMLM_DTYPE_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+constexpr int kAttnSmallRows = 32;   // tile rows of a sequence up to which it takes the few-row path
+constexpr int kAttnBigRows = 128;    // tile rows of a workgroup of the other
+constexpr int kAttnSmallItems = 2048, kAttnBigItems = 768;  // parts that the long axis is cut into, at most, over the card
+constexpr int kAttnMinKeys = 256;    // keys of a part, at least
+
+struct AttnItem {   // a tile of a sequence and a part of its keys
+  int row0, n, len, trow;  // the sequence: first row, rows, tokens, row of the page table
+  int first;               // first tile row
+  int kb, ke;              // keys
+  int part;                // where its part of the result goes, or -1: it is the whole
+};
+struct AttnJoin {   // a tile whose keys were cut
+  int row0, n, first, part, parts;
+  int pad[3];
+};
+struct AttnPlanView {
+  int* hdr;          // [16]: 0 items, 1 joins
+  int* start;        // [3][S + 1] running sums by sequence: items, joins, parts
+  AttnItem* items;
+  AttnJoin* joins;
+};
+
+inline int attn_tiles_max(int T, int S, int g) { return (int)((int64_t)T * g / kAttnBigRows) + S; }
+inline int attn_items_max(int T, int S, int g, int Hkv) { return attn_tiles_max(T, S, g) + (kAttnSmallItems + kAttnBigItems) / Hkv + 2; }
+inline int attn_joins_max(int T, int S, int g, int Hkv) {
+  const int cut = (kAttnSmallItems + kAttnBigItems) / Hkv + 2, tiles = attn_tiles_max(T, S, g);
+  return cut < tiles ? cut : tiles;
+}
+inline int attn_parts_max(int Hkv, int items) { return 2 * (items / Hkv + 1); }
+inline size_t attn_plan_carve(void* base, int T, int S, int g, int Hkv, AttnPlanView* pv) {
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = off;
+    off = align_up(off + bytes, 256);
+    return base ? reinterpret_cast<char*>(base) + o : nullptr;
+  };
+  AttnPlanView v;
+  v.hdr = reinterpret_cast<int*>(take(64));
+  v.start = reinterpret_cast<int*>(take((size_t)3 * (S + 1) * 4));
+  v.items = reinterpret_cast<AttnItem*>(take((size_t)attn_items_max(T, S, g, Hkv) * sizeof(AttnItem)));
+  v.joins = reinterpret_cast<AttnJoin*>(take((size_t)attn_joins_max(T, S, g, Hkv) * sizeof(AttnJoin)));
+  if (pv) *pv = v;
+  return off;
+}
+
+// ---- the plan ---------------------------------------------------------------------------------------------
+struct AttnPlanArgs {
+  AttnPlanView plan;
+  const int *q_indptr, *kv_len, *requests;  // [S + 1], [S], [S] rows of the page table (null: s)
+  int T, S, g, Hkv, R;
+  int most;                                 // tokens that a row of the table holds
+  int items_max, joins_max, parts_small_max, parts_big_max;
+};
+
+struct AttnSeq {
+  int row0, n, len, trow, tile, tiles;
+};
+__device__ __forceinline__ AttnSeq attn_seq(const AttnPlanArgs& a, int s) {
+  AttnSeq q;
+  const int r0 = a.q_indptr[s], r1 = a.q_indptr[s + 1];
+  q.row0 = r0 < 0 ? 0 : (r0 > a.T ? a.T : r0);
+  const int e = r1 > a.T ? a.T : r1;
+  q.n = e > q.row0 ? e - q.row0 : 0;
+  q.trow = a.requests ? a.requests[s] : s;
+  q.len = a.kv_len[s];
+  if (q.trow < 0 || q.trow >= a.R || q.len < 0) q.trow = 0, q.len = 0;
+  if (q.len > a.most) q.len = a.most;
+  const int rows = q.n * a.g;
+  q.tile = rows <= kAttnSmallRows ? kAttnSmallRows : kAttnBigRows;
+  q.tiles = (rows + q.tile - 1) / q.tile;
+  return q;
+}
+
+constexpr int kAttnPlanThreads = 1024;
+
+template <typename V>
+__device__ __forceinline__ V attn_block_sum(V v, V* red) {
+#pragma unroll
+  for (int d = 1; d < kWaveSize; d *= 2) v += __shfl_xor(v, d, kWaveSize);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  V t = 0;
+  for (int w = 0; w < kAttnPlanThreads / kWaveSize; ++w) t += red[w];
+  return t;
+}
+
+__device__ __forceinline__ int attn_scan(int v, int* wave_tot, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int d = 1; d < kWaveSize; d *= 2) {
+    const int u = __shfl_up(v, d, kWaveSize);
+    if (lane >= d) v += u;
+  }
+  __syncthreads();
+  if (lane == 63) wave_tot[wave] = v;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kAttnPlanThreads / kWaveSize; ++w) {
+    const int t = wave_tot[w];
+    before += w < wave ? t : 0;
+    total += t;
+  }
+  return v + before;
+}
+
+// One workgroup.  A sequence's tiles are cut alike, by its length; a part holds at least the batch's keys (times tiles and kv
+// heads) over the number of parts that the card is to get, so the numbers of items and parts have bounds that the host knows.
+__global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArgs a) {
+  __shared__ int wave_tot[16];
+  __shared__ int64_t red[16];
+  const int tid = threadIdx.x;
+  int64_t small = 0, big = 0;
+  for (int s = tid; s < a.S; s += kAttnPlanThreads) {
+    const AttnSeq q = attn_seq(a, s);
+    (q.tile == kAttnSmallRows ? small : big) += (int64_t)q.tiles * q.len;
+  }
+  small = attn_block_sum(small, red);
+  big = attn_block_sum(big, red);
+  // (keys of a part, a multiple of 64; ceil so that total / part stays within the bound)
+  auto part_of = [&](int64_t keys, int items) {
+    const int64_t c = (keys * a.Hkv + items - 1) / items;
+    const int64_t m = c < kAttnMinKeys ? kAttnMinKeys : c;
+    return (int)((m + 63) / 64 * 64 < 0x40000000 ? (m + 63) / 64 * 64 : 0x40000000);
+  };
+  const int cut_small = part_of(small, kAttnSmallItems), cut_big = part_of(big, kAttnBigItems);
+  int items = 0, joins = 0, parts_small = 0, parts_big = 0;
+  int* start = a.plan.start;
+  for (int base = 0; base < a.S; base += kAttnPlanThreads) {
+    const int s = base + tid;
+    int ni = 0, nj = 0, np = 0;
+    bool is_small = true;
+    if (s < a.S) {
+      const AttnSeq q = attn_seq(a, s);
+      is_small = q.tile == kAttnSmallRows;
+      const int cut = is_small ? cut_small : cut_big;
+      const int ns = q.len > cut ? (q.len + cut - 1) / cut : 1;
+      ni = q.tiles * ns;
+      nj = ns > 1 ? q.tiles : 0;
+      np = ns > 1 ? ni : 0;
+    }
+    int total;
+    int upto = attn_scan(ni, wave_tot, total);
+    if (s < a.S) start[s + 1] = items + upto;
+    items += total;
+    upto = attn_scan(nj, wave_tot, total);
+    if (s < a.S) start[(a.S + 1) + s + 1] = joins + upto;
+    joins += total;
+    upto = attn_scan(is_small ? np : 0, wave_tot, total);
+    const int at_small = parts_small + upto - np;
+    parts_small += total;
+    upto = attn_scan(is_small ? 0 : np, wave_tot, total);
+    const int at_big = parts_big + upto - np;
+    parts_big += total;
+    if (s < a.S) start[2 * (a.S + 1) + s] = is_small ? at_small : at_big;
+  }
+  if (tid == 0) {
+    start[0] = start[a.S + 1] = 0;
+    a.plan.hdr[0] = items < a.items_max ? items : a.items_max;
+    a.plan.hdr[1] = joins < a.joins_max ? joins : a.joins_max;
+  }
+  __syncthreads();
+  for (int i = tid; i < items && i < a.items_max; i += kAttnPlanThreads) {
+    int lo = 0, hi = a.S;
+    while (hi - lo > 1) {  // last s with start[s] <= i
+      const int mid = (lo + hi) >> 1;
+      if (start[mid] <= i) lo = mid;
+      else hi = mid;
+    }
+    const AttnSeq q = attn_seq(a, lo);
+    const int ns = (start[lo + 1] - start[lo]) / q.tiles, k = i - start[lo];
+    const int t = q.tiles - 1 - k / ns, j = k % ns;  // (the later tiles of a prompt see more keys: they go first)
+    AttnItem it;
+    it.row0 = q.row0, it.n = q.n, it.len = q.len, it.trow = q.trow, it.first = t * q.tile;
+    const int last = min(it.first + q.tile, q.n * a.g) - 1;
+    const int keys = max(0, min(q.len, q.len - q.n + last / a.g + 1));  // that the tile's last row sees
+    const int step = ((keys + ns - 1) / ns + 63) / 64 * 64;
+    it.kb = (int)min((int64_t)keys, (int64_t)j * step);
+    it.ke = (int)min((int64_t)keys, (int64_t)(j + 1) * step);
+    it.part = ns > 1 ? start[2 * (a.S + 1) + lo] + t * ns + j : -1;
+    // (sequences that overlap, which none should, could come to more parts than there is room for)
+    const int parts_max = q.tile == kAttnSmallRows ? a.parts_small_max : a.parts_big_max;
+    const bool fits = it.part < parts_max;
+    if (!fits) it.n = 0, it.kb = it.ke = 0, it.part = -1;
+    a.plan.items[i] = it;
+    if (ns > 1 && j == 0) {
+      const int at = start[(a.S + 1) + lo] + t;
+      if (at < a.joins_max) a.plan.joins[at] = AttnJoin{q.row0, fits && it.part + ns <= parts_max ? q.n : 0, it.first, it.part, ns, {0, 0, 0}};
+    }
+  }
+}
+
+// ---- attention --------------------------------------------------------------------------------------------
+struct AttnArgs {
+  uint16_t* out;
+  const uint16_t *q, *k, *v;
+  const int* table;          // [R, M]
+  AttnPlanView plan;
+  float *po_small, *po_big;  // parts of the results, [part][kv head][tile row][D], not divided by their sums
+  float *pm_small, *pm_big;  // [part][kv head][tile row][2]: maximum (of the scores times scale / log 2), sum
+  int64_t o_row, o_head, q_row, q_head, c_page, c_head, c_slot;
+  int M, n_pages, P, T, Hq, Hkv, g;
+  uint32_t div_mul;          // division by P: ((x * div_mul >> 32) + x) >> div_shift in 33 bits
+  int div_shift;
+  float scale;               // times log2 e
+};
+
+static __device__ __align__(16) const uint32_t attn_zeros[4] = {0u, 0u, 0u, 0u};
+
+__device__ __forceinline__ int attn_div(uint32_t x, uint32_t mul, int shift) {
+  return (int)(((uint64_t)__umulhi(x, mul) + x) >> shift);
+}
+
+// Element offset of a key within the pool (its kv head apart), -1 where there is none.
+__device__ __forceinline__ int64_t attn_find(const AttnArgs& a, const int* trow, int key, int ke) {
+  if (key >= ke) return -1;
+  const int j = attn_div((uint32_t)key, a.div_mul, a.div_shift);
+  const int page = trow[j];
+  if (page < 0 || page >= a.n_pages) return -1;
+  return (int64_t)page * a.c_page + (int64_t)(key - j * a.P) * a.c_slot;
+}
+__device__ __forceinline__ int64_t attn_shfl(int64_t v, int lane) {
+  const int lo = __shfl((int)(uint32_t)v, lane, kWaveSize), hi = __shfl((int)(v >> 32), lane, kWaveSize);
+  return ((int64_t)hi << 32) | (uint32_t)lo;
+}
+__device__ __forceinline__ u32x4 attn_ld(const uint16_t* base, int64_t off, int d) {
+  return ldg16(off >= 0 ? base + off + d : reinterpret_cast<const uint16_t*>(attn_zeros));
+}
+
+// A row of K or V in LDS: pieces of 16 bytes, the piece's place turned by the row so that the lanes of a matrix operand,
+// which read one piece of sixteen rows, meet all banks.
+template <int D>
+__device__ __forceinline__ int attn_place(int row, int piece) {
+  return row * D + ((D == 128 ? piece ^ (row & 15) : piece ^ ((row >> 1) & 7)) << 3);
+}
+
+// whether an element of a pair of 16-bit values is an infinity or NaN
+template <int DT>
+__device__ __forceinline__ uint32_t attn_not_finite(uint32_t x) {
+  return DT == SMLM_DTYPE_F16 ? ((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u : ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+}
+
+// Four elements of V by four keys: keys row, .. row + 3 (of this lane's sixteen), dimensions d0 + 0 .. 15, transposed.
+template <int D>
+__device__ __forceinline__ u32x2 attn_read_v(const uint16_t* lds, int row, int d0) {
+  const int l = threadIdx.x & 15, r = row + (l >> 2), d = d0 + (l & 3) * 4;
+  return lds_read_tr16(lds + attn_place<D>(r, d >> 3) + (d & 7));
+}
+
+template <int DT>
+__device__ __forceinline__ u32x2 attn_pack4(float a, float b, float c, float d) {
+  u32x2 o;
+  o[0] = pack2<DT>(a, b);
+  o[1] = pack2<DT>(c, d);
+  return o;
+}
+__device__ __forceinline__ uint16_t* attn_out_row(const AttnArgs& a, const AttnItem& it, int kvh, int p) {
+  return a.out + (int64_t)(it.row0 + p / a.g) * a.o_row + (int64_t)(kvh * a.g + p % a.g) * a.o_head;
+}
+
+// (the hardware's own: results under the smallest normal float are zero)
+__device__ __forceinline__ float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Up to 16 * MT tile rows.  Layouts of a 16 x 16 x 32 product by lane (c = lane & 15, b = lane >> 4): operands row or column c,
+// k = 8 b + 0..7; result column c, rows 4 b + 0..3.
+template <int DT, int D, int MT>
+__device__ __forceinline__ void attn_small(const AttnArgs& a, const AttnItem& it, int kvh, uint16_t* lds, float* ml) {
+  constexpr int kSteps = D / 32, kBlk = D / 16, kVLoads = D / 16;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, b = lane >> 4;
+  const int rows = it.n * a.g;
+  const int* trow = a.table + (int64_t)it.trow * a.M;
+  const uint16_t *kp = a.k + (int64_t)kvh * a.c_head, *vp = a.v + (int64_t)kvh * a.c_head;
+  uint16_t* vl = lds + wave * 32 * D;
+  const u32x4 zero4 = {0u, 0u, 0u, 0u};
+
+  u32x4 q[MT][kSteps];
+  int lim[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const int p = it.first + t * 16 + c, pc = p < rows ? p : 0;
+    const uint16_t* src = a.q + (int64_t)(it.row0 + pc / a.g) * a.q_row + (int64_t)(kvh * a.g + pc % a.g) * a.q_head;
+    lim[t] = min(it.ke - 1, it.len - it.n + pc / a.g);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const u32x4 x = ldg16(src + s * 32 + b * 8);
+      q[t][s] = p < rows ? x : zero4;
+    }
+  }
+  const int lim0 = it.len - it.n + it.first / a.g;  // the first row's: a tile up to it is seen whole by all
+
+  f32x4 o[MT][kBlk];
+  float m[MT], l[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    m[t] = -INFINITY, l[t] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kBlk; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  u32x4 kr[2][kSteps], vr[kVLoads];
+  constexpr int kRowLanes = D / 8, kRowsLoad = 64 / kRowLanes;  // lanes a row of V, rows a load
+  auto load = [&](int64_t off) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int64_t f = attn_shfl(off, u * 16 + c);
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) kr[u][s] = attn_ld(kp, f, s * 32 + b * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < kVLoads; ++i)
+      vr[i] = attn_ld(vp, attn_shfl(off, i * kRowsLoad + lane / kRowLanes), (lane % kRowLanes) * 8);
+  };
+  int64_t off = attn_find(a, trow, it.kb + wave * 32 + (lane & 31), it.ke), next = -1;
+  load(off);
+  next = attn_find(a, trow, it.kb + wave * 32 + 128 + (lane & 31), it.ke);
+  for (int base = it.kb + wave * 32; base < it.ke; base += 128) {
+    const uint32_t ok = (uint32_t)__ballot(off >= 0);
+    f32x4 s[MT][2];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        s[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) s[t][u] = Num<DT>::mfma(kr[u][k], q[t][k], s[t][u]);
+      }
+    const bool edge = base + 31 > lim0;
+    uint32_t odd = 0;
+#pragma unroll
+    for (int i = 0; i < kVLoads; ++i) {
+      const int r = i * kRowsLoad + lane / kRowLanes;
+      *(u32x4*)(vl + attn_place<D>(r, lane % kRowLanes)) = vr[i];
+      if (edge) odd |= attn_not_finite<DT>(vr[i][0]) | attn_not_finite<DT>(vr[i][1]) | attn_not_finite<DT>(vr[i][2]) | attn_not_finite<DT>(vr[i][3]);
+    }
+    off = next;
+    load(off);
+    next = attn_find(a, trow, base + 256 + (lane & 31), it.ke);
+
+    const bool guard = edge && __ballot(odd != 0) != 0;
+    u32x4 pf[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      if (edge || ok != 0xffffffffu) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = u * 16 + b * 4 + i;
+            if (!(ok >> key & 1) || base + key > lim[t]) s[t][u][i] = -INFINITY;
+          }
+      }
+      float mx = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
+                       fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
+      mx = fmaxf(mx, __shfl_xor(mx, 16, kWaveSize));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, kWaveSize));
+      const float mn = fmaxf(m[t], mx), ms = mn == -INFINITY ? 0.0f : mn * a.scale;
+      const float turn = attn_exp2(m[t] * a.scale - ms);
+      m[t] = mn;
+      float sum = 0.0f, p[8];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[u * 4 + i] = attn_exp2(s[t][u][i] * a.scale - ms);
+          sum += p[u * 4 + i];
+        }
+      l[t] = l[t] * turn + sum;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pf[t][i] = pack2<DT>(p[2 * i], p[2 * i + 1]);
+#pragma unroll
+      for (int i = 0; i < kBlk; ++i) o[t][i] *= turn;
+    }
+    if (!guard) {
+#pragma unroll
+      for (int i = 0; i < kBlk; ++i) {
+        const u32x2 v0 = attn_read_v<D>(vl, b * 4, i * 16), v1 = attn_read_v<D>(vl, 16 + b * 4, i * 16);
+        const u32x4 vf = {v0[0], v0[1], v1[0], v1[1]};
+#pragma unroll
+        for (int t = 0; t < MT; ++t) o[t][i] = Num<DT>::mfma(vf, pf[t], o[t][i]);
+      }
+    } else {  // key by key: slot j of lane group bb
+#pragma unroll 1
+      for (int x = 0; x < 32; ++x) {
+        const int bb = x >> 3, j = x & 7, key = (j >> 2) * 16 + bb * 4 + (j & 3);
+        u32x4 only;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) only[e] = b == bb && (j >> 1) == e ? (j & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
+#pragma unroll
+        for (int i = 0; i < kBlk; ++i) {
+          const u32x2 v0 = attn_read_v<D>(vl, b * 4, i * 16), v1 = attn_read_v<D>(vl, 16 + b * 4, i * 16);
+          const u32x4 vf = u32x4{v0[0], v0[1], v1[0], v1[1]} & only;
+#pragma unroll
+          for (int t = 0; t < MT; ++t) {
+            const f32x4 add = Num<DT>::mfma(vf, pf[t] & only, f32x4{0.f, 0.f, 0.f, 0.f});
+            if (base + key <= lim[t]) o[t][i] += add;
+          }
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();  // (this wave's LDS reads come before its next writes)
+  }
+
+  // the four waves' results, 16 rows at a time
+  float* ol = reinterpret_cast<float*>(lds);  // [4][16][D]
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    l[t] += __shfl_xor(l[t], 16, kWaveSize);
+    l[t] += __shfl_xor(l[t], 32, kWaveSize);
+    __syncthreads();  // V, or the last turn's results, have been read
+    if (b == 0) ml[(wave * 16 + c) * 2] = m[t] * a.scale, ml[(wave * 16 + c) * 2 + 1] = l[t];
+#pragma unroll
+    for (int i = 0; i < kBlk; ++i) *(f32x4*)(ol + (wave * 16 + c) * D + ((i * 4 + b) ^ (c & 7)) * 4) = o[t][i];
+    __syncthreads();
+    for (int x = threadIdx.x; x < 16 * (D / 4); x += 256) {
+      const int r = x / (D / 4), d4 = x % (D / 4), p = it.first + t * 16 + r;
+      if (p >= rows) continue;
+      float mw[4], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mw[w] = ml[(w * 16 + r) * 2], top = fmaxf(top, mw[w]);
+      const float ref = top == -INFINITY ? 0.0f : top;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = attn_exp2(mw[w] - ref);
+        sum += f * ml[(w * 16 + r) * 2 + 1];
+        const f32x4 v = *(const f32x4*)(ol + (w * 16 + r) * D + (d4 ^ (r & 7)) * 4);
+        acc += f * v;
+      }
+      if (it.part >= 0) {
+        const int64_t at = ((int64_t)it.part * a.Hkv + kvh) * kAttnSmallRows + t * 16 + r;
+        *(SMLM_GLOBAL f32x4*)(a.po_small + at * D + d4 * 4) = acc;
+        if (d4 == 0) a.pm_small[at * 2] = top, a.pm_small[at * 2 + 1] = sum;
+      } else {
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        *(SMLM_GLOBAL u32x2*)(attn_out_row(a, it, kvh, p) + d4 * 4) =
+            attn_pack4<DT>(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+      }
+    }
+  }
+}
+
+// 128 tile rows, 32 a wave.  Layouts of a 32 x 32 x 16 product by lane (c = lane & 31, h = lane >> 5): operands row or
+// column c, k = 8 h + 0..7; result column c, rows 8 (i / 4) + 4 h + i % 4, i = 0..15.
+template <int DT, int D>
+__device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, int kvh, uint16_t* lds, uint32_t* flags) {
+  constexpr int kSteps = D / 16, kBlk = D / 32, kKeys = 64;
+  constexpr int kRowLanes = D / 8, kRowsLoad = 64 / kRowLanes, kLoads = 16 / kRowsLoad;  // a wave loads 16 rows of K and of V
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  const int rows = it.n * a.g;
+  const int* trow = a.table + (int64_t)it.trow * a.M;
+  const uint16_t *kp = a.k + (int64_t)kvh * a.c_head, *vp = a.v + (int64_t)kvh * a.c_head;
+  const u32x4 zero4 = {0u, 0u, 0u, 0u};
+
+  const int p = it.first + wave * 32 + c, pc = p < rows ? p : 0;
+  const int lim = min(it.ke - 1, it.len - it.n + pc / a.g);
+  const int lim0 = it.len - it.n + it.first / a.g;  // of the workgroup's first row
+  u32x4 q[kSteps];
+  {
+    const uint16_t* src = a.q + (int64_t)(it.row0 + pc / a.g) * a.q_row + (int64_t)(kvh * a.g + pc % a.g) * a.q_head;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const u32x4 x = ldg16(src + s * 16 + h * 8);
+      q[s] = p < rows ? x : zero4;
+    }
+  }
+  f32x16 o[kBlk];
+  float m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kBlk; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
+
+  u32x4 kr[kLoads], vr[kLoads];
+  auto load = [&](int64_t off) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int64_t f = attn_shfl(off, i * kRowsLoad + lane / kRowLanes);
+      kr[i] = attn_ld(kp, f, (lane % kRowLanes) * 8);
+      vr[i] = attn_ld(vp, f, (lane % kRowLanes) * 8);
+    }
+  };
+  int64_t off = attn_find(a, trow, it.kb + wave * 16 + (lane & 15), it.ke);
+  load(off);
+  int64_t next = attn_find(a, trow, it.kb + kKeys + wave * 16 + (lane & 15), it.ke);
+  int turn_buf = 0;
+  for (int base = it.kb; base < it.ke; base += kKeys, turn_buf ^= 1) {
+    uint16_t *kl = lds + turn_buf * (2 * kKeys * D), *vl = kl + kKeys * D;
+    uint32_t* fl = flags + turn_buf * 4;
+    const bool edge = base + kKeys - 1 > lim0;
+    uint32_t odd = 0;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = wave * 16 + i * kRowsLoad + lane / kRowLanes;
+      *(u32x4*)(kl + attn_place<D>(r, lane % kRowLanes)) = kr[i];
+      *(u32x4*)(vl + attn_place<D>(r, lane % kRowLanes)) = vr[i];
+      if (edge) odd |= attn_not_finite<DT>(vr[i][0]) | attn_not_finite<DT>(vr[i][1]) | attn_not_finite<DT>(vr[i][2]) | attn_not_finite<DT>(vr[i][3]);
+    }
+    {
+      const uint32_t mine = (uint32_t)__ballot(off >= 0) & 0xffffu, any_odd = __ballot(odd != 0) != 0 ? 0x10000u : 0u;
+      if (lane == 0) fl[wave] = mine | any_odd;
+    }
+    __syncthreads();
+    off = next;
+    load(off);
+    next = attn_find(a, trow, base + 2 * kKeys + wave * 16 + (lane & 15), it.ke);
+    const uint32_t f0 = fl[0], f1 = fl[1], f2 = fl[2], f3 = fl[3];
+    const uint64_t ok = (uint64_t)((f0 & 0xffffu) | (f1 << 16)) | ((uint64_t)((f2 & 0xffffu) | (f3 << 16)) << 32);
+    const bool guard = ((f0 | f1 | f2 | f3) >> 16) != 0;
+
+    f32x16 s[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[u][e] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kSteps; ++k) {
+        const u32x4 kf = *(const u32x4*)(kl + attn_place<D>(u * 32 + c, k * 2 + h));
+        s[u] = mfma32<DT>(kf, q[k], s[u]);
+      }
+    }
+    if (edge || ok != ~0ull) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int key = u * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
+          if (!(ok >> key & 1) || base + key > lim) s[u][e] = -INFINITY;
+        }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[u][e]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, kWaveSize));
+    const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.0f : mn * a.scale;
+    if (__ballot(mn > m)) {  // some row's maximum has grown
+      const float turn = attn_exp2(m * a.scale - ms);
+      l *= turn;
+#pragma unroll
+      for (int i = 0; i < kBlk; ++i) o[i] *= turn;
+    }
+    m = mn;
+    u32x4 pf[2][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float p0 = attn_exp2(s[u][e] * a.scale - ms), p1 = attn_exp2(s[u][e + 1] * a.scale - ms);
+        l += p0 + p1;
+        pf[u][e >> 3][(e >> 1) & 3] = pack2<DT>(p0, p1);
+      }
+    if (!guard) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int i = 0; i < kBlk; ++i) {
+            const int r = u * 32 + ks * 16 + h * 4, d = i * 32 + ((lane >> 4) & 1) * 16;
+            const u32x2 v0 = attn_read_v<D>(vl, r, d), v1 = attn_read_v<D>(vl, r + 8, d);
+            o[i] = mfma32<DT>(u32x4{v0[0], v0[1], v1[0], v1[1]}, pf[u][ks], o[i]);
+          }
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll 1
+          for (int x = 0; x < 16; ++x) {  // slot j of half hh
+            const int hh = x >> 3, j = x & 7, key = u * 32 + ks * 16 + (j >> 2) * 8 + hh * 4 + (j & 3);
+            u32x4 only;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) only[e] = h == hh && (j >> 1) == e ? (j & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
+#pragma unroll
+            for (int i = 0; i < kBlk; ++i) {
+              const int r = u * 32 + ks * 16 + h * 4, d = i * 32 + ((lane >> 4) & 1) * 16;
+              const u32x2 v0 = attn_read_v<D>(vl, r, d), v1 = attn_read_v<D>(vl, r + 8, d);
+              f32x16 add;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) add[e] = 0.0f;
+              add = mfma32<DT>(u32x4{v0[0], v0[1], v1[0], v1[1]} & only, pf[u][ks] & only, add);
+              if (base + key <= lim) o[i] += add;
+            }
+          }
+    }
+  }
+  l += __shfl_xor(l, 32, kWaveSize);
+  if (p >= rows) return;  // (no barrier below)
+  if (it.part >= 0) {
+    const int64_t at = ((int64_t)it.part * a.Hkv + kvh) * kAttnBigRows + wave * 32 + c;
+#pragma unroll
+    for (int i = 0; i < kBlk; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *(SMLM_GLOBAL f32x4*)(a.po_big + at * D + i * 32 + 2 * e + 4 * h) = f32x4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+    if (h == 0) a.pm_big[at * 2] = m * a.scale, a.pm_big[at * 2 + 1] = l;
+  } else {
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* dst = attn_out_row(a, it, kvh, p);
+#pragma unroll
+    for (int i = 0; i < kBlk; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *(SMLM_GLOBAL u32x2*)(dst + i * 32 + 2 * e + 4 * h) =
+            attn_pack4<DT>(o[i][e] * inv, o[i][e + 1] * inv, o[i][e + 2] * inv, o[i][e + 3] * inv);
+  }
+}
+
+// Neighbouring workgroups take the kv heads of one item: with eight of them, or a multiple, a head's tiles meet in one XCD's L2.
+template <int DT, int D>
+__global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
+  __shared__ __align__(16) uint16_t lds[2 * 2 * 64 * D];
+  __shared__ uint32_t side[128];
+  const int i = (int)blockIdx.x / a.Hkv, kvh = (int)blockIdx.x - i * a.Hkv;
+  if (i >= a.plan.hdr[0]) return;
+  const AttnItem it = a.plan.items[i];
+  const int rows = it.n * a.g;
+  if (rows > kAttnSmallRows) attn_big<DT, D>(a, it, kvh, lds, side);
+  else if (rows > 16) attn_small<DT, D, 2>(a, it, kvh, lds, reinterpret_cast<float*>(side));
+  else attn_small<DT, D, 1>(a, it, kvh, lds, reinterpret_cast<float*>(side));
+}
+
+// The parts of a tile's rows: each weighed by its maximum against the largest, in order.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+  const int i = (int)blockIdx.x / a.Hkv, kvh = (int)blockIdx.x - i * a.Hkv;
+  if (i >= a.plan.hdr[1]) return;
+  const AttnJoin jn = a.plan.joins[i];
+  const int rows = jn.n * a.g;
+  const bool small = rows <= kAttnSmallRows;
+  const int tile = small ? kAttnSmallRows : kAttnBigRows;
+  const float *po = small ? a.po_small : a.po_big, *pm = small ? a.pm_small : a.pm_big;
+  AttnItem it;
+  it.row0 = jn.row0;
+  const int n = min(tile, rows - jn.first);
+  for (int x = threadIdx.x; x < n * (D / 4); x += 256) {
+    const int r = x / (D / 4), d4 = x % (D / 4);
+    float top = -INFINITY, sum = 0.0f;
+    for (int j = 0; j < jn.parts; ++j) top = fmaxf(top, pm[((((int64_t)jn.part + j) * a.Hkv + kvh) * tile + r) * 2]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < jn.parts; ++j) {
+      const int64_t at = (((int64_t)jn.part + j) * a.Hkv + kvh) * tile + r;
+      const float f = attn_exp2(pm[at * 2] - ref);
+      sum += f * pm[at * 2 + 1];
+      acc += f * ldg_f4(po + at * D + d4 * 4);
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    *(SMLM_GLOBAL u32x2*)(attn_out_row(a, it, kvh, jn.first + r) + d4 * 4) =
+        attn_pack4<DT>(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+  }
+}
+
+}  // namespace smlm

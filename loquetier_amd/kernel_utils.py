@@ -1,8 +1,8 @@
 """Host-side mirror of src/loquetier_src/kernel_utils.py for the SMLM path:
 `BatchLenInfo` (row layout of the flat batch) and the `add_lora` autograd
 Function, with the reference's positional arguments and `None`-padded backward
-tuple, running on the HIP kernels; and the `rms_norm` autograd Function
-(kernel_utils.py:149-176).
+tuple, running on the HIP kernels; the `rms_norm` autograd Function
+(kernel_utils.py:149-176); and `qk_norm_rope`, the same for queries and keys by head with their rotation.
 """
 from __future__ import annotations
 
@@ -294,3 +294,35 @@ class rms_norm(Function):
         d_weight = torch.empty_like(w)
         kernel.rms_norm_backward(dx, d_weight, grad_output.contiguous(), x, w, rms_1)
         return dx, d_weight, None
+
+
+class qk_norm_rope(Function):
+    """`qk_norm_rope.apply(q, k, q_weight, k_weight, table, positions, eps)`: queries [rows, q_heads, head_dim] and keys [rows,
+    kv_heads, head_dim] normed by head (where the weight is not None) and rotated by position, in one launch (see
+    ops/_kernels.qk_norm_rope); returns both.  The reference rotates with tensor expressions
+    (src/loquetier_src/models/mixed_llama.py:93-195).  The backward makes the root mean squares again, so only the inputs are
+    kept, and of those only what it reads: nothing of q and k where there is no norm."""
+
+    @staticmethod
+    def forward(ctx: FunctionCtx, q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor],
+                k_weight: Optional[torch.Tensor], table: torch.Tensor, positions: torch.Tensor, eps: float = 1e-6):
+        # (the layouts of views, an expanded one's too, do not carry over)
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        kernel.qk_norm_rope(q_out, k_out, q, k, table, positions, q_weight, k_weight, eps)
+        ctx.save_for_backward(None if q_weight is None else q, None if k_weight is None else k, q_weight, k_weight, table,
+                              positions)
+        ctx.eps = eps
+        return q_out, k_out
+
+    @staticmethod
+    def backward(ctx: FunctionCtx, gq: torch.Tensor, gk: torch.Tensor):
+        q, k, q_weight, k_weight, table, positions = ctx.saved_tensors
+        gq, gk = (g if kernel._heads_fit(g) and g.data_ptr() % 16 == 0 else g.clone(memory_format=torch.contiguous_format)
+                  for g in (gq, gk))
+        dq, dk = (torch.empty(g.shape, dtype=g.dtype, device=g.device) for g in (gq, gk))
+        dqw, dkw = (None if w is None else torch.empty_like(w) for w in (q_weight, k_weight))
+        # (without a norm the gradient stands for the input, which the kernel then does not read)
+        kernel.qk_norm_rope_backward(dq, dk, dqw, dkw, gq, gk, gq if q is None else q, gk if k is None else k, table, positions,
+                                     q_weight, k_weight, ctx.eps)
+        return dq, dk, dqw, dkw, None, None, None

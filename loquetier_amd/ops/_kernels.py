@@ -921,3 +921,357 @@ def segment_scales(seg_adapter: torch.Tensor, table: Optional[torch.Tensor] = No
                                              _stream(dev))
     _lib.check(rc, "segment_scales")
     return seg_out, part_seg, part_out
+
+
+# ---- between the projections: rotation of queries and keys, the cache's pages, attention over them --------------------
+
+def _heads_fit(t: torch.Tensor) -> bool:
+    """Whether the kernels read a tensor [rows, heads, head_dim] where it lies (its address has to be 16-byte aligned too)."""
+    return (t.size(2) == 1 or t.stride(2) == 1) and not any(s % 8 for n, s in zip(t.shape[:2], t.stride()[:2]) if n > 1)
+
+
+def _check_heads(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> None:
+    """[rows, heads, head_dim] of any strides the kernels read: views of one projection's output need no copy."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    _check_dim(3, t, name)
+    if t.numel() and not _heads_fit(t):
+        raise RuntimeError(f"{name} must have its head's dimensions next to each other and strides that are multiples of 8")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise RuntimeError(f"{name} must share q's dtype and device")
+
+
+def _heads(t: Optional[torch.Tensor]) -> _lib.Heads:
+    if t is None:
+        return _lib.Heads()
+    # (the stride of a dimension of one names nothing)
+    return _lib.Heads(t.data_ptr(), t.stride(0) if t.size(0) > 1 else 0, t.stride(1) if t.size(1) > 1 else 0)
+
+
+def _check_ints(dev: torch.device, dtype: torch.dtype, dim: int, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        _check_input(t, name)
+        _check_dim(dim, t, name)
+        if t.dtype != dtype or t.device != dev:
+            raise RuntimeError(f"{name} must be {dtype} on {dev}")
+
+
+def _check_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, like: torch.Tensor, kv_heads: int) -> Tuple[int, int, int]:
+    """Strides (page, head, place) of two caches [n_pages, kv_heads, page_size, head_dim]."""
+    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if not t.is_cuda:
+            raise RuntimeError(f"{n} must be a CUDA tensor")
+        _check_dim(4, t, n)
+        if t.dtype != like.dtype or t.device != like.device:
+            raise RuntimeError(f"{n} must share q's dtype and device")
+        if t.size(3) != like.size(2) or t.size(1) != kv_heads or t.size(2) < 1:
+            raise RuntimeError(f"{n} must be [n_pages, {kv_heads}, page_size, {like.size(2)}]")
+    if k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride():
+        raise RuntimeError("k_cache and v_cache must have the same shape and strides")
+    strides = tuple(s if n > 1 else 0 for n, s in zip(k_cache.shape, k_cache.stride()))
+    if strides[3] != 1 or any(s % 8 for s in strides[:3]):
+        raise RuntimeError("the caches must have a head's dimensions next to each other and strides that are multiples of 8")
+    return strides[:3]
+
+
+def rope_table(n_positions: int, rot_dim: int, base: float = 10000.0, device=None,
+               inv_freq: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """float32 [n_positions, rot_dim] for qk_norm_rope: by position rot_dim / 2 cosines, then the sines.  The angles,
+    position times base ** (-2 j / rot_dim) (or times inv_freq[j], for scaled variants), are taken in 64 bits: far positions lose
+    whole turns in 32."""
+    if rot_dim <= 0 or rot_dim % 16 or n_positions < 0:
+        raise RuntimeError("rot_dim must be a positive multiple of 16")
+    if inv_freq is None:
+        inv_freq = float(base) ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
+    if inv_freq.dim() != 1 or inv_freq.numel() != rot_dim // 2:
+        raise RuntimeError("inv_freq must have rot_dim / 2 entries")
+    angle = torch.arange(n_positions, dtype=torch.float64)[:, None] * inv_freq.detach().double().cpu()
+    return torch.cat([angle.cos(), angle.sin()], 1).float().to(device)
+
+
+def _rope_args(q, k, table, positions, q_weight, k_weight, eps) -> _lib.QkRope:
+    _check_heads(q, "q")
+    _check_heads(k, "k", q)
+    T, Hq, D = q.shape
+    if k.size(0) != T or k.size(2) != D:
+        raise RuntimeError("q and k must have the same rows and head size")
+    if Hq < 1 or k.size(1) < 1:
+        raise RuntimeError("q and k must have heads")
+    if q.dtype not in _DTYPE_CODE or D % 16 or not 0 < D <= 512:
+        raise RuntimeError(f"No suitable kernel. dtype={q.dtype} head_dim={D}")
+    dev = q.device
+    _check_ints(dev, torch.float32, 2, table=table)
+    rot = table.size(1)
+    if rot % 16 or not 0 < rot <= D:
+        raise RuntimeError(f"table must be [positions, rot_dim], rot_dim a multiple of 16 of at most {D}")
+    _check_ints(dev, torch.int32, 1, positions=positions)
+    if positions.size(0) != T:
+        raise RuntimeError("positions must have one entry per row")
+    _check_ints(dev, q.dtype, 1, q_weight=q_weight, k_weight=k_weight)
+    for w in (q_weight, k_weight):
+        if w is not None and w.size(0) != D:
+            raise RuntimeError(f"a weight must have {D} entries")
+    a = _lib.QkRope()
+    a.q, a.k = _heads(q), _heads(k)
+    a.q_weight, a.k_weight, a.table, a.positions = _ptr(q_weight), _ptr(k_weight), table.data_ptr(), positions.data_ptr()
+    a.rows, a.q_heads, a.kv_heads, a.head_dim, a.rot_dim, a.table_rows = T, Hq, k.size(1), D, rot, table.size(0)
+    a.dtype, a.eps = _DTYPE_CODE[q.dtype], float(eps)
+    return a
+
+
+def qk_norm_rope(q_out: torch.Tensor, k_out: Optional[torch.Tensor], q: torch.Tensor, k: torch.Tensor, table: torch.Tensor,
+                 positions: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, v: Optional[torch.Tensor] = None,
+                 k_cache: Optional[torch.Tensor] = None, v_cache: Optional[torch.Tensor] = None,
+                 slots: Optional[torch.Tensor] = None) -> None:
+    """Queries [rows, q_heads, head_dim] and keys [rows, kv_heads, head_dim], each head scaled to a root mean square of one and
+    by its weight [head_dim] (where there is one), then rotated by the row's position (see include/smlm.h).  table: rope_table's;
+    positions: int32 [rows], below 0 for padding.  q_out may be q, k_out may be k.
+
+    With the caches (k_cache, v_cache [n_pages, kv_heads, page_size, head_dim], any strides) and slots (int64 [rows],
+    page * page_size + place, -1: not cached) the keys and v also go there; k_out may then be None."""
+    a = _rope_args(q, k, table, positions, q_weight, k_weight, eps)
+    _check_heads(q_out, "q_out", q)
+    if q_out.shape != q.shape:
+        raise RuntimeError("q_out and q must have the same shape")
+    if k_out is not None:
+        _check_heads(k_out, "k_out", q)
+        if k_out.shape != k.shape:
+            raise RuntimeError("k_out and k must have the same shape")
+    a.q_out, a.k_out = _heads(q_out), _heads(k_out)
+    cache = (v, k_cache, v_cache, slots)
+    if any(t is not None for t in cache):
+        if any(t is None for t in cache):
+            raise RuntimeError("v, k_cache, v_cache and slots come together")
+        _check_heads(v, "v", q)
+        if v.shape != k.shape:
+            raise RuntimeError("v and k must have the same shape")
+        a.page_stride, a.head_stride, a.slot_stride = _check_caches(k_cache, v_cache, q, k.size(1))
+        _check_ints(q.device, torch.int64, 1, slots=slots)
+        if slots.size(0) != q.size(0):
+            raise RuntimeError("slots must have one entry per row")
+        a.v, a.slots = _heads(v), slots.data_ptr()
+        a.n_pages, a.page_size = k_cache.size(0), k_cache.size(2)
+        if a.n_pages > 0:
+            a.k_cache, a.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+    if k_out is None and k_cache is None:
+        raise RuntimeError("k_out may be left out only where keys go to a cache")
+    if k_out is None and a.n_pages == 0:
+        raise RuntimeError("the cache has no pages")
+    dev = q.device
+    with _on(dev):
+        rc = _lib.load().smlm_qk_norm_rope_fwd(C.byref(a), _stream(dev))
+    _lib.check(rc, "qk_norm_rope")
+
+
+def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, dq_weight: Optional[torch.Tensor],
+                          dk_weight: Optional[torch.Tensor], gq: torch.Tensor, gk: torch.Tensor, q: torch.Tensor,
+                          k: torch.Tensor, table: torch.Tensor, positions: torch.Tensor,
+                          q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                          eps: float = 1e-6, workspace: Optional[Workspace] = None) -> None:
+    """Gradients of qk_norm_rope's inputs from those of its outputs, the weights' summed over rows and heads in a fixed
+    order.  q, k, table, positions, weights: as in the forward."""
+    a = _rope_args(q, k, table, positions, q_weight, k_weight, eps)
+    for t, n, like in ((dq, "dq", q), (gq, "gq", q), (dk, "dk", k), (gk, "gk", k)):
+        _check_heads(t, n, q)
+        if t.shape != like.shape:
+            raise RuntimeError(f"{n} must have its tensor's shape")
+    for d, w, n in ((dq_weight, q_weight, "dq_weight"), (dk_weight, k_weight, "dk_weight")):
+        if (d is None) != (w is None):
+            raise RuntimeError(f"{n} and its weight come together")
+        if d is not None:
+            _check_ints(q.device, q.dtype, 1, **{n: d})
+            if d.shape != w.shape:
+                raise RuntimeError(f"{n} must match its weight")
+    dev = q.device
+    if q.size(0) == 0:
+        for d in (dq_weight, dk_weight):
+            if d is not None:
+                d.zero_()
+        return
+    with _on(dev):
+        ws = None
+        if q_weight is not None or k_weight is not None:
+            ws = _workspace(dev, _lib.size_query("smlm_qk_norm_rope_bwd_workspace_size", a.rows, a.q_heads, a.kv_heads,
+                                                 a.head_dim), workspace)
+        rc = _lib.load().smlm_qk_norm_rope_bwd(C.byref(a), C.byref(_heads(gq)), C.byref(_heads(gk)), C.byref(_heads(dq)),
+                                               C.byref(_heads(dk)), _ptr(dq_weight), _ptr(dk_weight), _ptr(ws),
+                                               0 if ws is None else ws.numel(), _stream(dev))
+    _lib.check(rc, "qk_norm_rope_backward")
+
+
+def _kv_state(table, length, refs, status, **lists) -> Tuple[torch.device, int, int, int]:
+    _check_input(table, "table")
+    dev = table.device
+    _check_ints(dev, torch.int32, 2, table=table)
+    _check_ints(dev, torch.int32, 1, length=length, refs=refs, status=status, **lists)
+    if length is not None and length.size(0) != table.size(0):
+        raise RuntimeError("length must have one entry per row of table")
+    if status is not None and status.numel() != 1:
+        raise RuntimeError("status must have one entry")
+    return dev, table.size(0), table.size(1), refs.size(0)
+
+
+def _kv_pool(pool: torch.Tensor, dev: torch.device, N: int) -> Tuple[int, int, int]:
+    """(blocks, page_size, bytes of a place) of a pool [n_pages, ..., page_size, head_dim]."""
+    _check_input(pool, "pool")
+    if pool.dim() < 3 or pool.device != dev or pool.size(0) != N:
+        raise RuntimeError("pool must be [n_pages, ..., page_size, head_dim], one page per entry of refs, on the tables' device")
+    place = pool.size(-1) * pool.element_size()
+    blocks = 1
+    for n in pool.shape[1:-2]:
+        blocks *= n
+    if place == 0 or place % 16 or blocks == 0 or pool.size(-2) == 0:
+        raise RuntimeError(f"No suitable kernel. {place} bytes a place")
+    return blocks, pool.size(-2), place
+
+
+def kv_extend(table: torch.Tensor, length: torch.Tensor, refs: torch.Tensor, requests: torch.Tensor, counts: torch.Tensor,
+              n_rows: int, page_size: int, status: Optional[torch.Tensor] = None, workspace: Optional[Workspace] = None):
+    """Room for counts[s] more tokens of requests[s], pages taken lowest number first, on the device (see include/smlm.h
+    for the state's tensors and `status`, which a call that cannot be done marks, changing nothing else).
+
+    Returns (q_indptr int32 [S + 1], kv_len int32 [S], positions int32 [n_rows], slots int64 [n_rows]): what qk_norm_rope and
+    AttentionPlan read.  n_rows: the counts' sum, or more (rows past it get position and slot -1)."""
+    dev, R, M, N = _kv_state(table, length, refs, status, requests=requests, counts=counts)
+    if requests.numel() != counts.numel():
+        raise RuntimeError("requests and counts must have one entry per sequence")
+    if n_rows < 0 or page_size < 1:
+        raise RuntimeError("n_rows and page_size must not be negative")
+    S = requests.numel()
+    q_indptr = torch.empty(S + 1, dtype=torch.int32, device=dev)
+    kv_len = torch.empty(S, dtype=torch.int32, device=dev)
+    positions = torch.empty(n_rows, dtype=torch.int32, device=dev)
+    slots = torch.empty(n_rows, dtype=torch.int64, device=dev)
+    with _on(dev):
+        ws = _workspace(dev, _lib.size_query("smlm_kv_workspace_size", R, N, S), workspace)
+        rc = _lib.load().smlm_kv_extend(_ptr(table), _ptr(length), _ptr(refs), _ptr(requests), _ptr(counts), q_indptr.data_ptr(),
+                                        _ptr(kv_len), _ptr(positions), _ptr(slots), ws.data_ptr(), ws.numel(), R, M, N, S,
+                                        n_rows, page_size, _ptr(status), _stream(dev))
+    _lib.check(rc, "kv_extend")
+    return q_indptr, kv_len, positions, slots
+
+
+def kv_free(table: torch.Tensor, length: torch.Tensor, refs: torch.Tensor, requests: torch.Tensor, page_size: int,
+            status: Optional[torch.Tensor] = None) -> None:
+    """Gives the requests' pages back (those that a fork shares stay with the others)."""
+    dev, R, M, N = _kv_state(table, length, refs, status, requests=requests)
+    if page_size < 1:
+        raise RuntimeError("page_size must be positive")
+    with _on(dev):
+        rc = _lib.load().smlm_kv_free(_ptr(table), _ptr(length), _ptr(refs), _ptr(requests), R, M, N, requests.numel(), page_size,
+                                      _ptr(status), _stream(dev))
+    _lib.check(rc, "kv_free")
+
+
+def kv_fork(pool: torch.Tensor, table: torch.Tensor, length: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor,
+            children: torch.Tensor, status: Optional[torch.Tensor] = None, workspace: Optional[Workspace] = None) -> None:
+    """children[i], empty so far, becomes a second parents[i]: full pages shared, the filled places of a part-filled last
+    page copied.  pool: [n_pages, ..., page_size, head_dim], contiguous (PagedKvCache.pool)."""
+    dev, R, M, N = _kv_state(table, length, refs, status, parents=parents, children=children)
+    blocks, P, place = _kv_pool(pool, dev, N)
+    if parents.numel() != children.numel():
+        raise RuntimeError("parents and children must have one entry per fork")
+    K = children.numel()
+    with _on(dev):
+        ws = _workspace(dev, _lib.size_query("smlm_kv_workspace_size", R, N, K), workspace)
+        rc = _lib.load().smlm_kv_fork(_ptr(pool), _ptr(table), _ptr(length), _ptr(refs), _ptr(parents), _ptr(children),
+                                      ws.data_ptr(), ws.numel(), R, M, N, K, blocks, P, place, _ptr(status), _stream(dev))
+    _lib.check(rc, "kv_fork")
+
+
+def kv_compact(pool: torch.Tensor, table: torch.Tensor, refs: torch.Tensor, workspace: Optional[Workspace] = None) -> None:
+    """Packs the pages in use to the pool's front; table and refs follow."""
+    dev, R, M, N = _kv_state(table, None, refs, None)
+    blocks, P, place = _kv_pool(pool, dev, N)
+    with _on(dev):
+        ws = _workspace(dev, _lib.size_query("smlm_kv_workspace_size", R, N, 0), workspace)
+        rc = _lib.load().smlm_kv_compact(_ptr(pool), _ptr(table), _ptr(refs), ws.data_ptr(), ws.numel(), R, M, N, blocks, P, place,
+                                         _stream(dev))
+    _lib.check(rc, "kv_compact")
+
+
+def kv_copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
+    """pool[dst[i]] = pool[src[i]] for int32 lists of pages; no page may be written twice, or read and written."""
+    _check_input(pool, "pool")
+    dev = pool.device
+    _check_ints(dev, torch.int32, 1, src=src, dst=dst)
+    if src.numel() != dst.numel():
+        raise RuntimeError("src and dst must have one entry per copy")
+    N = pool.size(0) if pool.dim() else 0
+    blocks, P, place = _kv_pool(pool, dev, N)
+    with _on(dev):
+        rc = _lib.load().smlm_kv_copy_pages(_ptr(pool), _ptr(src), _ptr(dst), src.numel(), N, blocks, P, place, _stream(dev))
+    _lib.check(rc, "kv_copy_pages")
+
+
+class AttentionPlan:
+    """How the card shares out the attention of one batch (see include/smlm.h): built once a step, for all its layers.
+
+    q_indptr int32 [S + 1]: rows of the sequences in the batch's n_rows; kv_len int32 [S]: tokens of each in the cache, the
+    new ones too; page_table int32 [R, M] (its contents are read by the attention calls); requests int32 [S]: the
+    sequences' rows of page_table (None: 0, 1, ...).  The tensors are read when the plan's launches run, and kept."""
+
+    def __init__(self, q_indptr: torch.Tensor, kv_len: torch.Tensor, page_table: torch.Tensor, n_rows: int, q_heads: int,
+                 kv_heads: int, page_size: int, requests: Optional[torch.Tensor] = None):
+        _check_input(q_indptr, "q_indptr")
+        dev = q_indptr.device
+        _check_ints(dev, torch.int32, 1, q_indptr=q_indptr, kv_len=kv_len, requests=requests)
+        _check_ints(dev, torch.int32, 2, page_table=page_table)
+        self.S = q_indptr.size(0) - 1
+        if self.S < 0 or kv_len.size(0) != self.S or (requests is not None and requests.size(0) != self.S):
+            raise RuntimeError("q_indptr needs one entry more than there are sequences, kv_len and requests one for each")
+        if requests is None and page_table.size(0) < self.S:
+            raise RuntimeError("page_table needs a row for each sequence")
+        if q_heads < 1 or kv_heads < 1 or q_heads % kv_heads:
+            raise RuntimeError("q_heads must be a multiple of kv_heads")
+        if n_rows < 0 or page_size < 1:
+            raise RuntimeError("n_rows and page_size must not be negative")
+        self.q_indptr, self.kv_len, self.page_table, self.requests = q_indptr, kv_len, page_table, requests
+        self.T, self.q_heads, self.kv_heads, self.page_size = int(n_rows), int(q_heads), int(kv_heads), int(page_size)
+        self.buf = torch.empty(_lib.size_query("smlm_attn_plan_size", self.T, self.S, self.q_heads, self.kv_heads),
+                               dtype=torch.uint8, device=dev)
+        R, M = page_table.shape
+        with _on(dev):
+            rc = _lib.load().smlm_attn_plan_build(self.buf.data_ptr(), self.buf.numel(), q_indptr.data_ptr(), _ptr(kv_len),
+                                                  _ptr(requests), self.T, self.S, R, M, self.page_size, self.q_heads,
+                                                  self.kv_heads, _stream(dev))
+        _lib.check(rc, "AttentionPlan")
+
+
+def paged_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, plan: AttentionPlan,
+                    scale: Optional[float] = None, workspace: Optional[Workspace] = None) -> None:
+    """Causal attention of the batch's rows q [rows, q_heads, head_dim] over the pages of k_cache and v_cache [n_pages, kv_heads,
+    page_size, head_dim] (any strides), prompts' chunks and single tokens in one call.  scale: head_dim ** -0.5 by default.
+    Rows that see no token become zero; rows of no sequence are left as they were."""
+    _check_heads(q, "q")
+    _check_heads(out, "out", q)
+    if out.shape != q.shape:
+        raise RuntimeError("out and q must have the same shape")
+    T, Hq, D = q.shape
+    if T != plan.T or Hq != plan.q_heads:
+        raise RuntimeError(f"the plan is for {plan.T} rows of {plan.q_heads} heads")
+    if plan.buf.device != q.device:
+        raise RuntimeError(f"the plan lives on {plan.buf.device}, q on {q.device}")
+    if q.dtype not in _DTYPE_CODE or D not in (64, 128):
+        raise RuntimeError(f"No suitable kernel. dtype={q.dtype} head_dim={D}")
+    page, head, place = _check_caches(k_cache, v_cache, q, plan.kv_heads)
+    if k_cache.size(2) != plan.page_size:
+        raise RuntimeError(f"the plan is for pages of {plan.page_size} tokens")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 3.0e38:
+        raise RuntimeError("scale must be positive")
+    dev = q.device
+    R, M = plan.page_table.shape
+    with _on(dev):
+        ws = None
+        need = _lib.size_query("smlm_paged_attn_workspace_size", T, plan.S, M, plan.page_size, Hq, plan.kv_heads, D)
+        if need:
+            ws = _workspace(dev, need, workspace)
+        rc = _lib.load().smlm_paged_attn(C.byref(_heads(out)), C.byref(_heads(q)), _ptr(k_cache), _ptr(v_cache), page, head, place,
+                                         _ptr(plan.page_table), plan.buf.data_ptr(), plan.buf.numel(), _ptr(ws),
+                                         0 if ws is None else ws.numel(), T, plan.S, R, M, k_cache.size(0), plan.page_size, Hq,
+                                         plan.kv_heads, D, _DTYPE_CODE[q.dtype], scale, _stream(dev))
+    _lib.check(rc, "paged_attention")
