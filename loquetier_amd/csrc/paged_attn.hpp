@@ -21,6 +21,8 @@
 // Keys of later rows of a chunk are in the cache already; their weight is zero, but zero times an infinity or NaN is
 // not, so the tiles that some rows see in part look whether their V has such a value and then add key by key to the rows that see it.
 #pragma once
+#include <type_traits>
+
 #include "smlm_common.hpp"
 
 namespace smlm {
@@ -249,13 +251,19 @@ __device__ __forceinline__ int attn_div(uint32_t x, uint32_t mul, int shift) {
   return (int)(((uint64_t)__umulhi(x, mul) + x) >> shift);
 }
 
-// Element offset of a key within the pool (its kv head apart), -1 where there is none.
-__device__ __forceinline__ int64_t attn_find(const AttnArgs& a, const int* trow, int key, int ke) {
-  if (key >= ke) return -1;
-  const int j = attn_div((uint32_t)key, a.div_mul, a.div_shift);
-  const int page = trow[j];
-  if (page < 0 || page >= a.n_pages) return -1;
-  return (int64_t)page * a.c_page + (int64_t)(key - j * a.P) * a.c_slot;
+// Element offset of a key within the pool (its kv head apart), -1 where there is none.  ke > 0.
+// In two steps, the page's number a tile ahead of its use: the read is on its way meanwhile.
+struct AttnKey {
+  int page, slot;
+};
+__device__ __forceinline__ AttnKey attn_key(const AttnArgs& a, const int* trow, int key, int ke) {
+  const int k = min(key, ke - 1);  // (no branch around the read)
+  const int j = attn_div((uint32_t)k, a.div_mul, a.div_shift);
+  return AttnKey{trow[j], key < ke ? k - j * a.P : -1};
+}
+__device__ __forceinline__ int64_t attn_offset(const AttnArgs& a, AttnKey k) {
+  const int64_t off = (int64_t)k.page * a.c_page + (int64_t)k.slot * a.c_slot;
+  return k.slot >= 0 && (uint32_t)k.page < (uint32_t)a.n_pages ? off : -1;
 }
 __device__ __forceinline__ int64_t attn_shfl(int64_t v, int lane) {
   const int lo = __shfl((int)(uint32_t)v, lane, kWaveSize), hi = __shfl((int)(v >> 32), lane, kWaveSize);
@@ -278,11 +286,17 @@ __device__ __forceinline__ uint32_t attn_not_finite(uint32_t x) {
   return DT == SMLM_DTYPE_F16 ? ((x & 0x7c007c00u) + 0x04000400u) & 0x80008000u : ((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
 }
 
-// Four elements of V by four keys: keys row, .. row + 3 (of this lane's sixteen), dimensions d0 + 0 .. 15, transposed.
+// Where a lane points the transposing load for keys row .. row + 3 of its sixteen lanes and dimensions d0 .. d0 + 15: it gets
+// dimension d0 + (lane & 15) of the four keys.  (Sixteen rows on, the place is the same sixteen rows on: the operands of a tile take
+// few different ones, kept in registers, and constants for the rest.)
 template <int D>
-__device__ __forceinline__ u32x2 attn_read_v(const uint16_t* lds, int row, int d0) {
+__device__ __forceinline__ int attn_v_place(int row, int d0) {
   const int l = threadIdx.x & 15, r = row + (l >> 2), d = d0 + (l & 3) * 4;
-  return lds_read_tr16(lds + attn_place<D>(r, d >> 3) + (d & 7));
+  return attn_place<D>(r, d >> 3) + (d & 7);
+}
+__device__ __forceinline__ u32x4 attn_v_pair(const uint16_t* a, const uint16_t* b) {
+  const u32x2 x = lds_read_tr16(a), y = lds_read_tr16(b);
+  return u32x4{x[0], x[1], y[0], y[1]};
 }
 
 template <int DT>
@@ -336,6 +350,9 @@ __device__ __forceinline__ void attn_small(const AttnArgs& a, const AttnItem& it
   }
   u32x4 kr[2][kSteps], vr[kVLoads];
   constexpr int kRowLanes = D / 8, kRowsLoad = 64 / kRowLanes;  // lanes a row of V, rows a load
+  int vat[kBlk];
+#pragma unroll
+  for (int i = 0; i < kBlk; ++i) vat[i] = attn_v_place<D>(b * 4, i * 16);
   auto load = [&](int64_t off) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -347,9 +364,13 @@ __device__ __forceinline__ void attn_small(const AttnArgs& a, const AttnItem& it
     for (int i = 0; i < kVLoads; ++i)
       vr[i] = attn_ld(vp, attn_shfl(off, i * kRowsLoad + lane / kRowLanes), (lane % kRowLanes) * 8);
   };
-  int64_t off = attn_find(a, trow, it.kb + wave * 32 + (lane & 31), it.ke), next = -1;
-  load(off);
-  next = attn_find(a, trow, it.kb + wave * 32 + 128 + (lane & 31), it.ke);
+  int64_t off = -1;
+  AttnKey next{0, -1};
+  if (it.kb < it.ke) {
+    off = attn_offset(a, attn_key(a, trow, it.kb + wave * 32 + (lane & 31), it.ke));
+    next = attn_key(a, trow, it.kb + wave * 32 + 128 + (lane & 31), it.ke);
+    load(off);
+  }
   for (int base = it.kb + wave * 32; base < it.ke; base += 128) {
     const uint32_t ok = (uint32_t)__ballot(off >= 0);
     f32x4 s[MT][2];
@@ -369,21 +390,23 @@ __device__ __forceinline__ void attn_small(const AttnArgs& a, const AttnItem& it
       *(u32x4*)(vl + attn_place<D>(r, lane % kRowLanes)) = vr[i];
       if (edge) odd |= attn_not_finite<DT>(vr[i][0]) | attn_not_finite<DT>(vr[i][1]) | attn_not_finite<DT>(vr[i][2]) | attn_not_finite<DT>(vr[i][3]);
     }
-    off = next;
+    off = attn_offset(a, next);
+    next = attn_key(a, trow, base + 256 + (lane & 31), it.ke);
     load(off);
-    next = attn_find(a, trow, base + 256 + (lane & 31), it.ke);
 
     const bool guard = edge && __ballot(odd != 0) != 0;
     u32x4 pf[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
       if (edge || ok != 0xffffffffu) {
+        const uint32_t there = ok >> (b * 4);
+        const int seen = lim[t] - base - b * 4;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int key = u * 16 + b * 4 + i;
-            if (!(ok >> key & 1) || base + key > lim[t]) s[t][u][i] = -INFINITY;
+            const int key = u * 16 + i;  // (and 4 b more)
+            if (!(there >> key & 1) || key > seen) s[t][u][i] = -INFINITY;
           }
       }
       float mx = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
@@ -410,8 +433,7 @@ __device__ __forceinline__ void attn_small(const AttnArgs& a, const AttnItem& it
     if (!guard) {
 #pragma unroll
       for (int i = 0; i < kBlk; ++i) {
-        const u32x2 v0 = attn_read_v<D>(vl, b * 4, i * 16), v1 = attn_read_v<D>(vl, 16 + b * 4, i * 16);
-        const u32x4 vf = {v0[0], v0[1], v1[0], v1[1]};
+        const u32x4 vf = attn_v_pair(vl + vat[i], vl + vat[i] + 16 * D);
 #pragma unroll
         for (int t = 0; t < MT; ++t) o[t][i] = Num<DT>::mfma(vf, pf[t], o[t][i]);
       }
@@ -419,13 +441,13 @@ __device__ __forceinline__ void attn_small(const AttnArgs& a, const AttnItem& it
 #pragma unroll 1
       for (int x = 0; x < 32; ++x) {
         const int bb = x >> 3, j = x & 7, key = (j >> 2) * 16 + bb * 4 + (j & 3);
+        asm volatile("" ::: "memory");  // (V is read again for each key: kept in registers it would cost the usual path)
         u32x4 only;
 #pragma unroll
         for (int e = 0; e < 4; ++e) only[e] = b == bb && (j >> 1) == e ? (j & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
 #pragma unroll
         for (int i = 0; i < kBlk; ++i) {
-          const u32x2 v0 = attn_read_v<D>(vl, b * 4, i * 16), v1 = attn_read_v<D>(vl, 16 + b * 4, i * 16);
-          const u32x4 vf = u32x4{v0[0], v0[1], v1[0], v1[1]} & only;
+          const u32x4 vf = attn_v_pair(vl + vat[i], vl + vat[i] + 16 * D) & only;
 #pragma unroll
           for (int t = 0; t < MT; ++t) {
             const f32x4 add = Num<DT>::mfma(vf, pf[t] & only, f32x4{0.f, 0.f, 0.f, 0.f});
@@ -478,11 +500,14 @@ __device__ __forceinline__ void attn_small(const AttnArgs& a, const AttnItem& it
 
 // 128 tile rows, 32 a wave.  Layouts of a 32 x 32 x 16 product by lane (c = lane & 31, h = lane >> 5): operands row or
 // column c, k = 8 h + 0..7; result column c, rows 8 (i / 4) + 4 h + i % 4, i = 0..15.
+// K and V tiles go from memory to LDS without passing through registers, the next tile's while one is worked on; the turned places are made
+// by what each lane reads, as the hardware writes the lanes' pieces one after the other.
 template <int DT, int D>
-__device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, int kvh, uint16_t* lds, uint32_t* flags) {
+__device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, int kvh, uint16_t* tile0, uint16_t* tile1,
+                                         uint32_t* flags) {
   constexpr int kSteps = D / 16, kBlk = D / 32, kKeys = 64;
   constexpr int kRowLanes = D / 8, kRowsLoad = 64 / kRowLanes, kLoads = 16 / kRowsLoad;  // a wave loads 16 rows of K and of V
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int rows = it.n * a.g;
   const int* trow = a.table + (int64_t)it.trow * a.M;
   const uint16_t *kp = a.k + (int64_t)kvh * a.c_head, *vp = a.v + (int64_t)kvh * a.c_head;
@@ -507,43 +532,32 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
 
-  u32x4 kr[kLoads], vr[kLoads];
-  auto load = [&](int64_t off) {
+  int kat[kSteps], vat[kBlk][2];
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) kat[k] = attn_place<D>(c, k * 2 + h);
+#pragma unroll
+  for (int i = 0; i < kBlk; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) vat[i][j] = attn_v_place<D>(h * 4 + j * 8, i * 32 + ((lane >> 4) & 1) * 16);
+
+  auto load = [&](int64_t off, uint16_t* tile) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int64_t f = attn_shfl(off, i * kRowsLoad + lane / kRowLanes);
-      kr[i] = attn_ld(kp, f, (lane % kRowLanes) * 8);
-      vr[i] = attn_ld(vp, f, (lane % kRowLanes) * 8);
+      const int r = i * kRowsLoad + lane / kRowLanes;
+      const int64_t f = attn_shfl(off, r);
+      int d = attn_place<D>(r, lane % kRowLanes) - r * D;  // (the turn undoes itself: the piece that belongs in this lane's place)
+      asm("" : "+v"(d));                                   // (its sum with the addresses is not kept over the loop: registers)
+      const uint16_t* zero = reinterpret_cast<const uint16_t*>(attn_zeros);
+      const uint16_t *ks = f >= 0 ? kp + f + d : zero, *vs = f >= 0 ? vp + f + d : zero;
+      uint16_t* dst = tile + (wave * 16 + i * kRowsLoad) * D;
+      __builtin_amdgcn_global_load_lds((SMLM_GLOBAL void*)ks, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((SMLM_GLOBAL void*)vs, (__attribute__((address_space(3))) void*)(dst + kKeys * D), 16, 0, 0);
     }
   };
-  int64_t off = attn_find(a, trow, it.kb + wave * 16 + (lane & 15), it.ke);
-  load(off);
-  int64_t next = attn_find(a, trow, it.kb + kKeys + wave * 16 + (lane & 15), it.ke);
-  int turn_buf = 0;
-  for (int base = it.kb; base < it.ke; base += kKeys, turn_buf ^= 1) {
-    uint16_t *kl = lds + turn_buf * (2 * kKeys * D), *vl = kl + kKeys * D;
-    uint32_t* fl = flags + turn_buf * 4;
-    const bool edge = base + kKeys - 1 > lim0;
-    uint32_t odd = 0;
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int r = wave * 16 + i * kRowsLoad + lane / kRowLanes;
-      *(u32x4*)(kl + attn_place<D>(r, lane % kRowLanes)) = kr[i];
-      *(u32x4*)(vl + attn_place<D>(r, lane % kRowLanes)) = vr[i];
-      if (edge) odd |= attn_not_finite<DT>(vr[i][0]) | attn_not_finite<DT>(vr[i][1]) | attn_not_finite<DT>(vr[i][2]) | attn_not_finite<DT>(vr[i][3]);
-    }
-    {
-      const uint32_t mine = (uint32_t)__ballot(off >= 0) & 0xffffu, any_odd = __ballot(odd != 0) != 0 ? 0x10000u : 0u;
-      if (lane == 0) fl[wave] = mine | any_odd;
-    }
-    __syncthreads();
-    off = next;
-    load(off);
-    next = attn_find(a, trow, base + 2 * kKeys + wave * 16 + (lane & 15), it.ke);
-    const uint32_t f0 = fl[0], f1 = fl[1], f2 = fl[2], f3 = fl[3];
-    const uint64_t ok = (uint64_t)((f0 & 0xffffu) | (f1 << 16)) | ((uint64_t)((f2 & 0xffffu) | (f3 << 16)) << 32);
-    const bool guard = ((f0 | f1 | f2 | f3) >> 16) != 0;
-
+  auto work = [&](auto may_edge, int base, const uint16_t* kl, const uint32_t* fl) {
+    const uint16_t* vl = kl + kKeys * D;
+    const bool edge = may_edge && base + kKeys - 1 > lim0;
+    const uint64_t ok = (uint64_t)((fl[0] & 0xffffu) | (fl[1] << 16)) | ((uint64_t)((fl[2] & 0xffffu) | (fl[3] << 16)) << 32);
     f32x16 s[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -551,17 +565,19 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
       for (int e = 0; e < 16; ++e) s[u][e] = 0.0f;
 #pragma unroll
       for (int k = 0; k < kSteps; ++k) {
-        const u32x4 kf = *(const u32x4*)(kl + attn_place<D>(u * 32 + c, k * 2 + h));
+        const u32x4 kf = *(const u32x4*)(kl + kat[k] + u * 32 * D);
         s[u] = mfma32<DT>(kf, q[k], s[u]);
       }
     }
     if (edge || ok != ~0ull) {
+      const uint64_t there = ok >> (4 * h);
+      const int seen = lim - base - 4 * h;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int key = u * 32 + 8 * (e >> 2) + 4 * h + (e & 3);
-          if (!(ok >> key & 1) || base + key > lim) s[u][e] = -INFINITY;
+          const int key = u * 32 + 8 * (e >> 2) + (e & 3);  // (and 4 h more)
+          if (!(there >> key & 1) || key > seen) s[u][e] = -INFINITY;
         }
     }
     float mx = s[0][0];
@@ -587,6 +603,17 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
         l += p0 + p1;
         pf[u][e >> 3][(e >> 1) & 3] = pack2<DT>(p0, p1);
       }
+    // a tile that some rows see in part: does its V hold a value that is no number?
+    bool guard = false;
+    if (edge) {
+      uint32_t odd = 0;
+#pragma unroll 1
+      for (int x = lane; x < kKeys * kRowLanes; x += kWaveSize) {
+        const u32x4 v = *(const u32x4*)(vl + x * 8);
+        odd |= attn_not_finite<DT>(v[0]) | attn_not_finite<DT>(v[1]) | attn_not_finite<DT>(v[2]) | attn_not_finite<DT>(v[3]);
+      }
+      guard = __ballot(odd != 0) != 0;
+    }
     if (!guard) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -594,33 +621,61 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
         for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
           for (int i = 0; i < kBlk; ++i) {
-            const int r = u * 32 + ks * 16 + h * 4, d = i * 32 + ((lane >> 4) & 1) * 16;
-            const u32x2 v0 = attn_read_v<D>(vl, r, d), v1 = attn_read_v<D>(vl, r + 8, d);
-            o[i] = mfma32<DT>(u32x4{v0[0], v0[1], v1[0], v1[1]}, pf[u][ks], o[i]);
+            const uint16_t* at = vl + (u * 32 + ks * 16) * D;
+            o[i] = mfma32<DT>(attn_v_pair(at + vat[i][0], at + vat[i][1]), pf[u][ks], o[i]);
           }
     } else {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
 #pragma unroll 1
-          for (int x = 0; x < 16; ++x) {  // slot j of half hh
-            const int hh = x >> 3, j = x & 7, key = u * 32 + ks * 16 + (j >> 2) * 8 + hh * 4 + (j & 3);
-            u32x4 only;
+      for (int x = 0; x < kKeys; ++x) {  // slot j of half hh in step st of sixteen keys
+        const int st = x >> 4, hh = (x >> 3) & 1, j = x & 7, key = st * 16 + (j >> 2) * 8 + hh * 4 + (j & 3);
+        asm volatile("" ::: "memory");  // (V is read again for each key: kept in registers it would cost the usual path)
+        u32x4 only, pj;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) only[e] = h == hh && (j >> 1) == e ? (j & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
+        for (int e = 0; e < 4; ++e) {
+          only[e] = h == hh && (j >> 1) == e ? (j & 1 ? 0xffff0000u : 0x0000ffffu) : 0u;
+          pj[e] = (st == 0 ? pf[0][0][e] : st == 1 ? pf[0][1][e] : st == 2 ? pf[1][0][e] : pf[1][1][e]) & only[e];
+        }
 #pragma unroll
-            for (int i = 0; i < kBlk; ++i) {
-              const int r = u * 32 + ks * 16 + h * 4, d = i * 32 + ((lane >> 4) & 1) * 16;
-              const u32x2 v0 = attn_read_v<D>(vl, r, d), v1 = attn_read_v<D>(vl, r + 8, d);
-              f32x16 add;
+        for (int i = 0; i < kBlk; ++i) {
+          const uint16_t* at = vl + st * 16 * D;
+          f32x16 add;
 #pragma unroll
-              for (int e = 0; e < 16; ++e) add[e] = 0.0f;
-              add = mfma32<DT>(u32x4{v0[0], v0[1], v1[0], v1[1]} & only, pf[u][ks] & only, add);
-              if (base + key <= lim) o[i] += add;
-            }
-          }
+          for (int e = 0; e < 16; ++e) add[e] = 0.0f;
+          add = mfma32<DT>(attn_v_pair(at + vat[i][0], at + vat[i][1]) & only, pj, add);
+          if (base + key <= lim) o[i] += add;
+        }
+      }
     }
+  };
+  // A tile's loads are waited for by the wave that gave them, then by all; at that point everybody is done with the tile before,
+  // whose place the next loads take.
+  int64_t off = -1;
+  AttnKey next{0, -1};
+  if (it.kb < it.ke) {
+    off = attn_offset(a, attn_key(a, trow, it.kb + wave * 16 + (lane & 15), it.ke));
+    next = attn_key(a, trow, it.kb + kKeys + wave * 16 + (lane & 15), it.ke);
+  }
+  auto turn = [&](auto may_edge, int base, uint16_t* mine, uint16_t* other, uint32_t* fl) {
+    const uint32_t valid = (uint32_t)__ballot(off >= 0) & 0xffffu;
+    if (lane == 0) fl[wave] = valid;
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    __syncthreads();
+    off = attn_offset(a, next);
+    next = attn_key(a, trow, base + 2 * kKeys + wave * 16 + (lane & 15), it.ke);
+    if (base + kKeys < it.ke) load(off, other);
+    work(may_edge, base, mine, fl);
+  };
+  if (it.kb < it.ke) load(off, tile0);
+  // pairs of tiles that every row sees, then the others (apart, so that the first loop keeps its registers to itself)
+  int base = it.kb;
+  for (; base + 2 * kKeys - 1 <= lim0 && base + kKeys < it.ke; base += 2 * kKeys) {
+    turn(std::false_type{}, base, tile0, tile1, flags);
+    turn(std::false_type{}, base + kKeys, tile1, tile0, flags + 4);
+  }
+#pragma unroll 1
+  for (; base < it.ke; base += 2 * kKeys) {
+    turn(std::true_type{}, base, tile0, tile1, flags);
+    if (base + kKeys < it.ke) turn(std::true_type{}, base + kKeys, tile1, tile0, flags + 4);
   }
   l += __shfl_xor(l, 32, kWaveSize);
   if (p >= rows) return;  // (no barrier below)
@@ -647,13 +702,13 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
 // Neighbouring workgroups take the kv heads of one item: with eight of them, or a multiple, a head's tiles meet in one XCD's L2.
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
-  __shared__ __align__(16) uint16_t lds[2 * 2 * 64 * D];
+  __shared__ __align__(16) uint16_t lds[2 * 64 * D], more[2 * 64 * D];
   __shared__ uint32_t side[128];
   const int i = (int)blockIdx.x / a.Hkv, kvh = (int)blockIdx.x - i * a.Hkv;
   if (i >= a.plan.hdr[0]) return;
   const AttnItem it = a.plan.items[i];
   const int rows = it.n * a.g;
-  if (rows > kAttnSmallRows) attn_big<DT, D>(a, it, kvh, lds, side);
+  if (rows > kAttnSmallRows) attn_big<DT, D>(a, it, kvh, lds, more, side);
   else if (rows > 16) attn_small<DT, D, 2>(a, it, kvh, lds, reinterpret_cast<float*>(side));
   else attn_small<DT, D, 1>(a, it, kvh, lds, reinterpret_cast<float*>(side));
 }
