@@ -142,8 +142,8 @@ _host = None
 
 class _NoHost:
     """In the native host path's place where it cannot be loaded: declines every call, and the Python functions take it."""
-    forward = staticmethod(lambda *args: False)
-    rms_norm = add_lora = fused_add_lora = staticmethod(lambda *args: None)
+    forward = rope = paged_attention = kv_free = kv_fork = staticmethod(lambda *args: False)
+    rms_norm = add_lora = fused_add_lora = qk_norm_rope = attention_plan = kv_extend = staticmethod(lambda *args: None)
 
 
 def host(default_workspace=None):

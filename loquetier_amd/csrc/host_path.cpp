@@ -25,6 +25,8 @@
 
 #include <string.h>
 
+#include <cmath>
+
 #include "smlm.h"
 
 namespace {
@@ -46,13 +48,25 @@ struct Lib {
   decltype(&smlm_rms_norm_bwd_workspace_size) rms_bwd_size;
   decltype(&smlm_rms_norm_bwd) rms_bwd;
   decltype(&smlm_put_words) put;
+  decltype(&smlm_qk_norm_rope_fwd) rope_fwd;
+  decltype(&smlm_qk_norm_rope_bwd_workspace_size) rope_bwd_size;
+  decltype(&smlm_qk_norm_rope_bwd) rope_bwd;
+  decltype(&smlm_attn_plan_size) attn_plan_size;
+  decltype(&smlm_attn_plan_build) attn_plan;
+  decltype(&smlm_paged_attn_workspace_size) attn_size;
+  decltype(&smlm_paged_attn) attn;
+  decltype(&smlm_kv_workspace_size) kv_size;
+  decltype(&smlm_kv_extend) kv_extend;
+  decltype(&smlm_kv_free) kv_free;
+  decltype(&smlm_kv_fork) kv_fork;
 } lib;
 PyObject* default_workspace = nullptr;  // ops._kernels._workspace
 
 struct Names {
   PyObject *T, *S, *kind, *built, *buf, *segment, *seg_key, *seg_key2, *ws_buf, *reserve, *workspace, *packed, *wa_table,
       *wb_table, *seg_scale, *plan, *rank, *train_len, *train_partition, *dropout, *adapter_rank, *part_segments, *bwd_plan,
-      *part_adapter, *a_tab, *b_tab, *grad_layout, *gather, *grad_uniform, *grad_tabs, *grad_offsets_a, *grad_offsets_b;
+      *part_adapter, *a_tab, *b_tab, *grad_layout, *gather, *grad_uniform, *grad_tabs, *grad_offsets_a, *grad_offsets_b,
+      *q_heads, *kv_heads, *page_size, *page_table;
 } names;
 
 void check(int rc, const char* what) {
@@ -691,6 +705,8 @@ PyObject* py_fused_add_lora(PyObject*, PyObject* const* p, Py_ssize_t n) {
   SMLM_PY_END
 }
 
+#include "host_layer.hpp"
+
 // bind({entry: address}, default_workspace)
 PyObject* py_bind(PyObject*, PyObject* args) {
   SMLM_PY_TRY
@@ -712,6 +728,17 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   get("smlm_rms_norm_bwd_workspace_size", &lib.rms_bwd_size);
   get("smlm_rms_norm_bwd", &lib.rms_bwd);
   get("smlm_put_words", &lib.put);
+  get("smlm_qk_norm_rope_fwd", &lib.rope_fwd);
+  get("smlm_qk_norm_rope_bwd_workspace_size", &lib.rope_bwd_size);
+  get("smlm_qk_norm_rope_bwd", &lib.rope_bwd);
+  get("smlm_attn_plan_size", &lib.attn_plan_size);
+  get("smlm_attn_plan_build", &lib.attn_plan);
+  get("smlm_paged_attn_workspace_size", &lib.attn_size);
+  get("smlm_paged_attn", &lib.attn);
+  get("smlm_kv_workspace_size", &lib.kv_size);
+  get("smlm_kv_extend", &lib.kv_extend);
+  get("smlm_kv_free", &lib.kv_free);
+  get("smlm_kv_fork", &lib.kv_fork);
   Py_INCREF(ws);
   Py_XSETREF(default_workspace, ws);
   Py_RETURN_NONE;
@@ -724,6 +751,13 @@ PyMethodDef methods[] = {
     {"rms_norm", (PyCFunction)(void (*)(void))py_rms_norm, METH_FASTCALL, nullptr},
     {"add_lora", (PyCFunction)(void (*)(void))py_add_lora, METH_FASTCALL, nullptr},
     {"fused_add_lora", (PyCFunction)(void (*)(void))py_fused_add_lora, METH_FASTCALL, nullptr},
+    {"qk_norm_rope", (PyCFunction)(void (*)(void))py_qk_norm_rope, METH_FASTCALL, nullptr},
+    {"rope", (PyCFunction)(void (*)(void))py_rope, METH_FASTCALL, nullptr},
+    {"attention_plan", (PyCFunction)(void (*)(void))py_attention_plan, METH_FASTCALL, nullptr},
+    {"paged_attention", (PyCFunction)(void (*)(void))py_paged_attention, METH_FASTCALL, nullptr},
+    {"kv_extend", (PyCFunction)(void (*)(void))py_kv_extend, METH_FASTCALL, nullptr},
+    {"kv_free", (PyCFunction)(void (*)(void))py_kv_free, METH_FASTCALL, nullptr},
+    {"kv_fork", (PyCFunction)(void (*)(void))py_kv_fork, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_smlm_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
@@ -735,7 +769,8 @@ PyMODINIT_FUNC PyInit__smlm_host(void) {
            s("reserve"), s("workspace"), s("packed"), s("wa_table"), s("wb_table"), s("seg_scale"), s("plan"), s("rank"),
            s("train_len"), s("train_partition"), s("dropout"), s("adapter_rank"), s("part_segments"), s("bwd_plan"),
            s("part_adapter"), s("a_tab"), s("b_tab"), s("grad_layout"), s("gather"), s("grad_uniform"), s("grad_tabs"),
-           s("grad_offsets_a"), s("grad_offsets_b")};
+           s("grad_offsets_a"), s("grad_offsets_b"), s("q_heads"), s("kv_heads"),
+           s("page_size"), s("page_table")};
   PyObject* m = PyModule_Create(&module);
   if (m && PyModule_AddStringConstant(m, "torch_version", TORCH_VERSION) < 0) Py_CLEAR(m);
   return m;

@@ -41,7 +41,7 @@ __device__ __forceinline__ int kv_scan(int v, int* wave_tot, int& total) {
   return v + before;
 }
 
-// Atomics reach memory past the CU's own cache, so what they wrote is read the same way.
+// Atomics reach memory past the CU's own cache, so what they wrote is read the same way (a barrier orders them in a workgroup).
 __device__ __forceinline__ int kv_load(const int* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ void kv_store(int* p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
@@ -82,7 +82,7 @@ struct KvExtendArgs {
   int R, M, N, S, rows, P;
 };
 
-// One workgroup: counts, checks, takes the pages and writes the step's tables.  q_indptr doubles as the counts' running sum.
+// One workgroup: counts, checks, takes the pages and writes the step's tables by sequence.  q_indptr doubles as the counts' running sum.
 __global__ __launch_bounds__(kKvThreads) void kv_extend_kernel(KvExtendArgs a) {
   __shared__ int wave_tot[16];
   __shared__ int bad;
@@ -92,13 +92,11 @@ __global__ __launch_bounds__(kKvThreads) void kv_extend_kernel(KvExtendArgs a) {
     const int r = a.requests[i];
     if (r >= 0 && r < a.R) kv_store(a.owner + r, 0x7fffffff);
   }
-  __threadfence();
   __syncthreads();
   for (int i = tid; i < a.S; i += kKvThreads) {
     const int r = a.requests[i];
     if (r >= 0 && r < a.R) atomicMin(a.owner + r, i);
   }
-  __threadfence();
   __syncthreads();
   int rows = 0, pages = 0;
   for (int base = 0; base < a.S; base += kKvThreads) {
@@ -144,25 +142,12 @@ __global__ __launch_bounds__(kKvThreads) void kv_extend_kernel(KvExtendArgs a) {
   const int err = bad;
   if (err) {
     for (int i = tid; i <= a.S; i += kKvThreads) {
-      a.q_indptr[i] = 0;
+      a.q_indptr[i] = a.start[i] = 0;
       if (i < a.S) a.kv_len[i] = 0;
     }
     if (tid == 0 && a.status) atomicOr(a.status, err);
     return;
   }
-  // (flat over the pages: one prompt may take most of them)
-  for (int p = tid; p < pages; p += kKvThreads) {
-    int lo = 0, hi = a.S;
-    while (hi - lo > 1) {  // last i with start[i] <= p; start[i + 1] > p there
-      const int mid = (lo + hi) >> 1;
-      if (a.start[mid] <= p) lo = mid;
-      else hi = mid;
-    }
-    const int r = a.requests[lo], id = a.fresh[p];
-    a.table[(int64_t)r * a.M + (a.length[r] + a.P - 1) / a.P + (p - a.start[lo])] = id;
-    a.refs[id] = 1;
-  }
-  __syncthreads();  // (the lengths are read above)
   for (int i = tid; i < a.S; i += kKvThreads) {
     const int r = a.requests[i];
     const int now = r < 0 ? 0 : a.length[r] + (a.q_indptr[i + 1] - a.q_indptr[i]);
@@ -171,26 +156,41 @@ __global__ __launch_bounds__(kKvThreads) void kv_extend_kernel(KvExtendArgs a) {
   }
 }
 
-// Positions and slots of the step's rows; rows past the last request's, and all of them where the step was refused, get -1.
+// last i in [0, n) with a[i] <= x, given a[0] <= x < a[n]
+__device__ __forceinline__ int kv_last_le(const int* a, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// The new pages' places in the table, and positions and slots of the step's rows: a thread a row (or page: there are at most as many
+// as rows).  Rows past the last request's, and all of them where the step was refused, get -1.
 __global__ __launch_bounds__(256) void kv_rows_kernel(KvExtendArgs a) {
-  const int row = (int)blockIdx.x * 256 + (int)threadIdx.x;
-  if (row >= a.rows) return;
+  const int t = (int)blockIdx.x * 256 + (int)threadIdx.x;
+  if (t >= a.rows) return;
+  // (a new page holds a new token, so pages do not outnumber rows)
+  if (a.S > 0 && t < a.start[a.S]) {
+    const int i = kv_last_le(a.start, a.S, t);
+    const int old = a.kv_len[i] - (a.q_indptr[i + 1] - a.q_indptr[i]), id = a.fresh[t];
+    a.table[(int64_t)a.requests[i] * a.M + (old + a.P - 1) / a.P + (t - a.start[i])] = id;
+    a.refs[id] = 1;
+  }
   int pos = -1;
   int64_t slot = -1;
-  if (a.S > 0 && row < a.q_indptr[a.S]) {
-    int lo = 0, hi = a.S;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.q_indptr[mid] <= row) lo = mid;
-      else hi = mid;
-    }
-    const int r = a.requests[lo];
-    pos = a.kv_len[lo] - (a.q_indptr[lo + 1] - row);
+  if (a.S > 0 && t < a.q_indptr[a.S]) {
+    const int i = kv_last_le(a.q_indptr, a.S, t);
+    const int n = a.q_indptr[i + 1] - a.q_indptr[i], had = (a.kv_len[i] - n + a.P - 1) / a.P;
+    pos = a.kv_len[i] - (a.q_indptr[i + 1] - t);
     const int j = pos / a.P;
-    slot = (int64_t)a.table[(int64_t)r * a.M + j] * a.P + (pos - j * a.P);
+    const int page = j < had ? a.table[(int64_t)a.requests[i] * a.M + j] : a.fresh[a.start[i] + j - had];
+    slot = (int64_t)page * a.P + (pos - j * a.P);
   }
-  a.positions[row] = pos;
-  a.slots[row] = slot;
+  a.positions[t] = pos;
+  a.slots[t] = slot;
 }
 
 struct KvFreeArgs {
@@ -282,13 +282,11 @@ __global__ __launch_bounds__(kKvThreads) void kv_fork_kernel(KvForkArgs a) {
     const int c = a.children[i];
     if (c >= 0 && c < a.R) kv_store(a.owner + c, 0x7fffffff);
   }
-  __threadfence();
   __syncthreads();
   for (int i = tid; i < a.K; i += kKvThreads) {
     const int c = a.children[i];
     if (c >= 0 && c < a.R) atomicMin(a.owner + c, i);
   }
-  __threadfence();
   __syncthreads();
   int pages = 0;
   for (int base = 0; base < a.K; base += kKvThreads) {

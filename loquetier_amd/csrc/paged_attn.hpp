@@ -38,7 +38,8 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 
 constexpr int kAttnSmallRows = 32;   // tile rows of a sequence up to which it takes the few-row path
 constexpr int kAttnBigRows = 128;    // tile rows of a workgroup of the other
-constexpr int kAttnSmallItems = 2048, kAttnBigItems = 768;  // parts that the long axis is cut into, at most, over the card
+constexpr int kAttnSlots = 512;      // workgroups on the card at a time: two a CU
+constexpr int kAttnSmallItems = 2048, kAttnBigItems = 1024;  // workgroups over the card that tiles are cut for, at most
 constexpr int kAttnMinKeys = 256;    // keys of a part, at least
 
 struct AttnItem {   // a tile of a sequence and a part of its keys
@@ -64,7 +65,8 @@ inline int attn_joins_max(int T, int S, int g, int Hkv) {
   const int cut = (kAttnSmallItems + kAttnBigItems) / Hkv + 2, tiles = attn_tiles_max(T, S, g);
   return cut < tiles ? cut : tiles;
 }
-inline int attn_parts_max(int Hkv, int items) { return 2 * (items / Hkv + 1); }
+// (a tile of x times the cut's keys has round(x) parts, which is more than one from x = 1.5 on: at most 4 x / 3)
+inline int attn_parts_max(int Hkv, int items) { return 4 * (items / Hkv + 1) / 3 + 1; }
 inline size_t attn_plan_carve(void* base, int T, int S, int g, int Hkv, AttnPlanView* pv) {
   size_t off = 0;
   auto take = [&](size_t bytes) {
@@ -111,122 +113,141 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnPlanArgs& a, int s) {
 
 constexpr int kAttnPlanThreads = 1024;
 
-template <typename V>
-__device__ __forceinline__ V attn_block_sum(V v, V* red) {
+constexpr int kAttnPlanLds = kAttnPlanThreads;  // up to here the sequences stay in LDS: every read of memory is most of a microsecond
+
+// The number of parts that a tile of the card's average length is cut into, for n tiles (times kv heads): as many as leave the
+// card's places for workgroups fullest, if that is worth the parts' traffic.  (Cutting 512 chunks' tiles, which just fill the card,
+// in two: 2048 rows over 14336 tokens 600 -> 657 us.)
+__device__ __forceinline__ int attn_parts(int n) {
+  if (n >= kAttnBigItems) return 1;
+  constexpr int kParts[8] = {1, 2, 3, 4, 6, 8, 12, 16};
+  int best = 1;
+  float cost = 1e30f;
 #pragma unroll
-  for (int d = 1; d < kWaveSize; d *= 2) v += __shfl_xor(v, d, kWaveSize);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  V t = 0;
-  for (int w = 0; w < kAttnPlanThreads / kWaveSize; ++w) t += red[w];
-  return t;
+  for (int i = 0; i < 8; ++i) {
+    const float c = (float)((n * kParts[i] + kAttnSlots - 1) / kAttnSlots) * (i ? 1.1f / (float)kParts[i] : 1.0f);
+    if (c < cost * 0.97f) cost = c, best = kParts[i];
+  }
+  return best;
 }
 
-__device__ __forceinline__ int attn_scan(int v, int* wave_tot, int& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < kWaveSize; d *= 2) {
-    const int u = __shfl_up(v, d, kWaveSize);
-    if (lane >= d) v += u;
-  }
-  __syncthreads();
-  if (lane == 63) wave_tot[wave] = v;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kAttnPlanThreads / kWaveSize; ++w) {
-    const int t = wave_tot[w];
-    before += w < wave ? t : 0;
-    total += t;
-  }
-  return v + before;
-}
-
-// One workgroup.  A sequence's tiles are cut alike, by its length; a part holds at least the batch's keys (times tiles and kv
-// heads) over the number of parts that the card is to get, so the numbers of items and parts have bounds that the host knows.
+// One workgroup.  The sequences' tiles are cut into parts of about `cut` keys, by the sequences' lengths; the cuts follow from the batch's
+// totals, so that the numbers of items and parts have bounds that the host knows.
 __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArgs a) {
-  __shared__ int wave_tot[16];
-  __shared__ int64_t red[16];
-  const int tid = threadIdx.x;
-  int64_t small = 0, big = 0;
+  __shared__ int wave_tot[4][16];
+  __shared__ int64_t red[2][16];
+  __shared__ int red_n[16];
+  __shared__ int first_s[kAttnPlanLds + 1], join_s[kAttnPlanLds], part_s[kAttnPlanLds];
+  __shared__ AttnSeq seq_s[kAttnPlanLds];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const bool local = a.S <= kAttnPlanLds;
+  int64_t keys[2] = {0, 0};  // of the few-row tiles, of the others
+  int n_big = 0;             // tiles of the others
   for (int s = tid; s < a.S; s += kAttnPlanThreads) {
     const AttnSeq q = attn_seq(a, s);
-    (q.tile == kAttnSmallRows ? small : big) += (int64_t)q.tiles * q.len;
+    const bool small = q.tile == kAttnSmallRows;
+    keys[0] += small ? (int64_t)q.tiles * q.len : 0;
+    keys[1] += small ? 0 : (int64_t)q.tiles * q.len;
+    n_big += small ? 0 : q.tiles;
+    if (local) seq_s[s] = q;
   }
-  small = attn_block_sum(small, red);
-  big = attn_block_sum(big, red);
-  // (keys of a part, a multiple of 64; ceil so that total / part stays within the bound)
-  auto part_of = [&](int64_t keys, int items) {
-    const int64_t c = (keys * a.Hkv + items - 1) / items;
-    const int64_t m = c < kAttnMinKeys ? kAttnMinKeys : c;
-    return (int)((m + 63) / 64 * 64 < 0x40000000 ? (m + 63) / 64 * 64 : 0x40000000);
+#pragma unroll
+  for (int d = 1; d < kWaveSize; d *= 2) {
+    keys[0] += __shfl_xor(keys[0], d, kWaveSize);
+    keys[1] += __shfl_xor(keys[1], d, kWaveSize);
+    n_big += __shfl_xor(n_big, d, kWaveSize);
+  }
+  if (lane == 0) red[0][wave] = keys[0], red[1][wave] = keys[1], red_n[wave] = n_big;
+  __syncthreads();
+  keys[0] = keys[1] = 0, n_big = 0;
+  for (int w = 0; w < kAttnPlanThreads / kWaveSize; ++w) keys[0] += red[0][w], keys[1] += red[1][w], n_big += red_n[w];
+  // keys of a part: total / items, and a little more than the rounding of a float may take
+  auto cut_of = [&](int64_t total, int items) {
+    const float c = (float)total * (float)a.Hkv / (float)(items > 0 ? items : 1) * 1.000002f + 1.0f;
+    return (int)fminf(fmaxf(c, (float)kAttnMinKeys), 1.0e9f);
   };
-  const int cut_small = part_of(small, kAttnSmallItems), cut_big = part_of(big, kAttnBigItems);
-  int items = 0, joins = 0, parts_small = 0, parts_big = 0;
+  const int heads_big = n_big < kAttnBigItems ? n_big * a.Hkv : kAttnBigItems;  // (no more is asked of it)
+  const int want = heads_big < kAttnBigItems ? heads_big * attn_parts(heads_big) : kAttnBigItems;
+  const int cut_small = cut_of(keys[0], kAttnSmallItems), cut_big = cut_of(keys[1], want < kAttnBigItems ? want : kAttnBigItems);
+  int at[4] = {0, 0, 0, 0};  // items, joins, parts of few-row tiles, of the others
   int* start = a.plan.start;
   for (int base = 0; base < a.S; base += kAttnPlanThreads) {
     const int s = base + tid;
-    int ni = 0, nj = 0, np = 0;
-    bool is_small = true;
+    int n[4] = {0, 0, 0, 0}, v[4];
+    bool small = true;
     if (s < a.S) {
-      const AttnSeq q = attn_seq(a, s);
-      is_small = q.tile == kAttnSmallRows;
-      const int cut = is_small ? cut_small : cut_big;
-      const int ns = q.len > cut ? (q.len + cut - 1) / cut : 1;
-      ni = q.tiles * ns;
-      nj = ns > 1 ? q.tiles : 0;
-      np = ns > 1 ? ni : 0;
+      const AttnSeq q = local ? seq_s[s] : attn_seq(a, s);
+      small = q.tile == kAttnSmallRows;
+      const uint32_t cut = (uint32_t)(small ? cut_small : cut_big), ns = max(1u, ((uint32_t)q.len + cut / 2) / cut);
+      n[0] = q.tiles * (int)ns;
+      n[1] = ns > 1 ? q.tiles : 0;
+      n[small ? 2 : 3] = ns > 1 ? n[0] : 0;
     }
-    int total;
-    int upto = attn_scan(ni, wave_tot, total);
-    if (s < a.S) start[s + 1] = items + upto;
-    items += total;
-    upto = attn_scan(nj, wave_tot, total);
-    if (s < a.S) start[(a.S + 1) + s + 1] = joins + upto;
-    joins += total;
-    upto = attn_scan(is_small ? np : 0, wave_tot, total);
-    const int at_small = parts_small + upto - np;
-    parts_small += total;
-    upto = attn_scan(is_small ? 0 : np, wave_tot, total);
-    const int at_big = parts_big + upto - np;
-    parts_big += total;
-    if (s < a.S) start[2 * (a.S + 1) + s] = is_small ? at_small : at_big;
+    __syncthreads();  // the last turn's sums have been read
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = n[i];
+#pragma unroll
+      for (int d = 1; d < kWaveSize; d *= 2) {
+        const int u = __shfl_up(v[i], d, kWaveSize);
+        if (lane >= d) v[i] += u;
+      }
+      if (lane == 63) wave_tot[i][wave] = v[i];
+    }
+    __syncthreads();
+    int all[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      all[i] = 0;
+#pragma unroll
+      for (int w = 0; w < kAttnPlanThreads / kWaveSize; ++w) {
+        const int t = wave_tot[i][w];
+        if (w < wave) v[i] += t;
+        all[i] += t;
+      }
+    }
+    if (s < a.S) {
+      const int first = at[0] + v[0], join = at[1] + v[1] - n[1], part = small ? at[2] + v[2] - n[2] : at[3] + v[3] - n[3];
+      if (local) first_s[s + 1] = first, join_s[s] = join, part_s[s] = part;
+      else start[s + 1] = first, start[(a.S + 1) + s] = join, start[2 * (a.S + 1) + s] = part;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) at[i] += all[i];
   }
   if (tid == 0) {
-    start[0] = start[a.S + 1] = 0;
-    a.plan.hdr[0] = items < a.items_max ? items : a.items_max;
-    a.plan.hdr[1] = joins < a.joins_max ? joins : a.joins_max;
+    first_s[0] = start[0] = 0;
+    a.plan.hdr[0] = at[0] < a.items_max ? at[0] : a.items_max;
+    a.plan.hdr[1] = at[1] < a.joins_max ? at[1] : a.joins_max;
   }
   __syncthreads();
-  for (int i = tid; i < items && i < a.items_max; i += kAttnPlanThreads) {
+  const int items = at[0] < a.items_max ? at[0] : a.items_max;
+  for (int i = tid; i < items; i += kAttnPlanThreads) {
     int lo = 0, hi = a.S;
-    while (hi - lo > 1) {  // last s with start[s] <= i
+    while (hi - lo > 1) {  // last s with first[s] <= i
       const int mid = (lo + hi) >> 1;
-      if (start[mid] <= i) lo = mid;
+      if ((local ? first_s[mid] : start[mid]) <= i) lo = mid;
       else hi = mid;
     }
-    const AttnSeq q = attn_seq(a, lo);
-    const int ns = (start[lo + 1] - start[lo]) / q.tiles, k = i - start[lo];
-    const int t = q.tiles - 1 - k / ns, j = k % ns;  // (the later tiles of a prompt see more keys: they go first)
+    const AttnSeq q = local ? seq_s[lo] : attn_seq(a, lo);
+    const int first = local ? first_s[lo] : start[lo], end = local ? first_s[lo + 1] : start[lo + 1];
+    const int join = local ? join_s[lo] : start[(a.S + 1) + lo], part = local ? part_s[lo] : start[2 * (a.S + 1) + lo];
+    const uint32_t ns = (uint32_t)(end - first) / (uint32_t)q.tiles, k = (uint32_t)(i - first);
+    const int t = q.tiles - 1 - (int)(k / ns), j = (int)(k % ns);  // (the later tiles of a prompt see more keys: they go first)
     AttnItem it;
     it.row0 = q.row0, it.n = q.n, it.len = q.len, it.trow = q.trow, it.first = t * q.tile;
     const int last = min(it.first + q.tile, q.n * a.g) - 1;
-    const int keys = max(0, min(q.len, q.len - q.n + last / a.g + 1));  // that the tile's last row sees
-    const int step = ((keys + ns - 1) / ns + 63) / 64 * 64;
-    it.kb = (int)min((int64_t)keys, (int64_t)j * step);
-    it.ke = (int)min((int64_t)keys, (int64_t)(j + 1) * step);
-    it.part = ns > 1 ? start[2 * (a.S + 1) + lo] + t * ns + j : -1;
+    const int seen = max(0, min(q.len, q.len - q.n + last / a.g + 1));  // keys that the tile's last row sees
+    const int64_t step = (int64_t)((seen + ns - 1) / ns + 63) / 64 * 64;
+    it.kb = (int)min((int64_t)seen, j * step);
+    it.ke = (int)min((int64_t)seen, (j + 1) * step);
+    it.part = ns > 1 ? part + t * (int)ns + j : -1;
     // (sequences that overlap, which none should, could come to more parts than there is room for)
     const int parts_max = q.tile == kAttnSmallRows ? a.parts_small_max : a.parts_big_max;
     const bool fits = it.part < parts_max;
     if (!fits) it.n = 0, it.kb = it.ke = 0, it.part = -1;
     a.plan.items[i] = it;
-    if (ns > 1 && j == 0) {
-      const int at = start[(a.S + 1) + lo] + t;
-      if (at < a.joins_max) a.plan.joins[at] = AttnJoin{q.row0, fits && it.part + ns <= parts_max ? q.n : 0, it.first, it.part, ns, {0, 0, 0}};
-    }
+    if (ns > 1 && j == 0 && join + t < a.joins_max)
+      a.plan.joins[join + t] = AttnJoin{q.row0, fits && it.part + (int)ns <= parts_max ? q.n : 0, it.first, it.part, (int)ns, {0, 0, 0}};
   }
 }
 
@@ -713,9 +734,13 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
   else attn_small<DT, D, 1>(a, it, kvh, lds, reinterpret_cast<float*>(side));
 }
 
-// The parts of a tile's rows: each weighed by its maximum against the largest, in order.
+// The parts of a tile's rows, each weighed by its maximum against the largest.  A thread takes four dimensions of a row and, where the parts
+// are many, every eighth of them; the eight are then added in order.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;  // threads a row; rows, or shares of the parts, at a time
+  __shared__ f32x4 acc_s[kGroups][kLanes];
+  __shared__ float sum_s[kGroups], top_s[kGroups];
   const int i = (int)blockIdx.x / a.Hkv, kvh = (int)blockIdx.x - i * a.Hkv;
   if (i >= a.plan.hdr[1]) return;
   const AttnJoin jn = a.plan.joins[i];
@@ -725,21 +750,61 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   const float *po = small ? a.po_small : a.po_big, *pm = small ? a.pm_small : a.pm_big;
   AttnItem it;
   it.row0 = jn.row0;
-  const int n = min(tile, rows - jn.first);
-  for (int x = threadIdx.x; x < n * (D / 4); x += 256) {
-    const int r = x / (D / 4), d4 = x % (D / 4);
+  const int n = min(tile, rows - jn.first), lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
+  const int64_t step = (int64_t)a.Hkv * tile;
+  const bool many = jn.parts >= 2 * kGroups;
+  const int by = many ? kGroups : 1;
+  for (int r0 = 0; r0 < n; r0 += many ? 1 : kGroups) {
+    const int r = many ? r0 : min(r0 + grp, n - 1);
+    const int64_t at0 = ((int64_t)jn.part * a.Hkv + kvh) * tile + r;
+    // running maximum over this thread's parts, four on their way at a time
     float top = -INFINITY, sum = 0.0f;
-    for (int j = 0; j < jn.parts; ++j) top = fmaxf(top, pm[((((int64_t)jn.part + j) * a.Hkv + kvh) * tile + r) * 2]);
-    const float ref = top == -INFINITY ? 0.0f : top;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int j = 0; j < jn.parts; ++j) {
-      const int64_t at = (((int64_t)jn.part + j) * a.Hkv + kvh) * tile + r;
-      const float f = attn_exp2(pm[at * 2] - ref);
-      sum += f * pm[at * 2 + 1];
-      acc += f * ldg_f4(po + at * D + d4 * 4);
+    for (int j = many ? grp : 0; j < jn.parts; j += 4 * by) {
+      float m[4], l[4];
+      f32x4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t at = at0 + (int64_t)min(j + u * by, jn.parts - 1) * step;
+        m[u] = j + u * by < jn.parts ? pm[at * 2] : -INFINITY;
+        l[u] = pm[at * 2 + 1];
+        v[u] = ldg_f4(po + at * D + lane * 4);
+      }
+      const float now = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top), ref = now == -INFINITY ? 0.0f : now;
+      const float old = attn_exp2(top - ref);
+      sum *= old;
+      acc *= old;
+      top = now;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (j + u * by >= jn.parts) continue;
+        const float f = attn_exp2(m[u] - ref);
+        sum += f * l[u];
+        acc += f * v[u];
+      }
+    }
+    if (many) {
+      __syncthreads();  // the last row's have been read
+      acc_s[grp][lane] = acc;
+      if (lane == 0) sum_s[grp] = sum, top_s[grp] = top;
+      __syncthreads();
+      if (grp != 0) continue;
+#pragma unroll
+      for (int w = 1; w < kGroups; ++w) top = fmaxf(top, top_s[w]);
+      const float ref = top == -INFINITY ? 0.0f : top;
+      sum = 0.0f;
+      acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kGroups; ++w) {
+        const float f = attn_exp2(top_s[w] - ref);
+        sum += f * sum_s[w];
+        acc += f * acc_s[w][lane];
+      }
+    } else if (r0 + grp >= n) {
+      continue;
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    *(SMLM_GLOBAL u32x2*)(attn_out_row(a, it, kvh, jn.first + r) + d4 * 4) =
+    *(SMLM_GLOBAL u32x2*)(attn_out_row(a, it, kvh, jn.first + r) + lane * 4) =
         attn_pack4<DT>(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
   }
 }

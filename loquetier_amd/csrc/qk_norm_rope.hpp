@@ -255,19 +255,33 @@ struct QkRopeFoldArgs {
   int D, blocks;           // workgroups a tensor
 };
 
-// dw from the workgroups' sums: sixteen columns a workgroup, sixteen rows of sums at a time.
+// dw from the workgroups' sums, sixteen columns a workgroup: a thread adds every 64th row of four columns, eight rows on their way
+// at a time, and the 64 sums are added in order of a tree.
 template <int DT>
 __global__ __launch_bounds__(256) void qk_rope_fold_kernel(QkRopeFoldArgs a) {
-  __shared__ float red[16][17];
-  const int t = (int)blockIdx.x / a.blocks, col = ((int)blockIdx.x % a.blocks) * 16 + (threadIdx.x & 15);
-  float s = 0.0f;
-  for (int p = threadIdx.x >> 4; p < a.n_part[t]; p += 16) s += a.partial[t][(int64_t)p * a.D + col];
-  red[threadIdx.x >> 4][threadIdx.x & 15] = s;
-  __syncthreads();
-  if (threadIdx.x >= 16) return;
+  __shared__ f32x4 red[64][4];
+  const int t = (int)blockIdx.x / a.blocks, c4 = threadIdx.x & 3, r = threadIdx.x >> 2;
+  const int col = ((int)blockIdx.x - t * a.blocks) * 16;
+  const float* from = a.partial[t] + col + c4 * 4;
+  const int n = a.n_part[t];
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  for (int p = r; p < n; p += 64 * 8) {
+    f32x4 v[8];
 #pragma unroll
-  for (int i = 1; i < 16; ++i) s += red[i][threadIdx.x];
-  a.dw[t][col] = (uint16_t)Num<DT>::bits(s);
+    for (int j = 0; j < 8; ++j) v[j] = ldg_f4(from + (int64_t)(p + 64 * j < n ? p + 64 * j : r) * a.D);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (p + 64 * j < n) s += v[j];
+  }
+  red[r][c4] = s;
+  for (int d = 32; d >= 1; d >>= 1) {
+    __syncthreads();
+    if (r < d) red[r][c4] += red[r + d][c4];
+  }
+  if (r == 0) {
+    const f32x4 v = red[0][c4];
+    *(SMLM_GLOBAL u32x2*)(a.dw[t] + col + c4 * 4) = u32x2{pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
+  }
 }
 
 }  // namespace smlm

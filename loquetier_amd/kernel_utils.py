@@ -303,6 +303,14 @@ class qk_norm_rope(Function):
     (src/loquetier_src/models/mixed_llama.py:93-195).  The backward makes the root mean squares again, so only the inputs are
     kept, and of those only what it reads: nothing of q and k where there is no norm."""
 
+    @classmethod
+    def apply(cls, *args, **kwargs):
+        if cls is qk_norm_rope and not kwargs and not torch._C._are_functorch_transforms_active():
+            out = kernel._host().qk_norm_rope(*args)  # (plain calls; None: nothing was done)
+            if out is not None:
+                return out
+        return super().apply(*args, **kwargs)
+
     @staticmethod
     def forward(ctx: FunctionCtx, q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor],
                 k_weight: Optional[torch.Tensor], table: torch.Tensor, positions: torch.Tensor, eps: float = 1e-6):

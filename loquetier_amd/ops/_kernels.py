@@ -1032,6 +1032,8 @@ def qk_norm_rope(q_out: torch.Tensor, k_out: Optional[torch.Tensor], q: torch.Te
 
     With the caches (k_cache, v_cache [n_pages, kv_heads, page_size, head_dim], any strides) and slots (int64 [rows],
     page * page_size + place, -1: not cached) the keys and v also go there; k_out may then be None."""
+    if _host().rope(q_out, k_out, q, k, table, positions, q_weight, k_weight, eps, v, k_cache, v_cache, slots):
+        return
     a = _rope_args(q, k, table, positions, q_weight, k_weight, eps)
     _check_heads(q_out, "q_out", q)
     if q_out.shape != q.shape:
@@ -1135,6 +1137,9 @@ def kv_extend(table: torch.Tensor, length: torch.Tensor, refs: torch.Tensor, req
 
     Returns (q_indptr int32 [S + 1], kv_len int32 [S], positions int32 [n_rows], slots int64 [n_rows]): what qk_norm_rope and
     AttentionPlan read.  n_rows: the counts' sum, or more (rows past it get position and slot -1)."""
+    done = _host().kv_extend(table, length, refs, requests, counts, n_rows, page_size, status, workspace)
+    if done is not None:
+        return done
     dev, R, M, N = _kv_state(table, length, refs, status, requests=requests, counts=counts)
     if requests.numel() != counts.numel():
         raise RuntimeError("requests and counts must have one entry per sequence")
@@ -1157,6 +1162,8 @@ def kv_extend(table: torch.Tensor, length: torch.Tensor, refs: torch.Tensor, req
 def kv_free(table: torch.Tensor, length: torch.Tensor, refs: torch.Tensor, requests: torch.Tensor, page_size: int,
             status: Optional[torch.Tensor] = None) -> None:
     """Gives the requests' pages back (those that a fork shares stay with the others)."""
+    if _host().kv_free(table, length, refs, requests, page_size, status):
+        return
     dev, R, M, N = _kv_state(table, length, refs, status, requests=requests)
     if page_size < 1:
         raise RuntimeError("page_size must be positive")
@@ -1170,6 +1177,8 @@ def kv_fork(pool: torch.Tensor, table: torch.Tensor, length: torch.Tensor, refs:
             children: torch.Tensor, status: Optional[torch.Tensor] = None, workspace: Optional[Workspace] = None) -> None:
     """children[i], empty so far, becomes a second parents[i]: full pages shared, the filled places of a part-filled last
     page copied.  pool: [n_pages, ..., page_size, head_dim], contiguous (PagedKvCache.pool)."""
+    if _host().kv_fork(pool, table, length, refs, parents, children, status, workspace):
+        return
     dev, R, M, N = _kv_state(table, length, refs, status, parents=parents, children=children)
     blocks, P, place = _kv_pool(pool, dev, N)
     if parents.numel() != children.numel():
@@ -1216,6 +1225,12 @@ class AttentionPlan:
 
     def __init__(self, q_indptr: torch.Tensor, kv_len: torch.Tensor, page_table: torch.Tensor, n_rows: int, q_heads: int,
                  kv_heads: int, page_size: int, requests: Optional[torch.Tensor] = None):
+        buf = _host().attention_plan(q_indptr, kv_len, page_table, n_rows, q_heads, kv_heads, page_size, requests)
+        if buf is not None:
+            self.buf, self.S, self.T = buf, q_indptr.size(0) - 1, n_rows
+            self.q_indptr, self.kv_len, self.page_table, self.requests = q_indptr, kv_len, page_table, requests
+            self.q_heads, self.kv_heads, self.page_size = q_heads, kv_heads, page_size
+            return
         _check_input(q_indptr, "q_indptr")
         dev = q_indptr.device
         _check_ints(dev, torch.int32, 1, q_indptr=q_indptr, kv_len=kv_len, requests=requests)
@@ -1246,6 +1261,8 @@ def paged_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v
     """Causal attention of the batch's rows q [rows, q_heads, head_dim] over the pages of k_cache and v_cache [n_pages, kv_heads,
     page_size, head_dim] (any strides), prompts' chunks and single tokens in one call.  scale: head_dim ** -0.5 by default.
     Rows that see no token become zero; rows of no sequence are left as they were."""
+    if _host().paged_attention(out, q, k_cache, v_cache, plan, scale, workspace):
+        return
     _check_heads(q, "q")
     _check_heads(out, "out", q)
     if out.shape != q.shape:
