@@ -113,6 +113,29 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnPlanArgs& a, int s) {
 
 constexpr int kAttnPlanThreads = 1024;
 
+// Inclusive sums over a wave: shifts inside rows of 16 lanes, then the rows' totals.
+#define SMLM_DPP(x, ctrl, rmask) __builtin_amdgcn_update_dpp(0, x, ctrl, rmask, 0xf, false)
+__device__ __forceinline__ int attn_wave_scan(int v) {
+  v += SMLM_DPP(v, 0x111, 0xf);  // row_shr:1
+  v += SMLM_DPP(v, 0x112, 0xf);
+  v += SMLM_DPP(v, 0x114, 0xf);
+  v += SMLM_DPP(v, 0x118, 0xf);
+  v += SMLM_DPP(v, 0x142, 0xa);  // row_bcast:15 into rows 1 and 3
+  v += SMLM_DPP(v, 0x143, 0xc);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+__device__ __forceinline__ float attn_wave_sum(float v) {
+  auto add = [&](int moved) { v += __builtin_bit_cast(float, moved); };
+  add(SMLM_DPP(__builtin_bit_cast(int, v), 0x111, 0xf));
+  add(SMLM_DPP(__builtin_bit_cast(int, v), 0x112, 0xf));
+  add(SMLM_DPP(__builtin_bit_cast(int, v), 0x114, 0xf));
+  add(SMLM_DPP(__builtin_bit_cast(int, v), 0x118, 0xf));
+  add(SMLM_DPP(__builtin_bit_cast(int, v), 0x142, 0xa));
+  add(SMLM_DPP(__builtin_bit_cast(int, v), 0x143, 0xc));
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+#undef SMLM_DPP
+
 constexpr int kAttnPlanLds = kAttnPlanThreads;  // up to here the sequences stay in LDS: every read of memory is most of a microsecond
 
 // The number of parts that a tile of the card's average length is cut into, for n tiles (times kv heads): as many as leave the
@@ -134,36 +157,31 @@ __device__ __forceinline__ int attn_parts(int n) {
 // One workgroup.  The sequences' tiles are cut into parts of about `cut` keys, by the sequences' lengths; the cuts follow from the batch's
 // totals, so that the numbers of items and parts have bounds that the host knows.
 __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArgs a) {
-  __shared__ int wave_tot[4][16];
-  __shared__ int64_t red[2][16];
-  __shared__ int red_n[16];
+  __shared__ __align__(16) int wave_tot[16][4];
+  __shared__ float red[3][16];
   __shared__ int first_s[kAttnPlanLds + 1], join_s[kAttnPlanLds], part_s[kAttnPlanLds];
   __shared__ AttnSeq seq_s[kAttnPlanLds];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, threads = (int)blockDim.x, waves = threads >> 6;
   const bool local = a.S <= kAttnPlanLds;
-  int64_t keys[2] = {0, 0};  // of the few-row tiles, of the others
-  int n_big = 0;             // tiles of the others
-  for (int s = tid; s < a.S; s += kAttnPlanThreads) {
+  float keys[2] = {0.0f, 0.0f};  // of the few-row tiles, of the others (only the cuts hang on them: a float will do)
+  float n_big_f = 0.0f;          // tiles of the others
+  for (int s = tid; s < a.S; s += threads) {
     const AttnSeq q = attn_seq(a, s);
     const bool small = q.tile == kAttnSmallRows;
-    keys[0] += small ? (int64_t)q.tiles * q.len : 0;
-    keys[1] += small ? 0 : (int64_t)q.tiles * q.len;
-    n_big += small ? 0 : q.tiles;
+    keys[0] += small ? (float)q.tiles * (float)q.len : 0.0f;
+    keys[1] += small ? 0.0f : (float)q.tiles * (float)q.len;
+    n_big_f += small ? 0.0f : (float)q.tiles;
     if (local) seq_s[s] = q;
   }
-#pragma unroll
-  for (int d = 1; d < kWaveSize; d *= 2) {
-    keys[0] += __shfl_xor(keys[0], d, kWaveSize);
-    keys[1] += __shfl_xor(keys[1], d, kWaveSize);
-    n_big += __shfl_xor(n_big, d, kWaveSize);
-  }
-  if (lane == 0) red[0][wave] = keys[0], red[1][wave] = keys[1], red_n[wave] = n_big;
+  keys[0] = attn_wave_sum(keys[0]), keys[1] = attn_wave_sum(keys[1]), n_big_f = attn_wave_sum(n_big_f);
+  if (lane == 0) red[0][wave] = keys[0], red[1][wave] = keys[1], red[2][wave] = n_big_f;
   __syncthreads();
-  keys[0] = keys[1] = 0, n_big = 0;
-  for (int w = 0; w < kAttnPlanThreads / kWaveSize; ++w) keys[0] += red[0][w], keys[1] += red[1][w], n_big += red_n[w];
+  keys[0] = keys[1] = n_big_f = 0.0f;
+  for (int w = 0; w < waves; ++w) keys[0] += red[0][w], keys[1] += red[1][w], n_big_f += red[2][w];
+  const int n_big = (int)fminf(n_big_f, 1.0e9f);
   // keys of a part: total / items, and a little more than the rounding of a float may take
-  auto cut_of = [&](int64_t total, int items) {
-    const float c = (float)total * (float)a.Hkv / (float)(items > 0 ? items : 1) * 1.000002f + 1.0f;
+  auto cut_of = [&](float total, int items) {
+    const float c = total * (float)a.Hkv / (float)(items > 0 ? items : 1) * 1.0001f + 1.0f;
     return (int)fminf(fmaxf(c, (float)kAttnMinKeys), 1.0e9f);
   };
   const int heads_big = n_big < kAttnBigItems ? n_big * a.Hkv : kAttnBigItems;  // (no more is asked of it)
@@ -171,7 +189,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
   const int cut_small = cut_of(keys[0], kAttnSmallItems), cut_big = cut_of(keys[1], want < kAttnBigItems ? want : kAttnBigItems);
   int at[4] = {0, 0, 0, 0};  // items, joins, parts of few-row tiles, of the others
   int* start = a.plan.start;
-  for (int base = 0; base < a.S; base += kAttnPlanThreads) {
+  for (int base = 0; base < a.S; base += threads) {
     const int s = base + tid;
     int n[4] = {0, 0, 0, 0}, v[4];
     bool small = true;
@@ -186,22 +204,15 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
     __syncthreads();  // the last turn's sums have been read
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      v[i] = n[i];
-#pragma unroll
-      for (int d = 1; d < kWaveSize; d *= 2) {
-        const int u = __shfl_up(v[i], d, kWaveSize);
-        if (lane >= d) v[i] += u;
-      }
-      if (lane == 63) wave_tot[i][wave] = v[i];
+      v[i] = attn_wave_scan(n[i]);
+      if (lane == 63) wave_tot[wave][i] = v[i];
     }
     __syncthreads();
-    int all[4];
+    int all[4] = {0, 0, 0, 0};
+    for (int w = 0; w < waves; ++w) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      all[i] = 0;
-#pragma unroll
-      for (int w = 0; w < kAttnPlanThreads / kWaveSize; ++w) {
-        const int t = wave_tot[i][w];
+      for (int i = 0; i < 4; ++i) {
+        const int t = wave_tot[w][i];
         if (w < wave) v[i] += t;
         all[i] += t;
       }
@@ -221,7 +232,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
   }
   __syncthreads();
   const int items = at[0] < a.items_max ? at[0] : a.items_max;
-  for (int i = tid; i < items; i += kAttnPlanThreads) {
+  for (int i = tid; i < items; i += threads) {
     int lo = 0, hi = a.S;
     while (hi - lo > 1) {  // last s with first[s] <= i
       const int mid = (lo + hi) >> 1;
@@ -263,6 +274,7 @@ struct AttnArgs {
   int M, n_pages, P, T, Hq, Hkv, g;
   uint32_t div_mul;          // division by P: ((x * div_mul >> 32) + x) >> div_shift in 33 bits
   int div_shift;
+  int whole;                 // sixteen keys from a multiple of sixteen on lie in one page
   float scale;               // times log2 e
 };
 
@@ -294,11 +306,18 @@ __device__ __forceinline__ u32x4 attn_ld(const uint16_t* base, int64_t off, int 
   return ldg16(off >= 0 ? base + off + d : reinterpret_cast<const uint16_t*>(attn_zeros));
 }
 
-// A row of K or V in LDS: pieces of 16 bytes, the piece's place turned by the row so that the lanes of a matrix operand,
-// which read one piece of sixteen rows, meet all banks.
+// A row of K or V in LDS: pieces of 16 bytes, the piece's place turned by the row.  The lanes of a matrix operand read one
+// piece of sixteen rows of K: the low bits of the row turn it, and they meet all banks.  Of V, sixteen lanes of the transposing load read a
+// pair of pieces of four rows, and the next sixteen the pair beside it (or the next four rows): the turn is by pairs, two apart from
+// row to row.  (V turned as K is: half of LDS's cycles were conflicts.)
 template <int D>
 __device__ __forceinline__ int attn_place(int row, int piece) {
   return row * D + ((D == 128 ? piece ^ (row & 15) : piece ^ ((row >> 1) & 7)) << 3);
+}
+template <int D>
+__device__ __forceinline__ int attn_place_v(int row, int piece) {
+  const int pairs = D == 128 ? ((row & 3) << 1) | ((row >> 2) & 1) : (row & 2) | ((row >> 2) & 1);
+  return row * D + ((piece ^ (pairs << 1)) << 3);
 }
 
 // whether an element of a pair of 16-bit values is an infinity or NaN
@@ -313,7 +332,7 @@ __device__ __forceinline__ uint32_t attn_not_finite(uint32_t x) {
 template <int D>
 __device__ __forceinline__ int attn_v_place(int row, int d0) {
   const int l = threadIdx.x & 15, r = row + (l >> 2), d = d0 + (l & 3) * 4;
-  return attn_place<D>(r, d >> 3) + (d & 7);
+  return attn_place_v<D>(r, d >> 3) + (d & 7);
 }
 __device__ __forceinline__ u32x4 attn_v_pair(const uint16_t* a, const uint16_t* b) {
   const u32x2 x = lds_read_tr16(a), y = lds_read_tr16(b);
@@ -408,7 +427,7 @@ __device__ __forceinline__ void attn_small(const AttnArgs& a, const AttnItem& it
 #pragma unroll
     for (int i = 0; i < kVLoads; ++i) {
       const int r = i * kRowsLoad + lane / kRowLanes;
-      *(u32x4*)(vl + attn_place<D>(r, lane % kRowLanes)) = vr[i];
+      *(u32x4*)(vl + attn_place_v<D>(r, lane % kRowLanes)) = vr[i];
       if (edge) odd |= attn_not_finite<DT>(vr[i][0]) | attn_not_finite<DT>(vr[i][1]) | attn_not_finite<DT>(vr[i][2]) | attn_not_finite<DT>(vr[i][3]);
     }
     off = attn_offset(a, next);
@@ -553,26 +572,54 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
 
-  int kat[kSteps], vat[kBlk][2];
+  int kat[kSteps], vat[kBlk];
 #pragma unroll
   for (int k = 0; k < kSteps; ++k) kat[k] = attn_place<D>(c, k * 2 + h);
 #pragma unroll
-  for (int i = 0; i < kBlk; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) vat[i][j] = attn_v_place<D>(h * 4 + j * 8, i * 32 + ((lane >> 4) & 1) * 16);
+  for (int i = 0; i < kBlk; ++i) vat[i] = attn_v_place<D>(h * 4, i * 32 + ((lane >> 4) & 1) * 16);  // (8 rows on: the same turn)
 
+  // What a lane reads: the turn undoes itself, so the piece that is turned into the lane's place.  Rows of a load are kRowsLoad
+  // apart from the next's, so their turns differ by constants.
+  constexpr int kTurnsK = kLoads, kTurnsV = kLoads < 2 ? kLoads : 2;
+  uint32_t kof[kTurnsK], vof[kTurnsV];  // bytes from the load's first row
+  const uint32_t slot_bytes = a.whole ? (uint32_t)a.c_slot * 2u : 0u;
+#pragma unroll
+  for (int i = 0; i < kTurnsK; ++i) {
+    const int r = i * kRowsLoad + lane / kRowLanes;
+    kof[i] = (uint32_t)(lane / kRowLanes) * slot_bytes + (uint32_t)(attn_place<D>(r, lane % kRowLanes) - r * D) * 2u;
+    if (i < kTurnsV) vof[i] = (uint32_t)(lane / kRowLanes) * slot_bytes + (uint32_t)(attn_place_v<D>(r, lane % kRowLanes) - r * D) * 2u;
+  }
+  typedef SMLM_GLOBAL const char* gptr;
+  auto to_lds = [&](gptr from, uint16_t* to) {
+    __builtin_amdgcn_global_load_lds((SMLM_GLOBAL void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+  };
   auto load = [&](int64_t off, uint16_t* tile) {
+    uint16_t* dst = tile + wave * 16 * D;
+    if (a.whole && (__ballot(off >= 0) & 0xffffu) == 0xffffu) {
+      // the wave's sixteen keys lie in one page: an address for all lanes and an offset that stays
+      const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)off), hi = __builtin_amdgcn_readfirstlane((uint32_t)(off >> 32));
+      const int64_t first = (int64_t)((uint64_t)hi << 32 | lo);
+      gptr ks = (gptr)(kp + first), vs = (gptr)(vp + first);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        uint32_t ko = kof[i], vo = vof[i % kTurnsV];
+        asm("" : "+v"(ko), "+v"(vo));  // (kept as 32 bits over the loop)
+        to_lds(ks + ko, dst + i * kRowsLoad * D);
+        to_lds(vs + vo, dst + i * kRowsLoad * D + kKeys * D);
+        ks += (uint32_t)kRowsLoad * slot_bytes, vs += (uint32_t)kRowsLoad * slot_bytes;
+      }
+      return;
+    }
+    int ln = lane;
+    asm volatile("" : "+v"(ln));  // (nothing of this is kept over the loop)
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int r = i * kRowsLoad + lane / kRowLanes;
+      const int r = i * kRowsLoad + ln / kRowLanes;
       const int64_t f = attn_shfl(off, r);
-      int d = attn_place<D>(r, lane % kRowLanes) - r * D;  // (the turn undoes itself: the piece that belongs in this lane's place)
-      asm("" : "+v"(d));                                   // (its sum with the addresses is not kept over the loop: registers)
+      const int dk = attn_place<D>(r, ln % kRowLanes) - r * D, dv = attn_place_v<D>(r, ln % kRowLanes) - r * D;
       const uint16_t* zero = reinterpret_cast<const uint16_t*>(attn_zeros);
-      const uint16_t *ks = f >= 0 ? kp + f + d : zero, *vs = f >= 0 ? vp + f + d : zero;
-      uint16_t* dst = tile + (wave * 16 + i * kRowsLoad) * D;
-      __builtin_amdgcn_global_load_lds((SMLM_GLOBAL void*)ks, (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
-      __builtin_amdgcn_global_load_lds((SMLM_GLOBAL void*)vs, (__attribute__((address_space(3))) void*)(dst + kKeys * D), 16, 0, 0);
+      to_lds((gptr)(f >= 0 ? kp + f + dk : zero), dst + i * kRowsLoad * D);
+      to_lds((gptr)(f >= 0 ? vp + f + dv : zero), dst + i * kRowsLoad * D + kKeys * D);
     }
   };
   auto work = [&](auto may_edge, int base, const uint16_t* kl, const uint32_t* fl) {
@@ -607,14 +654,16 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
 #pragma unroll
       for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[u][e]);
     mx = fmaxf(mx, __shfl_xor(mx, 32, kWaveSize));
-    const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.0f : mn * a.scale;
-    if (__ballot(mn > m)) {  // some row's maximum has grown
-      const float turn = attn_exp2(m * a.scale - ms);
+    // The reference that the exponents are taken against follows the running maximum only once that is 2^8 past it: the
+    // probabilities stay below 2^8, well inside the element types, and most tiles leave the accumulators alone.
+    if (__ballot((mx - m) * a.scale > 8.0f)) {
+      const float mn = fmaxf(m, mx), turn = attn_exp2((mn == -INFINITY ? 0.0f : m - mn) * a.scale);
       l *= turn;
 #pragma unroll
       for (int i = 0; i < kBlk; ++i) o[i] *= turn;
+      m = mn;
     }
-    m = mn;
+    const float ms = m == -INFINITY ? 0.0f : m * a.scale;
     u32x4 pf[2][2];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -643,7 +692,7 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
 #pragma unroll
           for (int i = 0; i < kBlk; ++i) {
             const uint16_t* at = vl + (u * 32 + ks * 16) * D;
-            o[i] = mfma32<DT>(attn_v_pair(at + vat[i][0], at + vat[i][1]), pf[u][ks], o[i]);
+            o[i] = mfma32<DT>(attn_v_pair(at + vat[i], at + vat[i] + 8 * D), pf[u][ks], o[i]);
           }
     } else {
 #pragma unroll 1
@@ -662,7 +711,7 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
           f32x16 add;
 #pragma unroll
           for (int e = 0; e < 16; ++e) add[e] = 0.0f;
-          add = mfma32<DT>(attn_v_pair(at + vat[i][0], at + vat[i][1]) & only, pj, add);
+          add = mfma32<DT>(attn_v_pair(at + vat[i], at + vat[i] + 8 * D) & only, pj, add);
           if (base + key <= lim) o[i] += add;
         }
       }
@@ -736,12 +785,14 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
 
 // The parts of a tile's rows, each weighed by its maximum against the largest.  A thread takes four dimensions of a row and, where the parts
 // are many, every eighth of them; the eight are then added in order.
+constexpr int kAttnJoinShares = 4;  // workgroups that share a tile's rows
 template <int DT, int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;  // threads a row; rows, or shares of the parts, at a time
   __shared__ f32x4 acc_s[kGroups][kLanes];
   __shared__ float sum_s[kGroups], top_s[kGroups];
-  const int i = (int)blockIdx.x / a.Hkv, kvh = (int)blockIdx.x - i * a.Hkv;
+  const int x = (int)blockIdx.x / kAttnJoinShares, share = (int)blockIdx.x % kAttnJoinShares;
+  const int i = x / a.Hkv, kvh = x - i * a.Hkv;
   if (i >= a.plan.hdr[1]) return;
   const AttnJoin jn = a.plan.joins[i];
   const int rows = jn.n * a.g;
@@ -754,7 +805,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   const int64_t step = (int64_t)a.Hkv * tile;
   const bool many = jn.parts >= 2 * kGroups;
   const int by = many ? kGroups : 1;
-  for (int r0 = 0; r0 < n; r0 += many ? 1 : kGroups) {
+  const int rows_turn = many ? 1 : kGroups;
+  for (int r0 = share * rows_turn; r0 < n; r0 += kAttnJoinShares * rows_turn) {
     const int r = many ? r0 : min(r0 + grp, n - 1);
     const int64_t at0 = ((int64_t)jn.part * a.Hkv + kvh) * tile + r;
     // running maximum over this thread's parts, four on their way at a time
