@@ -8,7 +8,9 @@
 // Arithmetic in float, rounded once; r is made again in the backward, which reads x anyway, so nothing is saved.
 //
 // Streaming kernels, bound by HBM: 2 bytes read and 2 written an element (backward: 4 and 2), and by launch latency
-// for decode batches.  A head takes D / 16 lanes (rounded up to a power of two), each with two pieces of eight
+// for decode batches.  2112 rows of 32 + 32 + 32 heads of 128 with norms into a cache 20 us (5.2 TB/s, as a plain copy of that size); 4096
+// rows of 32 + 8 heads 19 us forward, 26 + 4 us backward (4.8 TB/s); 256 rows without norms 4.4 us.  Outputs are stored
+// non-temporally (24.7 -> 21.0 us at 2112 rows): they would push out of L2 what is still to be read.  A head takes D / 16 lanes (rounded up to a power of two), each with two pieces of eight
 // dimensions that are partners in the rotation, so that the pairs meet inside a lane and only the norm's sum crosses
 // lanes.  A wave keeps one row: cosines and sines of its position are read once for all the heads it takes.
 #pragma once
@@ -33,6 +35,7 @@ struct QkRopeArgs {
   int64_t c_page, c_head, c_slot;       // strides of the caches
   int T, Hq, Hkv, D, rot, n_pos, page_size, n_slots;
   int lanes_log2;                       // lanes a head
+  int runs, parts;                      // runs of heads a wave, waves a row
   float eps, sign;                      // sign: -1 turns the other way
 };
 
@@ -77,83 +80,92 @@ __device__ __forceinline__ float group_sum(float x, int lanes_log2) {
   return x;
 }
 
-// A wave takes HEADS runs of (64 / lanes a head) heads of one row.  Heads are numbered q, then k, then v.
-template <int DT, bool NORM, int HEADS>
+// A run is as many heads as a wave has groups of lanes (64 / lanes a head); heads are numbered q, then k, then v.  A wave takes
+// up to HEADS runs of one row, a row's runs shared out evenly over its waves.
+// FULL: every dimension is rotated.
+template <int DT, bool NORM, bool FULL, int HEADS>
 __global__ __launch_bounds__(256) void qk_rope_kernel(QkRopeArgs a) {
   const int lane = threadIdx.x & 63, ll = a.lanes_log2;
   const int sub = lane & ((1 << ll) - 1), grp = lane >> ll, per = kWaveSize >> ll;
-  const int heads = a.Hq + a.Hkv + (a.v_cache ? a.Hkv : 0), parts = (heads + per * HEADS - 1) / (per * HEADS);
+  const int heads = a.Hq + a.Hkv + (a.v_cache ? a.Hkv : 0);
   const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int row = (int)(unit / parts), part = (int)(unit - (int64_t)row * parts);
+  const int row = (int)(unit / a.parts), part = (int)(unit - (int64_t)row * a.parts);
   if (row >= a.T) return;  // (no barrier below)
-  const bool lane_on = sub < (a.D >> 4), turns = sub < (a.rot >> 4);
+  const int first = part * a.runs * per;  // of this wave's heads
+  const bool lane_on = sub < (a.D >> 4), turns = FULL || sub < (a.rot >> 4);
   int c0, c1;
   rope_pieces(lane_on ? sub : 0, a.rot, c0, c1);
   const int pos = a.pos[row];
   const int64_t slot = a.k_cache ? a.slots[row] : -1;
 
   u32x4 x0[HEADS], x1[HEADS];
-  int head[HEADS];
 #pragma unroll
   for (int i = 0; i < HEADS; ++i) {
-    const int h = (part * HEADS + i) * per + grp;
-    head[i] = h;
-    const int hc = h < heads ? h : 0;  // (lanes past the last head read the first one)
-    const HeadsView src = hc < a.Hq ? a.q : (hc < a.Hq + a.Hkv ? a.k : a.v);
-    const int hh = hc < a.Hq ? hc : (hc < a.Hq + a.Hkv ? hc - a.Hq : hc - a.Hq - a.Hkv);
-    const uint16_t* p = src.data + row * src.row + hh * src.head;
+    if (i >= a.runs || first + i * per >= heads) break;  // uniform over the wave
+    const int h = min(first + i * per + grp, heads - 1);  // (lanes past the last head read it too)
+    const bool is_q = h < a.Hq, is_k = h < a.Hq + a.Hkv;
+    const uint16_t* p = is_q ? a.q.data + row * a.q.row + h * a.q.head
+                             : (is_k ? a.k.data + row * a.k.row + (h - a.Hq) * a.k.head
+                                     : a.v.data + row * a.v.row + (h - a.Hq - a.Hkv) * a.v.head);
     x0[i] = ldg16(p + c0);
     x1[i] = ldg16(p + c1);
   }
   float c[8], s[8];
   rope_angles(a.table, pos, a.n_pos, a.rot, lane_on ? sub : 0, a.sign, c, s);
+  u32x4 wq[2], wk[2];
+  if (NORM) {
+    constexpr uint32_t kOne = DT == SMLM_DTYPE_F16 ? 0x3c003c00u : 0x3f803f80u;
+    const u32x4 one = {kOne, kOne, kOne, kOne};
+    wq[0] = wq[1] = wk[0] = wk[1] = one;
+    if (a.wq) wq[0] = ldg16(a.wq + c0), wq[1] = ldg16(a.wq + c1);
+    if (a.wk) wk[0] = ldg16(a.wk + c0), wk[1] = ldg16(a.wk + c1);
+  }
   const bool keep = slot >= 0 && slot < a.n_slots;
   const int page = keep ? (int)slot / a.page_size : 0, at = keep ? (int)slot - page * a.page_size : 0;
 #pragma unroll
   for (int i = 0; i < HEADS; ++i) {
-    const bool is_q = head[i] < a.Hq, is_v = head[i] >= a.Hq + a.Hkv;
-    const int hh = is_q ? head[i] : (is_v ? head[i] - a.Hq - a.Hkv : head[i] - a.Hq);
-    float f0[8], f1[8];
-    unpack8f<DT>(x0[i], f0);
-    unpack8f<DT>(x1[i], f1);
-    if (NORM) {
-      float ss = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss += f0[e] * f0[e] + f1[e] * f1[e];
-      ss = group_sum(lane_on ? ss : 0.0f, ll);
-      const uint16_t* w = is_q ? a.wq : a.wk;
-      if (w && !is_v) {
-        const float r = 1.0f / sqrtf(ss / (float)a.D + a.eps);
-        float w0[8], w1[8];
-        unpack8f<DT>(ldg16(w + c0), w0);
-        unpack8f<DT>(ldg16(w + c1), w1);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f0[e] *= r * w0[e], f1[e] *= r * w1[e];
-      }
-    }
+    if (i >= a.runs || first + i * per >= heads) break;
+    const int h = first + i * per + grp;
+    const bool is_q = h < a.Hq, is_v = h >= a.Hq + a.Hkv;
     u32x4 o0 = x0[i], o1 = x1[i];
-    if (!is_v) {
+    if (first + i * per < a.Hq + a.Hkv) {  // (uniform: a run of values alone is a copy)
+      float f0[8], f1[8], cr[8], sr[8];
+      unpack8f<DT>(x0[i], f0);
+      unpack8f<DT>(x1[i], f1);
+      float r = 1.0f;
+      if (NORM) {
+        float ss = 0.0f, w0[8], w1[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss += f0[e] * f0[e] + f1[e] * f1[e];
+        ss = group_sum(lane_on ? ss : 0.0f, ll);
+        if (is_q ? a.wq : a.wk) r = 1.0f / sqrtf(ss / (float)a.D + a.eps);
+        unpack8f<DT>(is_q ? wq[0] : wk[0], w0);
+        unpack8f<DT>(is_q ? wq[1] : wk[1], w1);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f0[e] *= w0[e], f1[e] *= w1[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) cr[e] = NORM ? c[e] * r : c[e], sr[e] = NORM ? s[e] * r : s[e];
       float g0[8], g1[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        g0[e] = f0[e] * c[e] - (turns ? f1[e] * s[e] : 0.0f);  // (0 times an infinity beside it would be NaN)
-        g1[e] = f1[e] * c[e] + (turns ? f0[e] * s[e] : 0.0f);
+        g0[e] = f0[e] * cr[e] - (turns ? f1[e] * sr[e] : 0.0f);  // (0 times an infinity beside it would be NaN)
+        g1[e] = f1[e] * cr[e] + (turns ? f0[e] * sr[e] : 0.0f);
       }
-      o0 = pack8f<DT>(g0);
-      o1 = pack8f<DT>(g1);
+      if (!is_v) o0 = pack8f<DT>(g0), o1 = pack8f<DT>(g1);
     }
     if (pos < 0) o0 = u32x4{0u, 0u, 0u, 0u}, o1 = o0;
-    if (!lane_on || head[i] >= heads) continue;
+    if (!lane_on || h >= heads) continue;
+    const int hk = is_v ? h - a.Hq - a.Hkv : h - a.Hq;
     if (is_q || (!is_v && a.k_out.data)) {
-      const HeadsView dst = is_q ? a.q_out : a.k_out;
-      uint16_t* p = dst.data + row * dst.row + hh * dst.head;
-      stg16(p + c0, o0);
-      stg16(p + c1, o1);
+      uint16_t* p = is_q ? a.q_out.data + row * a.q_out.row + h * a.q_out.head : a.k_out.data + row * a.k_out.row + hk * a.k_out.head;
+      stg16_nt(p + c0, o0);
+      stg16_nt(p + c1, o1);
     }
     if (!is_q && keep) {
-      uint16_t* p = (is_v ? a.v_cache : a.k_cache) + page * a.c_page + hh * a.c_head + at * a.c_slot;
-      stg16(p + c0, o0);
-      stg16(p + c1, o1);
+      uint16_t* p = (is_v ? a.v_cache : a.k_cache) + page * a.c_page + hk * a.c_head + at * a.c_slot;
+      stg16_nt(p + c0, o0);
+      stg16_nt(p + c1, o1);
     }
   }
 }
@@ -173,6 +185,7 @@ struct QkRopeBwdPair {
 
 // The backward behind a norm.  A workgroup of four waves walks the rows of q or of k; a lane keeps its sixteen
 // dimensions' share of dw in registers over all rows and heads it meets.
+// (Two runs of heads on their way together take a wave a SIMD its registers: 33 us where this takes 26, 4096 rows of 32 and 8 heads of 128.)
 template <int DT>
 __global__ __launch_bounds__(256) void qk_rope_bwd_kernel(QkRopeBwdPair both) {
   __shared__ float red[4][kRopeMaxDim];
@@ -193,17 +206,15 @@ __global__ __launch_bounds__(256) void qk_rope_bwd_kernel(QkRopeBwdPair both) {
     const int pos = a.pos[row];
     float c[8], s[8];
     rope_angles(a.table, pos, a.n_pos, a.rot, lane_on ? sub : 0, -1.0f, c, s);
-    for (int h = grp; h < ((a.H + per - 1) / per) * per; h += per) {
-      const bool on = lane_on && h < a.H;
-      const int hc = h < a.H ? h : 0;
+    for (int h0 = 0; h0 < a.H; h0 += per) {
+      const int h = h0 + grp, hc = min(h, a.H - 1);  // (lanes past the last head read it too)
       const uint16_t* xp = a.x.data + row * a.x.row + hc * a.x.head;
       const uint16_t* gp = a.g.data + row * a.g.row + hc * a.g.head;
-      float x0[8], x1[8], g0[8], g1[8];
+      float x0[8], x1[8], g0[8], g1[8], ss = 0.0f, dot = 0.0f, y0[8], y1[8];
       unpack8f<DT>(ldg16(xp + c0), x0);
       unpack8f<DT>(ldg16(xp + c1), x1);
       unpack8f<DT>(ldg16(gp + c0), g0);
       unpack8f<DT>(ldg16(gp + c1), g1);
-      float ss = 0.0f, dot = 0.0f, y0[8], y1[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         y0[e] = g0[e] * c[e] - (turns ? g1[e] * s[e] : 0.0f);
@@ -213,7 +224,7 @@ __global__ __launch_bounds__(256) void qk_rope_bwd_kernel(QkRopeBwdPair both) {
       }
       ss = group_sum(lane_on ? ss : 0.0f, ll);
       dot = group_sum(lane_on ? dot : 0.0f, ll);
-      if (!on) continue;
+      if (!lane_on || h >= a.H) continue;
       const float r = 1.0f / sqrtf(ss * inv + a.eps), coef = dot * inv * r * r;
       u32x4 o0 = {0u, 0u, 0u, 0u}, o1 = o0;
       if (pos >= 0) {
@@ -228,9 +239,9 @@ __global__ __launch_bounds__(256) void qk_rope_bwd_kernel(QkRopeBwdPair both) {
         o0 = pack8f<DT>(d0);
         o1 = pack8f<DT>(d1);
       }
-      uint16_t* dp = a.dx.data + row * a.dx.row + hc * a.dx.head;
-      stg16(dp + c0, o0);
-      stg16(dp + c1, o1);
+      uint16_t* dp = a.dx.data + row * a.dx.row + h * a.dx.head;
+      stg16_nt(dp + c0, o0);
+      stg16_nt(dp + c1, o1);
     }
   }
   // the heads' groups of lanes, then the four waves, always in the same order
