@@ -54,7 +54,7 @@ struct AttnJoin {   // a tile whose keys were cut
 };
 struct AttnPlanView {
   int* hdr;          // [16]: 0 items, 1 joins
-  int* start;        // [3][S + 1] running sums by sequence: items, joins, parts
+  int* start;        // [4][S + 1] running sums by sequence: items with few rows, other items, joins, parts
   AttnItem* items;
   AttnJoin* joins;
 };
@@ -76,7 +76,7 @@ inline size_t attn_plan_carve(void* base, int T, int S, int g, int Hkv, AttnPlan
   };
   AttnPlanView v;
   v.hdr = reinterpret_cast<int*>(take(64));
-  v.start = reinterpret_cast<int*>(take((size_t)3 * (S + 1) * 4));
+  v.start = reinterpret_cast<int*>(take((size_t)4 * (S + 1) * 4));
   v.items = reinterpret_cast<AttnItem*>(take((size_t)attn_items_max(T, S, g, Hkv) * sizeof(AttnItem)));
   v.joins = reinterpret_cast<AttnJoin*>(take((size_t)attn_joins_max(T, S, g, Hkv) * sizeof(AttnJoin)));
   if (pv) *pv = v;
@@ -157,9 +157,9 @@ __device__ __forceinline__ int attn_parts(int n) {
 // One workgroup.  The sequences' tiles are cut into parts of about `cut` keys, by the sequences' lengths; the cuts follow from the batch's
 // totals, so that the numbers of items and parts have bounds that the host knows.
 __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArgs a) {
-  __shared__ __align__(16) int wave_tot[16][4];
+  __shared__ int wave_tot[16][5];
   __shared__ float red[3][16];
-  __shared__ int first_s[kAttnPlanLds + 1], join_s[kAttnPlanLds], part_s[kAttnPlanLds];
+  __shared__ int first_s[2][kAttnPlanLds + 1], join_s[kAttnPlanLds], part_s[kAttnPlanLds];
   __shared__ AttnSeq seq_s[kAttnPlanLds];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, threads = (int)blockDim.x, waves = threads >> 6;
   const bool local = a.S <= kAttnPlanLds;
@@ -187,62 +187,75 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
   const int heads_big = n_big < kAttnBigItems ? n_big * a.Hkv : kAttnBigItems;  // (no more is asked of it)
   const int want = heads_big < kAttnBigItems ? heads_big * attn_parts(heads_big) : kAttnBigItems;
   const int cut_small = cut_of(keys[0], kAttnSmallItems), cut_big = cut_of(keys[1], want < kAttnBigItems ? want : kAttnBigItems);
-  int at[4] = {0, 0, 0, 0};  // items, joins, parts of few-row tiles, of the others
+  int at[5] = {0, 0, 0, 0, 0};  // items with few rows, other items, joins, parts of the ones, of the others
   int* start = a.plan.start;
   for (int base = 0; base < a.S; base += threads) {
     const int s = base + tid;
-    int n[4] = {0, 0, 0, 0}, v[4];
+    int n[5] = {0, 0, 0, 0, 0}, v[5];
     bool small = true;
     if (s < a.S) {
       const AttnSeq q = local ? seq_s[s] : attn_seq(a, s);
       small = q.tile == kAttnSmallRows;
       const uint32_t cut = (uint32_t)(small ? cut_small : cut_big), ns = max(1u, ((uint32_t)q.len + cut / 2) / cut);
-      n[0] = q.tiles * (int)ns;
-      n[1] = ns > 1 ? q.tiles : 0;
-      n[small ? 2 : 3] = ns > 1 ? n[0] : 0;
+      const int items = q.tiles * (int)ns, parts = ns > 1 ? items : 0;
+      n[0] = small ? items : 0, n[1] = small ? 0 : items;
+      n[2] = ns > 1 ? q.tiles : 0;
+      n[3] = small ? parts : 0, n[4] = small ? 0 : parts;
     }
     __syncthreads();  // the last turn's sums have been read
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 5; ++i) {
       v[i] = attn_wave_scan(n[i]);
       if (lane == 63) wave_tot[wave][i] = v[i];
     }
     __syncthreads();
-    int all[4] = {0, 0, 0, 0};
+    int all[5] = {0, 0, 0, 0, 0};
     for (int w = 0; w < waves; ++w) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 5; ++i) {
         const int t = wave_tot[w][i];
         if (w < wave) v[i] += t;
         all[i] += t;
       }
     }
     if (s < a.S) {
-      const int first = at[0] + v[0], join = at[1] + v[1] - n[1], part = small ? at[2] + v[2] - n[2] : at[3] + v[3] - n[3];
-      if (local) first_s[s + 1] = first, join_s[s] = join, part_s[s] = part;
-      else start[s + 1] = first, start[(a.S + 1) + s] = join, start[2 * (a.S + 1) + s] = part;
+      const int join = at[2] + v[2] - n[2], part = small ? at[3] + v[3] - n[3] : at[4] + v[4] - n[4];
+      if (local) {
+        first_s[0][s + 1] = at[0] + v[0], first_s[1][s + 1] = at[1] + v[1];
+        join_s[s] = join, part_s[s] = part;
+      } else {
+        start[s + 1] = at[0] + v[0], start[(a.S + 1) + s + 1] = at[1] + v[1];
+        start[2 * (a.S + 1) + s] = join, start[3 * (a.S + 1) + s] = part;
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) at[i] += all[i];
+    for (int i = 0; i < 5; ++i) at[i] += all[i];
   }
+  const int items = at[0] + at[1] < a.items_max ? at[0] + at[1] : a.items_max;
   if (tid == 0) {
-    first_s[0] = start[0] = 0;
-    a.plan.hdr[0] = at[0] < a.items_max ? at[0] : a.items_max;
-    a.plan.hdr[1] = at[1] < a.joins_max ? at[1] : a.joins_max;
+    first_s[0][0] = first_s[1][0] = start[0] = start[a.S + 1] = 0;
+    a.plan.hdr[0] = items;
+    a.plan.hdr[1] = at[2] < a.joins_max ? at[2] : a.joins_max;
   }
   __syncthreads();
-  const int items = at[0] < a.items_max ? at[0] : a.items_max;
+  // Items with few rows stream, the others compute: they take turns, so that both have the card together (mixed batch of four prompts
+  // of 512 and 64 single tokens, 32 heads: the others all first 251 us, in turns 245; alone the two take 81 and 189).
+  const int both = min(at[0], at[1]);
   for (int i = tid; i < items; i += threads) {
+    const int kind = i < 2 * both ? !(i & 1) : at[1] > at[0];  // 1: the others
+    const int x = i < 2 * both ? i >> 1 : i - both;
+    const int* first_l = first_s[kind];
+    const int* first_g = start + kind * (a.S + 1);
     int lo = 0, hi = a.S;
-    while (hi - lo > 1) {  // last s with first[s] <= i
+    while (hi - lo > 1) {  // last s with first[s] <= x
       const int mid = (lo + hi) >> 1;
-      if ((local ? first_s[mid] : start[mid]) <= i) lo = mid;
+      if ((local ? first_l[mid] : first_g[mid]) <= x) lo = mid;
       else hi = mid;
     }
     const AttnSeq q = local ? seq_s[lo] : attn_seq(a, lo);
-    const int first = local ? first_s[lo] : start[lo], end = local ? first_s[lo + 1] : start[lo + 1];
-    const int join = local ? join_s[lo] : start[(a.S + 1) + lo], part = local ? part_s[lo] : start[2 * (a.S + 1) + lo];
-    const uint32_t ns = (uint32_t)(end - first) / (uint32_t)q.tiles, k = (uint32_t)(i - first);
+    const int first = local ? first_l[lo] : first_g[lo], end = local ? first_l[lo + 1] : first_g[lo + 1];
+    const int join = local ? join_s[lo] : start[2 * (a.S + 1) + lo], part = local ? part_s[lo] : start[3 * (a.S + 1) + lo];
+    const uint32_t ns = (uint32_t)(end - first) / (uint32_t)q.tiles, k = (uint32_t)(x - first);
     const int t = q.tiles - 1 - (int)(k / ns), j = (int)(k % ns);  // (the later tiles of a prompt see more keys: they go first)
     AttnItem it;
     it.row0 = q.row0, it.n = q.n, it.len = q.len, it.trow = q.trow, it.first = t * q.tile;
