@@ -352,6 +352,20 @@ __device__ __forceinline__ u32x4 attn_v_pair(const uint16_t* a, const uint16_t* 
   return u32x4{x[0], x[1], y[0], y[1]};
 }
 
+// The weights, and so their sums and the accumulators, are held 2^bias times as large: fp16 has no normal number under 2^-14, and
+// a long context's many small weights may add up to more than its few large ones.
+template <int DT>
+constexpr float kAttnBias = DT == SMLM_DTYPE_F16 ? 7.0f : 0.0f;
+
+// l + the two halves of x
+template <int DT>
+__device__ __forceinline__ float attn_add2(uint32_t x, float l) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  if (DT == SMLM_DTYPE_F16) return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, x), h2{(_Float16)1.0f, (_Float16)1.0f}, l, false);
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, x), b2{(__bf16)1.0f, (__bf16)1.0f}, l, false);
+}
+
 template <int DT>
 __device__ __forceinline__ u32x2 attn_pack4(float a, float b, float c, float d) {
   u32x2 o;
@@ -466,8 +480,8 @@ __device__ __forceinline__ void attn_small(const AttnArgs& a, const AttnItem& it
                        fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
       mx = fmaxf(mx, __shfl_xor(mx, 16, kWaveSize));
       mx = fmaxf(mx, __shfl_xor(mx, 32, kWaveSize));
-      const float mn = fmaxf(m[t], mx), ms = mn == -INFINITY ? 0.0f : mn * a.scale;
-      const float turn = attn_exp2(m[t] * a.scale - ms);
+      const float mn = fmaxf(m[t], mx), ref = mn == -INFINITY ? 0.0f : mn * a.scale, ms = ref - kAttnBias<DT>;
+      const float turn = attn_exp2(m[t] * a.scale - ref);
       m[t] = mn;
       float sum = 0.0f, p[8];
 #pragma unroll
@@ -606,23 +620,20 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
   auto to_lds = [&](gptr from, uint16_t* to) {
     __builtin_amdgcn_global_load_lds((SMLM_GLOBAL void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
   };
+  // the wave's sixteen keys lie in one page: an address for all lanes, made on the scalar side, and an offset that stays
+  auto load_page = [&](int64_t first, uint16_t* tile) {
+    uint16_t* dst = tile + wave * 16 * D;
+    gptr ks = (gptr)(kp + first), vs = (gptr)(vp + first);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      asm volatile("" : "+v"(kof[i]), "+v"(vof[i % kTurnsV]));  // (kept as 32 bits over the loop)
+      to_lds(ks + kof[i], dst + i * kRowsLoad * D);
+      to_lds(vs + vof[i % kTurnsV], dst + i * kRowsLoad * D + kKeys * D);
+      ks += (uint32_t)kRowsLoad * slot_bytes, vs += (uint32_t)kRowsLoad * slot_bytes;
+    }
+  };
   auto load = [&](int64_t off, uint16_t* tile) {
     uint16_t* dst = tile + wave * 16 * D;
-    if (a.whole && (__ballot(off >= 0) & 0xffffu) == 0xffffu) {
-      // the wave's sixteen keys lie in one page: an address for all lanes and an offset that stays
-      const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)off), hi = __builtin_amdgcn_readfirstlane((uint32_t)(off >> 32));
-      const int64_t first = (int64_t)((uint64_t)hi << 32 | lo);
-      gptr ks = (gptr)(kp + first), vs = (gptr)(vp + first);
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        uint32_t ko = kof[i], vo = vof[i % kTurnsV];
-        asm("" : "+v"(ko), "+v"(vo));  // (kept as 32 bits over the loop)
-        to_lds(ks + ko, dst + i * kRowsLoad * D);
-        to_lds(vs + vo, dst + i * kRowsLoad * D + kKeys * D);
-        ks += (uint32_t)kRowsLoad * slot_bytes, vs += (uint32_t)kRowsLoad * slot_bytes;
-      }
-      return;
-    }
     int ln = lane;
     asm volatile("" : "+v"(ln));  // (nothing of this is kept over the loop)
 #pragma unroll
@@ -668,7 +679,7 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
       for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[u][e]);
     mx = fmaxf(mx, __shfl_xor(mx, 32, kWaveSize));
     // The reference that the exponents are taken against follows the running maximum only once that is 2^8 past it: the
-    // probabilities stay below 2^8, well inside the element types, and most tiles leave the accumulators alone.
+    // probabilities stay below 2^8 (2^15 with the bias), inside the element types, and most tiles leave the accumulators alone.
     if (__ballot((mx - m) * a.scale > 8.0f)) {
       const float mn = fmaxf(m, mx), turn = attn_exp2((mn == -INFINITY ? 0.0f : m - mn) * a.scale);
       l *= turn;
@@ -676,15 +687,15 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
       for (int i = 0; i < kBlk; ++i) o[i] *= turn;
       m = mn;
     }
-    const float ms = m == -INFINITY ? 0.0f : m * a.scale;
+    const float ms = (m == -INFINITY ? 0.0f : m * a.scale) - kAttnBias<DT>;
     u32x4 pf[2][2];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
-        const float p0 = attn_exp2(s[u][e] * a.scale - ms), p1 = attn_exp2(s[u][e + 1] * a.scale - ms);
-        l += p0 + p1;
-        pf[u][e >> 3][(e >> 1) & 3] = pack2<DT>(p0, p1);
+        const uint32_t two = pack2<DT>(attn_exp2(s[u][e] * a.scale - ms), attn_exp2(s[u][e + 1] * a.scale - ms));
+        l = attn_add2<DT>(two, l);  // (the weights as V meets them: they add up to one whatever their rounding)
+        pf[u][e >> 3][(e >> 1) & 3] = two;
       }
     // a tile that some rows see in part: does its V hold a value that is no number?
     bool guard = false;
@@ -732,13 +743,41 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
   };
   // A tile's loads are waited for by the wave that gave them, then by all; at that point everybody is done with the tile before,
   // whose place the next loads take.
+  int base = it.kb;
+  if (base < it.ke) load(attn_offset(a, attn_key(a, trow, base + wave * 16 + (lane & 15), it.ke)), tile0);
+  // Pairs of tiles that every row sees, each sixteen keys of them and of the tile after in one page: apart, so that this loop keeps its
+  // registers to itself.  What it loads, and whether a page is there, is known on the scalar side.
+  if (a.whole && base + 2 * kKeys - 1 <= lim0 && base + 3 * kKeys <= it.ke) {
+    auto page_of = [&](int key, int* slot) {
+      const int j = attn_div((uint32_t)key, a.div_mul, a.div_shift);
+      *slot = key - j * a.P;
+      return uload(trow, j);
+    };
+    int slot, page = page_of(base + wave * 16, &slot);
+    uint32_t valid = (uint32_t)page < (uint32_t)a.n_pages ? 0xffffu : 0u;
+    page = page_of(base + kKeys + wave * 16, &slot);
+    auto turn = [&](int base, uint16_t* mine, uint16_t* other, uint32_t* fl) {
+      if (lane == 0) fl[wave] = valid;
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+      __syncthreads();
+      valid = (uint32_t)page < (uint32_t)a.n_pages ? 0xffffu : 0u;
+      if (valid) load_page((int64_t)page * a.c_page + (int64_t)slot * a.c_slot, other);
+      else load(-1, other);
+      page = page_of(min(base + 2 * kKeys + wave * 16, it.ke - 1), &slot);
+      work(std::false_type{}, base, mine, fl);
+    };
+    for (; base + 2 * kKeys - 1 <= lim0 && base + 3 * kKeys <= it.ke; base += 2 * kKeys) {
+      turn(base, tile0, tile1, flags);
+      turn(base + kKeys, tile1, tile0, flags + 4);
+    }
+  }
   int64_t off = -1;
   AttnKey next{0, -1};
-  if (it.kb < it.ke) {
-    off = attn_offset(a, attn_key(a, trow, it.kb + wave * 16 + (lane & 15), it.ke));
-    next = attn_key(a, trow, it.kb + kKeys + wave * 16 + (lane & 15), it.ke);
+  if (base < it.ke) {
+    off = attn_offset(a, attn_key(a, trow, base + wave * 16 + (lane & 15), it.ke));
+    next = attn_key(a, trow, base + kKeys + wave * 16 + (lane & 15), it.ke);
   }
-  auto turn = [&](auto may_edge, int base, uint16_t* mine, uint16_t* other, uint32_t* fl) {
+  auto turn = [&](int base, uint16_t* mine, uint16_t* other, uint32_t* fl) {
     const uint32_t valid = (uint32_t)__ballot(off >= 0) & 0xffffu;
     if (lane == 0) fl[wave] = valid;
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
@@ -746,19 +785,12 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
     off = attn_offset(a, next);
     next = attn_key(a, trow, base + 2 * kKeys + wave * 16 + (lane & 15), it.ke);
     if (base + kKeys < it.ke) load(off, other);
-    work(may_edge, base, mine, fl);
+    work(std::true_type{}, base, mine, fl);
   };
-  if (it.kb < it.ke) load(off, tile0);
-  // pairs of tiles that every row sees, then the others (apart, so that the first loop keeps its registers to itself)
-  int base = it.kb;
-  for (; base + 2 * kKeys - 1 <= lim0 && base + kKeys < it.ke; base += 2 * kKeys) {
-    turn(std::false_type{}, base, tile0, tile1, flags);
-    turn(std::false_type{}, base + kKeys, tile1, tile0, flags + 4);
-  }
 #pragma unroll 1
   for (; base < it.ke; base += 2 * kKeys) {
-    turn(std::true_type{}, base, tile0, tile1, flags);
-    if (base + kKeys < it.ke) turn(std::true_type{}, base + kKeys, tile1, tile0, flags + 4);
+    turn(base, tile0, tile1, flags);
+    if (base + kKeys < it.ke) turn(base + kKeys, tile1, tile0, flags + 4);
   }
   l += __shfl_xor(l, 32, kWaveSize);
   if (p >= rows) return;  // (no barrier below)

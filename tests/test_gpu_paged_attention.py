@@ -211,6 +211,25 @@ def test_large_scores_and_scale(K, dt):
     near(run(K, b, scale=0.01), *expected(b, 0.01))
 
 
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("new", [1, 9, 150])
+def test_many_small_weights(K, dt, new):
+    """One token of great weight and thousands whose weights, 2^-15 of it each, come to as much together: they count, and so does
+    their sum."""
+    b = batch(dt, [(new, 50000)], 4, 1, 64, 16, seed=6)
+    b["q"].zero_()
+    b["q"][..., 0] = 8.0
+    b["kc"].zero_()
+    b["vc"].copy_(torch.where(b["vc"] > 0, 1.0, 0.5))
+    page, at = int(b["table"][0, 700]), 5
+    b["kc"][page, 0, at, 0] = 8.0
+    b["vc"][page, 0, at] = 4.0
+    scale = 15 * math.log(2) / 64
+    want, bound = expected(b, scale)
+    assert 1.5 < float(want[0, 0, 0]) < 3.5  # (neither the one nor the others alone)
+    near(run(K, b, scale=scale), want, bound)
+
+
 def test_strided_tensors(K):
     b = batch("bf16", [(1, 70), (60, 30)], 4, 2, 64, 16)
     want = run(K, b)
