@@ -14,6 +14,7 @@
 // grows with tokens or page contents runs in a second launch that has the card.
 #pragma once
 #include "smlm_common.hpp"
+#include "wave_scan.hpp"
 
 namespace smlm {
 
@@ -22,11 +23,7 @@ constexpr int kKvThreads = 1024;
 // inclusive sum over the workgroup's 1024 threads; `total` gets the sum of all
 __device__ __forceinline__ int kv_scan(int v, int* wave_tot, int& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < kWaveSize; d *= 2) {
-    const int u = __shfl_up(v, d, kWaveSize);
-    if (lane >= d) v += u;
-  }
+  v = wave_scan(v);
   __syncthreads();  // earlier readers of wave_tot are done
   if (lane == 63) wave_tot[wave] = v;
   __syncthreads();
@@ -72,6 +69,28 @@ __device__ __forceinline__ int kv_take_free(const int* refs, int N, int want, in
   return found < want ? found : want;
 }
 
+// Marks, for each request of `list` (K entries), the first entry that names it; entry i is alone or first where kv_first gives i.
+// In LDS where the requests' rows fit, else in scratch memory (two trips to L2 and back: 3 us).
+constexpr int kKvOwners = 8192;
+__device__ __forceinline__ void kv_mark(const int* list, int K, int R, int* owner, int* owner_s) {
+  const bool local = R <= kKvOwners;
+  for (int i = threadIdx.x; i < K; i += kKvThreads) {
+    const int r = list[i];
+    if (r < 0 || r >= R) continue;
+    if (local) owner_s[r] = 0x7fffffff;
+    else kv_store(owner + r, 0x7fffffff);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < K; i += kKvThreads) {
+    const int r = list[i];
+    if (r >= 0 && r < R) atomicMin((local ? owner_s : owner) + r, i);
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ int kv_first(int r, int R, const int* owner, const int* owner_s) {
+  return R <= kKvOwners ? owner_s[r] : kv_load(owner + r);
+}
+
 struct KvExtendArgs {
   int *table, *length, *refs, *status;
   const int *requests, *counts;  // [S]; a request below 0 is skipped
@@ -85,19 +104,11 @@ struct KvExtendArgs {
 // One workgroup: counts, checks, takes the pages and writes the step's tables by sequence.  q_indptr doubles as the counts' running sum.
 __global__ __launch_bounds__(kKvThreads) void kv_extend_kernel(KvExtendArgs a) {
   __shared__ int wave_tot[16];
+  __shared__ int owner_s[kKvOwners];
   __shared__ int bad;
   const int tid = threadIdx.x;
   if (tid == 0) bad = 0;
-  for (int i = tid; i < a.S; i += kKvThreads) {
-    const int r = a.requests[i];
-    if (r >= 0 && r < a.R) kv_store(a.owner + r, 0x7fffffff);
-  }
-  __syncthreads();
-  for (int i = tid; i < a.S; i += kKvThreads) {
-    const int r = a.requests[i];
-    if (r >= 0 && r < a.R) atomicMin(a.owner + r, i);
-  }
-  __syncthreads();
+  kv_mark(a.requests, a.S, a.R, a.owner, owner_s);
   int rows = 0, pages = 0;
   for (int base = 0; base < a.S; base += kKvThreads) {
     const int i = base + tid;
@@ -108,7 +119,7 @@ __global__ __launch_bounds__(kKvThreads) void kv_extend_kernel(KvExtendArgs a) {
       if (r >= a.R || n < 0) {
         err = SMLM_KV_BAD_REQUEST;
       } else if (r >= 0) {
-        if (kv_load(a.owner + r) != i) err = SMLM_KV_BAD_REQUEST;
+        if (kv_first(r, a.R, a.owner, owner_s) != i) err = SMLM_KV_BAD_REQUEST;
         const int64_t old = a.length[r], now = old + n;
         const int64_t had = (old + a.P - 1) / a.P, has = (now + a.P - 1) / a.P;
         if (has > a.M || old < 0) err |= SMLM_KV_TOO_LONG;
@@ -275,19 +286,11 @@ struct KvForkArgs {
 
 __global__ __launch_bounds__(kKvThreads) void kv_fork_kernel(KvForkArgs a) {
   __shared__ int wave_tot[16];
+  __shared__ int owner_s[kKvOwners];
   __shared__ int bad;
   const int tid = threadIdx.x, P = a.pool.P;
   if (tid == 0) bad = 0;
-  for (int i = tid; i < a.K; i += kKvThreads) {
-    const int c = a.children[i];
-    if (c >= 0 && c < a.R) kv_store(a.owner + c, 0x7fffffff);
-  }
-  __syncthreads();
-  for (int i = tid; i < a.K; i += kKvThreads) {
-    const int c = a.children[i];
-    if (c >= 0 && c < a.R) atomicMin(a.owner + c, i);
-  }
-  __syncthreads();
+  kv_mark(a.children, a.K, a.R, a.owner, owner_s);
   int pages = 0;
   for (int base = 0; base < a.K; base += kKvThreads) {
     const int i = base + tid;
@@ -295,7 +298,7 @@ __global__ __launch_bounds__(kKvThreads) void kv_fork_kernel(KvForkArgs a) {
     if (i < a.K) {
       const int p = a.parents[i], c = a.children[i];
       if (c >= 0) {
-        if (p < 0 || p >= a.R || c >= a.R || kv_load(a.owner + c) != i || a.length[c] != 0) {
+        if (p < 0 || p >= a.R || c >= a.R || kv_first(c, a.R, a.owner, owner_s) != i || a.length[c] != 0) {
           err = SMLM_KV_BAD_REQUEST;
         } else {
           n = a.length[p];

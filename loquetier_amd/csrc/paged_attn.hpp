@@ -24,6 +24,7 @@
 #include <type_traits>
 
 #include "smlm_common.hpp"
+#include "wave_scan.hpp"
 
 namespace smlm {
 
@@ -113,29 +114,6 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnPlanArgs& a, int s) {
 
 constexpr int kAttnPlanThreads = 1024;
 
-// Inclusive sums over a wave: shifts inside rows of 16 lanes, then the rows' totals.
-#define SMLM_DPP(x, ctrl, rmask) __builtin_amdgcn_update_dpp(0, x, ctrl, rmask, 0xf, false)
-__device__ __forceinline__ int attn_wave_scan(int v) {
-  v += SMLM_DPP(v, 0x111, 0xf);  // row_shr:1
-  v += SMLM_DPP(v, 0x112, 0xf);
-  v += SMLM_DPP(v, 0x114, 0xf);
-  v += SMLM_DPP(v, 0x118, 0xf);
-  v += SMLM_DPP(v, 0x142, 0xa);  // row_bcast:15 into rows 1 and 3
-  v += SMLM_DPP(v, 0x143, 0xc);  // row_bcast:31 into rows 2 and 3
-  return v;
-}
-__device__ __forceinline__ float attn_wave_sum(float v) {
-  auto add = [&](int moved) { v += __builtin_bit_cast(float, moved); };
-  add(SMLM_DPP(__builtin_bit_cast(int, v), 0x111, 0xf));
-  add(SMLM_DPP(__builtin_bit_cast(int, v), 0x112, 0xf));
-  add(SMLM_DPP(__builtin_bit_cast(int, v), 0x114, 0xf));
-  add(SMLM_DPP(__builtin_bit_cast(int, v), 0x118, 0xf));
-  add(SMLM_DPP(__builtin_bit_cast(int, v), 0x142, 0xa));
-  add(SMLM_DPP(__builtin_bit_cast(int, v), 0x143, 0xc));
-  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
-}
-#undef SMLM_DPP
-
 constexpr int kAttnPlanLds = kAttnPlanThreads;  // up to here the sequences stay in LDS: every read of memory is most of a microsecond
 
 // The number of parts that a tile of the card's average length is cut into, for n tiles (times kv heads): as many as leave the
@@ -173,7 +151,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
     n_big_f += small ? 0.0f : (float)q.tiles;
     if (local) seq_s[s] = q;
   }
-  keys[0] = attn_wave_sum(keys[0]), keys[1] = attn_wave_sum(keys[1]), n_big_f = attn_wave_sum(n_big_f);
+  keys[0] = wave_total(keys[0]), keys[1] = wave_total(keys[1]), n_big_f = wave_total(n_big_f);
   if (lane == 0) red[0][wave] = keys[0], red[1][wave] = keys[1], red[2][wave] = n_big_f;
   __syncthreads();
   keys[0] = keys[1] = n_big_f = 0.0f;
@@ -205,7 +183,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
     __syncthreads();  // the last turn's sums have been read
 #pragma unroll
     for (int i = 0; i < 5; ++i) {
-      v[i] = attn_wave_scan(n[i]);
+      v[i] = wave_scan(n[i]);
       if (lane == 63) wave_tot[wave][i] = v[i];
     }
     __syncthreads();
