@@ -404,7 +404,7 @@ SMLM_API int smlm_paged_attn(const smlm_heads* out, const smlm_heads* q, const v
   a.table = table;
   a.o_row = out->row_stride, a.o_head = out->head_stride, a.q_row = q->row_stride, a.q_head = q->head_stride;
   a.c_page = page_stride, a.c_head = head_stride, a.c_slot = slot_stride;
-  a.M = M, a.n_pages = n_pages, a.P = page_size, a.T = T, a.Hq = q_heads, a.Hkv = kv_heads, a.g = g;
+  a.M = M, a.most = M * page_size, a.n_pages = n_pages, a.P = page_size, a.T = T, a.Hq = q_heads, a.Hkv = kv_heads, a.g = g;
   // x / P = (floor(x m / 2^32) + x) >> s for x < 2^32, with s = ceil(log2 P), m = floor(2^32 (2^s - P) / P) + 1
   // (Granlund and Montgomery, Division by Invariant Integers using Multiplication, 1994)
   while ((int64_t)1 << a.div_shift < page_size) ++a.div_shift;

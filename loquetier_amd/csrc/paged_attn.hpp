@@ -54,7 +54,7 @@ struct AttnJoin {   // a tile whose keys were cut
   int pad[3];
 };
 struct AttnPlanView {
-  int* hdr;          // [16]: 0 items, 1 joins
+  int* hdr;          // [16]: 0 items, 1 joins, 2 tokens that a row of the table holds
   int* start;        // [4][S + 1] running sums by sequence: items with few rows, other items, joins, parts
   AttnItem* items;
   AttnJoin* joins;
@@ -214,6 +214,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
     first_s[0][0] = first_s[1][0] = start[0] = start[a.S + 1] = 0;
     a.plan.hdr[0] = items;
     a.plan.hdr[1] = at[2] < a.joins_max ? at[2] : a.joins_max;
+    a.plan.hdr[2] = a.most;
   }
   __syncthreads();
   // Items with few rows stream, the others compute: they take turns, so that both have the card together (mixed batch of four prompts
@@ -233,8 +234,8 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
     const AttnSeq q = local ? seq_s[lo] : attn_seq(a, lo);
     const int first = local ? first_l[lo] : first_g[lo], end = local ? first_l[lo + 1] : first_g[lo + 1];
     const int join = local ? join_s[lo] : start[2 * (a.S + 1) + lo], part = local ? part_s[lo] : start[3 * (a.S + 1) + lo];
-    const uint32_t ns = (uint32_t)(end - first) / (uint32_t)q.tiles, k = (uint32_t)(x - first);
-    const int t = q.tiles - 1 - (int)(k / ns), j = (int)(k % ns);  // (the later tiles of a prompt see more keys: they go first)
+    const uint32_t ns = max(1u, (uint32_t)(end - first) / (uint32_t)max(1, q.tiles)), k = (uint32_t)(x - first);
+    const int t = max(0, q.tiles - 1 - (int)(k / ns)), j = (int)(k % ns);  // (the later tiles of a prompt see more keys: they go first)
     AttnItem it;
     it.row0 = q.row0, it.n = q.n, it.len = q.len, it.trow = q.trow, it.first = t * q.tile;
     const int last = min(it.first + q.tile, q.n * a.g) - 1;
@@ -263,6 +264,7 @@ struct AttnArgs {
   float *pm_small, *pm_big;  // [part][kv head][tile row][2]: maximum (of the scores times scale / log 2), sum
   int64_t o_row, o_head, q_row, q_head, c_page, c_head, c_slot;
   int M, n_pages, P, T, Hq, Hkv, g;
+  int most;                  // M * P: the plan has to be for as many
   uint32_t div_mul;          // division by P: ((x * div_mul >> 32) + x) >> div_shift in 33 bits
   int div_shift;
   int whole;                 // sixteen keys from a multiple of sixteen on lie in one page
@@ -798,7 +800,7 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
   __shared__ __align__(16) uint16_t lds[2 * 64 * D], more[2 * 64 * D];
   __shared__ uint32_t side[128];
   const int i = (int)blockIdx.x / a.Hkv, kvh = (int)blockIdx.x - i * a.Hkv;
-  if (i >= a.plan.hdr[0]) return;
+  if (i >= a.plan.hdr[0] || a.plan.hdr[2] != a.most) return;
   const AttnItem it = a.plan.items[i];
   const int rows = it.n * a.g;
   if (rows > kAttnSmallRows) attn_big<DT, D>(a, it, kvh, lds, more, side);
@@ -816,7 +818,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   __shared__ float sum_s[kGroups], top_s[kGroups];
   const int x = (int)blockIdx.x / kAttnJoinShares, share = (int)blockIdx.x % kAttnJoinShares;
   const int i = x / a.Hkv, kvh = x - i * a.Hkv;
-  if (i >= a.plan.hdr[1]) return;
+  if (i >= a.plan.hdr[1] || a.plan.hdr[2] != a.most) return;
   const AttnJoin jn = a.plan.joins[i];
   const int rows = jn.n * a.g;
   const bool small = rows <= kAttnSmallRows;

@@ -83,9 +83,9 @@ class PagedKvCache:
         k_cache, v_cache = self.layer(layer)
         q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         kernel.qk_norm_rope(q_out, None, q, k, table, step.positions, q_weight, k_weight, eps, v, k_cache, v_cache, step.slots)
-        out = torch.zeros_like(q_out) if plan.T else q_out
-        kernel.paged_attention(out, q_out, k_cache, v_cache, plan, scale, self.workspace)
-        return out
+        # in place: rows of no sequence have no position, so their queries are zero, and stay
+        kernel.paged_attention(q_out, q_out, k_cache, v_cache, plan, scale, self.workspace)
+        return q_out
 
     def check(self) -> None:
         """Raises where a call since the last check was refused (waits for the GPU)."""

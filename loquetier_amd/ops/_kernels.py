@@ -1260,7 +1260,7 @@ def paged_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v
                     scale: Optional[float] = None, workspace: Optional[Workspace] = None) -> None:
     """Causal attention of the batch's rows q [rows, q_heads, head_dim] over the pages of k_cache and v_cache [n_pages, kv_heads,
     page_size, head_dim] (any strides), prompts' chunks and single tokens in one call.  scale: head_dim ** -0.5 by default.
-    Rows that see no token become zero; rows of no sequence are left as they were."""
+    Rows that see no token become zero; rows of no sequence are left as they were.  out may be q."""
     if _host().paged_attention(out, q, k_cache, v_cache, plan, scale, workspace):
         return
     _check_heads(q, "q")

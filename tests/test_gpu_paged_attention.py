@@ -261,6 +261,42 @@ def test_same_bits_again(K):
         assert torch.equal(run(K, b), first)
 
 
+def test_in_place(K):
+    for seqs in ([(1, 9000)] * 2, [(1, 50), (300, 2000), (20, 7), (3, 0)]):
+        b = batch("bf16", seqs, 8, 2, 128, 16, seed=11)
+        want = run(K, b)
+        q = b["q"].clone()
+        assert torch.equal(run(K, dict(b, q=q), out=q), want)
+
+
+@pytest.mark.parametrize("g", [1, 4])
+def test_more_sequences_than_the_plan_keeps_in_lds(K, g):
+    import random
+    r = random.Random(g)
+    seqs = [(r.choice([0, 1, 1, 1, 2, 5, 40]), r.choice([0, 1, 30, 200, 900])) for _ in range(1500)]
+    b = batch("fp16", seqs, g, 1, 64, 16, seed=12)
+    near(run(K, b), *expected(b))
+
+
+def test_a_plan_for_another_table_does_nothing(K):
+    b = batch("bf16", [(1, 400), (200, 500)], 4, 2, 64, 16)
+    plan = K.AttentionPlan(b["indptr"], b["lens"], b["table"], b["T"], 4, 2, 16)
+    plan.page_table = b["table"][:, :3].contiguous()
+    out = torch.full_like(b["q"], 5.0)
+    K.paged_attention(out, b["q"], b["kc"], b["vc"], plan)
+    assert bool((out == 5).all())
+
+
+def test_sequences_that_overlap_stay_in_bounds(K):
+    """Row ranges that decrease, overlap or leave the batch break the contract; what is written stays within the batch's rows."""
+    b = batch("bf16", [(1, 400), (200, 2500), (1, 3)], 4, 2, 64, 16, after=3)
+    for indptr in ([0, 190, 10, 204], [0, 204, 0, 204], [-5, 300, 9, 400], [204, 1, 204, 0]):
+        out = torch.full((b["T"] + 2, 4, 64), 9.0, dtype=torch.bfloat16, device="cuda")
+        c = dict(b, indptr=torch.tensor(indptr, dtype=torch.int32).cuda())
+        run(K, c, out=out[1:-1])
+        assert bool((out[0] == 9).all()) and bool((out[-1] == 9).all())
+
+
 def test_empty_batches(K):
     b = batch("bf16", [(0, 5), (0, 0)], 4, 2, 64, 16, after=4)
     assert bool((run(K, b, fill=2.0) == 2).all())
