@@ -135,7 +135,8 @@ template <int DT, int D>
 int launch_attn(const AttnArgs& a, int items, int joins, hipStream_t st) {
   const int rc = launch(attn_kernel<DT, D>, dim3((unsigned)items * a.Hkv), dim3(256), st, a);
   if (rc || joins == 0) return rc;
-  return launch(attn_join_kernel<DT, D>, dim3((unsigned)joins * a.Hkv * kAttnJoinShares), dim3(256), st, a);
+  const int64_t work = (int64_t)joins * a.Hkv;
+  return launch(attn_join_kernel<DT, D>, dim3((unsigned)(work < kAttnJoinBlocks ? work : kAttnJoinBlocks)), dim3(256), st, a);
 }
 
 }  // namespace
@@ -362,7 +363,7 @@ SMLM_API int smlm_attn_plan_build(void* plan, size_t plan_bytes, const int32_t* 
   a.parts_small_max = attn_parts_max(kv_heads, kAttnSmallItems);
   a.parts_big_max = attn_parts_max(kv_heads, kAttnBigItems);
   // (fewer waves, fewer to wait for at a barrier)
-  return launch(attn_plan_kernel, dim3(1), dim3(S <= 256 ? 256 : kAttnPlanThreads), (hipStream_t)stream, a);
+  return launch(attn_plan_kernel, dim3(1), dim3(S <= 256 ? 512 : kAttnPlanThreads), (hipStream_t)stream, a);
 }
 
 SMLM_API int smlm_paged_attn_workspace_size(int T, int S, int M, int page_size, int q_heads, int kv_heads, int head_dim,
@@ -409,7 +410,8 @@ SMLM_API int smlm_paged_attn(const smlm_heads* out, const smlm_heads* q, const v
   // (Granlund and Montgomery, Division by Invariant Integers using Multiplication, 1994)
   while ((int64_t)1 << a.div_shift < page_size) ++a.div_shift;
   a.div_mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << a.div_shift) - page_size)) / page_size + 1);
-  a.whole = page_size % 16 == 0 && slot_stride >= 0 && slot_stride < (1 << 24);
+  const int load_rows = 512 / head_dim;
+  a.whole = slot_stride < 0 || slot_stride >= (1 << 24) ? 0 : (page_size % 16 == 0 ? 16 : (page_size % load_rows == 0 ? load_rows : 0));
   a.scale = scale * 1.4426950408889634f;
   const int items = attn_items_max(T, S, g, kv_heads), joins = cuts ? attn_joins_max(T, S, g, kv_heads) : 0;
   hipStream_t st = (hipStream_t)stream;

@@ -42,6 +42,7 @@ constexpr int kAttnBigRows = 128;    // tile rows of a workgroup of the other
 constexpr int kAttnSlots = 512;      // workgroups on the card at a time: two a CU
 constexpr int kAttnSmallItems = 2048, kAttnBigItems = 1024;  // workgroups over the card that tiles are cut for, at most
 constexpr int kAttnMinKeys = 256;    // keys of a part, at least
+constexpr int kAttnManyParts = 16;   // parts of a tile from which the threads of a join share them out
 
 struct AttnItem {   // a tile of a sequence and a part of its keys
   int row0, n, len, trow;  // the sequence: first row, rows, tokens, row of the page table
@@ -49,9 +50,11 @@ struct AttnItem {   // a tile of a sequence and a part of its keys
   int kb, ke;              // keys
   int part;                // where its part of the result goes, or -1: it is the whole
 };
-struct AttnJoin {   // a tile whose keys were cut
-  int row0, n, first, part, parts;
-  int pad[3];
+struct AttnJoin {   // rows of a tile whose keys were cut
+  int row0, first;         // the sequence's first row, the tile's first row
+  int big;                 // a tile of many rows
+  int part, parts;         // its parts
+  int from, step, rows;    // its rows from, from + step, ... below rows (eight at each, or one where the parts are many)
 };
 struct AttnPlanView {
   int* hdr;          // [16]: 0 items, 1 joins, 2 tokens that a row of the table holds
@@ -62,9 +65,10 @@ struct AttnPlanView {
 
 inline int attn_tiles_max(int T, int S, int g) { return (int)((int64_t)T * g / kAttnBigRows) + S; }
 inline int attn_items_max(int T, int S, int g, int Hkv) { return attn_tiles_max(T, S, g) + (kAttnSmallItems + kAttnBigItems) / Hkv + 2; }
+// (a tile's rows are joined by at most rows / 8 workgroups, or by eight where its parts are 16 and more)
 inline int attn_joins_max(int T, int S, int g, int Hkv) {
-  const int cut = (kAttnSmallItems + kAttnBigItems) / Hkv + 2, tiles = attn_tiles_max(T, S, g);
-  return cut < tiles ? cut : tiles;
+  const int64_t cut = (4 * kAttnSmallItems + 16 * kAttnBigItems) / Hkv + 16, tiles = (int64_t)attn_tiles_max(T, S, g) * 16;
+  return (int)(cut < tiles ? cut : tiles);
 }
 // (a tile of x times the cut's keys has round(x) parts, which is more than one from x = 1.5 on: at most 4 x / 3)
 inline int attn_parts_max(int Hkv, int items) { return 4 * (items / Hkv + 1) / 3 + 1; }
@@ -113,6 +117,12 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnPlanArgs& a, int s) {
 }
 
 constexpr int kAttnPlanThreads = 1024;
+
+// workgroups that share the join of one of a sequence's tiles
+__device__ __forceinline__ int attn_shares(const AttnSeq& q, int parts, int g) {
+  const int rows = min(q.tile, q.n * g);
+  return q.tile == kAttnSmallRows && parts >= kAttnManyParts ? min(8, rows) : (rows + 7) / 8;
+}
 
 constexpr int kAttnPlanLds = kAttnPlanThreads;  // up to here the sequences stay in LDS: every read of memory is most of a microsecond
 
@@ -177,7 +187,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
       const uint32_t cut = (uint32_t)(small ? cut_small : cut_big), ns = max(1u, ((uint32_t)q.len + cut / 2) / cut);
       const int items = q.tiles * (int)ns, parts = ns > 1 ? items : 0;
       n[0] = small ? items : 0, n[1] = small ? 0 : items;
-      n[2] = ns > 1 ? q.tiles : 0;
+      n[2] = ns > 1 ? q.tiles * attn_shares(q, (int)ns, a.g) : 0;
       n[3] = small ? parts : 0, n[4] = small ? 0 : parts;
     }
     __syncthreads();  // the last turn's sums have been read
@@ -243,14 +253,18 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
     const int64_t step = (int64_t)((seen + ns - 1) / ns + 63) / 64 * 64;
     it.kb = (int)min((int64_t)seen, j * step);
     it.ke = (int)min((int64_t)seen, (j + 1) * step);
-    it.part = ns > 1 ? part + t * (int)ns + j : -1;
+    const int part0 = part + t * (int)ns, parts_max = kind ? a.parts_big_max : a.parts_small_max;
+    it.part = ns > 1 ? part0 + j : -1;
     // (sequences that overlap, which none should, could come to more parts than there is room for)
-    const int parts_max = q.tile == kAttnSmallRows ? a.parts_small_max : a.parts_big_max;
-    const bool fits = it.part < parts_max;
+    const bool fits = ns == 1 || part0 + (int)ns <= parts_max;
     if (!fits) it.n = 0, it.kb = it.ke = 0, it.part = -1;
     a.plan.items[i] = it;
-    if (ns > 1 && j == 0 && join + t < a.joins_max)
-      a.plan.joins[join + t] = AttnJoin{q.row0, fits && it.part + (int)ns <= parts_max ? q.n : 0, it.first, it.part, (int)ns, {0, 0, 0}};
+    if (ns > 1) {
+      const int shares = attn_shares(q, (int)ns, a.g), by = kind || ns < kAttnManyParts ? 8 : 1;
+      const int rows = fits ? min(q.tile, q.n * a.g - it.first) : 0;
+      for (int h = j; h < shares && join + t * shares + h < a.joins_max; h += (int)ns)
+        a.plan.joins[join + t * shares + h] = AttnJoin{q.row0, it.first, kind, part0, (int)ns, h * by, shares * by, rows};
+    }
   }
 }
 
@@ -267,7 +281,7 @@ struct AttnArgs {
   int most;                  // M * P: the plan has to be for as many
   uint32_t div_mul;          // division by P: ((x * div_mul >> 32) + x) >> div_shift in 33 bits
   int div_shift;
-  int whole;                 // sixteen keys from a multiple of sixteen on lie in one page
+  int whole;                 // keys from a multiple of it on, as many, that lie in one page: 16, the rows of a load, or 0
   float scale;               // times log2 e
 };
 
@@ -560,6 +574,7 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
   const uint16_t *kp = a.k + (int64_t)kvh * a.c_head, *vp = a.v + (int64_t)kvh * a.c_head;
   const u32x4 zero4 = {0u, 0u, 0u, 0u};
 
+  const bool busy = it.first + wave * 32 < rows;  // (a wave without rows loads for the others)
   const int p = it.first + wave * 32 + c, pc = p < rows ? p : 0;
   const int lim = min(it.ke - 1, it.len - it.n + pc / a.g);
   const int lim0 = it.len - it.n + it.first / a.g;  // of the workgroup's first row
@@ -677,17 +692,7 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
         l = attn_add2<DT>(two, l);  // (the weights as V meets them: they add up to one whatever their rounding)
         pf[u][e >> 3][(e >> 1) & 3] = two;
       }
-    // a tile that some rows see in part: does its V hold a value that is no number?
-    bool guard = false;
-    if (edge) {
-      uint32_t odd = 0;
-#pragma unroll 1
-      for (int x = lane; x < kKeys * kRowLanes; x += kWaveSize) {
-        const u32x4 v = *(const u32x4*)(vl + x * 8);
-        odd |= attn_not_finite<DT>(v[0]) | attn_not_finite<DT>(v[1]) | attn_not_finite<DT>(v[2]) | attn_not_finite<DT>(v[3]);
-      }
-      guard = __ballot(odd != 0) != 0;
-    }
+    const bool guard = edge && ((fl[0] | fl[1] | fl[2] | fl[3]) >> 16) != 0;
     if (!guard) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -725,31 +730,64 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
   // whose place the next loads take.
   int base = it.kb;
   if (base < it.ke) load(attn_offset(a, attn_key(a, trow, base + wave * 16 + (lane & 15), it.ke)), tile0);
-  // Pairs of tiles that every row sees, each sixteen keys of them and of the tile after in one page: apart, so that this loop keeps its
-  // registers to itself.  What it loads, and whether a page is there, is known on the scalar side.
-  if (a.whole && base + 2 * kKeys - 1 <= lim0 && base + 3 * kKeys <= it.ke) {
-    auto page_of = [&](int key, int* slot) {
-      const int j = attn_div((uint32_t)key, a.div_mul, a.div_shift);
-      *slot = key - j * a.P;
-      return uload(trow, j);
+  // Pairs of tiles that every row sees, where the rows of a load lie in one page: apart, so that this loop keeps its registers to
+  // itself.  What it loads, and whether a page is there, is known on the scalar side: one page for a wave's sixteen keys, or one a load.
+  auto pairs = [&](auto sixteen) {  // (two loops: the test in one of them cost up to 5 percent)
+    constexpr uint32_t kAll = 0xffffu, kOne = (1u << kRowsLoad) - 1u;
+    int page[kLoads], slot[kLoads];
+    auto find = [&](int key) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        if (i && sixteen) break;
+        const int k = min(key + i * kRowsLoad, it.ke - 1), j = attn_div((uint32_t)k, a.div_mul, a.div_shift);
+        slot[i] = k - j * a.P;
+        page[i] = uload(trow, j);
+      }
     };
-    int slot, page = page_of(base + wave * 16, &slot);
-    uint32_t valid = (uint32_t)page < (uint32_t)a.n_pages ? 0xffffu : 0u;
-    page = page_of(base + kKeys + wave * 16, &slot);
+    auto fetch = [&](uint16_t* tile) -> uint32_t {  // the keys that are there
+      if (sixteen) {
+        const bool there = (uint32_t)page[0] < (uint32_t)a.n_pages;
+        if (there) load_page((int64_t)page[0] * a.c_page + (int64_t)slot[0] * a.c_slot, tile);
+        else load(-1, tile);
+        return there ? kAll : 0u;
+      }
+      uint32_t keys = 0;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const bool there = (uint32_t)page[i] < (uint32_t)a.n_pages;
+        const int64_t first = (int64_t)page[i] * a.c_page + (int64_t)slot[i] * a.c_slot;
+        const gptr zero = (gptr)(const void*)attn_zeros;
+        uint16_t* dst = tile + (wave * 16 + i * kRowsLoad) * D;
+        to_lds(there ? (gptr)(kp + first) + kof[i] : zero, dst);
+        to_lds(there ? (gptr)(vp + first) + vof[i % kTurnsV] : zero, dst + kKeys * D);
+        keys |= there ? kOne << (i * kRowsLoad) : 0u;
+      }
+      return keys;
+    };
+    find(base + wave * 16);
+    uint32_t valid = 0;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      if (i && sixteen) break;
+      if ((uint32_t)page[i] < (uint32_t)a.n_pages) valid |= sixteen ? kAll : kOne << (i * kRowsLoad);
+    }
+    find(base + kKeys + wave * 16);
     auto turn = [&](int base, uint16_t* mine, uint16_t* other, uint32_t* fl) {
       if (lane == 0) fl[wave] = valid;
       __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
       __syncthreads();
-      valid = (uint32_t)page < (uint32_t)a.n_pages ? 0xffffu : 0u;
-      if (valid) load_page((int64_t)page * a.c_page + (int64_t)slot * a.c_slot, other);
-      else load(-1, other);
-      page = page_of(min(base + 2 * kKeys + wave * 16, it.ke - 1), &slot);
-      work(std::false_type{}, base, mine, fl);
+      valid = fetch(other);
+      find(base + 2 * kKeys + wave * 16);
+      if (busy) work(std::false_type{}, base, mine, fl);
     };
     for (; base + 2 * kKeys - 1 <= lim0 && base + 3 * kKeys <= it.ke; base += 2 * kKeys) {
       turn(base, tile0, tile1, flags);
       turn(base + kKeys, tile1, tile0, flags + 4);
     }
+  };
+  if (base + 2 * kKeys - 1 <= lim0 && base + 3 * kKeys <= it.ke) {
+    if (a.whole == 16) pairs(std::true_type{});
+    else if (a.whole) pairs(std::false_type{});
   }
   int64_t off = -1;
   AttnKey next{0, -1};
@@ -759,13 +797,24 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
   }
   auto turn = [&](int base, uint16_t* mine, uint16_t* other, uint32_t* fl) {
     const uint32_t valid = (uint32_t)__ballot(off >= 0) & 0xffffu;
-    if (lane == 0) fl[wave] = valid;
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    // a tile that some rows see in part: does V, of the keys that this wave loaded, hold a value that is no number?
+    uint32_t odd = 0;
+    if (base + kKeys - 1 > lim0) {
+      const uint16_t* own = mine + (kKeys + wave * 16) * D + lane * 8;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const u32x4 v = *(const u32x4*)(own + i * kRowsLoad * D);
+        odd |= attn_not_finite<DT>(v[0]) | attn_not_finite<DT>(v[1]) | attn_not_finite<DT>(v[2]) | attn_not_finite<DT>(v[3]);
+      }
+    }
+    const uint32_t any_odd = __ballot(odd != 0) != 0 ? 0x10000u : 0u;
+    if (lane == 0) fl[wave] = valid | any_odd;
     __syncthreads();
     off = attn_offset(a, next);
     next = attn_key(a, trow, base + 2 * kKeys + wave * 16 + (lane & 15), it.ke);
     if (base + kKeys < it.ke) load(off, other);
-    work(std::true_type{}, base, mine, fl);
+    if (busy) work(std::true_type{}, base, mine, fl);
   };
 #pragma unroll 1
   for (; base < it.ke; base += 2 * kKeys) {
@@ -810,79 +859,78 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
 
 // The parts of a tile's rows, each weighed by its maximum against the largest.  A thread takes four dimensions of a row and, where the parts
 // are many, every eighth of them; the eight are then added in order.
-constexpr int kAttnJoinShares = 4;  // workgroups that share a tile's rows
+constexpr int kAttnJoinBlocks = 2048;  // workgroups of the join (the host knows a bound of the joins only, and workgroups without work cost too)
 template <int DT, int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;  // threads a row; rows, or shares of the parts, at a time
   __shared__ f32x4 acc_s[kGroups][kLanes];
   __shared__ float sum_s[kGroups], top_s[kGroups];
-  const int x = (int)blockIdx.x / kAttnJoinShares, share = (int)blockIdx.x % kAttnJoinShares;
-  const int i = x / a.Hkv, kvh = x - i * a.Hkv;
-  if (i >= a.plan.hdr[1] || a.plan.hdr[2] != a.most) return;
-  const AttnJoin jn = a.plan.joins[i];
-  const int rows = jn.n * a.g;
-  const bool small = rows <= kAttnSmallRows;
-  const int tile = small ? kAttnSmallRows : kAttnBigRows;
-  const float *po = small ? a.po_small : a.po_big, *pm = small ? a.pm_small : a.pm_big;
-  AttnItem it;
-  it.row0 = jn.row0;
-  const int n = min(tile, rows - jn.first), lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
-  const int64_t step = (int64_t)a.Hkv * tile;
-  const bool many = jn.parts >= 2 * kGroups;
-  const int by = many ? kGroups : 1;
-  const int rows_turn = many ? 1 : kGroups;
-  for (int r0 = share * rows_turn; r0 < n; r0 += kAttnJoinShares * rows_turn) {
-    const int r = many ? r0 : min(r0 + grp, n - 1);
-    const int64_t at0 = ((int64_t)jn.part * a.Hkv + kvh) * tile + r;
-    // running maximum over this thread's parts, four on their way at a time
-    float top = -INFINITY, sum = 0.0f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int j = many ? grp : 0; j < jn.parts; j += 4 * by) {
-      float m[4], l[4];
-      f32x4 v[4];
+  if (a.plan.hdr[2] != a.most) return;
+  const int work = a.plan.hdr[1] * a.Hkv;
+  for (int w = blockIdx.x; w < work; w += gridDim.x) {
+    const int i = w / a.Hkv, kvh = w - i * a.Hkv;
+    const AttnJoin jn = a.plan.joins[i];
+    const int tile = jn.big ? kAttnBigRows : kAttnSmallRows;
+    const float *po = jn.big ? a.po_big : a.po_small, *pm = jn.big ? a.pm_big : a.pm_small;
+    AttnItem it;
+    it.row0 = jn.row0;
+    const int lane = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
+    const int64_t step = (int64_t)a.Hkv * tile;
+    const bool many = jn.parts >= kAttnManyParts && !jn.big;
+    const int by = many ? kGroups : 1;
+    for (int r0 = jn.from; r0 < jn.rows; r0 += jn.step) {
+      const int row = many ? r0 : r0 + grp, r = min(row, jn.rows - 1);
+      const int64_t at0 = ((int64_t)jn.part * a.Hkv + kvh) * tile + r;
+      // running maximum over this thread's parts, four on their way at a time
+      float top = -INFINITY, sum = 0.0f;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      for (int j = many ? grp : 0; j < jn.parts; j += 4 * by) {
+        float m[4], l[4];
+        f32x4 v[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int64_t at = at0 + (int64_t)min(j + u * by, jn.parts - 1) * step;
-        m[u] = j + u * by < jn.parts ? pm[at * 2] : -INFINITY;
-        l[u] = pm[at * 2 + 1];
-        v[u] = ldg_f4(po + at * D + lane * 4);
-      }
-      const float now = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top), ref = now == -INFINITY ? 0.0f : now;
-      const float old = attn_exp2(top - ref);
-      sum *= old;
-      acc *= old;
-      top = now;
+        for (int u = 0; u < 4; ++u) {
+          const int64_t at = at0 + (int64_t)min(j + u * by, jn.parts - 1) * step;
+          m[u] = j + u * by < jn.parts ? pm[at * 2] : -INFINITY;
+          l[u] = pm[at * 2 + 1];
+          v[u] = ldg_f4(po + at * D + lane * 4);
+        }
+        const float now = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), top), ref = now == -INFINITY ? 0.0f : now;
+        const float old = attn_exp2(top - ref);
+        sum *= old;
+        acc *= old;
+        top = now;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (j + u * by >= jn.parts) continue;
-        const float f = attn_exp2(m[u] - ref);
-        sum += f * l[u];
-        acc += f * v[u];
+        for (int u = 0; u < 4; ++u) {
+          if (j + u * by >= jn.parts) continue;
+          const float f = attn_exp2(m[u] - ref);
+          sum += f * l[u];
+          acc += f * v[u];
+        }
       }
+      if (many) {
+        __syncthreads();  // the last row's have been read
+        acc_s[grp][lane] = acc;
+        if (lane == 0) sum_s[grp] = sum, top_s[grp] = top;
+        __syncthreads();
+        if (grp != 0) continue;
+#pragma unroll
+        for (int w = 1; w < kGroups; ++w) top = fmaxf(top, top_s[w]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        sum = 0.0f;
+        acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kGroups; ++w) {
+          const float f = attn_exp2(top_s[w] - ref);
+          sum += f * sum_s[w];
+          acc += f * acc_s[w][lane];
+        }
+      } else if (grp >= 8 || row >= jn.rows) {
+        continue;
+      }
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      *(SMLM_GLOBAL u32x2*)(attn_out_row(a, it, kvh, jn.first + r) + lane * 4) =
+          attn_pack4<DT>(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
     }
-    if (many) {
-      __syncthreads();  // the last row's have been read
-      acc_s[grp][lane] = acc;
-      if (lane == 0) sum_s[grp] = sum, top_s[grp] = top;
-      __syncthreads();
-      if (grp != 0) continue;
-#pragma unroll
-      for (int w = 1; w < kGroups; ++w) top = fmaxf(top, top_s[w]);
-      const float ref = top == -INFINITY ? 0.0f : top;
-      sum = 0.0f;
-      acc = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < kGroups; ++w) {
-        const float f = attn_exp2(top_s[w] - ref);
-        sum += f * sum_s[w];
-        acc += f * acc_s[w][lane];
-      }
-    } else if (r0 + grp >= n) {
-      continue;
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    *(SMLM_GLOBAL u32x2*)(attn_out_row(a, it, kvh, jn.first + r) + lane * 4) =
-        attn_pack4<DT>(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
   }
 }
 
