@@ -198,7 +198,7 @@ PyObject* py_paged_attention(PyObject*, PyObject* const* p, Py_ssize_t n) {
     Py_RETURN_FALSE;
   double scale = p[5] == Py_None ? 1.0 / std::sqrt((double)q.size(2)) : PyFloat_AsDouble(p[5]);
   if (scale == -1.0 && PyErr_Occurred()) throw python_raised();
-  if (!(scale > 0.0) || !(scale < 3.0e38)) Py_RETURN_FALSE;
+  if (!(scale > 0.0) || !(scale < 1.0e38)) Py_RETURN_FALSE;
   const int D = (int)q.size(2), M = (int)table.size(1);
   size_t need = 0;
   check(lib.attn_size((int)T, (int)S, M, (int)P, (int)Hq, (int)Hkv, D, &need), "smlm_paged_attn_workspace_size");

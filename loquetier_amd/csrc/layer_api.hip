@@ -382,7 +382,7 @@ SMLM_API int smlm_paged_attn(const smlm_heads* out, const smlm_heads* q, const v
   if (int rc = attn_check(T, S, q_heads, kv_heads)) return rc;
   if (int rc = kv_check(R, M, n_pages < 0 ? -1 : 0, S, page_size)) return rc;
   if (int rc = check_dtype(dtype)) return rc;
-  if (!(scale > 0.0f) || scale > 3.0e38f) return SMLM_ERR_ARG;
+  if (!(scale > 0.0f) || scale > 1.0e38f) return SMLM_ERR_ARG;
   if (head_dim != 64 && head_dim != 128) return SMLM_ERR_LIMIT;
   if (T == 0 || S == 0) return SMLM_OK;
   if (!out || !q || !out->data || !q->data || !plan || (n_pages > 0 && (!k_cache || !v_cache)) || (R > 0 && M > 0 && !table))

@@ -852,6 +852,7 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
   if (i >= a.plan.hdr[0] || a.plan.hdr[2] != a.most) return;
   const AttnItem it = a.plan.items[i];
   const int rows = it.n * a.g;
+  if (rows <= 0) return;
   if (rows > kAttnSmallRows) attn_big<DT, D>(a, it, kvh, lds, more, side);
   else if (rows > 16) attn_small<DT, D, 2>(a, it, kvh, lds, reinterpret_cast<float*>(side));
   else attn_small<DT, D, 1>(a, it, kvh, lds, reinterpret_cast<float*>(side));

@@ -120,7 +120,7 @@ __global__ __launch_bounds__(256) void qk_rope_kernel(QkRopeArgs a) {
     if (a.wq) wq[0] = ldg16(a.wq + c0), wq[1] = ldg16(a.wq + c1);
     if (a.wk) wk[0] = ldg16(a.wk + c0), wk[1] = ldg16(a.wk + c1);
   }
-  const bool keep = slot >= 0 && slot < a.n_slots;
+  const bool keep = slot >= 0 && slot < a.n_slots && pos >= 0;
   const int page = keep ? (int)slot / a.page_size : 0, at = keep ? (int)slot - page * a.page_size : 0;
 #pragma unroll
   for (int i = 0; i < HEADS; ++i) {

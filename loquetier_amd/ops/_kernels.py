@@ -1278,7 +1278,7 @@ def paged_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v
     if k_cache.size(2) != plan.page_size:
         raise RuntimeError(f"the plan is for pages of {plan.page_size} tokens")
     scale = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < 3.0e38:
+    if not 0.0 < scale < 1.0e38:
         raise RuntimeError("scale must be positive")
     dev = q.device
     R, M = plan.page_table.shape

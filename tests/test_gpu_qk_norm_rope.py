@@ -194,6 +194,52 @@ def test_padding_and_positions_past_the_table(K):
     assert torch.allclose(dwq.float(), ewq.float(), rtol=2 ** -7, atol=1e-3) and bool(dwk.isfinite().all())
 
 
+def test_padding_is_not_cached(K):
+    q, k, v, table, pos, _, _ = case("fp16", 6, 4, 2, 64, 64, (False, False), n_pos=50)
+    kc, vc = (torch.full((3, 2, 16, 64), 7.0, dtype=q.dtype, device="cuda") for _ in range(2))
+    pos[1] = pos[4] = -1
+    slots = torch.arange(6, device="cuda") * 5
+    K.qk_norm_rope(torch.empty_like(q.contiguous()), None, q, k, table, pos, v=v, k_cache=kc, v_cache=vc, slots=slots)
+    for c, x in ((kc, None), (vc, v)):
+        flat = c.transpose(1, 2).flatten(0, 1)
+        assert bool((flat[slots[[1, 4]]] == 7).all()) and not bool((flat[slots[[0, 2, 3, 5]]] == 7).any())
+        if x is not None:
+            assert torch.equal(flat[slots[[0, 2, 3, 5]]], x[[0, 2, 3, 5]])
+
+
+def test_training_step_in_a_graph(K):
+    """Forward and backward captured, replayed with new inputs between the program's own work, against eager passes."""
+    from loquetier_amd.kernel_utils import qk_norm_rope
+    q, k, _, table, pos, wq, wk = case("bf16", 60, 8, 2, 128, 128, (True, True), seed=12)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    inputs = [[torch.randn(t.shape, generator=g, device="cuda").to(t.dtype) for t in (q, k, q, k)] for _ in range(5)]
+
+    def step(q, k, gq, gk):
+        a, b = qk_norm_rope.apply(q, k, wq, wk, table, pos, 1e-6)
+        return [a.detach(), b.detach(), *torch.autograd.grad((a, b), (q, k, wq, wk), (gq, gk))]
+
+    wq.requires_grad_(True), wk.requires_grad_(True)
+    want = [[t.clone() for t in step(x[0].clone().requires_grad_(True), x[1].clone().requires_grad_(True), *x[2:])] for x in inputs]
+    static = [t.clone() for t in inputs[0]]
+    static[0].requires_grad_(True), static[1].requires_grad_(True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*static)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = step(*static)
+    for x, w in zip(inputs, want):
+        with torch.no_grad():
+            for s, t in zip(static, x):
+                s.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        torch.ones(3000, device="cuda").sum().item()
+        assert all(torch.equal(a, b) for a, b in zip(out, w))
+
+
 def test_infinities_stay_in_their_pairs(K):
     """A dimension that is not rotated passes through beside an infinity."""
     q, k, _, table, pos, _, _ = case("bf16", 4, 2, 1, 64, 32, (False, False))
