@@ -930,7 +930,7 @@ def _heads_fit(t: torch.Tensor) -> bool:
     return (t.size(2) == 1 or t.stride(2) == 1) and not any(s % 8 for n, s in zip(t.shape[:2], t.stride()[:2]) if n > 1)
 
 
-def _check_heads(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> None:
+def _check_heads(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None, written: bool = False) -> None:
     """[rows, heads, head_dim] of any strides the kernels read: views of one projection's output need no copy."""
     if not t.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor")
@@ -939,6 +939,8 @@ def _check_heads(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None
         raise RuntimeError(f"{name} must have its head's dimensions next to each other and strides that are multiples of 8")
     if like is not None and (t.dtype != like.dtype or t.device != like.device):
         raise RuntimeError(f"{name} must share q's dtype and device")
+    if written and any(s == 0 for n, s in zip(t.shape, t.stride()) if n > 1):
+        raise RuntimeError(f"{name} is written and must not be expanded")
 
 
 def _heads(t: Optional[torch.Tensor]) -> _lib.Heads:
@@ -1035,11 +1037,11 @@ def qk_norm_rope(q_out: torch.Tensor, k_out: Optional[torch.Tensor], q: torch.Te
     if _host().rope(q_out, k_out, q, k, table, positions, q_weight, k_weight, eps, v, k_cache, v_cache, slots):
         return
     a = _rope_args(q, k, table, positions, q_weight, k_weight, eps)
-    _check_heads(q_out, "q_out", q)
+    _check_heads(q_out, "q_out", q, True)
     if q_out.shape != q.shape:
         raise RuntimeError("q_out and q must have the same shape")
     if k_out is not None:
-        _check_heads(k_out, "k_out", q)
+        _check_heads(k_out, "k_out", q, True)
         if k_out.shape != k.shape:
             raise RuntimeError("k_out and k must have the same shape")
     a.q_out, a.k_out = _heads(q_out), _heads(k_out)
@@ -1051,6 +1053,8 @@ def qk_norm_rope(q_out: torch.Tensor, k_out: Optional[torch.Tensor], q: torch.Te
         if v.shape != k.shape:
             raise RuntimeError("v and k must have the same shape")
         a.page_stride, a.head_stride, a.slot_stride = _check_caches(k_cache, v_cache, q, k.size(1))
+        if any(s == 0 for n, s in zip(k_cache.shape, k_cache.stride()) if n > 1):
+            raise RuntimeError("the caches are written and must not be expanded")
         _check_ints(q.device, torch.int64, 1, slots=slots)
         if slots.size(0) != q.size(0):
             raise RuntimeError("slots must have one entry per row")
@@ -1077,7 +1081,7 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, dq_weight: Optiona
     order.  q, k, table, positions, weights: as in the forward."""
     a = _rope_args(q, k, table, positions, q_weight, k_weight, eps)
     for t, n, like in ((dq, "dq", q), (gq, "gq", q), (dk, "dk", k), (gk, "gk", k)):
-        _check_heads(t, n, q)
+        _check_heads(t, n, q, n in ("dq", "dk"))
         if t.shape != like.shape:
             raise RuntimeError(f"{n} must have its tensor's shape")
     for d, w, n in ((dq_weight, q_weight, "dq_weight"), (dk_weight, k_weight, "dk_weight")):
@@ -1264,7 +1268,7 @@ def paged_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v
     if _host().paged_attention(out, q, k_cache, v_cache, plan, scale, workspace):
         return
     _check_heads(q, "q")
-    _check_heads(out, "out", q)
+    _check_heads(out, "out", q, True)
     if out.shape != q.shape:
         raise RuntimeError("out and q must have the same shape")
     T, Hq, D = q.shape

@@ -222,6 +222,8 @@ def test_python_refusals(K):
                      (dict(q_out=k.clone()), "same shape"), (dict(k_out=None), "left out"), (dict(slots=slots), "come together"),
                      (dict(q=x.transpose(1, 2).contiguous().transpose(1, 2)), "next to each other"),
                      (dict(v=k, k_cache=cache, v_cache=cache.clone().transpose(1, 2).contiguous().transpose(1, 2), slots=slots), "same shape and strides"),
+                     (dict(q_out=x[:1].expand(4, HQ, D)), "expanded"), (dict(v=k, k_cache=cache[:1].expand(3, HKV, P, D),
+                      v_cache=cache[:1].expand(3, HKV, P, D), slots=slots), "expanded"),
                      (dict(v=k, k_cache=cache[..., :32], v_cache=cache[..., :32], slots=slots), "must be"),
                      (dict(v=k, k_cache=cache, v_cache=cache, slots=slots[:2]), "one entry per row"),
                      (dict(k_out=None, v=k, k_cache=cache[:0], v_cache=cache[:0], slots=slots), "no pages")):
@@ -237,7 +239,7 @@ def test_python_refusals(K):
     plan = K.AttentionPlan(i32(0, 2, 4), i32(2, 2), pt, 4, HQ, HKV, P)
     for args, what in (((x[:3], x[:3], cache, cache), "plan is for"), ((x, x, cache[:, :1], cache[:, :1]), "must be"),
                        ((x, x, cache[:, :, :8], cache[:, :, :8]), "pages of"), ((x, x.half(), cache, cache), "dtype"),
-                       ((x, x, cache, cache.half()), "dtype")):
+                       ((x, x, cache, cache.half()), "dtype"), ((x[:1].expand(4, HQ, D), x, cache, cache), "expanded")):
         with pytest.raises(RuntimeError, match=what):
             K.paged_attention(*args, plan)
     with pytest.raises(RuntimeError, match="scale"):

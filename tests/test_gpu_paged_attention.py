@@ -114,7 +114,7 @@ BATCHES = {
 
 @pytest.mark.parametrize("dt", ["fp16", "bf16"])
 @pytest.mark.parametrize("Hq,Hkv,D,P,nhd", [(8, 8, 128, 16, False), (8, 2, 128, 16, True), (8, 1, 64, 16, False), (6, 2, 64, 20, True),
-                                            (5, 1, 128, 7, False), (32, 8, 128, 64, False), (2, 1, 128, 1, False), (3, 3, 64, 128, False)])
+                                            (5, 1, 128, 7, False), (32, 8, 128, 64, False), (2, 1, 128, 1, False), (3, 3, 64, 128, False), (64, 1, 64, 1000, True), (40, 1, 128, 8, False)])
 @pytest.mark.parametrize("name", BATCHES)
 def test_batches(K, dt, Hq, Hkv, D, P, nhd, name):
     b = batch(dt, BATCHES[name], Hq, Hkv, D, P, nhd)
