@@ -117,15 +117,15 @@ int attn_check(int T, int S, int q_heads, int kv_heads) {
 // whether a row of the table holds keys enough for a sequence to be cut
 bool attn_cuts(int M, int page_size) { return (int64_t)M * page_size > kAttnMinKeys; }
 
-size_t attn_carve(void* base, int kv_heads, int head_dim, AttnArgs* a) {
+size_t attn_carve(void* base, int T, int S, int most, int q_heads, int kv_heads, int head_dim, AttnArgs* a) {
   size_t off = 0;
   auto take = [&](size_t floats) {
     const size_t o = off;
     off = align_up(off + floats * 4, 256);
     return base ? reinterpret_cast<float*>(reinterpret_cast<char*>(base) + o) : nullptr;
   };
-  const size_t small = (size_t)attn_parts_max(kv_heads, kAttnSmallItems) * kv_heads * kAttnSmallRows;
-  const size_t big = (size_t)attn_parts_max(kv_heads, kAttnBigItems) * kv_heads * kAttnBigRows;
+  const size_t small = (size_t)attn_parts_small(S, kv_heads, most) * kv_heads * kAttnSmallRows;
+  const size_t big = (size_t)attn_parts_big(T, S, q_heads / kv_heads, kv_heads, most) * kv_heads * kAttnBigRows;
   float *p0 = take(small * head_dim), *p1 = take(big * head_dim), *p2 = take(small * 2), *p3 = take(big * 2);
   if (a) a->po_small = p0, a->po_big = p1, a->pm_small = p2, a->pm_big = p3;
   return off;
@@ -360,8 +360,8 @@ SMLM_API int smlm_attn_plan_build(void* plan, size_t plan_bytes, const int32_t* 
   a.most = M * page_size;
   a.items_max = attn_items_max(T, S, g, kv_heads);
   a.joins_max = attn_joins_max(T, S, g, kv_heads);
-  a.parts_small_max = attn_parts_max(kv_heads, kAttnSmallItems);
-  a.parts_big_max = attn_parts_max(kv_heads, kAttnBigItems);
+  a.parts_small_max = attn_parts_small(S, kv_heads, a.most);
+  a.parts_big_max = attn_parts_big(T, S, g, kv_heads, a.most);
   // (fewer waves, fewer to wait for at a barrier)
   return launch(attn_plan_kernel, dim3(1), dim3(S <= 256 ? 512 : kAttnPlanThreads), (hipStream_t)stream, a);
 }
@@ -370,7 +370,8 @@ SMLM_API int smlm_paged_attn_workspace_size(int T, int S, int M, int page_size, 
                                             size_t* bytes) {
   if (!bytes || M < 0 || page_size <= 0 || head_dim <= 0) return SMLM_ERR_ARG;
   if (int rc = attn_check(T, S, q_heads, kv_heads)) return rc;
-  *bytes = attn_cuts(M, page_size) ? attn_carve(nullptr, kv_heads, head_dim, nullptr) : 0;
+  if ((int64_t)M * page_size > 0x7fffffff) return SMLM_ERR_LIMIT;
+  *bytes = attn_cuts(M, page_size) ? attn_carve(nullptr, T, S, M * page_size, q_heads, kv_heads, head_dim, nullptr) : 0;
   return SMLM_OK;
 }
 
@@ -396,7 +397,7 @@ SMLM_API int smlm_paged_attn(const smlm_heads* out, const smlm_heads* q, const v
   const bool cuts = attn_cuts(M, page_size);
   if (cuts) {
     if (!workspace) return SMLM_ERR_ARG;
-    if (workspace_bytes < attn_carve(workspace, kv_heads, head_dim, &a)) return SMLM_ERR_WORKSPACE;
+    if (workspace_bytes < attn_carve(workspace, T, S, M * page_size, q_heads, kv_heads, head_dim, &a)) return SMLM_ERR_WORKSPACE;
   }
   a.out = reinterpret_cast<uint16_t*>(out->data);
   a.q = reinterpret_cast<const uint16_t*>(q->data);
@@ -405,7 +406,7 @@ SMLM_API int smlm_paged_attn(const smlm_heads* out, const smlm_heads* q, const v
   a.table = table;
   a.o_row = out->row_stride, a.o_head = out->head_stride, a.q_row = q->row_stride, a.q_head = q->head_stride;
   a.c_page = page_stride, a.c_head = head_stride, a.c_slot = slot_stride;
-  a.M = M, a.most = M * page_size, a.n_pages = n_pages, a.P = page_size, a.T = T, a.Hq = q_heads, a.Hkv = kv_heads, a.g = g;
+  a.M = M, a.most = M * page_size, a.n_pages = n_pages, a.P = page_size, a.T = T, a.S = S, a.R = R, a.Hkv = kv_heads, a.g = g;
   // x / P = (floor(x m / 2^32) + x) >> s for x < 2^32, with s = ceil(log2 P), m = floor(2^32 (2^s - P) / P) + 1
   // (Granlund and Montgomery, Division by Invariant Integers using Multiplication, 1994)
   while ((int64_t)1 << a.div_shift < page_size) ++a.div_shift;

@@ -57,7 +57,7 @@ struct AttnJoin {   // rows of a tile whose keys were cut
   int from, step, rows;    // its rows from, from + step, ... below rows (eight at each, or one where the parts are many)
 };
 struct AttnPlanView {
-  int* hdr;          // [16]: 0 items, 1 joins, 2 tokens that a row of the table holds
+  int* hdr;          // [16]: 0 items, 1 joins, what the plan is for: 2 tokens that a row of the table holds, 3 T, 4 S, 5 g, 6 kv heads, 7 R
   int* start;        // [4][S + 1] running sums by sequence: items with few rows, other items, joins, parts
   AttnItem* items;
   AttnJoin* joins;
@@ -71,7 +71,16 @@ inline int attn_joins_max(int T, int S, int g, int Hkv) {
   return (int)(cut < tiles ? cut : tiles);
 }
 // (a tile of x times the cut's keys has round(x) parts, which is more than one from x = 1.5 on: at most 4 x / 3)
-inline int attn_parts_max(int Hkv, int items) { return 4 * (items / Hkv + 1) / 3 + 1; }
+// Parts of few-row tiles and of others, for sequences of at most `most` tokens; no more than the tiles there can be have at kAttnMinKeys.
+inline int attn_parts_max(int Hkv, int items, int64_t tiles, int most) {
+  const int64_t cut = 4 * (int64_t)(items / Hkv + 1) / 3 + 1, all = most > kAttnMinKeys ? tiles * (most / kAttnMinKeys + 1) : 0;
+  return (int)(cut < all ? cut : all);
+}
+inline int attn_parts_small(int S, int Hkv, int most) { return attn_parts_max(Hkv, kAttnSmallItems, S, most); }
+inline int attn_parts_big(int T, int S, int g, int Hkv, int most) {
+  const int64_t rows = (int64_t)T * g, seqs = rows / (kAttnSmallRows + 1);  // (sequences of more rows than a few)
+  return attn_parts_max(Hkv, kAttnBigItems, rows / kAttnBigRows + (seqs < S ? seqs : S), most);
+}
 inline size_t attn_plan_carve(void* base, int T, int S, int g, int Hkv, AttnPlanView* pv) {
   size_t off = 0;
   auto take = [&](size_t bytes) {
@@ -224,7 +233,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
     first_s[0][0] = first_s[1][0] = start[0] = start[a.S + 1] = 0;
     a.plan.hdr[0] = items;
     a.plan.hdr[1] = at[2] < a.joins_max ? at[2] : a.joins_max;
-    a.plan.hdr[2] = a.most;
+    a.plan.hdr[2] = a.most, a.plan.hdr[3] = a.T, a.plan.hdr[4] = a.S, a.plan.hdr[5] = a.g, a.plan.hdr[6] = a.Hkv, a.plan.hdr[7] = a.R;
   }
   __syncthreads();
   // Items with few rows stream, the others compute: they take turns, so that both have the card together (mixed batch of four prompts
@@ -277,13 +286,19 @@ struct AttnArgs {
   float *po_small, *po_big;  // parts of the results, [part][kv head][tile row][D], not divided by their sums
   float *pm_small, *pm_big;  // [part][kv head][tile row][2]: maximum (of the scores times scale / log 2), sum
   int64_t o_row, o_head, q_row, q_head, c_page, c_head, c_slot;
-  int M, n_pages, P, T, Hq, Hkv, g;
-  int most;                  // M * P: the plan has to be for as many
+  int M, n_pages, P, T, S, R, Hkv, g;
+  int most;                  // M * P
   uint32_t div_mul;          // division by P: ((x * div_mul >> 32) + x) >> div_shift in 33 bits
   int div_shift;
   int whole;                 // keys from a multiple of it on, as many, that lie in one page: 16, the rows of a load, or 0
   float scale;               // times log2 e
 };
+
+// A plan for other sizes names rows, or parts of the results, that may not be there: the call does nothing.
+__device__ __forceinline__ bool attn_fits(const AttnArgs& a) {
+  const int* h = a.plan.hdr;
+  return h[2] == a.most && h[3] == a.T && h[4] == a.S && h[5] == a.g && h[6] == a.Hkv && h[7] == a.R;
+}
 
 static __device__ __align__(16) const uint32_t attn_zeros[4] = {0u, 0u, 0u, 0u};
 
@@ -849,7 +864,7 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
   __shared__ __align__(16) uint16_t lds[2 * 64 * D], more[2 * 64 * D];
   __shared__ uint32_t side[128];
   const int i = (int)blockIdx.x / a.Hkv, kvh = (int)blockIdx.x - i * a.Hkv;
-  if (i >= a.plan.hdr[0] || a.plan.hdr[2] != a.most) return;
+  if (i >= a.plan.hdr[0] || !attn_fits(a)) return;
   const AttnItem it = a.plan.items[i];
   const int rows = it.n * a.g;
   if (rows <= 0) return;
@@ -866,7 +881,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;  // threads a row; rows, or shares of the parts, at a time
   __shared__ f32x4 acc_s[kGroups][kLanes];
   __shared__ float sum_s[kGroups], top_s[kGroups];
-  if (a.plan.hdr[2] != a.most) return;
+  if (!attn_fits(a)) return;
   const int work = a.plan.hdr[1] * a.Hkv;
   for (int w = blockIdx.x; w < work; w += gridDim.x) {
     const int i = w / a.Hkv, kvh = w - i * a.Hkv;

@@ -287,6 +287,21 @@ def test_a_plan_for_another_table_does_nothing(K):
     assert bool((out == 5).all())
 
 
+@pytest.mark.parametrize("T,S,heads", [(120, 2, (4, 2)), (201, 1, (4, 2)), (201, 2, (4, 1)), (201, 2, (2, 1))])
+def test_a_plan_for_other_sizes_does_nothing(K, T, S, heads):
+    b = batch("bf16", [(1, 400), (200, 500)], 4, 2, 64, 16)
+    plan = K.AttentionPlan(b["indptr"], b["lens"], b["table"], b["T"], 4, 2, 16)
+    plan.T, plan.S, (plan.q_heads, plan.kv_heads) = T, S, heads
+    q, (kc, vc) = b["q"][:T, :heads[0]], (c[:, :heads[1]] for c in (b["kc"], b["vc"]))
+    out = torch.full_like(b["q"], 5.0)
+    if heads[1] == 1:  # (one kv head's tiles are cut into more items than two's: the host knows that the plan is too small)
+        with pytest.raises(RuntimeError):
+            K.paged_attention(out[:T, :heads[0]], q, kc, vc, plan)
+    else:
+        K.paged_attention(out[:T, :heads[0]], q, kc, vc, plan)
+    assert bool((out == 5).all())
+
+
 def test_sequences_that_overlap_stay_in_bounds(K):
     """Row ranges that decrease, overlap or leave the batch break the contract; what is written stays within the batch's rows."""
     b = batch("bf16", [(1, 400), (200, 2500), (1, 3)], 4, 2, 64, 16, after=3)
