@@ -10,8 +10,11 @@
 // sets bits of `status`.
 //
 // The bookkeeping is a few kilobytes of integers, bound by latency: one workgroup of 1024 threads counts and takes the
-// pages (scans and a pass over refs, sixteen pages a thread at a time, ended as soon as enough are found); what
-// grows with tokens or page contents runs in a second launch that has the card.
+// pages (scans and a pass over refs, sixteen pages a thread at a time, the next ones on their way, ended as soon as enough are found);
+// what grows with tokens or page contents runs in a second launch that has the card.  us: a token for each of 256 requests, half of
+// 40000 pages free, 8.1 (an empty launch takes 2.5); prompts of 128000 tokens 9.4 + 4.3; freeing 64 requests of 4000 tokens 3.4;
+// forking 16 requests into 128 5.5 + 14.8 for copies of 32 MB.  Copies go at the rate of a plain copy: packing 610 MB 225 us,
+// 5.4 TB/s read and written.
 #pragma once
 #include "smlm_common.hpp"
 #include "wave_scan.hpp"
@@ -42,18 +45,31 @@ __device__ __forceinline__ int kv_scan(int v, int* wave_tot, int& total) {
 __device__ __forceinline__ int kv_load(const int* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ void kv_store(int* p, int v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
+// This thread's sixteen pages from number `first` on, where there are as many.  (A kernel asks for its first ones as it starts, so
+// that they are there when it knows how many it wants.)
+struct KvRefs {
+  i32x4 v[4];
+};
+__device__ __forceinline__ KvRefs kv_refs(const int* refs, int N, int first) {
+  KvRefs x;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x.v[j] = i32x4{1, 1, 1, 1};
+    if (first + 16 <= N) __builtin_memcpy(&x.v[j], refs + first + 4 * j, 16);
+  }
+  return x;
+}
+
 // The `want` lowest pages without holders into out[0, want); returns how many there are (at most want).
-__device__ __forceinline__ int kv_take_free(const int* refs, int N, int want, int* out, int* wave_tot) {
+__device__ __forceinline__ int kv_take_free(const int* refs, int N, int want, int* out, int* wave_tot, KvRefs x) {
   int found = 0;
   for (int base = 0; base < N && found < want; base += kKvThreads * 16) {
     const int first = base + (int)threadIdx.x * 16;
+    const KvRefs next = kv_refs(refs, N, first + kKvThreads * 16);
     uint32_t mask = 0;
     if (first + 16 <= N) {
-      i32x4 v[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) __builtin_memcpy(&v[j], refs + first + 4 * j, 16);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) mask |= (v[j >> 2][j & 3] == 0 ? 1u : 0u) << j;
+      for (int j = 0; j < 16; ++j) mask |= (x.v[j >> 2][j & 3] == 0 ? 1u : 0u) << j;
     } else {
       for (int j = 0; j < 16 && first + j < N; ++j) mask |= (refs[first + j] == 0 ? 1u : 0u) << j;
     }
@@ -65,6 +81,7 @@ __device__ __forceinline__ int kv_take_free(const int* refs, int N, int want, in
       mask &= mask - 1;
     }
     found += total;
+    x = next;
   }
   return found < want ? found : want;
 }
@@ -101,33 +118,41 @@ struct KvExtendArgs {
   int R, M, N, S, rows, P;
 };
 
+// A sequence's part of a step.
+struct KvNeed {
+  int n, pages, err;  // new tokens, new pages
+};
+__device__ __forceinline__ KvNeed kv_need(const KvExtendArgs& a, int r, int count, bool first, int old) {
+  KvNeed x{r < 0 ? 0 : max(count, 0), 0, 0};
+  if (r >= 0) {
+    if (r >= a.R || count < 0 || !first) x.err = SMLM_KV_BAD_REQUEST;
+    const int64_t now = (int64_t)old + x.n, had = ((int64_t)old + a.P - 1) / a.P, has = (now + a.P - 1) / a.P;
+    if (r < a.R && (has > a.M || old < 0)) x.err |= SMLM_KV_TOO_LONG;
+    if (x.n > a.rows) x.err |= SMLM_KV_ROWS, x.n = 0;  // (and so the sum stays small)
+    if (!x.err) x.pages = (int)(has - had);
+  }
+  return x;
+}
+
 // One workgroup: counts, checks, takes the pages and writes the step's tables by sequence.  q_indptr doubles as the counts' running sum.
 __global__ __launch_bounds__(kKvThreads) void kv_extend_kernel(KvExtendArgs a) {
   __shared__ int wave_tot[16];
   __shared__ int owner_s[kKvOwners];
   __shared__ int bad;
   const int tid = threadIdx.x;
+  const KvRefs refs0 = kv_refs(a.refs, a.N, tid * 16);
   if (tid == 0) bad = 0;
   kv_mark(a.requests, a.S, a.R, a.owner, owner_s);
   int rows = 0, pages = 0;
   for (int base = 0; base < a.S; base += kKvThreads) {
     const int i = base + tid;
-    int r = -1, n = 0, need = 0, err = 0;
+    int n = 0, need = 0, err = 0;
     if (i < a.S) {
-      r = a.requests[i];
-      n = r < 0 ? 0 : a.counts[i];
-      if (r >= a.R || n < 0) {
-        err = SMLM_KV_BAD_REQUEST;
-      } else if (r >= 0) {
-        if (kv_first(r, a.R, a.owner, owner_s) != i) err = SMLM_KV_BAD_REQUEST;
-        const int64_t old = a.length[r], now = old + n;
-        const int64_t had = (old + a.P - 1) / a.P, has = (now + a.P - 1) / a.P;
-        if (has > a.M || old < 0) err |= SMLM_KV_TOO_LONG;
-        else need = (int)(has - had);
-      }
-      if (err) n = 0, need = 0;
+      const int r = a.requests[i];
+      const bool in = r >= 0 && r < a.R;
+      const KvNeed x = kv_need(a, r, r < 0 ? 0 : a.counts[i], in && kv_first(r, a.R, a.owner, owner_s) == i, in ? a.length[r] : 0);
+      n = x.n, need = x.pages, err = x.err;
     }
-    if (n > a.rows) err |= SMLM_KV_ROWS, n = 0;  // (and so the sum stays small)
     if (err) atomicOr(&bad, err);
     int total;
     const int upto = kv_scan(n, wave_tot, total);
@@ -145,7 +170,7 @@ __global__ __launch_bounds__(kKvThreads) void kv_extend_kernel(KvExtendArgs a) {
   }
   __syncthreads();
   if (!bad) {
-    const int found = kv_take_free(a.refs, a.N, pages, a.fresh, wave_tot);
+    const int found = kv_take_free(a.refs, a.N, pages, a.fresh, wave_tot, refs0);
     if (tid == 0 && found < pages) bad = SMLM_KV_NO_PAGES;
   }
   __threadfence_block();
@@ -180,28 +205,113 @@ __device__ __forceinline__ int kv_last_le(const int* a, int n, int x) {
 
 // The new pages' places in the table, and positions and slots of the step's rows: a thread a row (or page: there are at most as many
 // as rows).  Rows past the last request's, and all of them where the step was refused, get -1.
+constexpr int kKvRowsLds = 1024;  // sequences up to which the running sums are searched in LDS
 __global__ __launch_bounds__(256) void kv_rows_kernel(KvExtendArgs a) {
+  __shared__ int start_s[kKvRowsLds + 1], indptr_s[kKvRowsLds + 1];
   const int t = (int)blockIdx.x * 256 + (int)threadIdx.x;
+  const bool local = a.S <= kKvRowsLds;
+  if (local) {
+    for (int i = threadIdx.x; i <= a.S; i += 256) start_s[i] = a.start[i], indptr_s[i] = a.q_indptr[i];
+    __syncthreads();
+  }
   if (t >= a.rows) return;
-  // (a new page holds a new token, so pages do not outnumber rows)
-  if (a.S > 0 && t < a.start[a.S]) {
-    const int i = kv_last_le(a.start, a.S, t);
-    const int old = a.kv_len[i] - (a.q_indptr[i + 1] - a.q_indptr[i]), id = a.fresh[t];
-    a.table[(int64_t)a.requests[i] * a.M + (old + a.P - 1) / a.P + (t - a.start[i])] = id;
+  auto start = [&](int i) { return local ? start_s[i] : a.start[i]; };
+  auto indptr = [&](int i) { return local ? indptr_s[i] : a.q_indptr[i]; };
+  if (t < start(a.S)) {
+    const int i = local ? kv_last_le(start_s, a.S, t) : kv_last_le(a.start, a.S, t);
+    const int old = a.kv_len[i] - (indptr(i + 1) - indptr(i)), id = a.fresh[t];
+    a.table[(int64_t)a.requests[i] * a.M + (old + a.P - 1) / a.P + (t - start(i))] = id;
     a.refs[id] = 1;
   }
   int pos = -1;
   int64_t slot = -1;
-  if (a.S > 0 && t < a.q_indptr[a.S]) {
-    const int i = kv_last_le(a.q_indptr, a.S, t);
-    const int n = a.q_indptr[i + 1] - a.q_indptr[i], had = (a.kv_len[i] - n + a.P - 1) / a.P;
-    pos = a.kv_len[i] - (a.q_indptr[i + 1] - t);
+  if (t < indptr(a.S)) {
+    const int i = local ? kv_last_le(indptr_s, a.S, t) : kv_last_le(a.q_indptr, a.S, t);
+    const int n = indptr(i + 1) - indptr(i), had = (a.kv_len[i] - n + a.P - 1) / a.P;
+    pos = a.kv_len[i] - (indptr(i + 1) - t);
     const int j = pos / a.P;
-    const int page = j < had ? a.table[(int64_t)a.requests[i] * a.M + j] : a.fresh[a.start[i] + j - had];
+    const int page = j < had ? a.table[(int64_t)a.requests[i] * a.M + j] : a.fresh[start(i) + j - had];
     slot = (int64_t)page * a.P + (pos - j * a.P);
   }
   a.positions[t] = pos;
   a.slots[t] = slot;
+}
+
+// The same where a thread has a sequence to itself: two trips to memory before the pages are looked for.  FEW: the rows too, which
+// then find what they look up in LDS: a token for each of 256 requests 8.1 us, 6.5 + 4.1 in two launches; 4096 rows of 256
+// requests 10.9 and 6.6 + 4.1, where the second launch's start is still to come; 8192 rows 14.9 and 6.7 + 4.6.
+constexpr int kKvFewRows = 4096;
+template <bool FEW>
+__global__ __launch_bounds__(kKvThreads) void kv_extend_one_kernel(KvExtendArgs a) {
+  __shared__ int wave_tot[16];
+  __shared__ int owner_s[kKvOwners];
+  __shared__ int indptr_s[kKvThreads + 1], start_s[kKvThreads + 1];  // running sums of new tokens and pages
+  __shared__ int req_s[kKvThreads], now_s[kKvThreads], tail_s[kKvThreads];  // request; tokens; the page that was filled in part
+  __shared__ int fresh_s[FEW ? kKvFewRows : 1];                                // (a new page holds a new token, so pages do not outnumber rows)
+  __shared__ int bad;
+  const int tid = threadIdx.x;
+  const int r = tid < a.S ? a.requests[tid] : -1, count = tid < a.S ? a.counts[tid] : 0;
+  const KvRefs refs0 = kv_refs(a.refs, a.N, tid * 16);
+  const bool in = r >= 0 && r < a.R, local = a.R <= kKvOwners;
+  if (tid == 0) bad = 0;
+  if (in) {
+    if (local) owner_s[r] = 0x7fffffff;
+    else kv_store(a.owner + r, 0x7fffffff);
+  }
+  __syncthreads();
+  if (in) atomicMin((local ? owner_s : a.owner) + r, tid);
+  const int old = in ? a.length[r] : 0;
+  __syncthreads();
+  KvNeed x{0, 0, 0};
+  if (tid < a.S) x = kv_need(a, r, count, in && kv_first(r, a.R, a.owner, owner_s) == tid, old);
+  if (x.err) atomicOr(&bad, x.err);
+  const int tail = FEW && in && old > 0 && old % a.P && old / a.P < a.M ? a.table[(int64_t)r * a.M + old / a.P] : -1;
+  int rows, pages;
+  const int rows_upto = kv_scan(x.n, wave_tot, rows), pages_upto = kv_scan(x.pages, wave_tot, pages);
+  if (rows > a.rows || pages > a.N) {
+    if (tid == 0) atomicOr(&bad, (rows > a.rows ? SMLM_KV_ROWS : 0) | (pages > a.N ? SMLM_KV_NO_PAGES : 0));
+  }
+  if (tid == 0) indptr_s[0] = start_s[0] = 0;
+  indptr_s[tid + 1] = rows_upto, start_s[tid + 1] = pages_upto;
+  req_s[tid] = r, now_s[tid] = old + x.n, tail_s[tid] = tail;
+  __syncthreads();
+  if (!bad) {
+    const int found = FEW ? kv_take_free(a.refs, a.N, pages, fresh_s, wave_tot, refs0) : kv_take_free(a.refs, a.N, pages, a.fresh, wave_tot, refs0);
+    if (tid == 0 && found < pages) bad = SMLM_KV_NO_PAGES;
+  }
+  __syncthreads();
+  const int err = bad;
+  if (tid == 0) {
+    a.q_indptr[0] = 0;
+    if (!FEW) a.start[0] = 0;
+    if (err && a.status) atomicOr(a.status, err);
+  }
+  if (tid < a.S) {
+    if (!FEW) a.start[tid + 1] = err ? 0 : pages_upto;
+    a.q_indptr[tid + 1] = err ? 0 : rows_upto;
+    a.kv_len[tid] = err || !in ? 0 : old + x.n;
+    if (in && !err) a.length[r] = old + x.n;
+  }
+  if (!FEW) return;
+  if (err) rows = pages = 0;
+  for (int t = tid; t < pages; t += kKvThreads) {
+    const int i = kv_last_le(start_s, a.S, t), n = indptr_s[i + 1] - indptr_s[i], id = fresh_s[t];
+    a.table[(int64_t)req_s[i] * a.M + (now_s[i] - n + a.P - 1) / a.P + (t - start_s[i])] = id;
+    a.refs[id] = 1;
+  }
+  for (int t = tid; t < a.rows; t += kKvThreads) {
+    int pos = -1;
+    int64_t slot = -1;
+    if (t < rows) {
+      const int i = kv_last_le(indptr_s, a.S, t);
+      const int n = indptr_s[i + 1] - indptr_s[i], had = (now_s[i] - n + a.P - 1) / a.P;
+      pos = now_s[i] - (indptr_s[i + 1] - t);
+      const int j = pos / a.P, page = j < had ? tail_s[i] : fresh_s[start_s[i] + j - had];
+      slot = (int64_t)page * a.P + (pos - j * a.P);
+    }
+    a.positions[t] = pos;
+    a.slots[t] = slot;
+  }
 }
 
 struct KvFreeArgs {
@@ -289,6 +399,7 @@ __global__ __launch_bounds__(kKvThreads) void kv_fork_kernel(KvForkArgs a) {
   __shared__ int owner_s[kKvOwners];
   __shared__ int bad;
   const int tid = threadIdx.x, P = a.pool.P;
+  const KvRefs refs0 = kv_refs(a.refs, a.pool.N, tid * 16);
   if (tid == 0) bad = 0;
   kv_mark(a.children, a.K, a.R, a.owner, owner_s);
   int pages = 0;
@@ -320,7 +431,7 @@ __global__ __launch_bounds__(kKvThreads) void kv_fork_kernel(KvForkArgs a) {
   }
   __syncthreads();
   if (!bad) {
-    const int found = kv_take_free(a.refs, a.pool.N, pages, a.fresh, wave_tot);
+    const int found = kv_take_free(a.refs, a.pool.N, pages, a.fresh, wave_tot, refs0);
     if (tid == 0 && found < pages) bad = SMLM_KV_NO_PAGES;
   }
   __threadfence_block();

@@ -268,7 +268,8 @@ SMLM_API int smlm_kv_extend(int32_t* table, int32_t* length, int32_t* refs, cons
   a.requests = requests, a.counts = counts;
   a.q_indptr = q_indptr, a.kv_len = kv_len, a.positions = positions, a.slots = slots;
   a.R = R, a.M = M, a.N = N, a.S = S, a.rows = rows, a.P = page_size;
-  const int rc = launch(kv_extend_kernel, dim3(1), dim3(kKvThreads), (hipStream_t)stream, a);
+  if (S <= kKvThreads && rows <= kKvFewRows) return launch(kv_extend_one_kernel<true>, dim3(1), dim3(kKvThreads), (hipStream_t)stream, a);
+  const int rc = launch(S <= kKvThreads ? kv_extend_one_kernel<false> : kv_extend_kernel, dim3(1), dim3(kKvThreads), (hipStream_t)stream, a);
   if (rc || rows == 0) return rc;
   return launch(kv_rows_kernel, dim3((unsigned)ceil_div(rows, 256)), dim3(256), (hipStream_t)stream, a);
 }

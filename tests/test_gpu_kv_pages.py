@@ -229,6 +229,36 @@ def test_many_pages_and_rows(K):
     do_extend(m, d, req, [1] * len(req), len(req) + 100)
 
 
+@pytest.mark.parametrize("S,rows,R", [(1024, 4096, 1100), (1025, 4096, 1100), (300, 4097, 400), (1, 4096, 3), (5, 40, 9000), (1030, 1500, 9000)])
+def test_steps_of_few_rows_and_others(K, S, rows, R):
+    """Around the sizes up to which a step takes one launch: steps that use all rows and fewer, and refusals."""
+    r = random.Random(S)
+    m, d = both(K, n_pages=6000, blocks=1, P=5, requests=R, width=900)
+    req = r.sample(range(R), S)
+    for used in (rows, rows // 2):
+        cuts = sorted(r.randint(0, used) for _ in range(S - 1))
+        do_extend(m, d, req, [b - a for a, b in zip([0] + cuts, cuts + [used])], rows)
+        r.shuffle(req)
+    ones = [1] * S
+    for names, counts, bits in ((req[:-1] + [R], ones, 1), (req[:-1] + [req[0]], ones, 1) if S > 1 else ([-3, R], [1, 1], 1),
+                                (req, [rows + 1] + ones[1:], 4), (req, [0] * (S - 1) + [-1], 1)):
+        m.status = 0
+        d.status.zero_()
+        do_extend(m, d, names, counts, rows)
+        assert m.status & bits
+    free = sum(x == 0 for x in m.refs)
+    m.refs[:] = [x or 1 for x in m.refs[:-2]] + m.refs[-2:]  # all but two pages held
+    d.refs.copy_(ints(m.refs))
+    m.status = 0
+    d.status.zero_()
+    do_extend(m, d, req, [min(11 * 5, rows)] + [0] * (S - 1), rows)
+    assert free > 2 and m.status & 8
+    m.status = 0
+    d.status.zero_()
+    do_extend(m, d, req, [min(2, rows)] + [0] * (S - 1), rows)
+    assert m.status == 0
+
+
 def test_empty_calls(K):
     m, d = both(K)
     do_extend(m, d, [], [], 0)
