@@ -475,8 +475,8 @@ typedef struct smlm_heads {
  *
  * With k_cache the rotated keys, and v, also go to a cache's pages: row t to place slots[t] % page_size of page
  * slots[t] / page_size, at data[page * page_stride + head * head_stride + place * slot_stride] (elements, multiples of 8) of both caches; a slot
- * outside [0, n_pages * page_size) (-1: rows that are not cached) is not written.  k_out's data may then be NULL.  Two rows of one
- * slot leave either.
+ * outside [0, n_pages * page_size) (-1: rows that are not cached) is not written.  k_out's data may then be NULL.  Of two rows of one
+ * slot each piece of eight elements is of either.
  */
 typedef struct smlm_qk_rope {
   smlm_heads q, k, v;         /* v: with k_cache only */

@@ -158,6 +158,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
   __shared__ float red[3][16];
   __shared__ int first_s[2][kAttnPlanLds + 1], join_s[kAttnPlanLds], part_s[kAttnPlanLds];
   __shared__ AttnSeq seq_s[kAttnPlanLds];
+  __shared__ int bin_s[256];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, threads = (int)blockDim.x, waves = threads >> 6;
   const bool local = a.S <= kAttnPlanLds;
   float keys[2] = {0.0f, 0.0f};  // of the few-row tiles, of the others (only the cuts hang on them: a float will do)
@@ -239,8 +240,15 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
   // Items with few rows stream, the others compute: they take turns, so that both have the card together (mixed batch of four prompts
   // of 512 and 64 single tokens, 32 heads: the others all first 251 us, in turns 245; alone the two take 81 and 189).
   const int both = min(at[0], at[1]);
-  for (int i = tid; i < items; i += threads) {
-    const int kind = i < 2 * both ? !(i & 1) : at[1] > at[0];  // 1: the others
+  struct Place {
+    AttnItem it;
+    AttnSeq q;
+    int kind, x;              // 1: the others; its number among its kind's
+    int lo, t, j, ns, part0;  // sequence, tile, part, parts of the tile
+    bool fits;
+  };
+  auto place = [&](int i) {
+    const int kind = i < 2 * both ? !(i & 1) : at[1] > at[0];
     const int x = i < 2 * both ? i >> 1 : i - both;
     const int* first_l = first_s[kind];
     const int* first_g = start + kind * (a.S + 1);
@@ -252,7 +260,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
     }
     const AttnSeq q = local ? seq_s[lo] : attn_seq(a, lo);
     const int first = local ? first_l[lo] : first_g[lo], end = local ? first_l[lo + 1] : first_g[lo + 1];
-    const int join = local ? join_s[lo] : start[2 * (a.S + 1) + lo], part = local ? part_s[lo] : start[3 * (a.S + 1) + lo];
+    const int part = local ? part_s[lo] : start[3 * (a.S + 1) + lo];
     const uint32_t ns = max(1u, (uint32_t)(end - first) / (uint32_t)max(1, q.tiles)), k = (uint32_t)(x - first);
     const int t = max(0, q.tiles - 1 - (int)(k / ns)), j = (int)(k % ns);  // (the later tiles of a prompt see more keys: they go first)
     AttnItem it;
@@ -267,12 +275,40 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
     // (sequences that overlap, which none should, could come to more parts than there is room for)
     const bool fits = ns == 1 || part0 + (int)ns <= parts_max;
     if (!fits) it.n = 0, it.kb = it.ke = 0, it.part = -1;
-    a.plan.items[i] = it;
-    if (ns > 1) {
-      const int shares = attn_shares(q, (int)ns, a.g), by = kind || ns < kAttnManyParts ? 8 : 1;
-      const int rows = fits ? min(q.tile, q.n * a.g - it.first) : 0;
-      for (int h = j; h < shares && join + t * shares + h < a.joins_max; h += (int)ns)
-        a.plan.joins[join + t * shares + h] = AttnJoin{q.row0, it.first, kind, part0, (int)ns, h * by, shares * by, rows};
+    return Place{it, q, kind, x, lo, t, j, (int)ns, part0, fits};
+  };
+  // Where the others are most of the items, and more than the card takes at a time, the long ones go first, over all sequences (by
+  // eighths of an octave): a long one that starts among the last keeps the rest of the card waiting.  In all, sequence by sequence and so:
+  // nine prompts of 700 rows over up to 3000 tokens 262 and 246 us, 64 of 16 rows over up to 4000 tokens 168 and 139; but beside many
+  // items with few rows the two ways to take turns quarrel (eight prompts of 512 rows, 128 single tokens 298 and 315).
+  const bool sorted = at[1] > kAttnSlots / a.Hkv && at[1] > at[0];
+  auto bin_of = [](const AttnItem& it) { return 255 - (int)((__float_as_uint((float)(it.ke - it.kb) + 1.0f) >> 20) - (127u << 3)); };
+  if (sorted) {
+    for (int b = tid; b < 256; b += threads) bin_s[b] = 0;
+    __syncthreads();
+    for (int i = tid; i < items; i += threads) {
+      const Place p = place(i);
+      if (p.kind) atomicAdd(&bin_s[bin_of(p.it)], 1);
+    }
+    __syncthreads();
+    const int n = tid < 256 ? bin_s[tid] : 0;
+    int before = wave_scan(n) - n;
+    if (lane == 63 && wave < 4) wave_tot[wave][0] = before + n;
+    __syncthreads();
+    for (int w = 0; w < 4; ++w) before += w < wave ? wave_tot[w][0] : 0;
+    if (tid < 256) bin_s[tid] = before;
+    __syncthreads();
+  }
+  for (int i = tid; i < items; i += threads) {
+    const Place p = place(i);
+    const int x = sorted && p.kind ? atomicAdd(&bin_s[bin_of(p.it)], 1) : p.x;
+    a.plan.items[x < both ? 2 * x + (p.kind ? 0 : 1) : x + both] = p.it;
+    if (p.ns > 1) {
+      const int join = local ? join_s[p.lo] : start[2 * (a.S + 1) + p.lo];
+      const int shares = attn_shares(p.q, p.ns, a.g), by = p.kind || p.ns < kAttnManyParts ? 8 : 1;
+      const int rows = p.fits ? min(p.q.tile, p.q.n * a.g - p.it.first) : 0;
+      for (int h = p.j; h < shares && join + p.t * shares + h < a.joins_max; h += p.ns)
+        a.plan.joins[join + p.t * shares + h] = AttnJoin{p.q.row0, p.it.first, p.kind, p.part0, p.ns, h * by, shares * by, rows};
     }
   }
 }
@@ -294,10 +330,11 @@ struct AttnArgs {
   float scale;               // times log2 e
 };
 
-// A plan for other sizes names rows, or parts of the results, that may not be there: the call does nothing.
-__device__ __forceinline__ bool attn_fits(const AttnArgs& a) {
-  const int* h = a.plan.hdr;
-  return h[2] == a.most && h[3] == a.T && h[4] == a.S && h[5] == a.g && h[6] == a.Hkv && h[7] == a.R;
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ i32x8 uload8(const void* p) { return *(const SMLM_CONST i32x8*)p; }
+// A plan for other sizes names rows, or parts of the results, that may not be there: the call does nothing.  (h: the header's start)
+__device__ __forceinline__ bool attn_fits(const AttnArgs& a, i32x8 h) {
+  return ((h[2] ^ a.most) | (h[3] ^ a.T) | (h[4] ^ a.S) | (h[5] ^ a.g) | (h[6] ^ a.Hkv) | (h[7] ^ a.R)) == 0;
 }
 
 static __device__ __align__(16) const uint32_t attn_zeros[4] = {0u, 0u, 0u, 0u};
@@ -743,77 +780,8 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
   };
   // A tile's loads are waited for by the wave that gave them, then by all; at that point everybody is done with the tile before,
   // whose place the next loads take.
-  int base = it.kb;
-  if (base < it.ke) load(attn_offset(a, attn_key(a, trow, base + wave * 16 + (lane & 15), it.ke)), tile0);
-  // Pairs of tiles that every row sees, where the rows of a load lie in one page: apart, so that this loop keeps its registers to
-  // itself.  What it loads, and whether a page is there, is known on the scalar side: one page for a wave's sixteen keys, or one a load.
-  auto pairs = [&](auto sixteen) {  // (two loops: the test in one of them cost up to 5 percent)
-    constexpr uint32_t kAll = 0xffffu, kOne = (1u << kRowsLoad) - 1u;
-    int page[kLoads], slot[kLoads];
-    auto find = [&](int key) {
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        if (i && sixteen) break;
-        const int k = min(key + i * kRowsLoad, it.ke - 1), j = attn_div((uint32_t)k, a.div_mul, a.div_shift);
-        slot[i] = k - j * a.P;
-        page[i] = uload(trow, j);
-      }
-    };
-    auto fetch = [&](uint16_t* tile) -> uint32_t {  // the keys that are there
-      if (sixteen) {
-        const bool there = (uint32_t)page[0] < (uint32_t)a.n_pages;
-        if (there) load_page((int64_t)page[0] * a.c_page + (int64_t)slot[0] * a.c_slot, tile);
-        else load(-1, tile);
-        return there ? kAll : 0u;
-      }
-      uint32_t keys = 0;
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const bool there = (uint32_t)page[i] < (uint32_t)a.n_pages;
-        const int64_t first = (int64_t)page[i] * a.c_page + (int64_t)slot[i] * a.c_slot;
-        const gptr zero = (gptr)(const void*)attn_zeros;
-        uint16_t* dst = tile + (wave * 16 + i * kRowsLoad) * D;
-        to_lds(there ? (gptr)(kp + first) + kof[i] : zero, dst);
-        to_lds(there ? (gptr)(vp + first) + vof[i % kTurnsV] : zero, dst + kKeys * D);
-        keys |= there ? kOne << (i * kRowsLoad) : 0u;
-      }
-      return keys;
-    };
-    find(base + wave * 16);
-    uint32_t valid = 0;
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      if (i && sixteen) break;
-      if ((uint32_t)page[i] < (uint32_t)a.n_pages) valid |= sixteen ? kAll : kOne << (i * kRowsLoad);
-    }
-    find(base + kKeys + wave * 16);
-    auto turn = [&](int base, uint16_t* mine, uint16_t* other, uint32_t* fl) {
-      if (lane == 0) fl[wave] = valid;
-      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-      __syncthreads();
-      valid = fetch(other);
-      find(base + 2 * kKeys + wave * 16);
-      if (busy) work(std::false_type{}, base, mine, fl);
-    };
-    for (; base + 2 * kKeys - 1 <= lim0 && base + 3 * kKeys <= it.ke; base += 2 * kKeys) {
-      turn(base, tile0, tile1, flags);
-      turn(base + kKeys, tile1, tile0, flags + 4);
-    }
-  };
-  if (base + 2 * kKeys - 1 <= lim0 && base + 3 * kKeys <= it.ke) {
-    if (a.whole == 16) pairs(std::true_type{});
-    else if (a.whole) pairs(std::false_type{});
-  }
-  int64_t off = -1;
-  AttnKey next{0, -1};
-  if (base < it.ke) {
-    off = attn_offset(a, attn_key(a, trow, base + wave * 16 + (lane & 15), it.ke));
-    next = attn_key(a, trow, base + kKeys + wave * 16 + (lane & 15), it.ke);
-  }
-  auto turn = [&](int base, uint16_t* mine, uint16_t* other, uint32_t* fl) {
-    const uint32_t valid = (uint32_t)__ballot(off >= 0) & 0xffffu;
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-    // a tile that some rows see in part: does V, of the keys that this wave loaded, hold a value that is no number?
+  // A tile that some rows see in part: does V, of the keys that this wave loaded, hold a value that is no number?
+  auto check = [&](int base, const uint16_t* mine) -> uint32_t {
     uint32_t odd = 0;
     if (base + kKeys - 1 > lim0) {
       const uint16_t* own = mine + (kKeys + wave * 16) * D + lane * 8;
@@ -823,18 +791,106 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
         odd |= attn_not_finite<DT>(v[0]) | attn_not_finite<DT>(v[1]) | attn_not_finite<DT>(v[2]) | attn_not_finite<DT>(v[3]);
       }
     }
-    const uint32_t any_odd = __ballot(odd != 0) != 0 ? 0x10000u : 0u;
-    if (lane == 0) fl[wave] = valid | any_odd;
-    __syncthreads();
-    off = attn_offset(a, next);
-    next = attn_key(a, trow, base + 2 * kKeys + wave * 16 + (lane & 15), it.ke);
-    if (base + kKeys < it.ke) load(off, other);
-    if (busy) work(std::true_type{}, base, mine, fl);
+    return __ballot(odd != 0) != 0 ? 0x10000u : 0u;
   };
+  int base = it.kb;
+  // Where the sixteen keys of a wave lie in one page, or those of a load, what is loaded, and whether a page is there, is known on the
+  // scalar side.  Of sixteen keys that reach past the end the page's other places are loaded too, and masked as later rows' keys are.
+  // Pairs of tiles that every row sees, and that are not the last, go apart, so that this loop keeps its registers to itself.
+  auto pages = [&](auto sixteen) {  // (two loops: the test in one of them cost up to 5 percent)
+    constexpr uint32_t kAll = 0xffffu, kOne = (1u << kRowsLoad) - 1u;
+    int page[kLoads], slot[kLoads];
+    auto find = [&](int key) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        if (i && sixteen) break;
+        const int at = key + i * kRowsLoad, k = min(at, it.ke - 1), j = attn_div((uint32_t)k, a.div_mul, a.div_shift);
+        const int pg = uload(trow, j);
+        slot[i] = k - j * a.P;
+        page[i] = at < it.ke ? pg : -1;
+      }
+    };
+    auto fetch = [&](uint16_t* tile) -> uint32_t {  // the keys that are there
+      const gptr zero = (gptr)(const void*)attn_zeros;
+      uint32_t keys = 0;
+      if (sixteen) {
+        const bool there = (uint32_t)page[0] < (uint32_t)a.n_pages;
+        uint16_t* dst = tile + wave * 16 * D;
+        if (there) {
+          load_page((int64_t)page[0] * a.c_page + (int64_t)slot[0] * a.c_slot, tile);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kLoads; ++i) to_lds(zero, dst + i * kRowsLoad * D), to_lds(zero, dst + i * kRowsLoad * D + kKeys * D);
+        }
+        return there ? kAll : 0u;
+      }
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const bool there = (uint32_t)page[i] < (uint32_t)a.n_pages;
+        const int64_t first = (int64_t)page[i] * a.c_page + (int64_t)slot[i] * a.c_slot;
+        uint16_t* dst = tile + (wave * 16 + i * kRowsLoad) * D;
+        to_lds(there ? (gptr)(kp + first) + kof[i] : zero, dst);
+        to_lds(there ? (gptr)(vp + first) + vof[i % kTurnsV] : zero, dst + kKeys * D);
+        keys |= there ? kOne << (i * kRowsLoad) : 0u;
+      }
+      return keys;
+    };
+    find(base + wave * 16);
+    uint32_t valid = fetch(tile0);
+    find(base + kKeys + wave * 16);
+    auto turn = [&](auto may_edge, int base, uint16_t* mine, uint16_t* other, uint32_t* fl) {
+      __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+      const uint32_t any_odd = may_edge ? check(base, mine) : 0u;
+      if (lane == 0) fl[wave] = valid | any_odd;
+      __syncthreads();
+      if (!may_edge || base + kKeys < it.ke) {
+        valid = fetch(other);
+        find(base + 2 * kKeys + wave * 16);
+      }
+      if (busy) work(may_edge, base, mine, fl);
+    };
+    for (; base + 2 * kKeys - 1 <= lim0 && base + 2 * kKeys < it.ke; base += 2 * kKeys) {
+      turn(std::false_type{}, base, tile0, tile1, flags);
+      turn(std::false_type{}, base + kKeys, tile1, tile0, flags + 4);
+    }
+    uint16_t *mine = tile0, *other = tile1;
+    uint32_t* fl = flags;
 #pragma unroll 1
-  for (; base < it.ke; base += 2 * kKeys) {
-    turn(base, tile0, tile1, flags);
-    if (base + kKeys < it.ke) turn(base + kKeys, tile1, tile0, flags + 4);
+    for (; base < it.ke; base += kKeys) {
+      turn(std::true_type{}, base, mine, other, fl);
+      uint16_t* const t = mine;
+      mine = other, other = t, fl = flags + (4 - (fl - flags));
+    }
+  };
+  if (base < it.ke) {
+    if (a.whole == 16) {
+      pages(std::true_type{});
+    } else if (a.whole) {
+      pages(std::false_type{});
+    } else {
+      load(attn_offset(a, attn_key(a, trow, base + wave * 16 + (lane & 15), it.ke)), tile0);
+      int64_t off = attn_offset(a, attn_key(a, trow, base + wave * 16 + (lane & 15), it.ke));
+      AttnKey next = attn_key(a, trow, base + kKeys + wave * 16 + (lane & 15), it.ke);
+      auto turn = [&](int base, uint16_t* mine, uint16_t* other, uint32_t* fl) {
+        const uint32_t valid = (uint32_t)__ballot(off >= 0) & 0xffffu;
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+        const uint32_t any_odd = check(base, mine);
+        if (lane == 0) fl[wave] = valid | any_odd;
+        __syncthreads();
+        off = attn_offset(a, next);
+        next = attn_key(a, trow, base + 2 * kKeys + wave * 16 + (lane & 15), it.ke);
+        if (base + kKeys < it.ke) load(off, other);
+        if (busy) work(std::true_type{}, base, mine, fl);
+      };
+      uint16_t *mine = tile0, *other = tile1;
+      uint32_t* fl = flags;
+#pragma unroll 1
+      for (; base < it.ke; base += kKeys) {
+        turn(base, mine, other, fl);
+        uint16_t* const t = mine;
+        mine = other, other = t, fl = flags + (4 - (fl - flags));
+      }
+    }
   }
   l += __shfl_xor(l, 32, kWaveSize);
   if (p >= rows) return;  // (no barrier below)
@@ -864,8 +920,11 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
   __shared__ __align__(16) uint16_t lds[2 * 64 * D], more[2 * 64 * D];
   __shared__ uint32_t side[128];
   const int i = (int)blockIdx.x / a.Hkv, kvh = (int)blockIdx.x - i * a.Hkv;
-  if (i >= a.plan.hdr[0] || !attn_fits(a)) return;
-  const AttnItem it = a.plan.items[i];
+  // (there is room for an item a workgroup: it is read beside the header, not after it)
+  i32x8 hdr = uload8(a.plan.hdr), item = uload8(a.plan.items + i);
+  asm volatile("" : "+s"(hdr), "+s"(item));
+  if (i >= hdr[0] || !attn_fits(a, hdr)) return;
+  const AttnItem it = __builtin_bit_cast(AttnItem, item);
   const int rows = it.n * a.g;
   if (rows <= 0) return;
   if (rows > kAttnSmallRows) attn_big<DT, D>(a, it, kvh, lds, more, side);
@@ -881,8 +940,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;  // threads a row; rows, or shares of the parts, at a time
   __shared__ f32x4 acc_s[kGroups][kLanes];
   __shared__ float sum_s[kGroups], top_s[kGroups];
-  if (!attn_fits(a)) return;
-  const int work = a.plan.hdr[1] * a.Hkv;
+  const i32x8 hdr = uload8(a.plan.hdr);
+  if (!attn_fits(a, hdr)) return;
+  const int work = hdr[1] * a.Hkv;
   for (int w = blockIdx.x; w < work; w += gridDim.x) {
     const int i = w / a.Hkv, kvh = w - i * a.Hkv;
     const AttnJoin jn = a.plan.joins[i];
