@@ -13,12 +13,15 @@
 // a step each, of random sign, so about as much as the rounding of the result itself.
 //
 // Sequences of up to 32 tile rows (decoding, short chunks) are bound by HBM: the four waves of a workgroup take 32 keys in turn,
-// K straight to registers, V through a part of LDS of the wave's own, no barrier until the end.  Others take 128 tile rows
-// a workgroup, 32 a wave, over K and V tiles of 64 keys that the four waves share.  A long axis is cut into parts where there are few
+// K straight to registers, V through a part of LDS of the wave's own, no barrier until the end.  256 single tokens over up to 4095,
+// 8 kv heads of 128: 2.13 GB in 376 us, 5.7 TB/s (a plain copy reaches 4.9); three over 131000 5.8 TB/s.  (Three or four workgroups a CU,
+// with fewer registers: 433 and 688 us.)  Others take 128 tile rows a workgroup, 32 a wave, over K and V tiles of 64 keys that the four
+// waves share: 2048 rows of 32 heads over 14336 tokens 512 us, 1.0 PFLOP/s (a library's matrix product of 8192 a side 1.17); the
+// matrix cores are busy half of the time at the 1.9 GHz that the card's power leaves them, and LDS a quarter of it, without conflicts.  A long axis is cut into parts where there are few
 // tiles (the plan decides, by the batch's total of keys); the parts' results are joined by a second launch, in order.
 //
-// Keys past a sequence's end and keys of pages that the pool does not hold read as zeros from a constant and get no weight.
-// Keys of later rows of a chunk are in the cache already; their weight is zero, but zero times an infinity or NaN is
+// Keys of pages that the pool does not hold, and mostly keys past a sequence's end, read as zeros from a constant and get no weight.
+// Keys of later rows of a chunk, and the other places of a last page, are in the cache; their weight is zero, but zero times an infinity or NaN is
 // not, so the tiles that some rows see in part look whether their V has such a value and then add key by key to the rows that see it.
 #pragma once
 #include <type_traits>
@@ -37,12 +40,20 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-constexpr int kAttnSmallRows = 32;   // tile rows of a sequence up to which it takes the few-row path
+// Tile rows of a sequence up to which it takes the few-row path.  (64 chunks of eight rows, four heads a kv head, over up to 4000
+// tokens, 32 tile rows each: 125 + 9 us, of the other path 144 + 4; more do not fit a wave's registers.)
+constexpr int kAttnSmallRows = 32;
 constexpr int kAttnBigRows = 128;    // tile rows of a workgroup of the other
 constexpr int kAttnSlots = 512;      // workgroups on the card at a time: two a CU
-constexpr int kAttnSmallItems = 2048, kAttnBigItems = 1024;  // workgroups over the card that tiles are cut for, at most
-constexpr int kAttnMinKeys = 256;    // keys of a part, at least
-constexpr int kAttnManyParts = 16;   // parts of a tile from which the threads of a join share them out
+// Workgroups over the card that tiles are cut for, at most: four turns of it even out sequences of uneven lengths, more cost more in
+// joins.  (1024, 2048, 4096 for few rows: 256 single tokens over up to 4095 tokens 389, 384, 382 us with the join, 64 chunks of eight
+// rows 127, 134, 159, one chunk of 128 rows over 30000 tokens 95, 88, 89.)
+constexpr int kAttnSmallItems = 2048, kAttnBigItems = 1024;
+// Keys of a part, at least: two turns of the four waves.  (128, 256, 512: a token over 2000 tokens 7.0, 8.5, 11.2 us, four over 4000
+// 19.8, 15.4, 15.9, 32 over up to 1500 36, 31, 28 with the join.)
+constexpr int kAttnMinKeys = 256;
+// Parts of a few-row tile from which the threads of a join share them out.  (85 parts: 30 us one after the other, 7 so; 8 parts 5.8 and 5.0.)
+constexpr int kAttnManyParts = 8;
 
 struct AttnItem {   // a tile of a sequence and a part of its keys
   int row0, n, len, trow;  // the sequence: first row, rows, tokens, row of the page table
@@ -65,7 +76,7 @@ struct AttnPlanView {
 
 inline int attn_tiles_max(int T, int S, int g) { return (int)((int64_t)T * g / kAttnBigRows) + S; }
 inline int attn_items_max(int T, int S, int g, int Hkv) { return attn_tiles_max(T, S, g) + (kAttnSmallItems + kAttnBigItems) / Hkv + 2; }
-// (a tile's rows are joined by at most rows / 8 workgroups, or by eight where its parts are 16 and more)
+// (a tile's rows are joined by at most rows / 8 workgroups, or by eight where its parts are eight and more)
 inline int attn_joins_max(int T, int S, int g, int Hkv) {
   const int64_t cut = (4 * kAttnSmallItems + 16 * kAttnBigItems) / Hkv + 16, tiles = (int64_t)attn_tiles_max(T, S, g) * 16;
   return (int)(cut < tiles ? cut : tiles);
@@ -136,8 +147,8 @@ __device__ __forceinline__ int attn_shares(const AttnSeq& q, int parts, int g) {
 constexpr int kAttnPlanLds = kAttnPlanThreads;  // up to here the sequences stay in LDS: every read of memory is most of a microsecond
 
 // The number of parts that a tile of the card's average length is cut into, for n tiles (times kv heads): as many as leave the
-// card's places for workgroups fullest, if that is worth the parts' traffic.  (Cutting 512 chunks' tiles, which just fill the card,
-// in two: 2048 rows over 14336 tokens 600 -> 657 us.)
+// card's places for workgroups fullest, if that is worth the parts' traffic.  (Cutting 512 tiles, which just fill the card, in two:
+// 2048 rows over 14336 tokens 524 -> 527 us and 17 for the join.)
 __device__ __forceinline__ int attn_parts(int n) {
   if (n >= kAttnBigItems) return 1;
   constexpr int kParts[8] = {1, 2, 3, 4, 6, 8, 12, 16};
@@ -238,7 +249,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
   }
   __syncthreads();
   // Items with few rows stream, the others compute: they take turns, so that both have the card together (mixed batch of four prompts
-  // of 512 and 64 single tokens, 32 heads: the others all first 251 us, in turns 245; alone the two take 81 and 189).
+  // of 512 rows over up to 1500 tokens and 64 single tokens, 32 heads: the others all first 246 us, in turns 235; alone 53 and 190).
   const int both = min(at[0], at[1]);
   struct Place {
     AttnItem it;
@@ -279,7 +290,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
   };
   // Where the others are most of the items, and more than the card takes at a time, the long ones go first, over all sequences (by
   // eighths of an octave): a long one that starts among the last keeps the rest of the card waiting.  In all, sequence by sequence and so:
-  // nine prompts of 700 rows over up to 3000 tokens 262 and 246 us, 64 of 16 rows over up to 4000 tokens 168 and 139; but beside many
+  // nine prompts of 700 rows over up to 3000 tokens 262 and 246 us, 64 of 16 rows over up to 4000 tokens 158 and 129; but beside many
   // items with few rows the two ways to take turns quarrel (eight prompts of 512 rows, 128 single tokens 298 and 315).
   const bool sorted = at[1] > kAttnSlots / a.Hkv && at[1] > at[0];
   auto bin_of = [](const AttnItem& it) { return 255 - (int)((__float_as_uint((float)(it.ke - it.kb) + 1.0f) >> 20) - (127u << 3)); };
@@ -934,7 +945,9 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
 
 // The parts of a tile's rows, each weighed by its maximum against the largest.  A thread takes four dimensions of a row and, where the parts
 // are many, every eighth of them; the eight are then added in order.
-constexpr int kAttnJoinBlocks = 2048;  // workgroups of the join (the host knows a bound of the joins only, and workgroups without work cost too)
+// Workgroups of the join: the host knows a bound of the joins only, and workgroups without work cost too.  (512, 2048, 8192: a mixed batch 13,
+// 8.4, 9.3 us, 256 single tokens 5.2, 4.3, 4.4.)
+constexpr int kAttnJoinBlocks = 2048;
 template <int DT, int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   constexpr int kLanes = D / 4, kGroups = 256 / kLanes;  // threads a row; rows, or shares of the parts, at a time
