@@ -434,6 +434,18 @@ __device__ __forceinline__ uint16_t* attn_out_row(const AttnArgs& a, const AttnI
   return a.out + (int64_t)(it.row0 + p / a.g) * a.o_row + (int64_t)(kvh * a.g + p % a.g) * a.o_head;
 }
 
+// the larger of a lane's and its partner's, 16 or 32 lanes on, without a trip through LDS
+__device__ __forceinline__ float attn_max16(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const auto both = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+__device__ __forceinline__ float attn_max32(float x) {
+  const uint32_t u = __float_as_uint(x);
+  const auto both = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1]));
+}
+
 // (the hardware's own: results under the smallest normal float are zero)
 __device__ __forceinline__ float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -535,8 +547,7 @@ __device__ __forceinline__ void attn_small(const AttnArgs& a, const AttnItem& it
       }
       float mx = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
                        fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
-      mx = fmaxf(mx, __shfl_xor(mx, 16, kWaveSize));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, kWaveSize));
+      mx = attn_max32(attn_max16(mx));
       const float mn = fmaxf(m[t], mx), ref = mn == -INFINITY ? 0.0f : mn * a.scale, ms = ref - kAttnBias<DT>;
       const float turn = attn_exp2(m[t] * a.scale - ref);
       m[t] = mn;
@@ -678,16 +689,19 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
   auto to_lds = [&](gptr from, uint16_t* to) {
     __builtin_amdgcn_global_load_lds((SMLM_GLOBAL void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
   };
-  // the wave's sixteen keys lie in one page: an address for all lanes, made on the scalar side, and an offset that stays
+  // Rows of one page: an address for all lanes, made on the scalar side, and an offset that stays.  (Through a buffer resource: a load
+  // to LDS with a lane's own address counts as an access to LDS too, and every wait for an operand then waits for all that are on their way.)
+  auto page_to_lds = [&](const uint16_t* rows, uint32_t lane_bytes, uint32_t bytes, uint16_t* to) {
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(rows), 0, 0xffffffffu, 0x00020000);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)to, 16, lane_bytes, bytes, 0, 0);
+  };
   auto load_page = [&](int64_t first, uint16_t* tile) {
     uint16_t* dst = tile + wave * 16 * D;
-    gptr ks = (gptr)(kp + first), vs = (gptr)(vp + first);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       asm volatile("" : "+v"(kof[i]), "+v"(vof[i % kTurnsV]));  // (kept as 32 bits over the loop)
-      to_lds(ks + kof[i], dst + i * kRowsLoad * D);
-      to_lds(vs + vof[i % kTurnsV], dst + i * kRowsLoad * D + kKeys * D);
-      ks += (uint32_t)kRowsLoad * slot_bytes, vs += (uint32_t)kRowsLoad * slot_bytes;
+      page_to_lds(kp + first, kof[i], (uint32_t)(i * kRowsLoad) * slot_bytes, dst + i * kRowsLoad * D);
+      page_to_lds(vp + first, vof[i % kTurnsV], (uint32_t)(i * kRowsLoad) * slot_bytes, dst + i * kRowsLoad * D + kKeys * D);
     }
   };
   auto load = [&](int64_t off, uint16_t* tile) {
@@ -704,7 +718,7 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
       to_lds((gptr)(f >= 0 ? vp + f + dv : zero), dst + i * kRowsLoad * D + kKeys * D);
     }
   };
-  auto work = [&](auto may_edge, int base, const uint16_t* kl, const uint32_t* fl) {
+  auto work = [&](auto may_edge, int base, const uint16_t* kl, const uint32_t* fl, auto between) {
     const uint16_t* vl = kl + kKeys * D;
     const bool edge = may_edge && base + kKeys - 1 > lim0;
     const uint64_t ok = (uint64_t)((fl[0] & 0xffffu) | (fl[1] << 16)) | ((uint64_t)((fl[2] & 0xffffu) | (fl[3] << 16)) << 32);
@@ -719,6 +733,15 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
         s[u] = mfma32<DT>(kf, q[k], s[u]);
       }
     }
+    // Six reads ahead of the products, and eight in the second: left to itself each product waits for the read before it.  (Both: 2 to 4
+    // percent where the card's power is not the bound, 1 where it is.)
+    __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+    for (int i = 0; i < 2 * kSteps - 6; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, 6, 0);
     if (edge || ok != ~0ull) {
       const uint64_t there = ok >> (4 * h);
       const int seen = lim - base - 4 * h;
@@ -735,7 +758,8 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[u][e]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32, kWaveSize));
+    mx = attn_max32(mx);
+    between();
     // The reference that the exponents are taken against follows the running maximum only once that is 2^8 past it: the
     // probabilities stay below 2^8 (2^15 with the bias), inside the element types, and most tiles leave the accumulators alone.
     if (__ballot((mx - m) * a.scale > 8.0f)) {
@@ -766,6 +790,13 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
             const uint16_t* at = vl + (u * 32 + ks * 16) * D;
             o[i] = mfma32<DT>(attn_v_pair(at + vat[i], at + vat[i] + 8 * D), pf[u][ks], o[i]);
           }
+      __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+#pragma unroll
+      for (int i = 0; i < 4 * kBlk - 4; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
     } else {
 #pragma unroll 1
       for (int x = 0; x < kKeys; ++x) {  // slot j of half hh in step st of sixteen keys
@@ -822,7 +853,7 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
       }
     };
     auto fetch = [&](uint16_t* tile) -> uint32_t {  // the keys that are there
-      const gptr zero = (gptr)(const void*)attn_zeros;
+      const uint16_t* zero = reinterpret_cast<const uint16_t*>(attn_zeros);
       uint32_t keys = 0;
       if (sixteen) {
         const bool there = (uint32_t)page[0] < (uint32_t)a.n_pages;
@@ -831,7 +862,10 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
           load_page((int64_t)page[0] * a.c_page + (int64_t)slot[0] * a.c_slot, tile);
         } else {
 #pragma unroll
-          for (int i = 0; i < kLoads; ++i) to_lds(zero, dst + i * kRowsLoad * D), to_lds(zero, dst + i * kRowsLoad * D + kKeys * D);
+          for (int i = 0; i < kLoads; ++i) {
+            page_to_lds(zero, 0, 0, dst + i * kRowsLoad * D);
+            page_to_lds(zero, 0, 0, dst + i * kRowsLoad * D + kKeys * D);
+          }
         }
         return there ? kAll : 0u;
       }
@@ -840,8 +874,8 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
         const bool there = (uint32_t)page[i] < (uint32_t)a.n_pages;
         const int64_t first = (int64_t)page[i] * a.c_page + (int64_t)slot[i] * a.c_slot;
         uint16_t* dst = tile + (wave * 16 + i * kRowsLoad) * D;
-        to_lds(there ? (gptr)(kp + first) + kof[i] : zero, dst);
-        to_lds(there ? (gptr)(vp + first) + vof[i % kTurnsV] : zero, dst + kKeys * D);
+        page_to_lds(there ? kp + first : zero, there ? kof[i] : 0u, 0, dst);
+        page_to_lds(there ? vp + first : zero, there ? vof[i % kTurnsV] : 0u, 0, dst + kKeys * D);
         keys |= there ? kOne << (i * kRowsLoad) : 0u;
       }
       return keys;
@@ -856,9 +890,10 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
       __syncthreads();
       if (!may_edge || base + kKeys < it.ke) {
         valid = fetch(other);
-        find(base + 2 * kKeys + wave * 16);
+        if (!busy) find(base + 2 * kKeys + wave * 16);
       }
-      if (busy) work(may_edge, base, mine, fl);
+      // (the pages' numbers are asked for where nothing is waited for in LDS: the counter is one)
+      if (busy) work(may_edge, base, mine, fl, [&] { find(base + 2 * kKeys + wave * 16); });
     };
     for (; base + 2 * kKeys - 1 <= lim0 && base + 2 * kKeys < it.ke; base += 2 * kKeys) {
       turn(std::false_type{}, base, tile0, tile1, flags);
@@ -891,7 +926,7 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
         off = attn_offset(a, next);
         next = attn_key(a, trow, base + 2 * kKeys + wave * 16 + (lane & 15), it.ke);
         if (base + kKeys < it.ke) load(off, other);
-        if (busy) work(std::true_type{}, base, mine, fl);
+        if (busy) work(std::true_type{}, base, mine, fl, [] {});
       };
       uint16_t *mine = tile0, *other = tile1;
       uint32_t* fl = flags;
