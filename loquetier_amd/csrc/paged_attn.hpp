@@ -12,13 +12,14 @@
 // and accumulators in float.  The probabilities are rounded to the element type for the second product: relative errors of half
 // a step each, of random sign, so about as much as the rounding of the result itself.
 //
-// Sequences of up to 32 tile rows (decoding, short chunks) are bound by HBM: the four waves of a workgroup take 32 keys in turn,
-// K straight to registers, V through a part of LDS of the wave's own, no barrier until the end.  256 single tokens over up to 4095,
-// 8 kv heads of 128: 2.13 GB in 376 us, 5.7 TB/s (a plain copy reaches 4.9); three over 131000 5.8 TB/s.  (Three or four workgroups a CU,
-// with fewer registers: 433 and 688 us.)  Others take 128 tile rows a workgroup, 32 a wave, over K and V tiles of 64 keys that the four
-// waves share: 2048 rows of 32 heads over 14336 tokens 512 us, 1.0 PFLOP/s (a library's matrix product of 8192 a side 1.17); the
-// matrix cores are busy half of the time at the 1.9 GHz that the card's power leaves them, and LDS a quarter of it, without conflicts.  A long axis is cut into parts where there are few
-// tiles (the plan decides, by the batch's total of keys); the parts' results are joined by a second launch, in order.
+// Sequences of up to 16 tile rows (decoding) are bound by HBM: the four waves of a workgroup take 32 keys in turn, K straight to
+// registers, V through a part of LDS of the wave's own, no barrier until the end.  256 single tokens over up to 4095, 8 kv heads of 128:
+// 2.13 GB in 362 to 382 us by the card, 5.6 to 5.9 TB/s (a plain copy reaches 4.9); three over 131000 5.8 TB/s.  (Three or four workgroups
+// a CU, with fewer registers: 433 and 688 us.)  Others take 128 tile rows a workgroup, 32 a wave, over K and V tiles of 64 keys that the
+// four waves share: 2048 rows of 32 heads over 14336 tokens 500 to 535 us by the card, 0.96 to 1.03 PFLOP/s (a library's matrix product of 8192
+// a side 1.17); the matrix cores are busy half of the time at the 1.9 GHz that the card's power leaves them, and LDS a quarter of it,
+// without conflicts.  A long axis is cut into parts where there are few tiles (the plan decides, by the batch's total of keys); the
+// parts' results are joined by a second launch, in order.
 //
 // Keys of pages that the pool does not hold, and mostly keys past a sequence's end, read as zeros from a constant and get no weight.
 // Keys of later rows of a chunk, and the other places of a last page, are in the cache; their weight is zero, but zero times an infinity or NaN is
@@ -40,17 +41,18 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Tile rows of a sequence up to which it takes the few-row path.  (64 chunks of eight rows, four heads a kv head, over up to 4000
-// tokens, 32 tile rows each: 125 + 9 us, of the other path 144 + 4; more do not fit a wave's registers.)
-constexpr int kAttnSmallRows = 32;
+// Tile rows of a sequence up to which it takes the few-row path: one operand's.  (Two operands, 32 rows, with the join: 64 chunks of eight
+// rows, four heads a kv head, over up to 4000 tokens 133 us, on the other path 119, 16 over 2000 43 and 31, four over 30000 123 and 95; with
+// heads of 64 73 and 76.)
+constexpr int kAttnSmallRows = 16;
 constexpr int kAttnBigRows = 128;    // tile rows of a workgroup of the other
 constexpr int kAttnSlots = 512;      // workgroups on the card at a time: two a CU
 // Workgroups over the card that tiles are cut for, at most: four turns of it even out sequences of uneven lengths, more cost more in
-// joins.  (1024, 2048, 4096 for few rows: 256 single tokens over up to 4095 tokens 389, 384, 382 us with the join, 64 chunks of eight
-// rows 127, 134, 159, one chunk of 128 rows over 30000 tokens 95, 88, 89.)
+// joins.  (1024, 2048, 4096 for few rows, with the join: 256 single tokens over up to 4095 tokens 394, 386, 387 us, three over up to 131000 251,
+// 259, 267, 64 chunks of four rows 118, 121, 137, eight prompts of 512 rows and 128 single tokens 282, 291, 317.)
 constexpr int kAttnSmallItems = 2048, kAttnBigItems = 1024;
-// Keys of a part, at least: two turns of the four waves.  (128, 256, 512: a token over 2000 tokens 7.0, 8.5, 11.2 us, four over 4000
-// 19.8, 15.4, 15.9, 32 over up to 1500 36, 31, 28 with the join.)
+// Keys of a part, at least: two turns of the four waves.  (128, 256, 512: a token over 2000 tokens 6.7, 8.2, 10.8 us, four over 4000
+// 19.3, 15.9, 15.6, 32 over up to 1500 with the join 34, 30, 28.)
 constexpr int kAttnMinKeys = 256;
 // Parts of a few-row tile from which the threads of a join share them out.  (85 parts: 30 us one after the other, 7 so; 8 parts 5.8 and 5.0.)
 constexpr int kAttnManyParts = 8;
@@ -148,14 +150,14 @@ constexpr int kAttnPlanLds = kAttnPlanThreads;  // up to here the sequences stay
 
 // The number of parts that a tile of the card's average length is cut into, for n tiles (times kv heads): as many as leave the
 // card's places for workgroups fullest, if that is worth the parts' traffic.  (Cutting 512 tiles, which just fill the card, in two:
-// 2048 rows over 14336 tokens 524 -> 527 us and 17 for the join.)
+// 2048 rows over 14336 tokens 502 -> 509 us and 17 for the join.  Up to 16, 32 and 64 parts: eight tiles over 100000 tokens 132, 89, 92 with the join.)
 __device__ __forceinline__ int attn_parts(int n) {
   if (n >= kAttnBigItems) return 1;
-  constexpr int kParts[8] = {1, 2, 3, 4, 6, 8, 12, 16};
+  constexpr int kParts[9] = {1, 2, 3, 4, 6, 8, 12, 16, 32};
   int best = 1;
   float cost = 1e30f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 9; ++i) {
     const float c = (float)((n * kParts[i] + kAttnSlots - 1) / kAttnSlots) * (i ? 1.1f / (float)kParts[i] : 1.0f);
     if (c < cost * 0.97f) cost = c, best = kParts[i];
   }
@@ -249,7 +251,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
   }
   __syncthreads();
   // Items with few rows stream, the others compute: they take turns, so that both have the card together (mixed batch of four prompts
-  // of 512 rows over up to 1500 tokens and 64 single tokens, 32 heads: the others all first 246 us, in turns 235; alone 53 and 190).
+  // of 512 rows over up to 1500 tokens and 64 single tokens, 32 heads: the others all first 240 us, in turns 231; alone 50 and 191).
   const int both = min(at[0], at[1]);
   struct Place {
     AttnItem it;
@@ -289,9 +291,9 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
     return Place{it, q, kind, x, lo, t, j, (int)ns, part0, fits};
   };
   // Where the others are most of the items, and more than the card takes at a time, the long ones go first, over all sequences (by
-  // eighths of an octave): a long one that starts among the last keeps the rest of the card waiting.  In all, sequence by sequence and so:
-  // nine prompts of 700 rows over up to 3000 tokens 262 and 246 us, 64 of 16 rows over up to 4000 tokens 158 and 129; but beside many
-  // items with few rows the two ways to take turns quarrel (eight prompts of 512 rows, 128 single tokens 298 and 315).
+  // eighths of an octave): a long one that starts among the last keeps the rest of the card waiting.  Sequence by sequence and so: nine
+  // prompts of 700 rows over up to 3000 tokens 242 and 227 us, 64 of 16 rows over up to 4000 151 and 123, four of 512 over up to 1500 57 and 50;
+  // but beside many items with few rows the two ways to take turns quarrel (eight prompts of 512 rows, 128 single tokens 280 and 294).
   const bool sorted = at[1] > kAttnSlots / a.Hkv && at[1] > at[0];
   auto bin_of = [](const AttnItem& it) { return 255 - (int)((__float_as_uint((float)(it.ke - it.kb) + 1.0f) >> 20) - (127u << 3)); };
   if (sorted) {
@@ -449,9 +451,9 @@ __device__ __forceinline__ float attn_max32(float x) {
 // (the hardware's own: results under the smallest normal float are zero)
 __device__ __forceinline__ float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Up to 16 * MT tile rows.  Layouts of a 16 x 16 x 32 product by lane (c = lane & 15, b = lane >> 4): operands row or column c,
+// Up to 16 tile rows.  Layouts of a 16 x 16 x 32 product by lane (c = lane & 15, b = lane >> 4): operands row or column c,
 // k = 8 b + 0..7; result column c, rows 4 b + 0..3.
-template <int DT, int D, int MT>
+template <int DT, int D>
 __device__ __forceinline__ void attn_small(const AttnArgs& a, const AttnItem& it, int kvh, uint16_t* lds, float* ml) {
   constexpr int kSteps = D / 32, kBlk = D / 16, kVLoads = D / 16;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, c = lane & 15, b = lane >> 4;
@@ -461,29 +463,23 @@ __device__ __forceinline__ void attn_small(const AttnArgs& a, const AttnItem& it
   uint16_t* vl = lds + wave * 32 * D;
   const u32x4 zero4 = {0u, 0u, 0u, 0u};
 
-  u32x4 q[MT][kSteps];
-  int lim[MT];
-#pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const int p = it.first + t * 16 + c, pc = p < rows ? p : 0;
+  const int p = it.first + c, pc = p < rows ? p : 0;
+  const int lim = min(it.ke - 1, it.len - it.n + pc / a.g);
+  u32x4 q[kSteps];
+  {
     const uint16_t* src = a.q + (int64_t)(it.row0 + pc / a.g) * a.q_row + (int64_t)(kvh * a.g + pc % a.g) * a.q_head;
-    lim[t] = min(it.ke - 1, it.len - it.n + pc / a.g);
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
       const u32x4 x = ldg16(src + s * 32 + b * 8);
-      q[t][s] = p < rows ? x : zero4;
+      q[s] = p < rows ? x : zero4;
     }
   }
   const int lim0 = it.len - it.n + it.first / a.g;  // the first row's: a tile up to it is seen whole by all
 
-  f32x4 o[MT][kBlk];
-  float m[MT], l[MT];
+  f32x4 o[kBlk];
+  float m = -INFINITY, l = 0.0f;
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    m[t] = -INFINITY, l[t] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kBlk; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int i = 0; i < kBlk; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   u32x4 kr[2][kSteps], vr[kVLoads];
   constexpr int kRowLanes = D / 8, kRowsLoad = 64 / kRowLanes;  // lanes a row of V, rows a load
   int vat[kBlk];
@@ -509,15 +505,13 @@ __device__ __forceinline__ void attn_small(const AttnArgs& a, const AttnItem& it
   }
   for (int base = it.kb + wave * 32; base < it.ke; base += 128) {
     const uint32_t ok = (uint32_t)__ballot(off >= 0);
-    f32x4 s[MT][2];
+    f32x4 s[2];
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
+    for (int u = 0; u < 2; ++u) {
+      s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        s[t][u] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) s[t][u] = Num<DT>::mfma(kr[u][k], q[t][k], s[t][u]);
-      }
+      for (int k = 0; k < kSteps; ++k) s[u] = Num<DT>::mfma(kr[u][k], q[k], s[u]);
+    }
     const bool edge = base + 31 > lim0;
     uint32_t odd = 0;
 #pragma unroll
@@ -531,46 +525,41 @@ __device__ __forceinline__ void attn_small(const AttnArgs& a, const AttnItem& it
     load(off);
 
     const bool guard = edge && __ballot(odd != 0) != 0;
-    u32x4 pf[MT];
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-      if (edge || ok != 0xffffffffu) {
-        const uint32_t there = ok >> (b * 4);
-        const int seen = lim[t] - base - b * 4;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = u * 16 + i;  // (and 4 b more)
-            if (!(there >> key & 1) || key > seen) s[t][u][i] = -INFINITY;
-          }
-      }
-      float mx = fmaxf(fmaxf(fmaxf(s[t][0][0], s[t][0][1]), fmaxf(s[t][0][2], s[t][0][3])),
-                       fmaxf(fmaxf(s[t][1][0], s[t][1][1]), fmaxf(s[t][1][2], s[t][1][3])));
-      mx = attn_max32(attn_max16(mx));
-      const float mn = fmaxf(m[t], mx), ref = mn == -INFINITY ? 0.0f : mn * a.scale, ms = ref - kAttnBias<DT>;
-      const float turn = attn_exp2(m[t] * a.scale - ref);
-      m[t] = mn;
-      float sum = 0.0f, p[8];
+    if (edge || ok != 0xffffffffu) {
+      const uint32_t there = ok >> (b * 4);
+      const int seen = lim - base - b * 4;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          p[u * 4 + i] = attn_exp2(s[t][u][i] * a.scale - ms);
-          sum += p[u * 4 + i];
+          const int key = u * 16 + i;  // (and 4 b more)
+          if (!(there >> key & 1) || key > seen) s[u][i] = -INFINITY;
         }
-      l[t] = l[t] * turn + sum;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) pf[t][i] = pack2<DT>(p[2 * i], p[2 * i + 1]);
-#pragma unroll
-      for (int i = 0; i < kBlk; ++i) o[t][i] *= turn;
     }
+    const float mx = attn_max32(attn_max16(fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                                                 fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])))));
+    const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.0f : mn * a.scale, ms = ref - kAttnBias<DT>;
+    const float turn = attn_exp2(m * a.scale - ref);
+    m = mn;
+    float sum = 0.0f, w[8];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[u * 4 + i] = attn_exp2(s[u][i] * a.scale - ms);
+        sum += w[u * 4 + i];
+      }
+    l = l * turn + sum;
+    u32x4 pf;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pf[i] = pack2<DT>(w[2 * i], w[2 * i + 1]);
+#pragma unroll
+    for (int i = 0; i < kBlk; ++i) o[i] *= turn;
     if (!guard) {
 #pragma unroll
       for (int i = 0; i < kBlk; ++i) {
         const u32x4 vf = attn_v_pair(vl + vat[i], vl + vat[i] + 16 * D);
-#pragma unroll
-        for (int t = 0; t < MT; ++t) o[t][i] = Num<DT>::mfma(vf, pf[t], o[t][i]);
+        o[i] = Num<DT>::mfma(vf, pf, o[i]);
       }
     } else {  // key by key: slot j of lane group bb
 #pragma unroll 1
@@ -583,52 +572,46 @@ __device__ __forceinline__ void attn_small(const AttnArgs& a, const AttnItem& it
 #pragma unroll
         for (int i = 0; i < kBlk; ++i) {
           const u32x4 vf = attn_v_pair(vl + vat[i], vl + vat[i] + 16 * D) & only;
-#pragma unroll
-          for (int t = 0; t < MT; ++t) {
-            const f32x4 add = Num<DT>::mfma(vf, pf[t] & only, f32x4{0.f, 0.f, 0.f, 0.f});
-            if (base + key <= lim[t]) o[t][i] += add;
-          }
+          const f32x4 add = Num<DT>::mfma(vf, pf & only, f32x4{0.f, 0.f, 0.f, 0.f});
+          if (base + key <= lim) o[i] += add;
         }
       }
     }
     __builtin_amdgcn_wave_barrier();  // (this wave's LDS reads come before its next writes)
   }
 
-  // the four waves' results, 16 rows at a time
+  // the four waves' results
   float* ol = reinterpret_cast<float*>(lds);  // [4][16][D]
+  l += __shfl_xor(l, 16, kWaveSize);
+  l += __shfl_xor(l, 32, kWaveSize);
+  __syncthreads();  // V has been read
+  if (b == 0) ml[(wave * 16 + c) * 2] = m * a.scale, ml[(wave * 16 + c) * 2 + 1] = l;
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    l[t] += __shfl_xor(l[t], 16, kWaveSize);
-    l[t] += __shfl_xor(l[t], 32, kWaveSize);
-    __syncthreads();  // V, or the last turn's results, have been read
-    if (b == 0) ml[(wave * 16 + c) * 2] = m[t] * a.scale, ml[(wave * 16 + c) * 2 + 1] = l[t];
+  for (int i = 0; i < kBlk; ++i) *(f32x4*)(ol + (wave * 16 + c) * D + ((i * 4 + b) ^ (c & 7)) * 4) = o[i];
+  __syncthreads();
+  for (int x = threadIdx.x; x < 16 * (D / 4); x += 256) {
+    const int r = x / (D / 4), d4 = x % (D / 4), row = it.first + r;
+    if (row >= rows) continue;
+    float mw[4], top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kBlk; ++i) *(f32x4*)(ol + (wave * 16 + c) * D + ((i * 4 + b) ^ (c & 7)) * 4) = o[t][i];
-    __syncthreads();
-    for (int x = threadIdx.x; x < 16 * (D / 4); x += 256) {
-      const int r = x / (D / 4), d4 = x % (D / 4), p = it.first + t * 16 + r;
-      if (p >= rows) continue;
-      float mw[4], top = -INFINITY, sum = 0.0f;
+    for (int w = 0; w < 4; ++w) mw[w] = ml[(w * 16 + r) * 2], top = fmaxf(top, mw[w]);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 0; w < 4; ++w) mw[w] = ml[(w * 16 + r) * 2], top = fmaxf(top, mw[w]);
-      const float ref = top == -INFINITY ? 0.0f : top;
-      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float f = attn_exp2(mw[w] - ref);
-        sum += f * ml[(w * 16 + r) * 2 + 1];
-        const f32x4 v = *(const f32x4*)(ol + (w * 16 + r) * D + (d4 ^ (r & 7)) * 4);
-        acc += f * v;
-      }
-      if (it.part >= 0) {
-        const int64_t at = ((int64_t)it.part * a.Hkv + kvh) * kAttnSmallRows + t * 16 + r;
-        *(SMLM_GLOBAL f32x4*)(a.po_small + at * D + d4 * 4) = acc;
-        if (d4 == 0) a.pm_small[at * 2] = top, a.pm_small[at * 2 + 1] = sum;
-      } else {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        *(SMLM_GLOBAL u32x2*)(attn_out_row(a, it, kvh, p) + d4 * 4) =
-            attn_pack4<DT>(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
-      }
+    for (int w = 0; w < 4; ++w) {
+      const float f = attn_exp2(mw[w] - ref);
+      sum += f * ml[(w * 16 + r) * 2 + 1];
+      const f32x4 v = *(const f32x4*)(ol + (w * 16 + r) * D + (d4 ^ (r & 7)) * 4);
+      acc += f * v;
+    }
+    if (it.part >= 0) {
+      const int64_t at = ((int64_t)it.part * a.Hkv + kvh) * kAttnSmallRows + r;
+      *(SMLM_GLOBAL f32x4*)(a.po_small + at * D + d4 * 4) = acc;
+      if (d4 == 0) a.pm_small[at * 2] = top, a.pm_small[at * 2 + 1] = sum;
+    } else {
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      *(SMLM_GLOBAL u32x2*)(attn_out_row(a, it, kvh, row) + d4 * 4) =
+          attn_pack4<DT>(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
     }
   }
 }
@@ -974,8 +957,7 @@ __global__ __launch_bounds__(256, 2) void attn_kernel(AttnArgs a) {
   const int rows = it.n * a.g;
   if (rows <= 0) return;
   if (rows > kAttnSmallRows) attn_big<DT, D>(a, it, kvh, lds, more, side);
-  else if (rows > 16) attn_small<DT, D, 2>(a, it, kvh, lds, reinterpret_cast<float*>(side));
-  else attn_small<DT, D, 1>(a, it, kvh, lds, reinterpret_cast<float*>(side));
+  else attn_small<DT, D>(a, it, kvh, lds, reinterpret_cast<float*>(side));
 }
 
 // The parts of a tile's rows, each weighed by its maximum against the largest.  A thread takes four dimensions of a row and, where the parts

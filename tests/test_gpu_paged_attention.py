@@ -312,6 +312,33 @@ def test_sequences_that_overlap_stay_in_bounds(K):
         assert bool((out[0] == 9).all()) and bool((out[-1] == 9).all())
 
 
+@pytest.mark.parametrize("P,D", [(16, 128), (48, 64), (20, 128), (8, 64), (7, 128)])
+def test_ends_of_tiles_and_pages(K, P, D):
+    """Lengths around tiles of 64 keys and pairs of them, for chunks of some rows and many, no number in any other place of the pool."""
+    seqs = [(n, length - n) for length in (40, 63, 64, 65, 127, 128, 129, 191, 192, 193, 255, 256, 257, 320) for n in (9, 40)]
+    b = batch("bf16", seqs, 4, 2, D, P, seed=21)
+    want, bound = expected(b)
+    used = torch.zeros(b["kc"].shape[0], P, dtype=torch.bool, device="cuda")
+    for i, (n, c) in enumerate(seqs):
+        tok = torch.arange(n + c, device="cuda")
+        used[b["table"][i].long()[tok // P], tok % P] = True
+    for cache in (b["kc"], b["vc"]):
+        cache.transpose(1, 2)[~used] = math.nan
+    near(run(K, b), want, bound)
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("Hq,Hkv", [(8, 8), (8, 2), (6, 2)])
+def test_tile_rows_around_the_paths(K, dt, Hq, Hkv):
+    """Rows of a kv head up to 16 and past it, up to 128 and past it, over lengths that are cut into few parts and many."""
+    g = Hq // Hkv
+    news = sorted({max(1, n // g + d) for n in (16, 32, 128) for d in (0, 1)})
+    near(*((lambda b: (run(K, b), *expected(b)))(batch(dt, [(n, c) for n in news for c in (0, 70, 600)], Hq, Hkv, 64, 16, seed=22))))
+    for n in news[:3]:
+        b = batch(dt, [(n, 17000)], Hq, Hkv, 64, 16, seed=23)
+        near(run(K, b), *expected(b))
+
+
 def test_empty_batches(K):
     b = batch("bf16", [(0, 5), (0, 0)], 4, 2, 64, 16, after=4)
     assert bool((run(K, b, fill=2.0) == 2).all())
