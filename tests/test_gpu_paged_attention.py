@@ -278,6 +278,19 @@ def test_more_sequences_than_the_plan_keeps_in_lds(K, g):
     near(run(K, b), *expected(b))
 
 
+@pytest.mark.parametrize("count,Hkv", [(300, 2), (1300, 1)])
+def test_more_chunks_than_the_card_takes_at_a_time(K, count, Hkv):
+    """The plan then sorts them by length, in LDS and past it: lengths of nothing and of one key among them, some single tokens."""
+    import random
+    r = random.Random(count)
+    seqs = [(r.choice([9, 20, 33, 70]), r.choice([0, 0, 1, 40, 300, 900])) for _ in range(count)] + [(1, 5), (1, 400)] * 10
+    r.shuffle(seqs)
+    b = batch("bf16", seqs, 4 * Hkv, Hkv, 64, 16, seed=24)
+    for i in range(0, len(seqs), 50):
+        b["lens"][i] = i // 50 % 3  # shorter than its rows
+    near(run(K, b), *expected(b))
+
+
 def test_a_plan_for_another_table_does_nothing(K):
     b = batch("bf16", [(1, 400), (200, 500)], 4, 2, 64, 16)
     plan = K.AttentionPlan(b["indptr"], b["lens"], b["table"], b["T"], 4, 2, 16)
