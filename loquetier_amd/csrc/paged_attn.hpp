@@ -54,6 +54,11 @@ constexpr int kAttnSmallItems = 2048, kAttnBigItems = 1024;
 // Keys of a part, at least: two turns of the four waves.  (128, 256, 512: a token over 2000 tokens 6.7, 8.2, 10.8 us, four over 4000
 // 19.3, 15.9, 15.6, 32 over up to 1500 with the join 34, 30, 28.)
 constexpr int kAttnMinKeys = 256;
+// Items with few rows for each of the others, in turns.  (None, 1, 2, 3, 4: eight prompts of 512 rows over up to 1500 tokens and 128 single tokens over
+// up to 4000 282, 282, 260, 297, 272 us, sixteen of 1024 from nothing and 40 single tokens 294, 325, 287, 340, 291, four of 512 and 64 with a kv
+// head a query head 240, 228, 229, 227, 227.  One and three are the bad ones, as if a CU got its second workgroup 32 items, its XCD's CUs, after the
+// first: with turns of two or four items it is then of the same kind.)
+constexpr int kAttnPer = 2;
 // Parts of a few-row tile from which the threads of a join share them out.  (85 parts: 30 us one after the other, 7 so; 8 parts 5.8 and 5.0.)
 constexpr int kAttnManyParts = 8;
 
@@ -250,9 +255,9 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
     a.plan.hdr[2] = a.most, a.plan.hdr[3] = a.T, a.plan.hdr[4] = a.S, a.plan.hdr[5] = a.g, a.plan.hdr[6] = a.Hkv, a.plan.hdr[7] = a.R;
   }
   __syncthreads();
-  // Items with few rows stream, the others compute: they take turns, so that both have the card together (mixed batch of four prompts
-  // of 512 rows over up to 1500 tokens and 64 single tokens, 32 heads: the others all first 240 us, in turns 231; alone 50 and 191).
-  const int both = min(at[0], at[1]);
+  // Items with few rows stream, the others compute: they take turns, one of the others and kAttnPer of these, so that both have the card
+  // together.
+  const int both = min(at[0] / kAttnPer, at[1]), mixed = (1 + kAttnPer) * both;
   struct Place {
     AttnItem it;
     AttnSeq q;
@@ -261,8 +266,9 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
     bool fits;
   };
   auto place = [&](int i) {
-    const int kind = i < 2 * both ? !(i & 1) : at[1] > at[0];
-    const int x = i < 2 * both ? i >> 1 : i - both;
+    const int turn = i / (1 + kAttnPer), in = i - turn * (1 + kAttnPer);
+    const int kind = i < mixed ? in == 0 : i - mixed < at[1] - both;
+    const int x = i < mixed ? (kind ? turn : turn * kAttnPer + in - 1) : (kind ? i - both * kAttnPer : i - at[1]);
     const int* first_l = first_s[kind];
     const int* first_g = start + kind * (a.S + 1);
     int lo = 0, hi = a.S;
@@ -293,7 +299,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
   // Where the others are most of the items, and more than the card takes at a time, the long ones go first, over all sequences (by
   // eighths of an octave): a long one that starts among the last keeps the rest of the card waiting.  Sequence by sequence and so: nine
   // prompts of 700 rows over up to 3000 tokens 242 and 227 us, 64 of 16 rows over up to 4000 151 and 123, four of 512 over up to 1500 57 and 50;
-  // but beside many items with few rows the two ways to take turns quarrel (eight prompts of 512 rows, 128 single tokens 280 and 294).
+  // beside as many items with few rows it gains nothing (eight prompts of 512 rows, 128 single tokens 260 and 266).
   const bool sorted = at[1] > kAttnSlots / a.Hkv && at[1] > at[0];
   auto bin_of = [](const AttnItem& it) { return 255 - (int)((__float_as_uint((float)(it.ke - it.kb) + 1.0f) >> 20) - (127u << 3)); };
   if (sorted) {
@@ -315,7 +321,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
   for (int i = tid; i < items; i += threads) {
     const Place p = place(i);
     const int x = sorted && p.kind ? atomicAdd(&bin_s[bin_of(p.it)], 1) : p.x;
-    a.plan.items[x < both ? 2 * x + (p.kind ? 0 : 1) : x + both] = p.it;
+    a.plan.items[!p.kind ? i : (x < both ? x * (1 + kAttnPer) : x + both * kAttnPer)] = p.it;
     if (p.ns > 1) {
       const int join = local ? join_s[p.lo] : start[2 * (a.S + 1) + p.lo];
       const int shares = attn_shares(p.q, p.ns, a.g), by = p.kind || p.ns < kAttnManyParts ? 8 : 1;
