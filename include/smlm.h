@@ -560,8 +560,9 @@ SMLM_API int smlm_kv_copy_pages(void* pool, const int32_t* src, const int32_t* d
  * Rows that see no token are zero; rows of no sequence are left alone.  Pages outside the pool, requests outside the table and
  * tokens past a row of the table do not count.  head_dim 64 or 128; any page size; scale > 0; strides multiples of 8 elements.
  *
- * out may be q.  The plan depends on q_indptr, kv_len and requests alone: one for all the layers of a step.  q_indptr must not decrease;
- * T, S, q_heads, kv_heads, R, M and page_size are the same for both (a call of other sizes than its plan's does nothing).
+ * out may be q.  The plan depends on q_indptr, kv_len and requests alone: one for all the layers of a step.  q_indptr must not decrease
+ * (a call with the plan of one that does does nothing); T, S, q_heads, kv_heads, R, M and page_size are the same for both (a call of other
+ * sizes than its plan's does nothing).
  */
 SMLM_API int smlm_attn_plan_size(int T, int S, int q_heads, int kv_heads, size_t* bytes);
 SMLM_API int smlm_attn_plan_build(void* plan, size_t plan_bytes, const int32_t* q_indptr, const int32_t* kv_len,

@@ -170,7 +170,8 @@ __device__ __forceinline__ int attn_parts(int n) {
 }
 
 // One workgroup.  The sequences' tiles are cut into parts of about `cut` keys, by the sequences' lengths; the cuts follow from the batch's
-// totals, so that the numbers of items and parts have bounds that the host knows.
+// totals, so that the numbers of items and parts have bounds that the host knows, as long as no two sequences share a row: the plan of
+// a q_indptr that decreases holds nothing, and a call with it does nothing.
 __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArgs a) {
   __shared__ int wave_tot[16][5];
   __shared__ float red[3][16];
@@ -180,13 +181,13 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, threads = (int)blockDim.x, waves = threads >> 6;
   const bool local = a.S <= kAttnPlanLds;
   float keys[2] = {0.0f, 0.0f};  // of the few-row tiles, of the others (only the cuts hang on them: a float will do)
-  float n_big_f = 0.0f;          // tiles of the others
+  float n_big_f = 0.0f;          // tiles of the others; infinite where q_indptr decreases
   for (int s = tid; s < a.S; s += threads) {
     const AttnSeq q = attn_seq(a, s);
     const bool small = q.tile == kAttnSmallRows;
     keys[0] += small ? (float)q.tiles * (float)q.len : 0.0f;
     keys[1] += small ? 0.0f : (float)q.tiles * (float)q.len;
-    n_big_f += small ? 0.0f : (float)q.tiles;
+    n_big_f += a.q_indptr[s + 1] < a.q_indptr[s] ? INFINITY : (small ? 0.0f : (float)q.tiles);
     if (local) seq_s[s] = q;
   }
   keys[0] = wave_total(keys[0]), keys[1] = wave_total(keys[1]), n_big_f = wave_total(n_big_f);
@@ -247,13 +248,16 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
 #pragma unroll
     for (int i = 0; i < 5; ++i) at[i] += all[i];
   }
-  const int items = at[0] + at[1] < a.items_max ? at[0] + at[1] : a.items_max;
+  const bool fits = n_big_f != INFINITY && at[0] + at[1] <= a.items_max && at[2] <= a.joins_max && at[3] <= a.parts_small_max &&
+                    at[4] <= a.parts_big_max;
+  const int items = fits ? at[0] + at[1] : 0;
   if (tid == 0) {
     first_s[0][0] = first_s[1][0] = start[0] = start[a.S + 1] = 0;
     a.plan.hdr[0] = items;
-    a.plan.hdr[1] = at[2] < a.joins_max ? at[2] : a.joins_max;
+    a.plan.hdr[1] = fits ? at[2] : 0;
     a.plan.hdr[2] = a.most, a.plan.hdr[3] = a.T, a.plan.hdr[4] = a.S, a.plan.hdr[5] = a.g, a.plan.hdr[6] = a.Hkv, a.plan.hdr[7] = a.R;
   }
+  if (!fits) return;
   __syncthreads();
   // Items with few rows stream, the others compute: they take turns, one of the others and kAttnPer of these, so that both have the card
   // together.
@@ -262,8 +266,7 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
     AttnItem it;
     AttnSeq q;
     int kind, x;              // 1: the others; its number among its kind's
-    int lo, t, j, ns, part0;  // sequence, tile, part, parts of the tile
-    bool fits;
+    int lo, t, j, ns, part0;  // sequence, tile, part, parts of the tile, the first of them
   };
   auto place = [&](int i) {
     const int turn = i / (1 + kAttnPer), in = i - turn * (1 + kAttnPer);
@@ -280,8 +283,8 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
     const AttnSeq q = local ? seq_s[lo] : attn_seq(a, lo);
     const int first = local ? first_l[lo] : first_g[lo], end = local ? first_l[lo + 1] : first_g[lo + 1];
     const int part = local ? part_s[lo] : start[3 * (a.S + 1) + lo];
-    const uint32_t ns = max(1u, (uint32_t)(end - first) / (uint32_t)max(1, q.tiles)), k = (uint32_t)(x - first);
-    const int t = max(0, q.tiles - 1 - (int)(k / ns)), j = (int)(k % ns);  // (the later tiles of a prompt see more keys: they go first)
+    const uint32_t ns = (uint32_t)(end - first) / (uint32_t)q.tiles, k = (uint32_t)(x - first);
+    const int t = q.tiles - 1 - (int)(k / ns), j = (int)(k % ns);  // (the later tiles of a prompt see more keys: they go first)
     AttnItem it;
     it.row0 = q.row0, it.n = q.n, it.len = q.len, it.trow = q.trow, it.first = t * q.tile;
     const int last = min(it.first + q.tile, q.n * a.g) - 1;
@@ -289,12 +292,9 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
     const int64_t step = (int64_t)((seen + ns - 1) / ns + 63) / 64 * 64;
     it.kb = (int)min((int64_t)seen, j * step);
     it.ke = (int)min((int64_t)seen, (j + 1) * step);
-    const int part0 = part + t * (int)ns, parts_max = kind ? a.parts_big_max : a.parts_small_max;
+    const int part0 = part + t * (int)ns;
     it.part = ns > 1 ? part0 + j : -1;
-    // (sequences that overlap, which none should, could come to more parts than there is room for)
-    const bool fits = ns == 1 || part0 + (int)ns <= parts_max;
-    if (!fits) it.n = 0, it.kb = it.ke = 0, it.part = -1;
-    return Place{it, q, kind, x, lo, t, j, (int)ns, part0, fits};
+    return Place{it, q, kind, x, lo, t, j, (int)ns, part0};
   };
   // Where the others are most of the items, and more than the card takes at a time, the long ones go first, over all sequences (by
   // eighths of an octave): a long one that starts among the last keeps the rest of the card waiting.  Sequence by sequence and so: nine
@@ -325,8 +325,8 @@ __global__ __launch_bounds__(kAttnPlanThreads) void attn_plan_kernel(AttnPlanArg
     if (p.ns > 1) {
       const int join = local ? join_s[p.lo] : start[2 * (a.S + 1) + p.lo];
       const int shares = attn_shares(p.q, p.ns, a.g), by = p.kind || p.ns < kAttnManyParts ? 8 : 1;
-      const int rows = p.fits ? min(p.q.tile, p.q.n * a.g - p.it.first) : 0;
-      for (int h = p.j; h < shares && join + p.t * shares + h < a.joins_max; h += p.ns)
+      const int rows = min(p.q.tile, p.q.n * a.g - p.it.first);
+      for (int h = p.j; h < shares; h += p.ns)
         a.plan.joins[join + p.t * shares + h] = AttnJoin{p.q.row0, p.it.first, p.kind, p.part0, p.ns, h * by, shares * by, rows};
     }
   }
