@@ -10,7 +10,8 @@
 // the registers as the next product, O^T = V^T P^T, reads them (the keys of a step may come in any order, as long as P and V
 // agree).  V is read from LDS through the transposing load.  One pass over the keys with the running maximum and sum; statistics
 // and accumulators in float.  The probabilities are rounded to the element type for the second product: relative errors of half
-// a step each, of random sign, so about as much as the rounding of the result itself.
+// a step each, of random sign, so about as much as the rounding of the result itself.  Their sum is taken of the rounded ones: what the errors
+// have in common leaves the result alone, and values that are all alike come back.
 //
 // Sequences of up to 16 tile rows (decoding) are bound by HBM: the four waves of a workgroup take 32 keys in turn, K straight to
 // registers, V through a part of LDS of the wave's own, no barrier until the end.  256 single tokens over up to 4095, 8 kv heads of 128:
@@ -547,18 +548,15 @@ __device__ __forceinline__ void attn_small(const AttnArgs& a, const AttnItem& it
     const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.0f : mn * a.scale, ms = ref - kAttnBias<DT>;
     const float turn = attn_exp2(m * a.scale - ref);
     m = mn;
-    float sum = 0.0f, w[8];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[u * 4 + i] = attn_exp2(s[u][i] * a.scale - ms);
-        sum += w[u * 4 + i];
-      }
-    l = l * turn + sum;
+    float sum = 0.0f;
     u32x4 pf;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) pf[i] = pack2<DT>(w[2 * i], w[2 * i + 1]);
+    for (int i = 0; i < 4; ++i) {
+      const f32x4& x = s[i >> 1];
+      pf[i] = pack2<DT>(attn_exp2(x[2 * i & 3] * a.scale - ms), attn_exp2(x[(2 * i & 3) + 1] * a.scale - ms));
+      sum = attn_add2<DT>(pf[i], sum);  // (the weights as V meets them: they add up to one whatever their rounding)
+    }
+    l = l * turn + sum;
 #pragma unroll
     for (int i = 0; i < kBlk; ++i) o[i] *= turn;
     if (!guard) {
@@ -765,7 +763,7 @@ __device__ __forceinline__ void attn_big(const AttnArgs& a, const AttnItem& it, 
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
         const uint32_t two = pack2<DT>(attn_exp2(s[u][e] * a.scale - ms), attn_exp2(s[u][e + 1] * a.scale - ms));
-        l = attn_add2<DT>(two, l);  // (the weights as V meets them: they add up to one whatever their rounding)
+        l = attn_add2<DT>(two, l);  // (as V meets them, as above)
         pf[u][e >> 3][(e >> 1) & 3] = two;
       }
     const bool guard = edge && ((fl[0] | fl[1] | fl[2] | fl[3]) >> 16) != 0;
