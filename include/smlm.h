@@ -514,7 +514,7 @@ SMLM_API int smlm_qk_norm_rope_bwd(const smlm_qk_rope* args, const smlm_heads* g
  * A call does all it is asked or, where it cannot, nothing, and then adds SMLM_KV_* bits to *status (int32 on the device; may be NULL).
  */
 #define SMLM_KV_BAD_REQUEST 1 /* past R, named twice, a child that is not empty, a count below 0 */
-#define SMLM_KV_TOO_LONG 2    /* more pages than a row of the table holds          */
+#define SMLM_KV_TOO_LONG 2    /* more pages than a row of the table holds, or more tokens than max_tokens */
 #define SMLM_KV_ROWS 4        /* more new tokens than rows                          */
 #define SMLM_KV_NO_PAGES 8    /* the pool has not enough free pages                 */
 
@@ -528,6 +528,12 @@ SMLM_API int smlm_kv_extend(int32_t* table, int32_t* length, int32_t* refs, cons
                             int32_t* q_indptr, int32_t* kv_len, int32_t* positions, int64_t* slots, void* workspace,
                             size_t workspace_bytes, int R, int M, int N, int S, int rows, int page_size, int32_t* status,
                             void* stream);
+
+/* The same where a request may have max_tokens tokens, fewer than a row of the table has places for (a last page's rest, say). */
+SMLM_API int smlm_kv_extend_upto(int32_t* table, int32_t* length, int32_t* refs, const int32_t* requests, const int32_t* counts,
+                                 int32_t* q_indptr, int32_t* kv_len, int32_t* positions, int64_t* slots, void* workspace,
+                                 size_t workspace_bytes, int R, int M, int N, int S, int rows, int page_size, int max_tokens,
+                                 int32_t* status, void* stream);
 
 /* The requests' pages lose a holder, their rows become -1 and their lengths 0.  One named twice is freed once; below 0 is skipped. */
 SMLM_API int smlm_kv_free(int32_t* table, int32_t* length, int32_t* refs, const int32_t* requests, int R, int M, int N, int K,

@@ -99,6 +99,7 @@ SIGNATURES = {
     "smlm_qk_norm_rope_bwd": (_i, [_prope, _pheads, _pheads, _pheads, _pheads, _vp, _vp, _vp, _sz, _vp]),
     "smlm_kv_workspace_size": (_i, [_i, _i, _i, _psz]),
     "smlm_kv_extend": (_i, [_vp] * 10 + [_sz] + [_i] * 6 + [_vp, _vp]),
+    "smlm_kv_extend_upto": (_i, [_vp] * 10 + [_sz] + [_i] * 7 + [_vp, _vp]),
     "smlm_kv_free": (_i, [_vp] * 4 + [_i] * 5 + [_vp, _vp]),
     "smlm_kv_fork": (_i, [_vp] * 7 + [_sz] + [_i] * 7 + [_vp, _vp]),
     "smlm_kv_compact": (_i, [_vp] * 4 + [_sz] + [_i] * 6 + [_vp]),

@@ -228,18 +228,19 @@ bool pages(const Tensor& table, const Tensor* length, const Tensor& refs, const 
          table.size(0) < (1 << 24) && table.size(1) < (1 << 20) && refs.size(0) < (1 << 28);
 }
 
-// kv_extend(table, length, refs, requests, counts, n_rows, page_size, status, workspace) -> the step's four tables, or None
+// kv_extend(table, length, refs, requests, counts, n_rows, page_size, status, workspace, max_tokens = None) -> the step's four tables, or None
 PyObject* py_kv_extend(PyObject*, PyObject* const* p, Py_ssize_t n) {
   SMLM_PY_TRY
-  TORCH_CHECK(n == 9, "kv_extend takes 9 arguments");
-  bool ok = plain_thread() && PyLong_CheckExact(p[5]) && PyLong_CheckExact(p[6]);
+  TORCH_CHECK(n == 9 || n == 10, "kv_extend takes 9 or 10 arguments");
+  const bool limit = n == 10 && p[9] != Py_None;
+  bool ok = plain_thread() && PyLong_CheckExact(p[5]) && PyLong_CheckExact(p[6]) && (!limit || PyLong_CheckExact(p[9]));
   for (int i = 0; i < 5; ++i) ok = ok && plain(p[i]);
   const Tensor* status = optional(p[7], &ok);
   if (!ok) Py_RETURN_NONE;
   const Tensor &table = THPVariable_Unpack(p[0]), &length = THPVariable_Unpack(p[1]), &refs = THPVariable_Unpack(p[2]),
                &req = THPVariable_Unpack(p[3]), &counts = THPVariable_Unpack(p[4]);
-  const int64_t rows = integer(p[5]), P = integer(p[6]);
-  if (!pages(table, &length, refs, status, req, counts) || rows < 0 || rows > (1 << 20) || P < 1 || P > (1 << 30)) Py_RETURN_NONE;
+  const int64_t rows = integer(p[5]), P = integer(p[6]), most = limit ? integer(p[9]) : 0x7fffffff;
+  if (most < 0 || most > 0x7fffffff || !pages(table, &length, refs, status, req, counts) || rows < 0 || rows > (1 << 20) || P < 1 || P > (1 << 30)) Py_RETURN_NONE;
   const int R = (int)table.size(0), M = (int)table.size(1), N = (int)refs.size(0), S = (int)req.size(0);
   const auto ints = table.options();
   Tensor indptr = at::empty({S + 1}, ints), len = at::empty({S}, ints), pos = at::empty({rows}, ints),
@@ -249,7 +250,7 @@ PyObject* py_kv_extend(PyObject*, PyObject* const* p, Py_ssize_t n) {
   const Tensor mem = scratch(p[8], need, table);
   auto i32 = [](const Tensor& t) { return (int32_t*)t.data_ptr(); };
   check(lib.kv_extend(i32(table), i32(length), i32(refs), i32(req), i32(counts), i32(indptr), i32(len), i32(pos),
-                      (int64_t*)slots.data_ptr(), mem.data_ptr(), (size_t)mem.numel(), R, M, N, S, (int)rows, (int)P,
+                      (int64_t*)slots.data_ptr(), mem.data_ptr(), (size_t)mem.numel(), R, M, N, S, (int)rows, (int)P, (int)most,
                       status ? i32(*status) : nullptr, stream(table)),
         "kv_extend");
   THPObjectPtr o[4] = {THPObjectPtr(THPVariable_Wrap(std::move(indptr))), THPObjectPtr(THPVariable_Wrap(std::move(len))),

@@ -56,7 +56,7 @@ struct Lib {
   decltype(&smlm_paged_attn_workspace_size) attn_size;
   decltype(&smlm_paged_attn) attn;
   decltype(&smlm_kv_workspace_size) kv_size;
-  decltype(&smlm_kv_extend) kv_extend;
+  decltype(&smlm_kv_extend_upto) kv_extend;
   decltype(&smlm_kv_free) kv_free;
   decltype(&smlm_kv_fork) kv_fork;
 } lib;
@@ -736,7 +736,7 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   get("smlm_paged_attn_workspace_size", &lib.attn_size);
   get("smlm_paged_attn", &lib.attn);
   get("smlm_kv_workspace_size", &lib.kv_size);
-  get("smlm_kv_extend", &lib.kv_extend);
+  get("smlm_kv_extend_upto", &lib.kv_extend);
   get("smlm_kv_free", &lib.kv_free);
   get("smlm_kv_fork", &lib.kv_fork);
   Py_INCREF(ws);

@@ -116,6 +116,7 @@ struct KvExtendArgs {
   int64_t* slots;                // [rows]
   int *owner, *start, *fresh;    // scratch: [R], [S + 1] running sum of new pages, [N]
   int R, M, N, S, rows, P;
+  int most;                      // tokens that a request may have, at most M * P
 };
 
 // A sequence's part of a step.
@@ -127,7 +128,7 @@ __device__ __forceinline__ KvNeed kv_need(const KvExtendArgs& a, int r, int coun
   if (r >= 0) {
     if (r >= a.R || count < 0 || !first) x.err = SMLM_KV_BAD_REQUEST;
     const int64_t now = (int64_t)old + x.n, had = ((int64_t)old + a.P - 1) / a.P, has = (now + a.P - 1) / a.P;
-    if (r < a.R && (has > a.M || old < 0)) x.err |= SMLM_KV_TOO_LONG;
+    if (r < a.R && (now > a.most || old < 0)) x.err |= SMLM_KV_TOO_LONG;
     if (x.n > a.rows) x.err |= SMLM_KV_ROWS, x.n = 0;  // (and so the sum stays small)
     if (!x.err) x.pages = (int)(has - had);
   }

@@ -253,12 +253,12 @@ SMLM_API int smlm_kv_workspace_size(int R, int N, int S, size_t* bytes) {
   return SMLM_OK;
 }
 
-SMLM_API int smlm_kv_extend(int32_t* table, int32_t* length, int32_t* refs, const int32_t* requests, const int32_t* counts,
-                            int32_t* q_indptr, int32_t* kv_len, int32_t* positions, int64_t* slots, void* workspace,
-                            size_t workspace_bytes, int R, int M, int N, int S, int rows, int page_size, int32_t* status,
-                            void* stream) {
+SMLM_API int smlm_kv_extend_upto(int32_t* table, int32_t* length, int32_t* refs, const int32_t* requests, const int32_t* counts,
+                                 int32_t* q_indptr, int32_t* kv_len, int32_t* positions, int64_t* slots, void* workspace,
+                                 size_t workspace_bytes, int R, int M, int N, int S, int rows, int page_size, int max_tokens,
+                                 int32_t* status, void* stream) {
   if (int rc = kv_check(R, M, N, S, page_size)) return rc;
-  if (rows < 0 || !q_indptr || !workspace || (S > 0 && (!requests || !counts || !kv_len)) ||
+  if (rows < 0 || max_tokens < 0 || !q_indptr || !workspace || (S > 0 && (!requests || !counts || !kv_len)) ||
       (rows > 0 && (!positions || !slots)) || (R > 0 && (!length || (M > 0 && !table))) || (N > 0 && !refs))
     return SMLM_ERR_ARG;
   if (rows > (1 << 20)) return SMLM_ERR_LIMIT;
@@ -270,10 +270,19 @@ SMLM_API int smlm_kv_extend(int32_t* table, int32_t* length, int32_t* refs, cons
   a.requests = requests, a.counts = counts;
   a.q_indptr = q_indptr, a.kv_len = kv_len, a.positions = positions, a.slots = slots;
   a.R = R, a.M = M, a.N = N, a.S = S, a.rows = rows, a.P = page_size;
+  a.most = max_tokens < M * page_size ? max_tokens : M * page_size;
   if (S <= kKvThreads && rows <= kKvFewRows) return launch(kv_extend_one_kernel<true>, dim3(1), dim3(kKvThreads), (hipStream_t)stream, a);
   const int rc = launch(S <= kKvThreads ? kv_extend_one_kernel<false> : kv_extend_kernel, dim3(1), dim3(kKvThreads), (hipStream_t)stream, a);
   if (rc || rows == 0) return rc;
   return launch(kv_rows_kernel, dim3((unsigned)ceil_div(rows, 256)), dim3(256), (hipStream_t)stream, a);
+}
+
+SMLM_API int smlm_kv_extend(int32_t* table, int32_t* length, int32_t* refs, const int32_t* requests, const int32_t* counts,
+                            int32_t* q_indptr, int32_t* kv_len, int32_t* positions, int64_t* slots, void* workspace,
+                            size_t workspace_bytes, int R, int M, int N, int S, int rows, int page_size, int32_t* status,
+                            void* stream) {
+  return smlm_kv_extend_upto(table, length, refs, requests, counts, q_indptr, kv_len, positions, slots, workspace, workspace_bytes, R,
+                             M, N, S, rows, page_size, 0x7fffffff, status, stream);
 }
 
 SMLM_API int smlm_kv_free(int32_t* table, int32_t* length, int32_t* refs, const int32_t* requests, int R, int M, int N, int K,

@@ -26,13 +26,14 @@ class KvStep(NamedTuple):
 
 class PagedKvCache:
     """`n_pages` pages of `page_size` tokens for all layers, [n_pages, n_layers, 2 (keys, values), kv_heads, page_size, head_dim] as the
-    reference's pages are laid out, and up to `max_requests` requests of up to `max_tokens` tokens each, known by their
-    number.  All calls are ordered on the current stream and may be captured into a graph after one eager pass."""
+    reference's pages are laid out, and up to `max_requests` requests of up to `max_tokens` tokens each (`extend` refuses more, so
+    a rotation table of `max_tokens` positions serves), known by their number.  All calls are ordered on the current stream and
+    may be captured into a graph after one eager pass."""
 
     def __init__(self, n_pages: int, n_layers: int, kv_heads: int, head_dim: int, max_requests: int, max_tokens: int,
                  page_size: int = 16, dtype: torch.dtype = torch.bfloat16, device="cuda"):
         self.pool = torch.zeros(n_pages, n_layers, 2, kv_heads, page_size, head_dim, dtype=dtype, device=device)
-        self.page_size, self.kv_heads = page_size, kv_heads
+        self.page_size, self.kv_heads, self.max_tokens = page_size, kv_heads, int(max_tokens)
         ints = dict(dtype=torch.int32, device=self.pool.device)
         self.table = torch.full((max_requests, -(-max_tokens // page_size)), -1, **ints)
         self.length = torch.zeros(max_requests, **ints)
@@ -58,7 +59,7 @@ class PagedKvCache:
             n_rows = sum(int(c) for c in counts)
         requests = self._ints(requests)
         return KvStep(*kernel.kv_extend(self.table, self.length, self.refs, requests, self._ints(counts), n_rows, self.page_size,
-                                        self.status, self.workspace), requests)
+                                        self.status, self.workspace, self.max_tokens), requests)
 
     def fork(self, parents: Ints, children: Ints) -> None:
         kernel.kv_fork(self.pool, self.table, self.length, self.refs, self._ints(parents), self._ints(children), self.status,
@@ -93,6 +94,6 @@ class PagedKvCache:
         if bits:
             self.status.zero_()
             names = {_lib.SMLM_KV_BAD_REQUEST: "a request that is unknown, named twice or not empty",
-                     _lib.SMLM_KV_TOO_LONG: "a request longer than its table", _lib.SMLM_KV_ROWS: "more tokens than rows",
+                     _lib.SMLM_KV_TOO_LONG: "a request longer than max_tokens", _lib.SMLM_KV_ROWS: "more tokens than rows",
                      _lib.SMLM_KV_NO_PAGES: "no free pages"}
             raise RuntimeError("the cache refused a call: " + ", ".join(n for b, n in names.items() if bits & b))

@@ -1135,13 +1135,15 @@ def _kv_pool(pool: torch.Tensor, dev: torch.device, N: int) -> Tuple[int, int, i
 
 
 def kv_extend(table: torch.Tensor, length: torch.Tensor, refs: torch.Tensor, requests: torch.Tensor, counts: torch.Tensor,
-              n_rows: int, page_size: int, status: Optional[torch.Tensor] = None, workspace: Optional[Workspace] = None):
+              n_rows: int, page_size: int, status: Optional[torch.Tensor] = None, workspace: Optional[Workspace] = None,
+              max_tokens: Optional[int] = None):
     """Room for counts[s] more tokens of requests[s], pages taken lowest number first, on the device (see include/smlm.h
     for the state's tensors and `status`, which a call that cannot be done marks, changing nothing else).
 
     Returns (q_indptr int32 [S + 1], kv_len int32 [S], positions int32 [n_rows], slots int64 [n_rows]): what qk_norm_rope and
-    AttentionPlan read.  n_rows: the counts' sum, or more (rows past it get position and slot -1)."""
-    done = _host().kv_extend(table, length, refs, requests, counts, n_rows, page_size, status, workspace)
+    AttentionPlan read.  n_rows: the counts' sum, or more (rows past it get position and slot -1).  max_tokens: what a request
+    may have, where that is less than its row of the table has places for."""
+    done = _host().kv_extend(table, length, refs, requests, counts, n_rows, page_size, status, workspace, max_tokens)
     if done is not None:
         return done
     dev, R, M, N = _kv_state(table, length, refs, status, requests=requests, counts=counts)
@@ -1149,6 +1151,9 @@ def kv_extend(table: torch.Tensor, length: torch.Tensor, refs: torch.Tensor, req
         raise RuntimeError("requests and counts must have one entry per sequence")
     if n_rows < 0 or page_size < 1:
         raise RuntimeError("n_rows and page_size must not be negative")
+    if max_tokens is not None and max_tokens < 0:
+        raise RuntimeError("max_tokens must not be negative")
+    most = 0x7fffffff if max_tokens is None else min(int(max_tokens), 0x7fffffff)
     S = requests.numel()
     q_indptr = torch.empty(S + 1, dtype=torch.int32, device=dev)
     kv_len = torch.empty(S, dtype=torch.int32, device=dev)
@@ -1156,9 +1161,9 @@ def kv_extend(table: torch.Tensor, length: torch.Tensor, refs: torch.Tensor, req
     slots = torch.empty(n_rows, dtype=torch.int64, device=dev)
     with _on(dev):
         ws = _workspace(dev, _lib.size_query("smlm_kv_workspace_size", R, N, S), workspace)
-        rc = _lib.load().smlm_kv_extend(_ptr(table), _ptr(length), _ptr(refs), _ptr(requests), _ptr(counts), q_indptr.data_ptr(),
-                                        _ptr(kv_len), _ptr(positions), _ptr(slots), ws.data_ptr(), ws.numel(), R, M, N, S,
-                                        n_rows, page_size, _ptr(status), _stream(dev))
+        rc = _lib.load().smlm_kv_extend_upto(_ptr(table), _ptr(length), _ptr(refs), _ptr(requests), _ptr(counts),
+                                             q_indptr.data_ptr(), _ptr(kv_len), _ptr(positions), _ptr(slots), ws.data_ptr(),
+                                             ws.numel(), R, M, N, S, n_rows, page_size, most, _ptr(status), _stream(dev))
     _lib.check(rc, "kv_extend")
     return q_indptr, kv_len, positions, slots
 

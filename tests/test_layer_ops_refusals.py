@@ -126,3 +126,11 @@ def test_division_by_the_page_size():
         assert m < 1 << 32
         for x in [0, 1, P - 1, P, P + 1, 2 * P - 1, 2 ** 31 - 1] + [r.randrange(2 ** 31) for _ in range(20)]:
             assert (((x * m) >> 32) + x) >> s == x // P
+
+
+def test_extend_with_a_limit(L):
+    n = C.c_size_t()
+    assert L.smlm_kv_workspace_size(4, 10, 3, C.byref(n)) == 0
+    ext = lambda most=9, ws=A, size=n.value, P=16: L.smlm_kv_extend_upto(
+        A, A, A, A, A, A, A, A, A, ws, size, 4, 4, 10, 3, 5, P, most, None, None)
+    assert ext(most=-1) == ARG and ext(P=0) == ARG and ext(ws=None) == ARG and ext(size=16) == WORKSPACE
