@@ -52,6 +52,19 @@ bool caches(const Tensor& k, const Tensor& v, const Tensor& q, int64_t kv_heads)
 }
 int64_t stride_of(const Tensor& t, int i) { return t.size(i) > 1 ? t.stride(i) : 0; }
 
+// Gradients that hang on `of` in a graph that is being made of a backward: to differentiate them is refused, as there is no kernel for it.
+struct QkGradients : public Function<QkGradients> {
+  static variable_list forward(AutogradContext*, at::TensorList gradients, at::TensorList of) {
+    (void)of;
+    variable_list out;
+    for (const Tensor& t : gradients) out.push_back(t.variable_data());
+    return out;
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "the gradients of qk_norm_rope cannot be differentiated");
+  }
+};
+
 struct QkNormRope : public Function<QkNormRope> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const std::optional<Tensor>& q_weight,
                                const std::optional<Tensor>& k_weight, const Tensor& table, const Tensor& pos, double eps) {
@@ -95,6 +108,18 @@ struct QkNormRope : public Function<QkNormRope> {
     check(lib.rope_bwd(&a, &gq, &gk, &dq, &dk, dw[0].defined() ? dw[0].data_ptr() : nullptr,
                        dw[1].defined() ? dw[1].data_ptr() : nullptr, need ? mem.data_ptr() : nullptr, need, stream(g[0])),
           "qk_norm_rope_backward");
+    if (at::GradMode::is_enabled()) {
+      variable_list made, of;
+      for (const Tensor& t : {d[0], d[1], dw[0], dw[1]})
+        if (t.defined()) made.push_back(t);
+      for (const Tensor& t : {grads[0], grads[1], s[0], s[1], s[2], s[3]})
+        if (t.defined()) of.push_back(t);
+      const variable_list out = QkGradients::apply(at::TensorList(made), at::TensorList(of));
+      d[0] = out[0], d[1] = out[1];
+      size_t n = 2;
+      for (Tensor& t : dw)
+        if (t.defined()) t = out[n++];
+    }
     return {d[0], d[1], dw[0], dw[1], Tensor(), Tensor(), Tensor()};
   }
 };

@@ -296,12 +296,33 @@ class rms_norm(Function):
         return dx, d_weight, None
 
 
+class _qk_norm_rope_gradients(Function):
+    """The backward of `qk_norm_rope`, as a function of its own so that a graph made of it (create_graph) knows what the
+    gradients hang on: to differentiate them is refused, as there is no kernel for it."""
+
+    @staticmethod
+    def forward(ctx: FunctionCtx, gq, gk, q, k, q_weight, k_weight, table, positions, eps: float):
+        gq, gk = (g if kernel._heads_fit(g) and g.data_ptr() % 16 == 0 else g.clone(memory_format=torch.contiguous_format)
+                  for g in (gq, gk))
+        dq, dk = (torch.empty(g.shape, dtype=g.dtype, device=g.device) for g in (gq, gk))
+        dqw, dkw = (None if w is None else torch.empty_like(w) for w in (q_weight, k_weight))
+        # (without a norm the gradient stands for the input, which the kernel then does not read)
+        kernel.qk_norm_rope_backward(dq, dk, dqw, dkw, gq, gk, gq if q is None else q, gk if k is None else k, table, positions,
+                                     q_weight, k_weight, eps)
+        return dq, dk, dqw, dkw
+
+    @staticmethod
+    def backward(ctx: FunctionCtx, *grads):
+        raise RuntimeError("the gradients of qk_norm_rope cannot be differentiated")
+
+
 class qk_norm_rope(Function):
     """`qk_norm_rope.apply(q, k, q_weight, k_weight, table, positions, eps)`: queries [rows, q_heads, head_dim] and keys [rows,
     kv_heads, head_dim] normed by head (where the weight is not None) and rotated by position, in one launch (see
     ops/_kernels.qk_norm_rope); returns both.  The reference rotates with tensor expressions
     (src/loquetier_src/models/mixed_llama.py:93-195).  The backward makes the root mean squares again, so only the inputs are
-    kept, and of those only what it reads: nothing of q and k where there is no norm."""
+    kept, and of those only what it reads: nothing of q and k where there is no norm.  Its gradients cannot be differentiated
+    again: a graph of them (create_graph) raises where it is asked to."""
 
     @classmethod
     def apply(cls, *args, **kwargs):
@@ -325,12 +346,4 @@ class qk_norm_rope(Function):
 
     @staticmethod
     def backward(ctx: FunctionCtx, gq: torch.Tensor, gk: torch.Tensor):
-        q, k, q_weight, k_weight, table, positions = ctx.saved_tensors
-        gq, gk = (g if kernel._heads_fit(g) and g.data_ptr() % 16 == 0 else g.clone(memory_format=torch.contiguous_format)
-                  for g in (gq, gk))
-        dq, dk = (torch.empty(g.shape, dtype=g.dtype, device=g.device) for g in (gq, gk))
-        dqw, dkw = (None if w is None else torch.empty_like(w) for w in (q_weight, k_weight))
-        # (without a norm the gradient stands for the input, which the kernel then does not read)
-        kernel.qk_norm_rope_backward(dq, dk, dqw, dkw, gq, gk, gq if q is None else q, gk if k is None else k, table, positions,
-                                     q_weight, k_weight, ctx.eps)
-        return dq, dk, dqw, dkw, None, None, None
+        return *_qk_norm_rope_gradients.apply(gq, gk, *ctx.saved_tensors, ctx.eps), None, None, None

@@ -288,3 +288,37 @@ def test_no_rows(K):
     a, b = qk_norm_rope.apply(*leaves, table, pos, 1e-6)
     (a.sum() + b.sum()).backward()
     assert a.shape == (0, 4, 64) and not bool(leaves[2].grad.any()) and not bool(leaves[3].grad.any())
+
+
+@pytest.fixture(params=["native", "python"])
+def path(request, monkeypatch, K):
+    from loquetier_amd import _lib
+    if request.param == "python":
+        monkeypatch.setattr(K, "_host", lambda: _lib._NoHost)
+
+
+@pytest.mark.parametrize("norm", [(True, True), (True, False), (False, False)], ids=["norms", "qnorm", "plain"])
+def test_gradients_are_not_differentiated(K, path, norm):
+    """A graph of the gradients raises where it is differentiated, by every way to what they hang on; without one nothing changes."""
+    from loquetier_amd.kernel_utils import qk_norm_rope
+    q, k, _, table, pos, wq, wk = case("bf16", 6, 4, 2, 64, 64, norm, seed=14)
+    leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, wq, wk) if t is not None]
+    args = lambda: (leaves[0], leaves[1], leaves[2] if norm[0] else None, leaves[-1] if norm[1] else None, table, pos, 1e-6)
+    gq, gk = torch.ones_like(leaves[0]), torch.ones_like(leaves[1])
+    want = torch.autograd.grad(qk_norm_rope.apply(*args()), leaves, (gq, gk))
+    got = torch.autograd.grad(qk_norm_rope.apply(*args()), leaves, (gq, gk), create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    again = "cannot be differentiated"
+    if any(norm):  # the gradients hang on q, which other terms lead to as well
+        for x, g in zip(leaves, got):
+            with pytest.raises(RuntimeError, match=again):
+                torch.autograd.grad(g.float().square().sum() + leaves[0].float().square().sum(), leaves[0], retain_graph=True)
+        with pytest.raises(RuntimeError, match=again):
+            (sum(g.float().square().sum() for g in got) + leaves[0].float().sum()).backward()
+    else:  # a rotation by itself: the gradients hang on the outputs' alone
+        assert not any(g.requires_grad for g in got)
+    gq.requires_grad_(True)
+    got = torch.autograd.grad(qk_norm_rope.apply(*args()), leaves, (gq, gk), create_graph=True)
+    with pytest.raises(RuntimeError, match=again):
+        torch.autograd.grad(got[0].float().sum(), gq)
+    assert leaves[0].grad is None
