@@ -1225,6 +1225,9 @@ def kv_copy_pages(pool: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> N
     _lib.check(rc, "kv_copy_pages")
 
 
+_ATTENTION_DIMS = (64, 128)  # head sizes of paged_attention
+
+
 class AttentionPlan:
     """How the card shares out the attention of one batch (see include/smlm.h): built once a step, for all its layers.
 
@@ -1281,7 +1284,7 @@ def paged_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v
         raise RuntimeError(f"the plan is for {plan.T} rows of {plan.q_heads} heads")
     if plan.buf.device != q.device:
         raise RuntimeError(f"the plan lives on {plan.buf.device}, q on {q.device}")
-    if q.dtype not in _DTYPE_CODE or D not in (64, 128):
+    if q.dtype not in _DTYPE_CODE or D not in _ATTENTION_DIMS:
         raise RuntimeError(f"No suitable kernel. dtype={q.dtype} head_dim={D}")
     page, head, place = _check_caches(k_cache, v_cache, q, plan.kv_heads)
     if k_cache.size(2) != plan.page_size:

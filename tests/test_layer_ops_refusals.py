@@ -134,3 +134,17 @@ def test_extend_with_a_limit(L):
     ext = lambda most=9, ws=A, size=n.value, P=16: L.smlm_kv_extend_upto(
         A, A, A, A, A, A, A, A, A, ws, size, 4, 4, 10, 3, 5, P, most, None, None)
     assert ext(most=-1) == ARG and ext(P=0) == ARG and ext(ws=None) == ARG and ext(size=16) == WORKSPACE
+
+
+@pytest.mark.parametrize("dim,dtype", [(96, torch.bfloat16), (256, torch.float16), (0, torch.bfloat16), (128, torch.float32), (64, torch.int8)])
+def test_a_cache_that_attention_cannot_read(dim, dtype):
+    """Refused when it is made, not when its pages have been written."""
+    from loquetier_amd.kvcache import PagedKvCache
+    with pytest.raises(RuntimeError, match="No suitable kernel"):
+        PagedKvCache(2, 1, 1, dim, 1, 16, dtype=dtype, device="cpu")
+
+
+def test_a_cache_that_it_can_read():
+    from loquetier_amd.kvcache import PagedKvCache
+    for dim, dtype in ((64, torch.float16), (128, torch.bfloat16)):
+        assert PagedKvCache(2, 1, 1, dim, 1, 16, dtype=dtype, device="cpu").pool.shape == (2, 1, 2, 1, 16, dim)
