@@ -511,7 +511,8 @@ SMLM_API int smlm_qk_norm_rope_bwd(const smlm_qk_rope* args, const smlm_heads* g
  * int32: table [R, M] (the pages of request r in order, -1 past the last), length [R] (its tokens), refs [N] (requests that
  * hold page n, 0: free); the requests' rows start with tables of -1 and lengths of 0.  Free pages are taken lowest number first.  A
  * request's last page, where it is part-filled, is its own.
- * A call does all it is asked or, where it cannot, nothing, and then adds SMLM_KV_* bits to *status (int32 on the device; may be NULL).
+ * smlm_kv_extend and smlm_kv_fork do all they are asked or, where they cannot, nothing, and then add SMLM_KV_* bits to *status (int32 on the
+ * device; may be NULL).  smlm_kv_free frees every request that is there, and adds SMLM_KV_BAD_REQUEST for one that is not.
  */
 #define SMLM_KV_BAD_REQUEST 1 /* past R, named twice, a child that is not empty, a count below 0 */
 #define SMLM_KV_TOO_LONG 2    /* more pages than a row of the table holds, or more tokens than max_tokens */
@@ -535,7 +536,10 @@ SMLM_API int smlm_kv_extend_upto(int32_t* table, int32_t* length, int32_t* refs,
                                  size_t workspace_bytes, int R, int M, int N, int S, int rows, int page_size, int max_tokens,
                                  int32_t* status, void* stream);
 
-/* The requests' pages lose a holder, their rows become -1 and their lengths 0.  One named twice is freed once; below 0 is skipped. */
+/*
+ * The requests' pages lose a holder, their rows become -1 and their lengths 0, each request by itself: one named twice is freed once, below
+ * 0 is skipped, past R is reported (and the others are freed).
+ */
 SMLM_API int smlm_kv_free(int32_t* table, int32_t* length, int32_t* refs, const int32_t* requests, int R, int M, int N, int K,
                           int page_size, int32_t* status, void* stream);
 

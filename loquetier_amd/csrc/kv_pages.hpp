@@ -6,8 +6,8 @@
 // function of the inputs alone; the counts are changed by integer atomics, whose order does not show.  A request's
 // part-filled last page belongs to it alone (a fork copies it), so growing never has to copy.
 //
-// A call changes all it should or nothing: what it needs is counted and checked first, and a call that cannot be done
-// sets bits of `status`.
+// extend and fork change all they should or nothing: what they need is counted and checked first, and a call that cannot be done
+// sets bits of `status`.  free takes each request by itself: there is nothing it could lack, and a number that is no request's sets a bit.
 //
 // The bookkeeping is a few kilobytes of integers, bound by latency: one workgroup of 1024 threads counts and takes the
 // pages (scans and a pass over refs, sixteen pages a thread at a time, the next ones on their way, ended as soon as enough are found);
@@ -321,7 +321,7 @@ struct KvFreeArgs {
   int R, M, N, K, P;
 };
 
-// A workgroup a request; who takes its length away gives its pages back, so a request named twice is freed once.
+// A workgroup a request, the known ones of a list that names an unknown one too; who takes its length away gives its pages back, so a request named twice is freed once.
 __global__ __launch_bounds__(256) void kv_free_kernel(KvFreeArgs a) {
   __shared__ int had;
   const int r = a.requests[blockIdx.x];

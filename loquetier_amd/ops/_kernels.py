@@ -1170,7 +1170,8 @@ def kv_extend(table: torch.Tensor, length: torch.Tensor, refs: torch.Tensor, req
 
 def kv_free(table: torch.Tensor, length: torch.Tensor, refs: torch.Tensor, requests: torch.Tensor, page_size: int,
             status: Optional[torch.Tensor] = None) -> None:
-    """Gives the requests' pages back (those that a fork shares stay with the others)."""
+    """Gives the requests' pages back (those that a fork shares stay with the others).  Each request by itself: one that is
+    unknown marks `status`, and the others are freed all the same."""
     if _host().kv_free(table, length, refs, requests, page_size, status):
         return
     dev, R, M, N = _kv_state(table, length, refs, status, requests=requests)

@@ -281,3 +281,18 @@ def test_copy_pages(K, shape):
     want[[0, 3]] = pool[[2, 1]]
     K.kv_copy_pages(pool, ints([2, 1, 0, 99, -1]), ints([0, 3, 77, 2, 2]))  # three of them with a page that is not there
     assert torch.equal(pool, want)
+
+
+def test_free_takes_each_request_by_itself(K):
+    """A list that names an unknown request, one twice and one that is skipped: the rest is freed, the unknown one reported."""
+    m, d = both(K, n_pages=30, P=4, requests=6, width=5)
+    do_extend(m, d, [0, 1, 2, 3], [9, 17, 4, 1], 31)
+    m.fork([1], [4])
+    K.kv_fork(d.pool, d.table, d.length, d.refs, ints([1]), ints([4]), d.status)
+    K.kv_free(d.table, d.length, d.refs, ints([0, 6, 1, -2, 1, 2 ** 31 - 1]), d.P, d.status)
+    assert d.status.item() == 1 and d.length.tolist() == [0, 0, 4, 1, 17, 0]
+    assert d.table.tolist()[0] == d.table.tolist()[1] == [-1] * 5
+    assert [n for n, r in enumerate(d.refs.tolist()) if r] == sorted({i for row in d.table.tolist() for i in row if i >= 0})
+    assert set(d.refs.tolist()) == {0, 1}  # (what the fork shares has one holder left)
+    m.free([0, 6, 1, -2, 1, 2 ** 31 - 1])
+    d.same(m)
