@@ -2,7 +2,8 @@
 step that read them (the reference keeps both in Python lists, kernel_src/src/loquetier/utils/kvcache.py, and hands
 pointers to its init_kv / append_kv / batch_prefill / batch_decode, kernel_src/csrc/loquetier_ops.cc:90-273).
 
-Nothing here waits for the GPU except `check`."""
+Nothing here waits for the GPU except `check`, and lists of more than 3584 entries, which are copied where shorter ones travel in a
+launch's arguments (tensors on the device are read where they lie)."""
 from __future__ import annotations
 
 from typing import NamedTuple, Optional, Sequence, Tuple, Union
