@@ -511,6 +511,9 @@ SMLM_API int smlm_qk_norm_rope_bwd(const smlm_qk_rope* args, const smlm_heads* g
  * int32: table [R, M] (the pages of request r in order, -1 past the last), length [R] (its tokens), refs [N] (requests that
  * hold page n, 0: free); the requests' rows start with tables of -1 and lengths of 0.  Free pages are taken lowest number first.  A
  * request's last page, where it is part-filled, is its own.
+ * smlm_kv_extend gives places out before anything is written there.  So a step's writes to its slots, and its attention, come before the next
+ * smlm_kv_fork of its requests (which copies places that count as filled), the next smlm_kv_free of them and the next smlm_kv_compact (after which
+ * the slots' pages are free or somebody else's).
  * smlm_kv_extend and smlm_kv_fork do all they are asked or, where they cannot, nothing, and then add SMLM_KV_* bits to *status (int32 on the
  * device; may be NULL).  smlm_kv_free frees every request that is there, and adds SMLM_KV_BAD_REQUEST for one that is not.
  */
@@ -520,7 +523,7 @@ SMLM_API int smlm_qk_norm_rope_bwd(const smlm_qk_rope* args, const smlm_heads* g
 #define SMLM_KV_NO_PAGES 8    /* the pool has not enough free pages                 */
 
 /*
- * Room for counts[s] more tokens of requests[s] (int32 [S]; below 0: skipped), and the step's tables: q_indptr int32 [S + 1] (running sum of
+ * Room for counts[s] more tokens of requests[s] (int32 [S]; below 0: skipped, without rows), and the step's tables: q_indptr int32 [S + 1] (running sum of
  * the counts), kv_len int32 [S] (tokens with the new ones), and for each of `rows` rows (at least the counts' sum) positions int32 and
  * slots int64 (page * page_size + place); rows past the sum get -1.  A refused step has zeros in q_indptr and kv_len, and -1.
  */

@@ -55,7 +55,8 @@ class PagedKvCache:
 
     def extend(self, requests: Ints, counts: Ints, n_rows: Optional[int] = None) -> KvStep:
         """Room for counts[s] new tokens of requests[s], in the batch's order, and the step's tables.  n_rows: rows of the batch
-        (the counts' sum, which a caller with counts on the device names)."""
+        (the counts' sum, which a caller with counts on the device names).  The places are given out before they are written: the
+        step's `attend` calls, all layers', come before the next `fork` or `free` of its requests and the next `compact`."""
         if n_rows is None:
             if isinstance(counts, torch.Tensor):
                 raise RuntimeError("n_rows is needed where the counts are on the device")
@@ -72,6 +73,8 @@ class PagedKvCache:
         kernel.kv_free(self.table, self.length, self.refs, self._ints(requests), self.page_size, self.status)
 
     def compact(self) -> None:
+        """Packs the pages in use to the pool's front.  Between steps: the slots of a step that was extended before name pages as they
+        lay then."""
         kernel.kv_compact(self.pool, self.table, self.refs, self.workspace)
 
     def plan(self, step: KvStep, q_heads: int) -> kernel.AttentionPlan:

@@ -1202,7 +1202,7 @@ def kv_fork(pool: torch.Tensor, table: torch.Tensor, length: torch.Tensor, refs:
 
 
 def kv_compact(pool: torch.Tensor, table: torch.Tensor, refs: torch.Tensor, workspace: Optional[Workspace] = None) -> None:
-    """Packs the pages in use to the pool's front; table and refs follow."""
+    """Packs the pages in use to the pool's front; table and refs follow (slots that kv_extend gave out before do not)."""
     dev, R, M, N = _kv_state(table, None, refs, None)
     blocks, P, place = _kv_pool(pool, dev, N)
     with _on(dev):
