@@ -96,3 +96,23 @@ def test_append(K, dt, norm, T, Hq, Hkv, D, rot, P):
         flat = torch.full((pages * P, Hkv, D), 7.0, dtype=q.dtype, device="cuda")
         flat[slots[ok]] = x[ok]
         assert torch.equal(cache.transpose(1, 2).flatten(0, 1), flat)
+
+
+@pytest.mark.parametrize("T", [1, 4, 5, 129, 2048, 2049, 2053, 4097])
+@pytest.mark.parametrize("H,D,rot", [(1, 128, 128), (9, 128, 64), (32, 128, 128), (5, 80, 80), (3, 512, 512), (33, 64, 16)])
+def test_one_gradient(K, T, H, D, rot):
+    """A gradient of one row and head alone, first, last and between: the weights' gradient is its term, the sums of all others are zero."""
+    q, k, _, table, pos, wq, wk = case("bf16", T, H, H, D, rot, (True, True), seed=T + H)
+    cos, sin = angles(table, pos)
+    for row, head in {(0, 0), (T - 1, H - 1), (T - 1, 0), (0, H - 1), (T // 2, H // 2)}:
+        gq, gk = torch.zeros_like(q), torch.zeros_like(k)
+        gq[row, head] = torch.randn(D, device="cuda").to(q.dtype)
+        gk[T - 1 - row, head] = torch.randn(D, device="cuda").to(q.dtype)
+        dq, dk, dwq, dwk = (torch.full(t.shape, 5.0, dtype=t.dtype, device="cuda") for t in (q, k, wq, wk))
+        K.qk_norm_rope_backward(dq, dk, dwq, dwk, gq, gk, q, k, table, pos, wq, wk, 1e-5)
+        for g, x, dx, dw, at in ((gq, q, dq, dwq, row), (gk, k, dk, dwk, T - 1 - row)):
+            gd, xd, c, s = g[at:at + 1].double(), x[at:at + 1].double(), cos[at:at + 1], sin[at:at + 1]
+            r = (xd.pow(2).mean(-1, keepdim=True) + 1e-5).rsqrt()
+            # (one term is not zero, so no addition rounds)
+            near(dw, (turn(gd, c, -s) * xd * r).sum((0, 1)), (sizes(gd, c, -s) * xd.abs() * r).sum((0, 1)))
+            assert bool(dx[at, head].any()) and int((dx != 0).any(-1).sum()) == 1
