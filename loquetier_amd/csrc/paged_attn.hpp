@@ -15,7 +15,7 @@
 //
 // Sequences of up to 16 tile rows (decoding) are bound by HBM: the four waves of a workgroup take 32 keys in turn, K straight to
 // registers, V through a part of LDS of the wave's own, no barrier until the end.  256 single tokens over up to 4095, 8 kv heads of 128:
-// 2.13 GB in 362 to 382 us by the card, 5.6 to 5.9 TB/s (a plain copy reaches 4.9); three over 131000 5.8 TB/s.  (Three or four workgroups
+// 2.13 GB in 362 to 382 us by the card, 5.6 to 5.9 TB/s (a plain copy reaches 4.9); three over 131000 5.6 to 5.8 TB/s.  (Three or four workgroups
 // a CU, with fewer registers: 433 and 688 us.)  Others take 128 tile rows a workgroup, 32 a wave, over K and V tiles of 64 keys that the
 // four waves share: 2048 rows of 32 heads over 14336 tokens 500 to 535 us by the card, 0.96 to 1.03 PFLOP/s (a library's matrix product of 8192
 // a side 1.17); the matrix cores are busy half of the time at the 1.9 GHz that the card's power leaves them, and LDS a quarter of it,

@@ -9,7 +9,7 @@
 //
 // Streaming kernels, bound by HBM: 2 bytes read and 2 written an element (backward: 4 and 2), and by launch latency
 // for decode batches.  2112 rows of 32 + 32 + 32 heads of 128 with norms into a cache 20 us (5.2 TB/s, as a plain copy of that size); 4096
-// rows of 32 + 8 heads 19 us forward, 26.7 + 3.4 us backward (4.8 TB/s); 256 rows without norms into a cache 3.4 us.  Outputs are stored
+// rows of 32 + 8 heads 19 us forward, 25.0 + 3.4 us backward (5.2 TB/s); 256 rows without norms into a cache 3.4 to 3.8 us.  Outputs are stored
 // non-temporally (24.7 -> 21.0 us at 2112 rows): they would push out of L2 what is still to be read.  A head takes D / 16 lanes (rounded up to a power of two), each with two pieces of eight
 // dimensions that are partners in the rotation, so that the pairs meet inside a lane and only the norm's sum crosses
 // lanes.  A wave keeps one row: cosines and sines of its position are read once for all the heads it takes.
