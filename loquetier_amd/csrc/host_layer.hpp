@@ -265,7 +265,9 @@ PyObject* py_kv_extend(PyObject*, PyObject* const* p, Py_ssize_t n) {
   const Tensor &table = THPVariable_Unpack(p[0]), &length = THPVariable_Unpack(p[1]), &refs = THPVariable_Unpack(p[2]),
                &req = THPVariable_Unpack(p[3]), &counts = THPVariable_Unpack(p[4]);
   const int64_t rows = integer(p[5]), P = integer(p[6]), most = limit ? integer(p[9]) : 0x7fffffff;
-  if (most < 0 || most > 0x7fffffff || !pages(table, &length, refs, status, req, counts) || rows < 0 || rows > (1 << 20) || P < 1 || P > (1 << 30)) Py_RETURN_NONE;
+  if (most < 0 || most > 0x7fffffff || !pages(table, &length, refs, status, req, counts) || rows < 0 || rows > (1 << 20) || P < 1 ||
+      P > (1 << 30))
+    Py_RETURN_NONE;
   const int R = (int)table.size(0), M = (int)table.size(1), N = (int)refs.size(0), S = (int)req.size(0);
   const auto ints = table.options();
   Tensor indptr = at::empty({S + 1}, ints), len = at::empty({S}, ints), pos = at::empty({rows}, ints),

@@ -33,7 +33,7 @@ class PagedKvCache:
 
     def __init__(self, n_pages: int, n_layers: int, kv_heads: int, head_dim: int, max_requests: int, max_tokens: int,
                  page_size: int = 16, dtype: torch.dtype = torch.bfloat16, device="cuda"):
-        if dtype not in kernel._DTYPE_CODE or head_dim not in kernel._ATTENTION_DIMS:  # (not first when its pages hold keys)
+        if dtype not in kernel._DTYPE_CODE or head_dim not in kernel._ATTENTION_DIMS:  # (now, not once its pages hold keys)
             raise RuntimeError(f"No suitable kernel. dtype={dtype} head_dim={head_dim}")
         self.pool = torch.zeros(n_pages, n_layers, 2, kv_heads, page_size, head_dim, dtype=dtype, device=device)
         self.page_size, self.kv_heads, self.max_tokens = page_size, kv_heads, int(max_tokens)
