@@ -1232,9 +1232,9 @@ _ATTENTION_DIMS = (64, 128)  # head sizes of paged_attention
 class AttentionPlan:
     """How the card shares out the attention of one batch (see include/smlm.h): built once a step, for all its layers.
 
-    q_indptr int32 [S + 1]: rows of the sequences in the batch's n_rows, never decreasing (or the plan holds nothing); kv_len int32 [S]: tokens of each in the cache, the
-    new ones too; page_table int32 [R, M] (its contents are read by the attention calls); requests int32 [S]: the
-    sequences' rows of page_table (None: 0, 1, ...).  The tensors are read when the plan's launches run, and kept."""
+    q_indptr int32 [S + 1]: rows of the sequences in the batch's n_rows, never decreasing (or the plan holds nothing); kv_len
+    int32 [S]: tokens of each in the cache, the new ones too; page_table int32 [R, M] (its contents are read by the attention
+    calls); requests int32 [S]: the sequences' rows of page_table (None: 0, 1, ...).  The tensors are read when the plan's launches run, and kept."""
 
     def __init__(self, q_indptr: torch.Tensor, kv_len: torch.Tensor, page_table: torch.Tensor, n_rows: int, q_heads: int,
                  kv_heads: int, page_size: int, requests: Optional[torch.Tensor] = None):
