@@ -590,6 +590,29 @@ SMLM_API int smlm_paged_attn(const smlm_heads* out, const smlm_heads* q, const v
                              void* stream);
 
 /*
+ * Softmax cross entropy of rows against a vocabulary's matrix, without the logits in memory (the reference makes them and takes torch's
+ * loss a train partition: src/loquetier_src/models/mixed_llama.py:382-415).  x [T, H], w [V, H] of `dtype`, labels int64 [T]; a label
+ * outside [0, V) (-100, say) is none.
+ *   lse[t] = log sum_v exp(x[t] . w[v]),  loss[t] = lse[t] - x[t] . w[labels[t]]     float [T]; both 0 without a label
+ * With partition (int32 [P + 1], not decreasing, rows [partition[p], partition[p + 1]) of the batch) also, float [P],
+ *   means[p] = the mean of its labelled rows' losses (0 where there are none), weight[p] = one over their number (0)
+ * and rows outside every partition have no label.  H a multiple of 8.  Sums are taken in a fixed order.
+ */
+SMLM_API int smlm_vocab_loss_workspace_size(int T, int H, int V, int what, size_t* bytes); /* what: 0 forward; backward: 1 dx, 2 dw, 3 both */
+SMLM_API int smlm_vocab_loss_fwd(float* loss, float* lse, float* means, float* weight, const void* x, const void* w,
+                                 const int64_t* labels, const int32_t* partition, int P, void* workspace, size_t workspace_bytes,
+                                 int T, int H, int V, int dtype, void* stream);
+
+/*
+ * Its gradients: dx [T, H] and dw [V, H] (either may be NULL) of sum_t grad[t] loss[t], or with partition of sum_p grad[p] means[p].
+ * lse, weight: the forward's.  The logits are made again, a piece of the vocabulary at a time; rows that nothing hangs on (no label, or
+ * a gradient of 0) cost nothing and get zeros.  dx is rounded once; the products' left operand is rounded to 16 bits as in any product.
+ */
+SMLM_API int smlm_vocab_loss_bwd(void* dx, void* dw, const float* grad, const float* lse, const void* x, const void* w,
+                                 const int64_t* labels, const int32_t* partition, const float* weight, int P, void* workspace,
+                                 size_t workspace_bytes, int T, int H, int V, int dtype, void* stream);
+
+/*
  * Copies `bytes` (a multiple of 4) of host memory to device memory (4-byte aligned) in the
  * arguments of launches on `stream`, 3584 bytes each: src has been read when the call
  * returns, and the host waits for nothing.  For the small tables a call needs (row

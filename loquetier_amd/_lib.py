@@ -108,6 +108,9 @@ SIGNATURES = {
     "smlm_attn_plan_build": (_i, [_vp, _sz, _vp, _vp, _vp] + [_i] * 7 + [_vp]),
     "smlm_paged_attn_workspace_size": (_i, [_i] * 7 + [_psz]),
     "smlm_paged_attn": (_i, [_pheads, _pheads, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _sz, _vp, _sz] + [_i] * 10 + [_f, _vp]),
+    "smlm_vocab_loss_workspace_size": (_i, [_i] * 4 + [_psz]),
+    "smlm_vocab_loss_fwd": (_i, [_vp] * 8 + [_i, _vp, _sz] + [_i] * 4 + [_vp]),
+    "smlm_vocab_loss_bwd": (_i, [_vp] * 9 + [_i, _vp, _sz] + [_i] * 4 + [_vp]),
     "smlm_put_words": (_i, [_vp, _vp, _sz, _vp]),
 }
 

@@ -18,7 +18,7 @@ HOST_PATH = os.path.join(LIB_DIR, "_smlm_host.so")  # Python extension: csrc/hos
 PROBE_PATH = os.path.join(LIB_DIR, "libsmlm_probe.so")
 # library -> its translation units (headers are found through -I csrc)
 LIBRARIES = {
-    LIB_PATH: ["smlm_api.hip", "layer_api.hip"],  # the operator library (include/smlm.h)
+    LIB_PATH: ["smlm_api.hip", "layer_api.hip", "train_api.hip"],  # the operator library (include/smlm.h)
     PROBE_PATH: ["stream_probe.hip"],  # plain streaming kernels bench.py calibrates against
 }
 

@@ -347,3 +347,47 @@ class qk_norm_rope(Function):
     @staticmethod
     def backward(ctx: FunctionCtx, gq: torch.Tensor, gk: torch.Tensor):
         return *_qk_norm_rope_gradients.apply(gq, gk, *ctx.saved_tensors, ctx.eps), None, None, None
+
+
+class _linear_cross_entropy_gradients(Function):
+    """The backward of `linear_cross_entropy`, as a function of its own so that a graph made of it (create_graph) knows what the
+    gradients hang on: to differentiate them is refused, as there is no kernel for it."""
+
+    @staticmethod
+    def forward(ctx: FunctionCtx, grad, x, w, labels, lse, partition, weight, want_x: bool, want_w: bool):
+        dx, dw = torch.empty_like(x) if want_x else None, torch.empty_like(w) if want_w else None
+        kernel.linear_cross_entropy_backward(dx, dw, grad.contiguous(), lse, x, w, labels, partition, weight)
+        return dx, dw
+
+    @staticmethod
+    def backward(ctx: FunctionCtx, *grads):
+        raise RuntimeError("the gradients of linear_cross_entropy cannot be differentiated")
+
+
+class linear_cross_entropy(Function):
+    """`linear_cross_entropy.apply(x, w, labels, partition=None)`: the softmax cross entropy of the logits x w^T against the labels,
+    float32, without the logits in memory (see ops/_kernels.linear_cross_entropy): row by row [rows], or with a partition of the
+    rows, as the flat batch's training sequences are one, the mean over each partition's labelled rows [P] (the reference takes
+    such a loss a train partition: src/loquetier_src/models/mixed_llama.py:382-415).  x and w contiguous, of one 16-bit type.
+    Kept for the backward: the inputs and a float a row.  Its gradients cannot be differentiated again."""
+
+    @staticmethod
+    def forward(ctx: FunctionCtx, x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
+                partition: Optional[torch.Tensor] = None):
+        floats = dict(dtype=torch.float32, device=x.device)
+        loss, lse = torch.empty(x.size(0), **floats), torch.empty(x.size(0), **floats)
+        means = weight = None
+        if partition is not None:
+            means, weight = (torch.empty(max(partition.numel() - 1, 0), **floats) for _ in range(2))
+        kernel.linear_cross_entropy(loss, lse, x, w, labels, partition, means, weight)
+        ctx.save_for_backward(x, w, labels, lse, partition, weight)
+        return loss if partition is None else means
+
+    @staticmethod
+    def backward(ctx: FunctionCtx, grad: torch.Tensor):
+        if not (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]):
+            return None, None, None, None
+        x, w, labels, lse, partition, weight = ctx.saved_tensors
+        dx, dw = _linear_cross_entropy_gradients.apply(grad, x, w, labels, lse, partition, weight, ctx.needs_input_grad[0],
+                                                       ctx.needs_input_grad[1])
+        return dx, dw, None, None

@@ -1305,3 +1305,82 @@ def paged_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v
                                          0 if ws is None else ws.numel(), T, plan.S, R, M, k_cache.size(0), plan.page_size, Hq,
                                          plan.kv_heads, D, _DTYPE_CODE[q.dtype], scale, _stream(dev))
     _lib.check(rc, "paged_attention")
+
+
+# ---- around a fine-tuning step: the loss over the vocabulary ------------------------------------------------------------
+
+def _loss_shapes(x, w, labels, partition):
+    for t, n in ((x, "x"), (w, "w")):
+        _check_input(t, n)
+        _check_dim(2, t, n)
+    dev = x.device
+    if w.dtype != x.dtype or w.device != dev:
+        raise RuntimeError("w must share x's dtype and device")
+    (T, H), V = x.shape, w.size(0)
+    if w.size(1) != H:
+        raise RuntimeError("x and w must have the same columns")
+    if V < 1 or H < 1 or H % 8:
+        raise RuntimeError(f"No suitable kernel. dtype={x.dtype} columns={H} vocabulary={V}")
+    _check_ints(dev, torch.int64, 1, labels=labels)
+    if labels.size(0) != T:
+        raise RuntimeError("labels must have one entry per row")
+    _check_ints(dev, torch.int32, 1, partition=partition)
+    if partition is not None and partition.size(0) < 1:
+        raise RuntimeError("partition needs one entry more than there are partitions")
+    return dev, T, H, V, 0 if partition is None else partition.size(0) - 1
+
+
+def linear_cross_entropy(loss: torch.Tensor, lse: torch.Tensor, x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
+                         partition: Optional[torch.Tensor] = None, means: Optional[torch.Tensor] = None,
+                         weight: Optional[torch.Tensor] = None, workspace: Optional[Workspace] = None) -> None:
+    """loss[t] = logsumexp(x[t] w^T) - x[t] . w[labels[t]] and the logsumexp itself, both float32 [rows], for rows x [rows, columns]
+    and a vocabulary's matrix w [vocabulary, columns] (fp16 or bf16), without the logits in memory.  labels: int64 [rows]; one
+    outside [0, vocabulary) is none, and its row's loss is 0.
+
+    partition (int32 [P + 1]: rows partition[p] to partition[p + 1], not decreasing): means [P] becomes the mean loss of each partition's
+    labelled rows (0 where there are none) and weight [P] one over their number; rows outside every partition have no label."""
+    dev, T, H, V, P = _loss_shapes(x, w, labels, partition)
+    code = _dtype_code(x)
+    _check_ints(dev, torch.float32, 1, loss=loss, lse=lse, means=means, weight=weight)
+    if loss.size(0) != T or lse.size(0) != T:
+        raise RuntimeError("loss and lse must have one entry per row")
+    if P and (means is None or weight is None or means.size(0) != P or weight.size(0) != P):
+        raise RuntimeError("means and weight must have one entry per partition")
+    with _on(dev):
+        ws = _workspace(dev, _lib.size_query("smlm_vocab_loss_workspace_size", T, H, V, 0), workspace)
+        rc = _lib.load().smlm_vocab_loss_fwd(_ptr(loss), _ptr(lse), _ptr(means), _ptr(weight), _ptr(x), _ptr(w), _ptr(labels),
+                                             _ptr(partition) if P else None, P, ws.data_ptr(), ws.numel(), T, H, V, code, _stream(dev))
+    _lib.check(rc, "linear_cross_entropy")
+
+
+def linear_cross_entropy_backward(dx: Optional[torch.Tensor], dw: Optional[torch.Tensor], grad: torch.Tensor, lse: torch.Tensor,
+                                  x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
+                                  partition: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
+                                  workspace: Optional[Workspace] = None) -> None:
+    """Gradients of linear_cross_entropy's losses (grad float32 [rows]) or, with partition, of its means (grad float32 [P]) by x and w;
+    either may be None.  lse, weight: the forward's.  Rows without a label, or with a gradient of 0, get zeros and cost nothing."""
+    dev, T, H, V, P = _loss_shapes(x, w, labels, partition)
+    code = _dtype_code(x)
+    for d, like, n in ((dx, x, "dx"), (dw, w, "dw")):
+        if d is not None:
+            _check_ints(dev, x.dtype, 2, **{n: d})
+            if d.shape != like.shape:
+                raise RuntimeError(f"{n} must match {n[1:]}")
+    if dx is None and dw is None:
+        raise RuntimeError("dx or dw is needed")
+    _check_ints(dev, torch.float32, 1, grad=grad, lse=lse, weight=weight)
+    if lse.size(0) != T or grad.size(0) != (T if partition is None else P):
+        raise RuntimeError("lse must have one entry per row, grad one for each loss")
+    if partition is not None and (weight is None or weight.size(0) != P):
+        raise RuntimeError("weight must have one entry per partition")
+    if T == 0 or (partition is not None and P == 0):
+        for d in (dx, dw):
+            if d is not None:
+                d.zero_()
+        return
+    with _on(dev):
+        what = (dx is not None) + 2 * (dw is not None)
+        ws = _workspace(dev, _lib.size_query("smlm_vocab_loss_workspace_size", T, H, V, what), workspace)
+        rc = _lib.load().smlm_vocab_loss_bwd(_ptr(dx), _ptr(dw), _ptr(grad), _ptr(lse), _ptr(x), _ptr(w), _ptr(labels), _ptr(partition),
+                                             _ptr(weight), P, ws.data_ptr(), ws.numel(), T, H, V, code, _stream(dev))
+    _lib.check(rc, "linear_cross_entropy_backward")

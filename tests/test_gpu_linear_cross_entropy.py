@@ -1,0 +1,299 @@
+"""linear_cross_entropy against its definition in 64 bits: rows and vocabularies around the tiles' edges, rows without labels,
+partitions, gradients of both inputs.
+
+Tolerances.  Logits are sums of H exact products in float, in an order that the matrix cores choose: off by at most H 2^-24 sum |x w|,
+here far less (errors of random sign); 2e-6 of the largest |x||w| covers them, and losses, differences of two such numbers, are taken
+to 1e-5 of it.  An entry G = c (p - [label]) has p = exp(z - lse): off by p times the logits' error, and by some steps of a float
+of the exponential and the logarithm (v_exp_f32 and v_log_f32, 2^-23 each; 1e-6 in all) - of p, not of G, which is near 0 where a label is
+nearly certain.  It is then rounded to 16 bits, at most eps / 2 of |G|, multiplied in float, and the result is rounded once more:
+|error| <= sum |G w| eps / 2 + sum |c p w| (2e-6 |x||w| + 1e-6) + |dx| eps / 2, and a float's rounding of the sums, 1e-7 of their largest."""
+import math
+
+import pytest
+import torch
+
+from loquetier_amd.kernel_utils import linear_cross_entropy
+from loquetier_amd.ops import _kernels as K
+
+pytestmark = pytest.mark.gpu
+FP16, BF16 = torch.float16, torch.bfloat16
+
+
+def make(T, H, V, dt, seed=0, labelled=1.0, spread=2.5):
+    g = torch.Generator().manual_seed(seed)
+    w = (torch.randn(V, H, generator=g) * (spread / math.sqrt(H))).to(dt)
+    labels = torch.randint(0, V, (T,), generator=g)
+    x = (torch.randn(T, H, generator=g) + torch.rand(T, 1, generator=g) * w[labels].float()).to(dt)
+    labels[torch.rand(T, generator=g) >= labelled] = -100
+    return x.cuda(), w.cuda(), labels.cuda()
+
+
+def want(x, w, labels, c):
+    """losses, dx, dw and the sums of absolute values that bound their errors, in 64 bits; c: each row's weight."""
+    x, w = x.double().cpu(), w.double().cpu()
+    labels, c = labels.cpu(), c.double().cpu()
+    V = w.shape[0]
+    ok = (labels >= 0) & (labels < V)
+    z = x @ w.t()
+    lse = torch.logsumexp(z, 1)
+    safe = labels.clamp(0, V - 1)
+    loss = torch.where(ok, lse - z.gather(1, safe[:, None])[:, 0], 0)
+    P = torch.exp(z - lse[:, None]) * torch.where(ok, c, 0)[:, None]
+    G = P.clone()
+    G[torch.arange(len(labels)), safe] -= torch.where(ok, c, 0)
+    bx, bw = [M.abs() @ w.abs() for M in (G, P)], [M.abs().t() @ x.abs() for M in (G, P)]
+    return loss, torch.where(ok, lse, 0), G @ w, G.t() @ x, bx, bw
+
+
+def close(got, exact, bounds, eps, top):
+    off, (bound, soft) = (got.double().cpu() - exact).abs(), bounds
+    limit = bound * eps / 2 + soft * (2e-6 * top + 1e-6) + exact.abs() * eps / 2 + 1e-7 * bound.max()
+    limit += torch.finfo(got.dtype).smallest_normal * eps  # (a step of the subnormal numbers)
+    assert torch.isfinite(got).all()
+    assert (off <= limit).all(), (off / limit).max()
+
+
+def check(x, w, labels, partition=None, want_w=True, grad=None):
+    T = x.shape[0]
+    x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(want_w)
+    out = linear_cross_entropy.apply(x, w, labels, partition)
+    g = torch.rand(out.shape, generator=torch.Generator().manual_seed(3)).cuda() + 0.5 if grad is None else grad
+    grads = torch.autograd.grad(out, [x, w] if want_w else [x], g)
+    ok = (labels >= 0) & (labels < w.shape[0])
+    if partition is None:
+        c = g
+    else:
+        c = torch.zeros(T, device="cuda")
+        for p, (a, b) in enumerate(zip(partition.tolist(), partition.tolist()[1:])):
+            c[a:b] = g[p] / max(1, int(ok[a:b].sum()))
+    loss, lse, dx, dw, bx, bw = want(x.detach(), w.detach(), labels, c)
+    top = (x.detach().double().norm(dim=1).max() * w.detach().double().norm(dim=1).max()).item()
+    if partition is None:
+        assert out.dtype == torch.float32 and (out.double().cpu() - loss).abs().max() <= 1e-5 * max(1, top)
+    else:
+        edges = partition.tolist()
+        means = torch.stack([loss[a:b].sum() / max(1, int(ok[a:b].sum())) for a, b in zip(edges, edges[1:])])
+        assert (out.double().cpu() - means).abs().max() <= 1e-5 * max(1, top)
+    eps = torch.finfo(x.dtype).eps
+    close(grads[0], dx, bx, eps, top)
+    if want_w:
+        close(grads[1], dw, bw, eps, top)
+    return out, grads
+
+
+@pytest.mark.parametrize("dt", [FP16, BF16])
+@pytest.mark.parametrize("T,H,V", [(1, 64, 100), (1, 8, 1), (3, 72, 257), (33, 512, 2000), (64, 128, 300), (65, 128, 300), (130, 200, 1023),
+                                   (256, 64, 256), (257, 264, 513), (300, 1032, 777), (600, 256, 4097)])
+def test_rows_and_gradients(T, H, V, dt):
+    x, w, labels = make(T, H, V, dt, T + V)
+    check(x, w, labels)
+
+
+@pytest.mark.parametrize("dt", [FP16, BF16])
+@pytest.mark.parametrize("T,H,V,labelled", [(40, 136, 500, 0.5), (512, 256, 1500, 0.6), (700, 520, 900, 0.1)])
+def test_rows_without_labels(T, H, V, labelled, dt):
+    x, w, labels = make(T, H, V, dt, T, labelled)
+    x[labels < 0] = float("nan")  # (nothing of them is used)
+    xz = torch.where(labels[:, None] < 0, torch.zeros_like(x), x)
+    edges = torch.tensor([0, T // 3, T // 3, T // 2, T], dtype=torch.int32, device="cuda")  # (one has no rows)
+    a = x.detach().requires_grad_(True)
+    out = linear_cross_entropy.apply(a, w, labels, edges)
+    got = torch.autograd.grad(out, a, torch.ones_like(out))[0]
+    ref_out, ref = check(xz, w, labels, edges, grad=torch.ones_like(out))
+    assert torch.equal(out, ref_out) and torch.equal(got, ref[0])
+    assert out[1] == 0 and not got[labels < 0].any()
+
+
+def test_no_row_has_a_label():
+    x, w, labels = make(100, 64, 300, BF16)
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    for bad in (-100, 300, 1 << 40, -(1 << 40)):
+        labels.fill_(bad)
+        out = linear_cross_entropy.apply(x, w, labels)
+        dx, dw = torch.autograd.grad(out.sum(), (x, w))
+        assert not out.any() and not dx.any() and not dw.any()
+    part = torch.tensor([0, 50, 100], dtype=torch.int32, device="cuda")
+    out = linear_cross_entropy.apply(x, w, labels, part)
+    dx, dw = torch.autograd.grad(out.sum(), (x, w))
+    assert not out.any() and not dx.any() and not dw.any()
+
+
+def test_rows_outside_the_partitions():
+    x, w, labels = make(90, 64, 300, FP16)
+    part = torch.tensor([20, 50, 70], dtype=torch.int32, device="cuda")
+    check(x, w, labels, part)
+    x = x.requires_grad_(True)
+    out = linear_cross_entropy.apply(x, w, labels, part)
+    dx = torch.autograd.grad(out.sum(), x)[0]
+    assert not dx[:20].any() and not dx[70:].any() and dx[20:70].any()
+
+
+def test_one_partitions_loss_alone():
+    x, w, labels = make(600, 128, 700, BF16)
+    part = torch.tensor([0, 200, 600], dtype=torch.int32, device="cuda")
+    check(x, w, labels, part, grad=torch.tensor([0.0, 2.0], device="cuda"))
+    x = x.requires_grad_(True)
+    dx = torch.autograd.grad(linear_cross_entropy.apply(x, w, labels, part)[1], x)[0]
+    assert not dx[:200].any() and dx[200:].any()
+
+
+def test_frozen_head_and_frozen_rows():
+    x, w, labels = make(100, 64, 300, BF16)
+    a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    both = torch.autograd.grad(linear_cross_entropy.apply(a, b, labels).sum(), (a, b))
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy.apply(a, w, labels).sum(), a)[0], both[0])
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy.apply(x, b, labels).sum(), b)[0], both[1])
+
+
+@pytest.mark.parametrize("dt", [FP16, BF16])
+def test_pieces_of_the_vocabulary(dt):
+    """G of more than one piece (128 MiB of it at a time)."""
+    T, V = 700, 100001
+    x, w, labels = make(T, 64, V, dt, 5)
+    x = x.requires_grad_(True)
+    w = w.requires_grad_(True)
+    out = linear_cross_entropy.apply(x, w, labels)
+    dx, dw = torch.autograd.grad(out.sum(), (x, w))
+    z = x.detach().double() @ w.detach().double().t().contiguous()
+    lse = torch.logsumexp(z, 1)
+    at = torch.arange(T, device="cuda")
+    assert (out.double() - (lse - z[at, labels])).abs().max() < 2e-5
+    G = torch.exp(z - lse[:, None])
+    G[at, labels] -= 1
+    eps = torch.finfo(dt).eps
+    for got, a, b in ((dx, G, w.detach().double()), (dw, G.t().contiguous(), x.detach().double())):
+        exact, bound = a @ b, a.abs() @ b.abs()
+        assert ((got.double() - exact).abs() <= bound * (eps / 2 + 1e-5) + exact.abs() * eps / 2 + 1e-7).all()
+
+
+def test_small_gradients_in_fp16():
+    """Gradients far below one, and rows whose weights differ by 2^20: G is held relative to the largest."""
+    x, w, labels = make(80, 128, 5000, FP16, 1)
+    x = x.requires_grad_(True)
+    g = torch.full((80,), 2.0 ** -6, device="cuda")
+    g[40:] = 2.0 ** -26
+    dx, = torch.autograd.grad(linear_cross_entropy.apply(x, w, labels), x, g * 2.0 ** 20)
+    loss, _, want_x, _, bound, _ = want(x.detach(), w, labels, g * 2.0 ** 20)
+    off = (dx.double().cpu() - want_x).abs()
+    limit = bound[0] * 2.0 ** -11 + bound[1] * 1e-4 + want_x.abs() * 2.0 ** -11 + 2.0 ** -25
+    assert (off <= limit).all(), (off / limit).max()
+
+
+def test_infinities_and_nan_stay_in_their_rows():
+    x, w, labels = make(70, 64, 300, BF16, 2)
+    x[3], x[5, 0] = float("nan"), float("inf")
+    x = x.requires_grad_(True)
+    out = linear_cross_entropy.apply(x, w, labels)
+    dx, = torch.autograd.grad(out.sum(), x)
+    bad = torch.zeros(70, dtype=torch.bool, device="cuda")
+    bad[3] = bad[5] = True
+    assert torch.isnan(out[bad]).all() and torch.isfinite(out[~bad]).all()
+    assert torch.isnan(dx[bad]).any(1).all() and torch.isfinite(dx[~bad]).all()
+
+
+def test_large_logits():
+    """Logits of some thousands: the maximum is taken off before the exponentials."""
+    x, w, labels = make(50, 128, 700, BF16, 4, spread=400.0)
+    x = x.requires_grad_(True)
+    out = linear_cross_entropy.apply(x, w, labels)
+    loss, *_ = want(x.detach(), w, labels, torch.ones(50))
+    assert ((out.double().cpu() - loss).abs() <= 1e-5 * (1 + loss.abs()) + 5e-3).all()
+    assert torch.isfinite(torch.autograd.grad(out.sum(), x)[0]).all()
+
+
+def test_differences():
+    """The gradient against central differences of the loss: x moves along a direction by powers of two that bf16 holds."""
+    x, w, labels = make(8, 64, 200, BF16, 6)
+    x = (x.float() * 16).round().clamp(-64, 64).div(16).to(BF16)  # (multiples of 2^-4 up to 4: sums with 2^-5 are exact)
+    a = x.clone().requires_grad_(True)
+    dx, = torch.autograd.grad(linear_cross_entropy.apply(a, w, labels).sum(), a)
+    d = (torch.rand(8, 64, generator=torch.Generator().manual_seed(1)) < 0.5).to(BF16).cuda() * 2 - 1
+    step = 2.0 ** -5
+    up, down = (linear_cross_entropy.apply(x + s * d, w, labels) for s in (step, -step))
+    slope = (up - down) / (2 * step)
+    along = (dx.float() * d.float()).sum(1)
+    # third derivative of a logsumexp along d: at most 2 max |w . d|^3, the difference quotient off by step^2 / 6 of it
+    far = (w.double() @ d.double().t()).abs().amax(0).cpu()
+    limit = step ** 2 / 3 * far ** 3 + 2e-5 / step + 2.0 ** -8 * 2 * (dx.float().abs() * 2).sum(1).cpu() + 64 * 2.0 ** -9 * w.abs().max().item()
+    assert ((slope - along).abs().cpu() <= limit).all()
+
+
+def test_captured_and_replayed():
+    x, w, labels = make(300, 128, 1000, BF16, 7, 0.7)
+    part = torch.tensor([0, 100, 300], dtype=torch.int32, device="cuda")
+    ws = K.Workspace(x.device)
+    f = lambda n: torch.empty(n, device="cuda")
+    loss, lse, means, weight, dx, dw = f(300), f(300), f(2), f(2), torch.empty_like(x), torch.empty_like(w)
+    g = torch.ones(2, device="cuda")
+
+    def step():
+        K.linear_cross_entropy(loss, lse, x, w, labels, part, means, weight, ws)
+        K.linear_cross_entropy_backward(dx, dw, g, lse, x, w, labels, part, weight, ws)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            step()
+    torch.cuda.current_stream().wait_stream(s)
+    for seed in (8, 9, 10):
+        x2, w2, l2 = make(300, 128, 1000, BF16, seed, 0.4 + 0.1 * (seed - 8))
+        x.copy_(x2), w.copy_(w2), labels.copy_(l2)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (means, dx, dw)]
+        step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, (means, dx, dw)))
+        check(x, w, labels, part)
+
+
+def test_another_stream_and_the_same_bits():
+    x, w, labels = make(500, 256, 3000, FP16, 8)
+    x = x.requires_grad_(True)
+    run = lambda: (lambda o: (o.detach(), torch.autograd.grad(o.sum(), x)[0]))(linear_cross_entropy.apply(x, w, labels))
+    first = run()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        second = run()
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+
+
+def test_second_derivatives_are_refused():
+    x, w, labels = make(8, 64, 100, BF16)
+    x = x.requires_grad_(True)
+    dx, = torch.autograd.grad(linear_cross_entropy.apply(x, w, labels).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="cannot be differentiated"):
+        torch.autograd.grad(dx.float().sum(), x)
+
+
+@pytest.mark.parametrize("T", [0, 4])
+def test_empty(T):
+    x = torch.randn(T, 64, device="cuda").to(BF16).requires_grad_(True)
+    w = torch.randn(10, 64, device="cuda").to(BF16).requires_grad_(True)
+    labels = torch.zeros(T, dtype=torch.int64, device="cuda")
+    out = linear_cross_entropy.apply(x, w, labels, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    assert out.shape == (0,)
+    dx, dw = torch.autograd.grad(out.sum(), (x, w))
+    assert not dx.any() and not dw.any() and dx.shape == x.shape
+    if T == 0:
+        out = linear_cross_entropy.apply(x, w, labels)
+        assert out.shape == (0,) and not torch.autograd.grad(out.sum(), w)[0].any()
+
+
+def test_refusals():
+    x, w, labels = make(8, 64, 100, BF16)
+    ok = lambda **k: linear_cross_entropy.apply(*{**dict(x=x, w=w, labels=labels, partition=None), **k}.values())
+    part = torch.tensor([0, 8], dtype=torch.int32, device="cuda")
+    for bad, text in ((dict(x=x.float(), w=w.float()), "No suitable kernel"), (dict(x=x.half()), "dtype"),
+                      (dict(x=x[:, :60].contiguous(), w=w[:, :60].contiguous()), "No suitable kernel"),
+                      (dict(x=x[:, :32]), "contiguous"), (dict(w=w[:, :32].contiguous()), "columns"),
+                      (dict(labels=labels.int()), "int64"), (dict(labels=labels[:4]), "one entry per row"),
+                      (dict(x=x.cpu()), "CUDA"), (dict(partition=part.long()), "int32"), (dict(x=x[0]), "2D"),
+                      (dict(partition=part[:0]), "partition"), (dict(w=w[:0]), "No suitable kernel")):
+        with pytest.raises(RuntimeError, match=text):
+            ok(**bad)
