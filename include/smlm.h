@@ -590,6 +590,26 @@ SMLM_API int smlm_paged_attn(const smlm_heads* out, const smlm_heads* q, const v
                              void* stream);
 
 /*
+ * The residual's addition, the RMSNorm behind it and the norm's 8-bit form in one pass (the reference adds in a tensor expression and
+ * norms the sum: src/loquetier_src/models/mixed_llama.py:53-66), in float, each output rounded once:
+ *   h = x + residual (rounded to `dtype`),  y = h * rms * w,  rms[t] = 1 / sqrt(mean_j h[t,j]^2 + eps)
+ *   out = y in `dtype`;  out8 = y / scale in e4m3 (OCP), scale = max |y| / 448 of the row (group 0: float [rows]) or of 128 columns
+ *   (group 128: float [rows, cols / 128], cols a multiple of 128)
+ * x, residual, h, out: [rows, cols]; w: [cols]; cols a multiple of 8.  residual NULL: h is x (and the argument h NULL).  h, out, rms, and out8
+ * with scale may be NULL where they are not wanted (one of h, out, out8 is).  h and out may be x or residual.  A scale below the
+ * normal floats is 0 and its values are zeros; where y holds an infinity or NaN the scale is infinite or NaN.
+ */
+SMLM_API int smlm_add_rms_norm_fwd(void* out, float* rms, void* h, const void* x, const void* residual, const void* w, void* out8,
+                                   float* scale, int group, int rows, int cols, float eps, int dtype, void* stream);
+
+/*
+ * Its backward: g the gradient of out, gh that of h (NULL: none); dh = gh + (g*w - h*dot*rms^2/cols) * rms, rounded once, is the gradient
+ * of x and of the residual, dw as smlm_rms_norm_bwd's, and so is the workspace (smlm_rms_norm_bwd_workspace_size).  dh may be g or gh.
+ */
+SMLM_API int smlm_add_rms_norm_bwd(void* dh, void* dw, const void* g, const void* gh, const void* h, const void* w, const float* rms,
+                                   void* workspace, size_t workspace_bytes, int rows, int cols, int dtype, void* stream);
+
+/*
  * Softmax cross entropy of rows against a vocabulary's matrix, without the logits in memory (the reference makes them and takes torch's
  * loss a train partition: src/loquetier_src/models/mixed_llama.py:382-415).  x [T, H], w [V, H] of `dtype`, labels int64 [T]; a label
  * outside [0, V) (-100, say) is none.
@@ -597,20 +617,60 @@ SMLM_API int smlm_paged_attn(const smlm_heads* out, const smlm_heads* q, const v
  * With partition (int32 [P + 1], not decreasing, rows [partition[p], partition[p + 1]) of the batch) also, float [P],
  *   means[p] = the mean of its labelled rows' losses (0 where there are none), weight[p] = one over their number (0)
  * and rows outside every partition have no label.  H a multiple of 8.  Sums are taken in a fixed order.
+ * kept (16-byte aligned; NULL: not wanted) is filled with what smlm_vocab_loss_bwd_kept makes dx of: a product more here, none there.
  */
-SMLM_API int smlm_vocab_loss_workspace_size(int T, int H, int V, int what, size_t* bytes); /* what: 0 forward; backward: 1 dx, 2 dw, 3 both */
-SMLM_API int smlm_vocab_loss_fwd(float* loss, float* lse, float* means, float* weight, const void* x, const void* w,
-                                 const int64_t* labels, const int32_t* partition, int P, void* workspace, size_t workspace_bytes,
-                                 int T, int H, int V, int dtype, void* stream);
+SMLM_API int smlm_vocab_loss_workspace_size(int T, int H, int V, int what, size_t* bytes); /* what: 0 forward, 4 forward with kept; backward:
+                                                                                              1 dx, 2 dw, 3 both; 5: bytes of kept */
+SMLM_API int smlm_vocab_loss_fwd(float* loss, float* lse, float* means, float* weight, void* kept, size_t kept_bytes, const void* x,
+                                 const void* w, const int64_t* labels, const int32_t* partition, int P, void* workspace,
+                                 size_t workspace_bytes, int T, int H, int V, int dtype, void* stream);
 
 /*
- * Its gradients: dx [T, H] and dw [V, H] (either may be NULL) of sum_t grad[t] loss[t], or with partition of sum_p grad[p] means[p].
- * lse, weight: the forward's.  The logits are made again, a piece of the vocabulary at a time; rows that nothing hangs on (no label, or
- * a gradient of 0) cost nothing and get zeros.  dx is rounded once; the products' left operand is rounded to 16 bits as in any product.
+ * dx [T, H] of sum_t grad[t] loss[t], or with partition of sum_p grad[p] means[p], from what the forward kept (w, partition and weight as there).
+ * Rows that nothing hangs on (no label, or a gradient of 0) get zeros.  Rounded once; the exponentials, the left operand of a product,
+ * are rounded to 16 bits as in any.
  */
-SMLM_API int smlm_vocab_loss_bwd(void* dx, void* dw, const float* grad, const float* lse, const void* x, const void* w,
-                                 const int64_t* labels, const int32_t* partition, const float* weight, int P, void* workspace,
+SMLM_API int smlm_vocab_loss_bwd_kept(void* dx, const float* grad, const void* kept, size_t kept_bytes, const void* w,
+                                      const int32_t* partition, const float* weight, int P, int T, int H, int V, int dtype, void* stream);
+
+/*
+ * dx and dw [V, H] (either may be NULL) without anything kept but loss and lse: the logits are made again, a piece of the vocabulary at a time;
+ * rows that nothing hangs on cost nothing.
+ */
+SMLM_API int smlm_vocab_loss_bwd(void* dx, void* dw, const float* grad, const float* loss, const float* lse, const void* x,
+                                 const void* w, const int64_t* labels, const int32_t* partition, const float* weight, int P, void* workspace,
                                  size_t workspace_bytes, int T, int H, int V, int dtype, void* stream);
+
+/*
+ * One AdamW step of many tensors in place, each in a group of its own rates and with a step count of its own (the reference keeps an
+ * optimizer an adapter: src/loquetier_src/trainer_utils.py).  params, grads, sizes are HOST arrays; grads[i] NULL: tensor i stays as
+ * it is and its step does not count on.  Everything else is device memory:
+ *   step [n] int32, counted on;  group [n] int32 in [0, n_groups) (a tensor of another group stays as it is);
+ *   hyper [n_groups][5] float: lr, b1, b2, eps, weight decay
+ *   exp_avg, exp_avg_sq: flat, tensor i from element 256 * sum_{j < i} ceil(sizes[j] / 256) on, each tensor's last 256 filled up with
+ *   zeros.  state_bits 32: float, the averages m of g and v of g^2.  8: e4m3, m and the ROOT of v, relative to the floats
+ *   avg_scale, sq_scale of every 256 elements (a root above 0 is held as 2^-9 of its scale at least)
+ *   master: NULL, or float weights, flat as the states; the 16-bit weights become their rounding.  One that is not its float weight's
+ *   rounding before the step takes that one's place.
+ *     m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  w = w - lr wd w - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * dtype: SMLM_DTYPE_* of weights and gradients, or 2: float (master NULL).  No two tensors may overlap.
+ */
+typedef struct smlm_adamw {
+  void* const* params;
+  const void* const* grads;
+  const int64_t* sizes;
+  int32_t* step;
+  const int32_t* group;
+  const float* hyper;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* avg_scale;
+  float* sq_scale;
+  float* master;
+  int n_tensors, n_groups, state_bits, dtype;
+} smlm_adamw;
+SMLM_API int smlm_adamw_workspace_size(int n_tensors, size_t* bytes);
+SMLM_API int smlm_adamw_step(const smlm_adamw* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Copies `bytes` (a multiple of 4) of host memory to device memory (4-byte aligned) in the

@@ -20,6 +20,7 @@ SMLM_ERR_SCRATCH = -7
 SMLM_STATIC_SCRATCH_BYTES = 8 << 20
 SMLM_STAGE_SHRINK, SMLM_STAGE_EXPAND = 1, 2
 SMLM_BWD_PRODUCTS, SMLM_BWD_DX, SMLM_BWD_WGRAD = 1, 2, 4
+SMLM_DTYPE_F32 = 2  # of smlm_adamw alone
 SMLM_KV_BAD_REQUEST, SMLM_KV_TOO_LONG, SMLM_KV_ROWS, SMLM_KV_NO_PAGES = 1, 2, 4, 8
 
 _vp, _i, _sz, _f = C.c_void_p, C.c_int, C.c_size_t, C.c_float
@@ -56,6 +57,13 @@ class QkRope(C.Structure):
                 ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("slot_stride", C.c_int64),
                 *[(n, C.c_int) for n in ("rows", "q_heads", "kv_heads", "head_dim", "rot_dim", "table_rows", "n_pages",
                                          "page_size", "dtype")], ("eps", C.c_float)]
+
+
+class AdamW(C.Structure):
+    """struct smlm_adamw of include/smlm.h."""
+    _fields_ = [*[(n, C.c_void_p) for n in ("params", "grads", "sizes", "step", "group", "hyper", "exp_avg", "exp_avg_sq",
+                                            "avg_scale", "sq_scale", "master")],
+                *[(n, C.c_int) for n in ("n_tensors", "n_groups", "state_bits", "dtype")]]
 
 
 _pheads, _prope, _i64 = C.POINTER(Heads), C.POINTER(QkRope), C.c_int64
@@ -108,9 +116,14 @@ SIGNATURES = {
     "smlm_attn_plan_build": (_i, [_vp, _sz, _vp, _vp, _vp] + [_i] * 7 + [_vp]),
     "smlm_paged_attn_workspace_size": (_i, [_i] * 7 + [_psz]),
     "smlm_paged_attn": (_i, [_pheads, _pheads, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _sz, _vp, _sz] + [_i] * 10 + [_f, _vp]),
+    "smlm_add_rms_norm_fwd": (_i, [_vp] * 8 + [_i] * 3 + [_f, _i, _vp]),
+    "smlm_add_rms_norm_bwd": (_i, [_vp] * 8 + [_sz] + [_i] * 3 + [_vp]),
+    "smlm_adamw_workspace_size": (_i, [_i, _psz]),
+    "smlm_adamw_step": (_i, [C.POINTER(AdamW), _vp, _sz, _vp]),
     "smlm_vocab_loss_workspace_size": (_i, [_i] * 4 + [_psz]),
-    "smlm_vocab_loss_fwd": (_i, [_vp] * 8 + [_i, _vp, _sz] + [_i] * 4 + [_vp]),
-    "smlm_vocab_loss_bwd": (_i, [_vp] * 9 + [_i, _vp, _sz] + [_i] * 4 + [_vp]),
+    "smlm_vocab_loss_fwd": (_i, [_vp] * 5 + [_sz] + [_vp] * 4 + [_i, _vp, _sz] + [_i] * 4 + [_vp]),
+    "smlm_vocab_loss_bwd_kept": (_i, [_vp] * 3 + [_sz] + [_vp] * 3 + [_i] * 5 + [_vp]),
+    "smlm_vocab_loss_bwd": (_i, [_vp] * 10 + [_i, _vp, _sz] + [_i] * 4 + [_vp]),
     "smlm_put_words": (_i, [_vp, _vp, _sz, _vp]),
 }
 
@@ -146,8 +159,9 @@ _host = None
 
 class _NoHost:
     """In the native host path's place where it cannot be loaded: declines every call, and the Python functions take it."""
-    forward = rope = paged_attention = kv_free = kv_fork = staticmethod(lambda *args: False)
+    forward = rope = paged_attention = kv_free = kv_fork = add_rms = adamw_step = staticmethod(lambda *args: False)
     rms_norm = add_lora = fused_add_lora = qk_norm_rope = attention_plan = kv_extend = staticmethod(lambda *args: None)
+    add_rms_norm = linear_cross_entropy = staticmethod(lambda *args: None)
 
 
 def host(default_workspace=None):

@@ -25,6 +25,7 @@
 
 #include <string.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "smlm.h"
@@ -59,6 +60,14 @@ struct Lib {
   decltype(&smlm_kv_extend_upto) kv_extend;
   decltype(&smlm_kv_free) kv_free;
   decltype(&smlm_kv_fork) kv_fork;
+  decltype(&smlm_add_rms_norm_fwd) add_rms_fwd;
+  decltype(&smlm_add_rms_norm_bwd) add_rms_bwd;
+  decltype(&smlm_vocab_loss_workspace_size) loss_size;
+  decltype(&smlm_vocab_loss_fwd) loss_fwd;
+  decltype(&smlm_vocab_loss_bwd) loss_bwd;
+  decltype(&smlm_vocab_loss_bwd_kept) loss_bwd_kept;
+  decltype(&smlm_adamw_workspace_size) adamw_size;
+  decltype(&smlm_adamw_step) adamw;
 } lib;
 PyObject* default_workspace = nullptr;  // ops._kernels._workspace
 
@@ -706,6 +715,7 @@ PyObject* py_fused_add_lora(PyObject*, PyObject* const* p, Py_ssize_t n) {
 }
 
 #include "host_layer.hpp"
+#include "host_train.hpp"
 
 // bind({entry: address}, default_workspace)
 PyObject* py_bind(PyObject*, PyObject* args) {
@@ -739,6 +749,14 @@ PyObject* py_bind(PyObject*, PyObject* args) {
   get("smlm_kv_extend_upto", &lib.kv_extend);
   get("smlm_kv_free", &lib.kv_free);
   get("smlm_kv_fork", &lib.kv_fork);
+  get("smlm_add_rms_norm_fwd", &lib.add_rms_fwd);
+  get("smlm_add_rms_norm_bwd", &lib.add_rms_bwd);
+  get("smlm_vocab_loss_workspace_size", &lib.loss_size);
+  get("smlm_vocab_loss_fwd", &lib.loss_fwd);
+  get("smlm_vocab_loss_bwd", &lib.loss_bwd);
+  get("smlm_vocab_loss_bwd_kept", &lib.loss_bwd_kept);
+  get("smlm_adamw_workspace_size", &lib.adamw_size);
+  get("smlm_adamw_step", &lib.adamw);
   Py_INCREF(ws);
   Py_XSETREF(default_workspace, ws);
   Py_RETURN_NONE;
@@ -758,6 +776,10 @@ PyMethodDef methods[] = {
     {"kv_extend", (PyCFunction)(void (*)(void))py_kv_extend, METH_FASTCALL, nullptr},
     {"kv_free", (PyCFunction)(void (*)(void))py_kv_free, METH_FASTCALL, nullptr},
     {"kv_fork", (PyCFunction)(void (*)(void))py_kv_fork, METH_FASTCALL, nullptr},
+    {"add_rms_norm", (PyCFunction)(void (*)(void))py_add_rms_norm, METH_FASTCALL, nullptr},
+    {"add_rms", (PyCFunction)(void (*)(void))py_add_rms, METH_FASTCALL, nullptr},
+    {"linear_cross_entropy", (PyCFunction)(void (*)(void))py_linear_cross_entropy, METH_FASTCALL, nullptr},
+    {"adamw_step", (PyCFunction)(void (*)(void))py_adamw_step, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_smlm_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

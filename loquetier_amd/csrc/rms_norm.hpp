@@ -150,6 +150,7 @@ struct RmsBwdArgs {
   const uint16_t* w;    // [cols]
   const float* rms;     // [rows]
   int rows, cols;
+  const uint16_t* gh;   // [rows, cols] what dx gets besides (ADD)
 };
 
 // A workgroup walks the rows R at a time, blockIdx.x * R, + gridDim.x * R, ...; a thread takes 8 columns (CH = 1, up to
@@ -163,7 +164,7 @@ struct RmsBwdArgs {
 // wider one / contiguous shares / interleaved: 4096 x 4096 26.0 / 24.3 / 23.2, 8192 x 4096 46.4 / 41.0 / 38.0,
 // 8192 x 6144 80.6 / 67.2 / 55.0, 4096 x 12288 66.7 / 70.1 / 57.6, 1000 x 16384 30.4 / 31.1 / 29.8,
 // 4096 x 16384 85.6 / 83.0 / 76.7, 300 x 1024 12.0 / 6.5 / 6.3, 4096 x 2048 17.4 / 17.1 / 16.5.
-template <int DT, int CH, int R>
+template <int DT, int CH, int R, bool ADD = false>
 __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4))) void rms_bwd_kernel(RmsBwdArgs a) {
   typedef float dots_t __attribute__((ext_vector_type(R)));
   __shared__ dots_t part[2][16];  // the rows' dots by wave, two halves in turn
@@ -185,7 +186,7 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4))) void 
     for (int e = 0; e < 8; ++e) dw[i][e] = 0.0f;
   }
   // rows past the last re-read it and are not used
-  auto load = [&](int row, u32x4 (&xr)[R][CH], u32x4 (&gr)[R][CH], float (&r)[R]) {
+  auto load = [&](int row, u32x4 (&xr)[R][CH], u32x4 (&gr)[R][CH], u32x4 (&hr)[R][CH], float (&r)[R]) {
 #pragma unroll
     for (int t = 0; t < R; ++t) {
       const int rr = row + t < a.rows ? row + t : a.rows - 1;
@@ -193,20 +194,21 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4))) void 
       for (int i = 0; i < CH; ++i) {
         xr[t][i] = ldg16_nt(a.x + (long)rr * a.cols + col[i]);
         gr[t][i] = ldg16_nt(a.g + (long)rr * a.cols + col[i]);
+        if (ADD) hr[t][i] = ldg16_nt(a.gh + (long)rr * a.cols + col[i]);
       }
       r[t] = uload(a.rms, rr);
     }
   };
-  u32x4 xv[R][CH], gv[R][CH];
+  u32x4 xv[R][CH], gv[R][CH], hv[R][CH];
   float rms[R];
-  load((int)blockIdx.x * R, xv, gv, rms);
+  load((int)blockIdx.x * R, xv, gv, hv, rms);
   int parity = 0;
   for (int row = (int)blockIdx.x * R; row < a.rows; row += step) {  // uniform over the workgroup
-    u32x4 xn[R][CH], gn[R][CH];
+    u32x4 xn[R][CH], gn[R][CH], hn[R][CH];
     float rn[R];
     // unconditional (past the end it re-reads these rows): a branch around the loads would make the wave wait
     // for everything in flight where the paths join
-    load(row + step < a.rows ? row + step : row, xn, gn, rn);
+    load(row + step < a.rows ? row + step : row, xn, gn, hn, rn);
     __builtin_amdgcn_sched_barrier(0);  // the next rows' loads are issued before these rows are used
     dots_t dots;
 #pragma unroll
@@ -241,10 +243,14 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4))) void 
         unpack8<DT>(gv[t][i], gf);
         unpack8<DT>(wv[i], wf);
         u32x4 o;
+        float hf[8];
+        if (ADD) unpack8<DT>(hv[t][i], hf);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          o[e] = pack2<DT>((gf[2 * e] * wf[2 * e] - xf[2 * e] * coef) * rms[t],
-                           (gf[2 * e + 1] * wf[2 * e + 1] - xf[2 * e + 1] * coef) * rms[t]);
+        for (int e = 0; e < 4; ++e) {
+          const float d0 = (gf[2 * e] * wf[2 * e] - xf[2 * e] * coef) * rms[t];
+          const float d1 = (gf[2 * e + 1] * wf[2 * e + 1] - xf[2 * e + 1] * coef) * rms[t];
+          o[e] = ADD ? pack2<DT>(hf[2 * e] + d0, hf[2 * e + 1] + d1) : pack2<DT>(d0, d1);
+        }
         if (ok[i]) stg16_nt(a.dx + (long)(row + t) * a.cols + col[i], o);
 #pragma unroll
         for (int e = 0; e < 8; ++e) dw[i][e] += xf[e] * rms[t] * gf[e];
@@ -253,7 +259,10 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4))) void 
 #pragma unroll
     for (int t = 0; t < R; ++t) {
 #pragma unroll
-      for (int i = 0; i < CH; ++i) xv[t][i] = xn[t][i], gv[t][i] = gn[t][i];
+      for (int i = 0; i < CH; ++i) {
+        xv[t][i] = xn[t][i], gv[t][i] = gn[t][i];
+        if (ADD) hv[t][i] = hn[t][i];
+      }
       rms[t] = rn[t];
     }
   }
@@ -308,7 +317,7 @@ __global__ __launch_bounds__(256) void rms_fwd_wide_kernel(RmsFwdArgs a) {
   }
 }
 
-template <int DT>
+template <int DT, bool ADD = false>
 __global__ __launch_bounds__(256) void rms_bwd_wide_kernel(RmsBwdArgs a) {
   __shared__ float red4[4];
   const float inv_n = 1.0f / (float)a.cols;
@@ -333,10 +342,14 @@ __global__ __launch_bounds__(256) void rms_bwd_wide_kernel(RmsBwdArgs a) {
       unpack8<DT>(ldg16(a.g + off + col), gf);
       unpack8<DT>(ldg16(a.w + col), wf);
       u32x4 o;
+      float hf[8];
+      if (ADD) unpack8<DT>(ldg16(a.gh + off + col), hf);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        o[e] = pack2<DT>((gf[2 * e] * wf[2 * e] - xf[2 * e] * coef) * rms,
-                         (gf[2 * e + 1] * wf[2 * e + 1] - xf[2 * e + 1] * coef) * rms);
+      for (int e = 0; e < 4; ++e) {
+        const float d0 = (gf[2 * e] * wf[2 * e] - xf[2 * e] * coef) * rms;
+        const float d1 = (gf[2 * e + 1] * wf[2 * e + 1] - xf[2 * e + 1] * coef) * rms;
+        o[e] = ADD ? pack2<DT>(hf[2 * e] + d0, hf[2 * e + 1] + d1) : pack2<DT>(d0, d1);
+      }
       stg16_nt(a.dx + off + col, o);
       // this thread's columns of the workgroup's partial row: nobody else touches them
       f32x4 p0 = {0.f, 0.f, 0.f, 0.f}, p1 = p0;

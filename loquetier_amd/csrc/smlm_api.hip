@@ -9,7 +9,7 @@
 
 #include "api_common.hpp"
 #include "put_words.hpp"
-#include "rms_norm.hpp"
+#include "rms_launch.hpp"
 #include "segments.hpp"
 #include "smlm.h"
 #include "smlm_backward.hpp"
@@ -903,18 +903,6 @@ void* static_scratch() {
   return p;
 }
 
-// Columns a workgroup of the RMSNorm backward's fold takes: 16 where a row is short, so that its workgroups fill the
-// chip; of wider rows 32 and 64, as the pieces of 64 bytes that 16 columns read of every partial row fetch the lines
-// twice.  Whole backward, us, 16 / 32 / 64 columns: 4096 x 2048 16.9 / 16.9 / -, 1000 x 4096 12.4 / 11.0 / -,
-// 1000 x 8192 21.8 / 18.8 / 18.6, 1000 x 11008 28.7 / 25.1 / 24.8, 64 x 20480 16.9 / - / 14.5.
-template <int DT>
-int launch_rms_fold(hipStream_t st, const RmsFoldArgs& a) {
-  const dim3 bl(256);
-  if (a.cols <= 2048) return launch(rms_fold_kernel<DT, 4>, dim3((unsigned)ceil_div(a.cols, 16)), bl, st, a);
-  if (a.cols <= 4096) return launch(rms_fold_kernel<DT, 8>, dim3((unsigned)ceil_div(a.cols, 32)), bl, st, a);
-  return launch(rms_fold_kernel<DT, 16>, dim3((unsigned)ceil_div(a.cols, 64)), bl, st, a);
-}
-
 }  // namespace
 
 extern "C" {
@@ -1613,38 +1601,6 @@ SMLM_API int smlm_lora_bwd_multi_ex(int n_proj, void* const* dx, void* const* co
                                  : launch_wgrad<SMLM_DTYPE_BF16, false>(nbj, split, grid, st, wa);
 }
 
-static int rms_bwd_threads(int cols) {
-  const int pieces = cols / 8;  // a piece a thread, or two where a row has more than 1024
-  return round_up(pieces <= 1024 ? pieces : ceil_div(pieces, 2), kWaveSize);
-}
-// workgroups of the RMSNorm kernels: the forward gives every row group its own workgroup; the backward's fill the
-// chip once (up to 512 threads a CU, the same number on every CU) with two rows each or more, so that the partial sums
-// of dw stay small next to x and g.  (4096 x 3072, 384 threads: 341 workgroups 21.9 us, 512 23.5, 256 19.2.)
-static int rms_blocks(int rows, int cols, bool backward) {
-  int nb, cap = 1 << 22;
-  if (cols > kRmsMaxCols) {  // wide rows: a workgroup per row; the backward's partial rows are whole rows of floats
-    nb = rows;
-    if (backward) cap = 128;
-  } else if (backward) {
-    const int threads = rms_bwd_threads(cols);
-    nb = ceil_div(rows, 2);
-    cap = 256 * (threads >= 512 ? 1 : 512 / threads);
-  } else {
-    nb = ceil_div(rows, cols <= kRmsWaveCols ? 4 : 1);
-  }
-  if (nb > cap) nb = cap;
-  return nb < 1 ? 1 : nb;
-}
-static int rms_bwd_blocks(int rows, int cols) { return rms_blocks(rows, cols, true); }
-
-static int rms_check(int rows, int cols, int dtype) {
-  if (rows < 0 || cols <= 0) return SMLM_ERR_ARG;
-  if (dtype != SMLM_DTYPE_F16 && dtype != SMLM_DTYPE_BF16) return SMLM_ERR_DTYPE;
-  if (cols & 7) return SMLM_ERR_ALIGN;
-  if (cols > (1 << 24) || rows > (1 << 30)) return SMLM_ERR_LIMIT;
-  return SMLM_OK;
-}
-
 SMLM_API int smlm_rms_norm_fwd(void* out, float* rms, const void* x, const void* w, int rows,
                                int cols, float eps, int dtype, void* stream) {
   int rc = rms_check(rows, cols, dtype);
@@ -1702,17 +1658,8 @@ SMLM_API int smlm_rms_norm_bwd(void* dx, void* dw, const void* g, const void* x,
   const bool f16 = dtype == SMLM_DTYPE_F16;
   const RmsBwdArgs a{reinterpret_cast<uint16_t*>(dx), reinterpret_cast<float*>(workspace),
                      reinterpret_cast<const uint16_t*>(g), reinterpret_cast<const uint16_t*>(x),
-                     reinterpret_cast<const uint16_t*>(w), rms, rows, cols};
-  const dim3 grid((unsigned)nb);
-  if (cols > kRmsMaxCols)
-    rc = f16 ? launch(rms_bwd_wide_kernel<SMLM_DTYPE_F16>, grid, dim3(256), st, a)
-             : launch(rms_bwd_wide_kernel<SMLM_DTYPE_BF16>, grid, dim3(256), st, a);
-  else if (cols <= 8192)
-    rc = f16 ? launch(rms_bwd_kernel<SMLM_DTYPE_F16, 1, 2>, grid, dim3(rms_bwd_threads(cols)), st, a)
-             : launch(rms_bwd_kernel<SMLM_DTYPE_BF16, 1, 2>, grid, dim3(rms_bwd_threads(cols)), st, a);
-  else
-    rc = f16 ? launch(rms_bwd_kernel<SMLM_DTYPE_F16, 2, 1>, grid, dim3(rms_bwd_threads(cols)), st, a)
-             : launch(rms_bwd_kernel<SMLM_DTYPE_BF16, 2, 1>, grid, dim3(rms_bwd_threads(cols)), st, a);
+                     reinterpret_cast<const uint16_t*>(w), rms, rows, cols, nullptr};
+  rc = f16 ? launch_rms_bwd<SMLM_DTYPE_F16, false>(nb, st, a) : launch_rms_bwd<SMLM_DTYPE_BF16, false>(nb, st, a);
   if (rc) return rc;
   const RmsFoldArgs fa{reinterpret_cast<uint16_t*>(dw), reinterpret_cast<const float*>(workspace), nb, cols};
   return f16 ? launch_rms_fold<SMLM_DTYPE_F16>(st, fa) : launch_rms_fold<SMLM_DTYPE_BF16>(st, fa);

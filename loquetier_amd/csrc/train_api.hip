@@ -1,6 +1,8 @@
-// C ABI of the operators around a fine-tuning step (see include/smlm.h): the loss over the vocabulary, the update of many
-// tensors.  Argument checks, workspace carving, launch shapes.  No allocation, no host synchronisation, no state.
+// C ABI of the operators around a fine-tuning step (see include/smlm.h): the residual's addition with its norm, the loss over the
+// vocabulary, the update of many tensors.  Argument checks, workspace carving, launch shapes.  No allocation, no host synchronisation, no state.
+#include "adamw.hpp"
 #include "api_common.hpp"
+#include "rms_launch.hpp"
 #include "vocab_loss.hpp"
 
 using namespace smlm;
@@ -44,143 +46,320 @@ struct LossSpace {
   uint16_t* g;
   int pad, parts, piece;
 };
-// what: 0 the forward, 1 the backward with dx, 2 with dw, 3 with both.
-size_t loss_carve(void* base, int T, int H, int V, int what, LossSpace* out) {
+struct LossTaker {
+  char* base;
   size_t off = 0;
-  auto take = [&](size_t bytes) {
+  template <typename P>
+  void take(P*& p, size_t bytes) {
     const size_t o = off;
     off = align_up(off + bytes, 256);
-    return base ? reinterpret_cast<char*>(base) + o : nullptr;
-  };
-  LossSpace s{};
-  const size_t t = (size_t)T;
-  s.rows.count = reinterpret_cast<int32_t*>(take(256));
-  s.rows.unit = reinterpret_cast<float*>(base ? s.rows.count + 16 : nullptr);
-  s.rows.row = reinterpret_cast<int32_t*>(take(4 * t));
-  s.rows.label = reinterpret_cast<int32_t*>(take(4 * t));
-  s.rows.x = reinterpret_cast<uint16_t*>(take(2 * t * H));
-  s.pad = round_up(T, 64);
-  s.parts = ceil_div(V, kLossTileV) * (loss_few(T) ? 4 : 2);
-  s.piece = loss_piece(T, V);
-  if (what == 0) {
-    s.part = reinterpret_cast<float*>(take(8 * (size_t)s.parts * s.pad));
-    s.at_label = reinterpret_cast<float*>(take(4 * (size_t)s.pad));
-  } else {
-    s.rows.number = reinterpret_cast<int32_t*>(take(4 * t));
-    s.rows.coef = reinterpret_cast<float*>(take(4 * t));
-    s.rows.lse2 = reinterpret_cast<float*>(take(4 * t));
-    s.g = reinterpret_cast<uint16_t*>(take(2 * t * s.piece));
-    if (what & 1) s.dx = reinterpret_cast<float*>(take(4 * (size_t)loss_dx_floats(T, H)));
+    p = base ? reinterpret_cast<P*>(base + o) : nullptr;
   }
-  if (out) *out = s;
-  return off;
+};
+// What the forward keeps for the gradient of x: its sums, and what the fold needs.
+size_t loss_keep(void* base, int T, int H, LossSpace* s) {
+  LossTaker k{reinterpret_cast<char*>(base)};
+  const size_t t = (size_t)T;
+  k.take(s->rows.count, 256);
+  k.take(s->rows.number, 4 * t);
+  k.take(s->rows.label, 4 * t);
+  k.take(s->rows.sum, 4 * t);
+  k.take(s->rows.share, 4 * t);
+  k.take(s->dx, 4 * (size_t)loss_dx_floats(T, H));
+  return k.off;
+}
+// what: 0 the forward, 1 the backward with dx, 2 with dw, 3 with both, 4 the forward that keeps.
+size_t loss_carve(void* base, int T, int H, int V, int what, LossSpace* s) {
+  LossTaker k{reinterpret_cast<char*>(base)};
+  const size_t t = (size_t)T;
+  if (what != 4) {
+    k.take(s->rows.count, 256);
+    s->rows.unit = reinterpret_cast<float*>(base ? s->rows.count + 16 : nullptr);
+    k.take(s->rows.label, 4 * t);
+    k.take(s->rows.sum, 4 * t);
+    k.take(s->rows.share, 4 * t);
+  }
+  k.take(s->rows.row, 4 * t);
+  k.take(s->rows.x, 2 * t * H);
+  s->pad = round_up(T, 64);
+  s->piece = what == 0 ? round_up(V, kLossTileV) : loss_piece(T, V);
+  s->parts = s->piece / kLossTileV * (loss_few(T) ? 4 : 2);
+  if (what == 0 || what == 4) {
+    k.take(s->part, 8 * (size_t)s->parts * s->pad);
+    k.take(s->at_label, 4 * (size_t)s->pad);
+    k.take(s->rows.ref, 4 * t);
+    k.take(s->rows.turn, 4 * t);
+  } else {
+    k.take(s->rows.number, 4 * t);
+    k.take(s->rows.coef, 4 * t);
+    k.take(s->rows.lse2, 4 * t);
+    k.take(s->rows.own, 4 * t);
+    k.take(s->rows.lost, 4 * t);
+  }
+  if (what) k.take(s->g, 2 * t * s->piece);
+  if (what == 1 || what == 3) k.take(s->dx, 4 * (size_t)loss_dx_floats(T, H));
+  return k.off;
 }
 
 dim3 loss_grid(int64_t units) { return dim3((unsigned)((units + 7) / 8 * 8)); }
 
-template <int DT>
-int loss_logits(bool few, bool grad, dim3 grid, hipStream_t st, const LossTileArgs& a) {
+template <int MODE>
+int loss_logits(bool f16, bool few, dim3 grid, hipStream_t st, const LossTileArgs& a) {
   const dim3 bl(256);
   if (few)
-    return grad ? launch(loss_logits_kernel<DT, true, true>, grid, bl, st, a)
-                : launch(loss_logits_kernel<DT, true, false>, grid, bl, st, a);
-  return grad ? launch(loss_logits_kernel<DT, false, true>, grid, bl, st, a)
-              : launch(loss_logits_kernel<DT, false, false>, grid, bl, st, a);
+    return f16 ? launch(loss_logits_kernel<SMLM_DTYPE_F16, true, MODE>, grid, bl, st, a)
+               : launch(loss_logits_kernel<SMLM_DTYPE_BF16, true, MODE>, grid, bl, st, a);
+  return f16 ? launch(loss_logits_kernel<SMLM_DTYPE_F16, false, MODE>, grid, bl, st, a)
+             : launch(loss_logits_kernel<SMLM_DTYPE_BF16, false, MODE>, grid, bl, st, a);
 }
+int loss_dx(bool f16, bool few, hipStream_t st, const LossTileArgs& a) {
+  const int tile = few ? kLossFewRows : kLossRows, h_tiles = ceil_div(a.H, 256);
+  int most = 0;  // units, whatever the number of labelled rows
+  for (int r = 1; r <= ceil_div(a.T, tile); ++r) {
+    const int u = r * h_tiles * loss_splits(r, h_tiles, a.most_splits);
+    if (u > most) most = u;
+  }
+  const dim3 grid = loss_grid(most), bl(256);
+  if (few)
+    return f16 ? launch(loss_dx_kernel<SMLM_DTYPE_F16, true>, grid, bl, st, a) : launch(loss_dx_kernel<SMLM_DTYPE_BF16, true>, grid, bl, st, a);
+  return f16 ? launch(loss_dx_kernel<SMLM_DTYPE_F16, false>, grid, bl, st, a) : launch(loss_dx_kernel<SMLM_DTYPE_BF16, false>, grid, bl, st, a);
+}
+#define LOSS_TRY(call) \
+  if (int rc = (call)) return rc
 
 }  // namespace
 
 SMLM_API int smlm_vocab_loss_workspace_size(int T, int H, int V, int what, size_t* bytes) {
-  if (!bytes || what < 0 || what > 3) return SMLM_ERR_ARG;
+  if (!bytes || what < 0 || what > 5) return SMLM_ERR_ARG;
   if (int rc = loss_check(T, H, V, SMLM_DTYPE_F16)) return rc;
-  *bytes = loss_carve(nullptr, T, H, V, what, nullptr);
+  LossSpace s{};
+  *bytes = what == 5 ? loss_keep(nullptr, T, H, &s) : loss_carve(nullptr, T, H, V, what, &s);
   return SMLM_OK;
 }
 
-SMLM_API int smlm_vocab_loss_fwd(float* loss, float* lse, float* means, float* weight, const void* x, const void* w,
-                                 const int64_t* labels, const int32_t* partition, int P, void* workspace, size_t workspace_bytes,
-                                 int T, int H, int V, int dtype, void* stream) {
+SMLM_API int smlm_vocab_loss_fwd(float* loss, float* lse, float* means, float* weight, void* kept, size_t kept_bytes, const void* x,
+                                 const void* w, const int64_t* labels, const int32_t* partition, int P, void* workspace,
+                                 size_t workspace_bytes, int T, int H, int V, int dtype, void* stream) {
   if (int rc = loss_check(T, H, V, dtype)) return rc;
   if (P < 0 || (partition && P > 0 && (!means || !weight))) return SMLM_ERR_ARG;
   if (!partition) P = 0;
   if (T == 0 && P == 0) return SMLM_OK;
   if (T > 0 && (!loss || !lse || !x || !w || !labels || !workspace)) return SMLM_ERR_ARG;
-  if (!aligned16(x) || !aligned16(w) || !aligned16(workspace)) return SMLM_ERR_ALIGN;
+  if (!aligned16(x) || !aligned16(w) || !aligned16(workspace) || !aligned16(kept)) return SMLM_ERR_ALIGN;
   hipStream_t st = (hipStream_t)stream;
   if (T > 0) {
-    LossSpace s;
-    if (workspace_bytes < loss_carve(workspace, T, H, V, 0, &s)) return SMLM_ERR_WORKSPACE;
-    const LossScanArgs sa{s.rows, labels, loss, lse, nullptr, P ? partition : nullptr, nullptr, T, V, P, 0};
-    if (int rc = launch(loss_scan_kernel<false>, dim3(1), dim3(kLossScanThreads), st, sa)) return rc;
+    LossSpace s{};
+    if (kept && kept_bytes < loss_keep(kept, T, H, &s)) return SMLM_ERR_WORKSPACE;
+    if (workspace_bytes < loss_carve(workspace, T, H, V, kept ? 4 : 0, &s)) return SMLM_ERR_WORKSPACE;
+    const LossScanArgs sa{s.rows, labels, loss, lse, nullptr, P ? partition : nullptr, nullptr, T, V, P, 0, kept != nullptr};
+    LOSS_TRY(launch(loss_scan_kernel<false>, dim3(1), dim3(kLossScanThreads), st, sa));
     const LossGatherArgs ga{s.rows, reinterpret_cast<const uint16_t*>(x), T, H};
-    if (int rc = launch(loss_gather_kernel, dim3((unsigned)ceil_div(T, 4)), dim3(256), st, ga)) return rc;
+    LOSS_TRY(launch(loss_gather_kernel, dim3((unsigned)ceil_div(T, 4)), dim3(256), st, ga));
     LossTileArgs a{};
     a.rows = s.rows, a.x = ga.x, a.w = reinterpret_cast<const uint16_t*>(w), a.part = s.part, a.at_label = s.at_label;
-    a.T = T, a.H = H, a.V = V, a.pad = s.pad, a.v0 = 0, a.v1 = V;
-    const bool few = loss_few(T);
-    const dim3 grid = loss_grid((int64_t)ceil_div(T, few ? kLossFewRows : kLossRows) * ceil_div(V, kLossTileV));
-    int rc = dtype == SMLM_DTYPE_F16 ? loss_logits<SMLM_DTYPE_F16>(few, false, grid, st, a)
-                                     : loss_logits<SMLM_DTYPE_BF16>(few, false, grid, st, a);
-    if (rc) return rc;
-    const LossFoldArgs fa{s.rows, s.part, s.at_label, loss, lse, s.parts, s.pad};
-    rc = launch(loss_fold_kernel, dim3((unsigned)ceil_div(T, 16)), dim3(256), st, fa);
-    if (rc) return rc;
+    a.g = s.g, a.dx = s.dx, a.T = T, a.H = H, a.V = V, a.pad = s.pad, a.ldg = s.piece, a.most_splits = kLossMostSplits, a.turned = 1;
+    const bool few = loss_few(T), f16 = dtype == SMLM_DTYPE_F16;
+    for (int v0 = 0; v0 < V; v0 += s.piece) {
+      a.v0 = v0, a.v1 = V - v0 < s.piece ? V : v0 + s.piece, a.add = v0 > 0;
+      const int v_tiles = ceil_div(a.v1 - v0, kLossTileV), parts = v_tiles * (few ? 4 : 2);
+      const dim3 grid = loss_grid((int64_t)ceil_div(T, few ? kLossFewRows : kLossRows) * v_tiles);
+      LOSS_TRY(kept ? loss_logits<kLossSoft>(f16, few, grid, st, a) : loss_logits<kLossSums>(f16, few, grid, st, a));
+      const LossRefsArgs ra{s.rows, s.part, s.at_label, loss, lse, parts, s.pad, v0 == 0, a.v1 == V,
+                            kept && f16 ? kLossBias<SMLM_DTYPE_F16> : 0.0f};
+      const dim3 rows16((unsigned)ceil_div(T, 16));
+      LOSS_TRY(launch(loss_refs_kernel, rows16, dim3(256), st, ra));
+      if (!kept) continue;
+      const LossTurnArgs ta{s.rows, s.part, s.g, parts, s.pad, s.piece, few ? 64 : 128};
+      const dim3 gt(rows16.x, (unsigned)(ceil_div(parts, 8) < 16 ? ceil_div(parts, 8) : 16));
+      LOSS_TRY(f16 ? launch(loss_turn_kernel<SMLM_DTYPE_F16>, gt, dim3(256), st, ta)
+                   : launch(loss_turn_kernel<SMLM_DTYPE_BF16>, gt, dim3(256), st, ta));
+      LOSS_TRY(loss_dx(f16, few, st, a));
+    }
   }
   if (P == 0) return SMLM_OK;
   const LossMeansArgs ma{loss, labels, partition, means, weight, T, V};
   return launch(loss_means_kernel, dim3((unsigned)P), dim3(1024), st, ma);
 }
 
-SMLM_API int smlm_vocab_loss_bwd(void* dx, void* dw, const float* grad, const float* lse, const void* x, const void* w,
+SMLM_API int smlm_vocab_loss_bwd_kept(void* dx, const float* grad, const void* kept, size_t kept_bytes, const void* w,
+                                      const int32_t* partition, const float* weight, int P, int T, int H, int V, int dtype, void* stream) {
+  if (int rc = loss_check(T, H, V, dtype)) return rc;
+  if (P < 0 || (partition && P > 0 && !weight)) return SMLM_ERR_ARG;
+  if (T == 0) return SMLM_OK;
+  if (!dx || !grad || !kept || !w) return SMLM_ERR_ARG;
+  if (!aligned16(dx) || !aligned16(kept) || !aligned16(w)) return SMLM_ERR_ALIGN;
+  LossSpace s{};
+  if (kept_bytes < loss_keep(const_cast<void*>(kept), T, H, &s)) return SMLM_ERR_WORKSPACE;
+  const LossDxFoldArgs fa{s.rows, s.dx, reinterpret_cast<uint16_t*>(dx), reinterpret_cast<const uint16_t*>(w), T, H, loss_few(T),
+                          kLossMostSplits, grad, partition, weight, P};
+  const dim3 grid((unsigned)ceil_div(T, 4)), bl(256);
+  hipStream_t st = (hipStream_t)stream;
+  return dtype == SMLM_DTYPE_F16 ? launch(loss_dx_fold_kernel<SMLM_DTYPE_F16, true>, grid, bl, st, fa)
+                                 : launch(loss_dx_fold_kernel<SMLM_DTYPE_BF16, true>, grid, bl, st, fa);
+}
+
+SMLM_API int smlm_vocab_loss_bwd(void* dx, void* dw, const float* grad, const float* loss, const float* lse, const void* x, const void* w,
                                  const int64_t* labels, const int32_t* partition, const float* weight, int P, void* workspace,
                                  size_t workspace_bytes, int T, int H, int V, int dtype, void* stream) {
   if (int rc = loss_check(T, H, V, dtype)) return rc;
   if (P < 0 || (partition && P > 0 && !weight) || (!dx && !dw)) return SMLM_ERR_ARG;
   if (T == 0) return dw ? SMLM_ERR_ARG : SMLM_OK;  // (dw would have nothing to sum)
-  if (!grad || !lse || !x || !w || !labels || !workspace) return SMLM_ERR_ARG;
+  if (!grad || !loss || !lse || !x || !w || !labels || !workspace) return SMLM_ERR_ARG;
   if (!aligned16(x) || !aligned16(w) || !aligned16(workspace) || !aligned16(dx) || !aligned16(dw)) return SMLM_ERR_ALIGN;
-  LossSpace s;
+  LossSpace s{};
   if (workspace_bytes < loss_carve(workspace, T, H, V, (dx ? 1 : 0) | (dw ? 2 : 0), &s)) return SMLM_ERR_WORKSPACE;
   hipStream_t st = (hipStream_t)stream;
   const bool f16 = dtype == SMLM_DTYPE_F16, few = loss_few(T);
-  const LossScanArgs sa{s.rows, labels, nullptr, const_cast<float*>(lse), grad, partition, weight, T, V, P, f16};
-  if (int rc = launch(loss_scan_kernel<true>, dim3(1), dim3(kLossScanThreads), st, sa)) return rc;
+  const LossScanArgs sa{s.rows, labels, const_cast<float*>(loss), const_cast<float*>(lse), grad, partition, weight, T, V, P, f16, 1};
+  LOSS_TRY(launch(loss_scan_kernel<true>, dim3(1), dim3(kLossScanThreads), st, sa));
   const LossGatherArgs ga{s.rows, reinterpret_cast<const uint16_t*>(x), T, H};
-  if (int rc = launch(loss_gather_kernel, dim3((unsigned)ceil_div(T, 4)), dim3(256), st, ga)) return rc;
+  LOSS_TRY(launch(loss_gather_kernel, dim3((unsigned)ceil_div(T, 4)), dim3(256), st, ga));
   LossTileArgs a{};
   a.rows = s.rows, a.x = ga.x, a.w = reinterpret_cast<const uint16_t*>(w), a.g = s.g, a.dx = s.dx;
   a.dw = reinterpret_cast<uint16_t*>(dw), a.T = T, a.H = H, a.V = V, a.ldg = s.piece, a.most_splits = kLossMostSplits;
   const int tile = few ? kLossFewRows : kLossRows, h_tiles = ceil_div(H, 256);
-  int most_units = 0;  // of dx, whatever the number of labelled rows
-  for (int r = 1; r <= ceil_div(T, tile); ++r) {
-    const int u = r * h_tiles * loss_splits(r, h_tiles, kLossMostSplits);
-    if (u > most_units) most_units = u;
-  }
+  const dim3 bl(256);
   for (int v0 = 0; v0 < V; v0 += s.piece) {
     a.v0 = v0, a.v1 = V - v0 < s.piece ? V : v0 + s.piece, a.add = v0 > 0;
     const int v_tiles = ceil_div(a.v1 - v0, kLossTileV);
-    const dim3 bl(256), grid = loss_grid((int64_t)ceil_div(T, tile) * v_tiles);
-    int rc = f16 ? loss_logits<SMLM_DTYPE_F16>(few, true, grid, st, a) : loss_logits<SMLM_DTYPE_BF16>(few, true, grid, st, a);
-    if (rc) return rc;
-    if (dx) {
-      const dim3 gx = loss_grid(most_units);
-      if (few)
-        rc = f16 ? launch(loss_dx_kernel<SMLM_DTYPE_F16, true>, gx, bl, st, a)
-                 : launch(loss_dx_kernel<SMLM_DTYPE_BF16, true>, gx, bl, st, a);
-      else
-        rc = f16 ? launch(loss_dx_kernel<SMLM_DTYPE_F16, false>, gx, bl, st, a)
-                 : launch(loss_dx_kernel<SMLM_DTYPE_BF16, false>, gx, bl, st, a);
-      if (rc) return rc;
-    }
+    LOSS_TRY(loss_logits<kLossGrad>(f16, few, loss_grid((int64_t)ceil_div(T, tile) * v_tiles), st, a));
+    if (dx) LOSS_TRY(loss_dx(f16, few, st, a));
     if (dw) {
       const dim3 gw = loss_grid((int64_t)h_tiles * v_tiles);
-      rc = f16 ? launch(loss_dw_kernel<SMLM_DTYPE_F16>, gw, bl, st, a) : launch(loss_dw_kernel<SMLM_DTYPE_BF16>, gw, bl, st, a);
-      if (rc) return rc;
+      LOSS_TRY(f16 ? launch(loss_dw_kernel<SMLM_DTYPE_F16>, gw, bl, st, a) : launch(loss_dw_kernel<SMLM_DTYPE_BF16>, gw, bl, st, a));
     }
   }
   if (!dx) return SMLM_OK;
-  const LossDxFoldArgs fa{s.rows, s.dx, reinterpret_cast<uint16_t*>(dx), T, H, few, kLossMostSplits};
+  const LossDxFoldArgs fa{s.rows, s.dx, reinterpret_cast<uint16_t*>(dx), a.w, T, H, few, kLossMostSplits, nullptr, nullptr, nullptr, 0};
   const dim3 grid((unsigned)ceil_div(T, 4));
-  return f16 ? launch(loss_dx_fold_kernel<SMLM_DTYPE_F16>, grid, dim3(256), st, fa)
-             : launch(loss_dx_fold_kernel<SMLM_DTYPE_BF16>, grid, dim3(256), st, fa);
+  return f16 ? launch(loss_dx_fold_kernel<SMLM_DTYPE_F16, false>, grid, bl, st, fa)
+             : launch(loss_dx_fold_kernel<SMLM_DTYPE_BF16, false>, grid, bl, st, fa);
+}
+
+// ---- the residual's addition and its norm ----
+
+namespace {
+
+template <int DT>
+int launch_add_rms(hipStream_t st, const AddRmsArgs& a) {
+  const dim3 bl(256);
+  if (a.cols > kRmsMaxCols) return launch(add_rms_wide_kernel<DT>, dim3((unsigned)a.rows), bl, st, a);
+  if (a.cols > kRmsWaveCols) {
+    const dim3 grid((unsigned)a.rows);
+    return a.cols <= 8192 ? launch(add_rms_kernel<DT, 4, 4>, grid, bl, st, a) : launch(add_rms_kernel<DT, 4, 8>, grid, bl, st, a);
+  }
+  if (a.rows <= 1024 && a.cols > 1024) return launch(add_rms_kernel<DT, 4, 2>, dim3((unsigned)a.rows), bl, st, a);
+  const dim3 grid((unsigned)ceil_div(a.rows, 4));
+  if (a.cols <= 512) return launch(add_rms_kernel<DT, 1, 1>, grid, bl, st, a);
+  if (a.cols <= 1024) return launch(add_rms_kernel<DT, 1, 2>, grid, bl, st, a);
+  return a.cols <= 2048 ? launch(add_rms_kernel<DT, 1, 4>, grid, bl, st, a) : launch(add_rms_kernel<DT, 1, 8>, grid, bl, st, a);
+}
+
+}  // namespace
+
+SMLM_API int smlm_add_rms_norm_fwd(void* out, float* rms, void* h, const void* x, const void* residual, const void* w, void* out8,
+                                   float* scale, int group, int rows, int cols, float eps, int dtype, void* stream) {
+  if (int rc = rms_check(rows, cols, dtype)) return rc;
+  if (group != 0 && group != 128) return SMLM_ERR_ARG;
+  if (group && (cols & 127)) return SMLM_ERR_ALIGN;
+  if (rows == 0) return SMLM_OK;
+  if ((!out && !out8 && !h) || (h && !residual) || (!out8) != (!scale)) return SMLM_ERR_ARG;
+  if (!x || !w) return SMLM_ERR_ARG;
+  if (!aligned16(out) || !aligned16(h) || !aligned16(x) || !aligned16(residual) || !aligned16(w) || !aligned16(out8))
+    return SMLM_ERR_ALIGN;
+  const AddRmsArgs a{reinterpret_cast<uint16_t*>(out), rms, reinterpret_cast<uint16_t*>(h), reinterpret_cast<const uint16_t*>(x),
+                     reinterpret_cast<const uint16_t*>(residual), reinterpret_cast<const uint16_t*>(w),
+                     reinterpret_cast<uint8_t*>(out8), scale, rows, cols, group == 128, eps};
+  hipStream_t st = (hipStream_t)stream;
+  return dtype == SMLM_DTYPE_F16 ? launch_add_rms<SMLM_DTYPE_F16>(st, a) : launch_add_rms<SMLM_DTYPE_BF16>(st, a);
+}
+
+SMLM_API int smlm_add_rms_norm_bwd(void* dh, void* dw, const void* g, const void* gh, const void* h, const void* w, const float* rms,
+                                   void* workspace, size_t workspace_bytes, int rows, int cols, int dtype, void* stream) {
+  if (int rc = rms_check(rows, cols, dtype)) return rc;
+  if (!dh || !dw || !g || !h || !w || !rms || !workspace) return SMLM_ERR_ARG;
+  if (!aligned16(dh) || !aligned16(dw) || !aligned16(g) || !aligned16(gh) || !aligned16(h) || !aligned16(w) || !aligned16(workspace))
+    return SMLM_ERR_ALIGN;
+  if (rows == 0) return SMLM_ERR_ARG;  // (dw would have nothing to sum)
+  const int nb = rms_bwd_blocks(rows, cols);
+  if (workspace_bytes < (size_t)nb * cols * 4) return SMLM_ERR_WORKSPACE;
+  hipStream_t st = (hipStream_t)stream;
+  const bool f16 = dtype == SMLM_DTYPE_F16;
+  const RmsBwdArgs a{reinterpret_cast<uint16_t*>(dh), reinterpret_cast<float*>(workspace), reinterpret_cast<const uint16_t*>(g),
+                     reinterpret_cast<const uint16_t*>(h), reinterpret_cast<const uint16_t*>(w), rms, rows, cols,
+                     reinterpret_cast<const uint16_t*>(gh)};
+  const int rc = gh ? f16 ? launch_rms_bwd<SMLM_DTYPE_F16, true>(nb, st, a) : launch_rms_bwd<SMLM_DTYPE_BF16, true>(nb, st, a)
+                    : f16 ? launch_rms_bwd<SMLM_DTYPE_F16, false>(nb, st, a) : launch_rms_bwd<SMLM_DTYPE_BF16, false>(nb, st, a);
+  if (rc) return rc;
+  const RmsFoldArgs fa{reinterpret_cast<uint16_t*>(dw), reinterpret_cast<const float*>(workspace), nb, cols};
+  return f16 ? launch_rms_fold<SMLM_DTYPE_F16>(st, fa) : launch_rms_fold<SMLM_DTYPE_BF16>(st, fa);
+}
+
+// ---- the update of many tensors ----
+
+SMLM_API int smlm_adamw_workspace_size(int n_tensors, size_t* bytes) {
+  if (!bytes || n_tensors < 0) return SMLM_ERR_ARG;
+  *bytes = align_up((size_t)(n_tensors > 0 ? n_tensors : 1) * sizeof(AdamTensor), 256);
+  return SMLM_OK;
+}
+
+namespace {
+
+template <int PT>
+int launch_adam(bool eight, bool master, dim3 grid, hipStream_t st, const AdamArgs& a) {
+  const dim3 bl(256);
+  if (eight)
+    return master ? launch(adam_kernel<PT, true, true>, grid, bl, st, a) : launch(adam_kernel<PT, true, false>, grid, bl, st, a);
+  return master ? launch(adam_kernel<PT, false, true>, grid, bl, st, a) : launch(adam_kernel<PT, false, false>, grid, bl, st, a);
+}
+
+template <int N>
+int adam_begin(const smlm_adamw* p, AdamTensor* table, int at, int n, int64_t first, int align, hipStream_t st) {
+  AdamBeginArgs<N> a;
+  a.table = table, a.step = p->step, a.hyper = p->hyper, a.group = p->group, a.at = at, a.n = n, a.n_groups = p->n_groups, a.pad = 0;
+  a.first = first;
+  for (int i = 0; i < n; ++i) {
+    const uint64_t w = (uint64_t)(uintptr_t)p->params[at + i], g = (uint64_t)(uintptr_t)p->grads[at + i];
+    a.entry[i] = AdamEntry{w, g, p->sizes[at + i] | (((w | g) & (uint64_t)(align - 1)) ? INT64_MIN : 0)};
+  }
+  return launch(adam_begin_kernel<N>, dim3(1), dim3(256), st, a);
+}
+
+}  // namespace
+
+SMLM_API int smlm_adamw_step(const smlm_adamw* p, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!p || p->n_tensors < 0 || p->n_groups < 0 || (p->state_bits != 8 && p->state_bits != 32)) return SMLM_ERR_ARG;
+  const bool f32 = p->dtype == kAdamF32, eight = p->state_bits == 8;
+  if (!f32)
+    if (int rc = check_dtype(p->dtype)) return rc;
+  if (f32 && p->master) return SMLM_ERR_ARG;
+  if (p->n_tensors == 0) return SMLM_OK;
+  if (!p->params || !p->grads || !p->sizes || !p->step || !p->hyper || !p->group || !workspace) return SMLM_ERR_ARG;
+  int64_t blocks = 0;
+  for (int i = 0; i < p->n_tensors; ++i) {
+    if (p->sizes[i] < 0 || p->sizes[i] > ((int64_t)1 << 40)) return SMLM_ERR_LIMIT;
+    if (p->sizes[i] > 0 && !p->params[i]) return SMLM_ERR_ARG;
+    blocks += (p->sizes[i] + kAdamBlock - 1) / kAdamBlock;
+  }
+  if (blocks > ((int64_t)1 << 32) - 64) return SMLM_ERR_LIMIT;
+  if (blocks > 0 && (!p->exp_avg || !p->exp_avg_sq || (eight && (!p->avg_scale || !p->sq_scale)))) return SMLM_ERR_ARG;
+  if (!aligned16(p->exp_avg) || !aligned16(p->exp_avg_sq) || !aligned16(p->master) || !aligned16(workspace)) return SMLM_ERR_ALIGN;
+  if (workspace_bytes < (size_t)p->n_tensors * sizeof(AdamTensor)) return SMLM_ERR_WORKSPACE;
+  hipStream_t st = (hipStream_t)stream;
+  AdamTensor* table = reinterpret_cast<AdamTensor*>(workspace);
+  int64_t first = 0;
+  const int align = f32 ? 16 : 8;  // (bytes of a lane's four elements)
+  for (int at = 0; at < p->n_tensors;) {
+    const int n = p->n_tensors - at < kAdamEntries ? p->n_tensors - at : kAdamEntries;
+    const int rc = n <= 16 ? adam_begin<16>(p, table, at, n, first, align, st) : adam_begin<kAdamEntries>(p, table, at, n, first, align, st);
+    if (rc) return rc;
+    for (int i = 0; i < n; ++i) first += (p->sizes[at + i] + kAdamBlock - 1) / kAdamBlock;
+    at += n;
+  }
+  if (blocks == 0) return SMLM_OK;
+  const AdamArgs a{table, p->exp_avg, p->exp_avg_sq, p->avg_scale, p->sq_scale, p->master, p->n_tensors, blocks};
+  const dim3 grid((unsigned)((blocks + 4 * kAdamRun - 1) / (4 * kAdamRun)));
+  if (f32) return launch_adam<kAdamF32>(eight, false, grid, st, a);
+  return p->dtype == SMLM_DTYPE_F16 ? launch_adam<SMLM_DTYPE_F16>(eight, p->master != nullptr, grid, st, a)
+                                    : launch_adam<SMLM_DTYPE_BF16>(eight, p->master != nullptr, grid, st, a);
 }

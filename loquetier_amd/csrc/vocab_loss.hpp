@@ -5,15 +5,30 @@
 //   G[t, v] = c[t] (exp(z[t, v] - lse[t]) - [v == label[t]]),  dx = G w,  dw = G^T x
 //
 // Rows without a label cost nothing but their zeros: the labelled ones are numbered on the device, copied side by side where they
-// are not already, and everything below runs over these n rows.  The forward multiplies tile by tile and keeps of each tile its
-// rows' maximum and sum; the backward makes the logits again, a piece of the vocabulary at a time, turns them into G in 16 bits,
-// and multiplies that with w and x.  All three are gemm_tile's products, bound by the matrix cores from some hundred rows on and by
-// the reading of w below.
+// are not already, and everything below runs over these n rows.  All products are gemm_tile's, bound by the matrix cores from some
+// hundred rows on and by the reading of w below.
 //
-// G's rounding: half a step of 16 bits an entry, as any product of 16-bit operands has it.  In fp16 G is held 2^15 times as large,
-// relative to the largest |c|: probabilities of a large vocabulary lie below fp16's normal numbers.
+// The loss alone: tile by tile, of each row and 128 (64) entries of the vocabulary the sum of exponentials against a whole power of two.
+//
+// The loss and the gradient of x (the usual fine-tuning step: the vocabulary's matrix is frozen) take two products, no third that makes the
+// logits again: dx is linear in c, so what it needs is sum_v exp(z - ref) w[v] and sum_v exp(z - ref), and ref need not be the maximum.
+// A piece of the vocabulary at a time the exponentials are stored in 16 bits, each row's against its reference of the pieces
+// before, and multiplied with w.  Where the piece outgrows the reference (or there is none yet) a part is stored against its own,
+// and turned to the row's new one before the product, as the sums so far are: references are whole powers of two, so turning rounds
+// nothing.  The backward divides and multiplies with c.
+//
+// With the gradient of w the backward makes the logits again, by piece, turns them into G in 16 bits, and multiplies that with w and x.
+//
+// The label has no part in the sums and the 16-bit entries: with `others` = sum_{v != label} exp(z - ref) and e = exp(z[label] - ref), the
+// loss is log(1 + others / e) and dx = c (sum_{v != label} exp(z - ref) w[v] - others w[label]) / (others + e), the label's share in
+// float: where a label is nearly certain nothing cancels, and the gradient is as exact, relative to its size, as anywhere.
+//
+// Rounding to 16 bits: half a step of each entry, as any product of 16-bit operands has it (of G at the label too, where dw is
+// wanted: what dx loses by it is given back in float).  fp16 entries are held 2^15 times as large (G relative to the largest |c|):
+// probabilities of a large vocabulary lie below fp16's normal numbers.
 #pragma once
 #include "gemm_tile.hpp"
+#include "rms_norm.hpp"
 #include "wave_scan.hpp"
 
 namespace smlm {
@@ -32,19 +47,25 @@ struct LossRows {
   int32_t* number;   // [T] of a row of the batch, -1: none (backward)
   float* coef;       // [T] c, in fp16 relative to `unit` (backward)
   float* lse2;       // [T] lse in powers of two (backward)
+  float* own;        // [T] exp(-loss) - 1 (backward)
+  float* lost;       // [T] what rounding took from G at the label (backward)
   float* unit;       // [1] what gradients are multiplied with in the end (backward)
+  float* ref;        // [T] the power of two that a row's exponentials are taken against
+  float* sum;        // [T] of them without the label's; in the end one over their sum with it
+  float* share;      // [T] in the end: the part of them that is not the label's
+  float* turn;       // [T] what the sums so far are multiplied with
   uint16_t* x;       // [n, H] the rows side by side, unless n == T
 };
 
 struct LossScanArgs {
   LossRows to;
   const int64_t* labels;  // [T]
-  float* loss;            // [T], zeros where there is no label (forward)
-  float* lse;             // [T] (forward: written; backward: read)
+  float* loss;            // [T] (forward: zeros where there is no label; backward: read)
+  float* lse;             // [T] (the same)
   const float* grad;      // [T], or [P] (backward)
   const int32_t* partition;  // [P + 1] or NULL
   const float* weight;       // [P] (backward)
-  int T, V, P, f16;
+  int T, V, P, f16, number;  // number: rows' numbers are wanted
 };
 
 // Index of the partition that row t lies in, -1: none.
@@ -105,12 +126,12 @@ __global__ __launch_bounds__(kLossScanThreads) void loss_scan_kernel(LossScanArg
       const int t = t0 + e;
       if (t >= a.T) break;
       const bool ok = label[e] >= 0;
-      if (BWD) a.to.number[t] = ok ? at : -1;
+      if (a.number) a.to.number[t] = ok ? at : -1;
       if (!BWD && !ok) a.loss[t] = 0.0f, a.lse[t] = 0.0f;
       if (!ok) continue;
       a.to.row[at] = t;
       a.to.label[at] = (int32_t)label[e];
-      if (BWD) a.to.coef[at] = c[e], a.to.lse2[at] = a.lse[t] * kLog2e;
+      if (BWD) a.to.coef[at] = c[e], a.to.lse2[at] = a.lse[t] * kLog2e, a.to.own[at] = expm1f(-a.loss[t]);
       ++at;
     }
     __syncthreads();
@@ -148,14 +169,15 @@ struct LossTileArgs {
   LossRows rows;
   const uint16_t* x;  // [T, H]
   const uint16_t* w;  // [V, H]
-  float* part;        // [parts][pad][2] a row's maximum and sum of a part of the vocabulary (forward)
+  float* part;        // [parts][pad][2] a row's reference and sum of a part of the vocabulary (forward)
   float* at_label;    // [pad] (forward)
-  uint16_t* g;        // [n, ldg] (backward)
-  float* dx;          // [splits][n, H] (backward)
+  uint16_t* g;        // [n, ldg] G, or the exponentials
+  float* dx;          // [splits][n, H]
   uint16_t* dw;       // [V, H] (backward)
   int T, H, V, pad;
   int v0, v1, ldg;    // the piece of the vocabulary
-  int most_splits, add;
+  int most_splits, add;  // add: to what is there of dx, turned (`turned`)
+  int turned;
 };
 
 __device__ __forceinline__ const uint16_t* loss_x(const LossTileArgs& a, int n) { return n == a.T ? a.x : a.rows.x; }
@@ -218,8 +240,19 @@ __device__ __forceinline__ void loss_lds_free() {
   __syncthreads();
 }
 
-// The logits' tiles.  FEW: one tile of kLossFewRows rows holds all of them.  GRAD: they become G, otherwise their rows' statistics.
-template <int DT, bool FEW, bool GRAD>
+constexpr int kLossSums = 0, kLossSoft = 1, kLossGrad = 2;  // what becomes of the logits: sums alone, exponentials too, G
+
+// References are above a row's maximum by less than one, or by the room that is left for later pieces: bf16 has exponents enough for
+// any (60 above), fp16 gets 2^4 at the price of entries below 2^-28 of the maximum losing bits.
+template <int DT>
+constexpr float kLossRoom = DT == SMLM_DTYPE_F16 ? 4.0f : 0.0f;
+template <int DT>
+constexpr float kLossAbove = DT == SMLM_DTYPE_F16 ? 0.0f : 60.0f;
+template <int DT>
+constexpr float kLossBias = DT == SMLM_DTYPE_F16 ? 15.0f : 0.0f;  // fp16 entries are 2^15 times as large, and so are their sums
+
+// The logits' tiles.  FEW: one tile of kLossFewRows rows holds all of them.
+template <int DT, bool FEW, int MODE>
 __global__ __launch_bounds__(256, 1) void loss_logits_kernel(LossTileArgs a) {
   constexpr int WA = FEW ? 4 : 2, IA = FEW ? 2 : 4, WB = FEW ? 1 : 2, JB = FEW ? 2 : 4;
   typedef GemmShape<WA, IA, false, WB, JB, false> S;
@@ -235,70 +268,73 @@ __global__ __launch_bounds__(256, 1) void loss_logits_kernel(LossTileArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
   const int v = first_v + (wave / WB) * IA * 32, t = first_t + (wave % WB) * JB * 32 + (lane & 31);
   const bool ends = v + IA * 32 > a.v1;  // the vocabulary ends inside the wave's part
-  if (!GRAD) {
 #pragma unroll
-    for (int j = 0; j < JB; ++j) {
-      const int tj = t + j * 32;
-      if (ends) {
+  for (int j = 0; j < JB; ++j) {
+    const int tj = t + j * 32, tc = min(tj, n - 1);
+    if (ends) {
 #pragma unroll
-        for (int i = 0; i < IA; ++i)
+      for (int i = 0; i < IA; ++i)
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (v + i * 32 + 8 * (e >> 2) + 4 * h + (e & 3) >= a.v1) acc[i][j][e] = -INFINITY;
-      }
+        for (int e = 0; e < 16; ++e)
+          if (v + i * 32 + 8 * (e >> 2) + 4 * h + (e & 3) >= a.v1) acc[i][j][e] = -INFINITY;
+    }
+    const int at = a.rows.label[tc] - v - 4 * h;  // the label's place among the lane's logits
+    const bool near = __ballot(at >= 0 && at < IA * 32) != 0;
+    if (MODE != kLossGrad) {
       float m = -INFINITY, l = 0.0f;
-#pragma unroll
-      for (int i = 0; i < IA; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[i][j][e]);
-      m = fmaxf(m, __shfl_xor(m, 32, kWaveSize));
-      const float m2 = m == -INFINITY ? 0.0f : m * kLog2e;
-#pragma unroll
-      for (int i = 0; i < IA; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) l += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, -m2));
-      l += __shfl_xor(l, 32, kWaveSize);
-      const bool there = tj < n;
-      const int at = there ? a.rows.label[tj] - v : -1;
-      if (__ballot(at >= 0 && at < IA * 32)) {
+      if (near) {
         float z = 0.0f;
         bool here = false;
 #pragma unroll
         for (int i = 0; i < IA; ++i)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (at == i * 32 + 8 * (e >> 2) + 4 * h + (e & 3)) z = acc[i][j][e], here = true;
-        if (here) a.at_label[tj] = z;
+            if (at == i * 32 + 8 * (e >> 2) + (e & 3)) z = acc[i][j][e], acc[i][j][e] = -INFINITY, here = true;
+        if (here && tj < n) a.at_label[tj] = z;
       }
-      if (there && h == 0) {
-        typedef float f32x2_t __attribute__((ext_vector_type(2)));
-        *(SMLM_GLOBAL f32x2_t*)(a.part + ((int64_t)(u.other * WA + wave / WB) * a.pad + tj) * 2) = f32x2_t{m == -INFINITY ? m : m2, l};
-      }
-    }
-  } else {
 #pragma unroll
-    for (int j = 0; j < JB; ++j) {
-      const int tj = min(t + j * 32, n - 1);
-      const float c = a.rows.coef[tj], lse2 = a.rows.lse2[tj];
-      const int at = a.rows.label[tj] - v - 4 * h;
+      for (int i = 0; i < IA; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) m = fmaxf(m, acc[i][j][e]);
+      m = fmaxf(m, __shfl_xor(m, 32, kWaveSize)) * kLog2e;
+      float c = MODE == kLossSoft && a.add ? a.rows.ref[tc] : -INFINITY;
+      if (!(m <= c + kLossAbove<DT>)) c = ceilf(m) + (MODE == kLossSoft ? kLossRoom<DT> : 0.0f);
+      const float to = (c == -INFINITY ? 0.0f : c) - (MODE == kLossSoft ? kLossBias<DT> : 0.0f);
+#pragma unroll
+      for (int i = 0; i < IA; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, -to));
+          if (MODE == kLossSoft) acc[i][j][e] = x;
+          l += x;
+        }
+      l += __shfl_xor(l, 32, kWaveSize);
+      if (tj < n && h == 0) {
+        typedef float f32x2_t __attribute__((ext_vector_type(2)));
+        *(SMLM_GLOBAL f32x2_t*)(a.part + ((int64_t)(u.other * WA + wave / WB) * a.pad + tj) * 2) = f32x2_t{c, l};
+      }
+    } else {
+      const float c = a.rows.coef[tc], lse2 = a.rows.lse2[tc];
 #pragma unroll
       for (int i = 0; i < IA; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, -lse2)) * c;
-      if (__ballot(at >= -4 && at < IA * 32)) {
-#pragma unroll
-        for (int i = 0; i < IA; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) acc[i][j][e] -= at == i * 32 + 8 * (e >> 2) + (e & 3) ? c : 0.0f;
-      }
-      if (ends) {
+      if (near) {
+        float lost = 0.0f;
+        bool here = false;
 #pragma unroll
         for (int i = 0; i < IA; ++i)
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            if (v + i * 32 + 8 * (e >> 2) + 4 * h + (e & 3) >= a.v1) acc[i][j][e] = 0.0f;
+            if (at == i * 32 + 8 * (e >> 2) + (e & 3)) {
+              acc[i][j][e] = c * a.rows.own[tc];
+              lost = acc[i][j][e] - Num<DT>::lo(pack2<DT>(acc[i][j][e], 0.0f)), here = true;
+            }
+        if (here && tj < n) a.rows.lost[tj] = lost;
       }
     }
+  }
+  if (MODE != kLossSums) {
     loss_lds_free();
     const int row = first_t + (wave % WB) * JB * 32;
     loss_store<DT>(acc, lds + wave * IA * JB * 1024, a.g + (int64_t)row * a.ldg + (v - a.v0), a.ldg, n - row, IA * 32);
@@ -340,7 +376,8 @@ __global__ __launch_bounds__(256, 1) void loss_dx_kernel(LossTileArgs a) {
 #pragma unroll
         for (int e = 0; e < 16; e += 4)
           if (t + j * 32 < n && hh + i * 32 + 2 * e < a.H) {
-            const f32x4 v = ldg_f4(out + (int64_t)(t + j * 32) * a.H + hh + i * 32 + 2 * e);
+            f32x4 v = ldg_f4(out + (int64_t)(t + j * 32) * a.H + hh + i * 32 + 2 * e);
+            if (a.turned) v *= a.rows.turn[t + j * 32];
             acc[i][j][e] = v[0], acc[i][j][e + 1] = v[1], acc[i][j][e + 2] = v[2], acc[i][j][e + 3] = v[3];
           }
   }
@@ -382,16 +419,18 @@ __global__ __launch_bounds__(256, 1) void loss_dw_kernel(LossTileArgs a) {
   loss_store<DT>(acc, lds + wave * IA * JB * 1024, a.dw + (int64_t)v * a.H + hh, a.H, a.v1 - v, a.H - hh);
 }
 
-struct LossFoldArgs {
+struct LossRefsArgs {
   LossRows rows;
   const float* part;      // [parts][pad][2]
   const float* at_label;
   float* loss;
   float* lse;
-  int parts, pad;
+  int parts, pad, first, last;  // the piece's parts; whether it is the first, the last
+  float bias;                   // the sums are 2^bias as large
 };
-// Sixteen rows a workgroup, sixteen threads a row: a line of sixteen rows' parts a load.
-__global__ __launch_bounds__(256) void loss_fold_kernel(LossFoldArgs a) {
+// The rows' references and sums after a piece of the vocabulary; after the last, the losses.  Sixteen rows a workgroup, sixteen threads a
+// row: a line of sixteen rows' parts a load.
+__global__ __launch_bounds__(256) void loss_refs_kernel(LossRefsArgs a) {
   typedef float f32x2_t __attribute__((ext_vector_type(2)));
   __shared__ f32x2_t sums[16][16];
   const int n = uload(a.rows.count, 0), r = threadIdx.x & 15, q = threadIdx.x >> 4;
@@ -419,12 +458,59 @@ __global__ __launch_bounds__(256) void loss_fold_kernel(LossFoldArgs a) {
   __syncthreads();
   if (q || t >= n) return;
   for (int p = 1; p < 16; ++p) join(sums[p][r][0], sums[p][r][1]);
-  // (the label's logit meets the maximum in the product that made it: what m lost in rounding is in l, and a certain label's loss is
-  // 0 however large the logits are)
+  if (!a.first) {
+    const float was = a.rows.ref[t];
+    join(was, a.rows.sum[t]);
+    a.rows.turn[t] = m == was ? 1.0f : __builtin_amdgcn_exp2f(was - m);
+  }
+  a.rows.ref[t] = m, a.rows.sum[t] = l;
+  if (!a.last) return;
+  // e = 2^x, in the sums' units; on the side where neither overflows
+  const float z = a.at_label[t], x = (m == -INFINITY ? INFINITY : __builtin_fmaf(z, kLog2e, -m)) + a.bias;
+  float loss, over, share;
+  if (x >= 0.0f) {
+    const float e = __builtin_amdgcn_exp2f(-x), y = l * e;
+    loss = y < 0x1p-10f ? y * (1.0f - y * (0.5f - y * (1.0f / 3.0f))) : __builtin_amdgcn_logf(1.0f + y) * kLn2;
+    over = e / (1.0f + y), share = y / (1.0f + y);
+  } else {
+    const float all = l + __builtin_amdgcn_exp2f(x);
+    loss = (__builtin_amdgcn_logf(all) - x) * kLn2;
+    over = 1.0f / all, share = l / all;
+  }
   const int row = a.rows.row[t];
-  const float log_l = __builtin_amdgcn_logf(l);
-  a.lse[row] = (m + log_l) * kLn2;
-  a.loss[row] = (__builtin_fmaf(-a.at_label[t], kLog2e, m) + log_l) * kLn2;
+  a.loss[row] = loss, a.lse[row] = z + loss;
+  a.rows.sum[t] = over, a.rows.share[t] = share;
+}
+
+struct LossTurnArgs {
+  LossRows rows;
+  const float* part;  // [parts][pad][2]
+  uint16_t* g;        // [n, ldg]
+  int parts, pad, ldg, wide;  // wide: entries a part, 128 or 64
+};
+// Exponentials that were stored against another reference than their row's: turned to it, by whole powers of two.  Sixteen lanes a row and
+// a part of 128; blockIdx.y deals out the parts.
+template <int DT>
+__global__ __launch_bounds__(256) void loss_turn_kernel(LossTurnArgs a) {
+  const int n = uload(a.rows.count, 0), i = (int)blockIdx.x * 16 + (threadIdx.x >> 4), l = threadIdx.x & 15;
+  if (i >= n) return;
+  const float ref = a.rows.ref[i];
+  uint16_t* row = a.g + (int64_t)i * a.ldg;
+  const int lanes = a.wide >> 3, each = 16 / lanes;  // (64 entries: two parts at a time)
+#pragma unroll 4
+  for (int p0 = (int)blockIdx.y * each; p0 < a.parts; p0 += (int)gridDim.y * each) {
+    const int p = p0 + l / lanes;
+    if (p >= a.parts) break;
+    const float c = a.part[((int64_t)p * a.pad + i) * 2];
+    if (c == ref || c == -INFINITY) continue;
+    const float by = __builtin_amdgcn_exp2f(c - ref);
+    uint16_t* at = row + p * a.wide + (l % lanes) * 8;
+    const u32x4 v = ldg16(at);
+    u32x4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = pack2<DT>(Num<DT>::lo(v[e]) * by, Num<DT>::hi(v[e]) * by);
+    stg16(at, o);
+  }
 }
 
 struct LossMeansArgs {
@@ -460,31 +546,58 @@ struct LossDxFoldArgs {
   LossRows rows;
   const float* part;  // [splits][n, H]
   uint16_t* dx;       // [T, H]
+  const uint16_t* w;  // [V, H]
   int T, H, few, most_splits;
+  // of exponentials (KEPT): the rows' coefficients are found here
+  const float* grad;         // [T], or [P]
+  const int32_t* partition;  // [P + 1] or NULL
+  const float* weight;       // [P]
+  int P;
 };
-// A wave a row of the batch: its parts summed in order, rounded once; zeros without a label.
-template <int DT>
+// A wave a row of the batch: its parts summed in order, and what the label adds; zeros without one.
+template <int DT, bool KEPT>
 __global__ __launch_bounds__(256) void loss_dx_fold_kernel(LossDxFoldArgs a) {
   const int n = uload(a.rows.count, 0), lane = threadIdx.x & 63, tile = a.few ? kLossFewRows : kLossRows;
   const int splits = loss_splits((n + tile - 1) / tile, (a.H + 255) / 256, a.most_splits);
-  const float unit = uload(a.rows.unit, 0);
   const int t = (int)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= a.T) return;
   const int i = a.rows.number[t];
   uint16_t* to = a.dx + (int64_t)t * a.H;
+  float by = 0.0f, label = 0.0f;  // of the sums, of w[label]
+  bool none = i < 0;
+  if (KEPT && i >= 0) {
+    float c;
+    if (a.partition) {
+      const int p = loss_partition(a.partition, a.P, t);
+      c = p < 0 ? 0.0f : a.grad[p] * a.weight[p];
+    } else {
+      c = a.grad[t];
+    }
+    by = c * a.rows.sum[i], label = -c * a.rows.share[i];
+    none = c == 0.0f;  // (nothing hangs on this row)
+  } else if (i >= 0) {
+    by = a.rows.unit[0], label = a.rows.lost[i] * by;
+  }
+  if (none) {
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    for (int c = lane * 8; c < a.H; c += 512) stg16(to + c, zero);
+    return;
+  }
+  const uint16_t* w = a.w + (int64_t)a.rows.label[i] * a.H;
   for (int c = lane * 8; c < a.H; c += 512) {
     f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
-    if (i >= 0)
-      for (int s = 0; s < splits; ++s) {
-        const float* p = a.part + ((int64_t)s * n + i) * a.H + c;
-        lo += ldg_f4(p);
-        hi += ldg_f4(p + 4);
-      }
+    float f[8];
+    unpack8<DT>(ldg16(w + c), f);
+    for (int s = 0; s < splits; ++s) {
+      const float* p = a.part + ((int64_t)s * n + i) * a.H + c;
+      lo += ldg_f4(p);
+      hi += ldg_f4(p + 4);
+    }
     u32x4 o;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      o[e] = pack2<DT>(lo[2 * e] * unit, lo[2 * e + 1] * unit);
-      o[2 + e] = pack2<DT>(hi[2 * e] * unit, hi[2 * e + 1] * unit);
+      o[e] = pack2<DT>(lo[2 * e] * by + f[2 * e] * label, lo[2 * e + 1] * by + f[2 * e + 1] * label);
+      o[2 + e] = pack2<DT>(hi[2 * e] * by + f[4 + 2 * e] * label, hi[2 * e + 1] * by + f[5 + 2 * e] * label);
     }
     stg16(to + c, o);
   }

@@ -349,14 +349,61 @@ class qk_norm_rope(Function):
         return *_qk_norm_rope_gradients.apply(gq, gk, *ctx.saved_tensors, ctx.eps), None, None, None
 
 
+class _add_rms_norm_gradients(Function):
+    """The backward of `add_rms_norm`, as a function of its own so that a graph made of it (create_graph) knows what the gradients
+    hang on: to differentiate them is refused, as there is no kernel for it."""
+
+    @staticmethod
+    def forward(ctx: FunctionCtx, g, gh, h, w, rms):
+        dh, dw = torch.empty_like(h), torch.empty_like(w)
+        kernel.add_rms_norm_backward(dh, dw, g.contiguous(), None if gh is None else gh.contiguous(), h, w, rms)
+        return dh, dw
+
+    @staticmethod
+    def backward(ctx: FunctionCtx, *grads):
+        raise RuntimeError("the gradients of add_rms_norm cannot be differentiated")
+
+
+class add_rms_norm(Function):
+    """`add_rms_norm.apply(x, residual, w, eps)`: (norm, sum), the sum x + residual [rows, cols] and its RMSNorm with the weight
+    [cols], in one launch (see ops/_kernels.add_rms_norm): what a decoder layer does before each of its norms, where the
+    reference adds in a tensor expression (src/loquetier_src/models/mixed_llama.py:53-66).  The backward adds the gradient of the sum in its own
+    launch.  Its gradients cannot be differentiated again."""
+
+    @classmethod
+    def apply(cls, *args, **kwargs):
+        if cls is add_rms_norm and not kwargs and not torch._C._are_functorch_transforms_active():
+            out = kernel._host().add_rms_norm(*args)  # (plain calls; None: nothing was done)
+            if out is not None:
+                return out
+        return super().apply(*args, **kwargs)
+
+    @staticmethod
+    def forward(ctx: FunctionCtx, x: torch.Tensor, residual: torch.Tensor, w: torch.Tensor, eps: float = 1e-6):
+        rms = torch.empty((x.size(0), 1), dtype=torch.float32, device=x.device)
+        out, h = torch.empty_like(x), torch.empty_like(x)
+        kernel.add_rms_norm(out, rms, h, x, residual, w, eps)
+        ctx.save_for_backward(h, w, rms)
+        ctx.set_materialize_grads(False)
+        return out, h
+
+    @staticmethod
+    def backward(ctx: FunctionCtx, g: Optional[torch.Tensor], gh: Optional[torch.Tensor]):
+        if g is None:  # (nothing hangs on the norm)
+            return gh, gh, None, None
+        h, w, rms = ctx.saved_tensors
+        dh, dw = _add_rms_norm_gradients.apply(g, gh, h, w, rms)
+        return dh, dh, dw, None
+
+
 class _linear_cross_entropy_gradients(Function):
     """The backward of `linear_cross_entropy`, as a function of its own so that a graph made of it (create_graph) knows what the
     gradients hang on: to differentiate them is refused, as there is no kernel for it."""
 
     @staticmethod
-    def forward(ctx: FunctionCtx, grad, x, w, labels, lse, partition, weight, want_x: bool, want_w: bool):
+    def forward(ctx: FunctionCtx, grad, x, w, labels, loss, lse, partition, weight, kept, want_x: bool, want_w: bool):
         dx, dw = torch.empty_like(x) if want_x else None, torch.empty_like(w) if want_w else None
-        kernel.linear_cross_entropy_backward(dx, dw, grad.contiguous(), lse, x, w, labels, partition, weight)
+        kernel.linear_cross_entropy_backward(dx, dw, grad.contiguous(), loss, lse, x, w, labels, partition, weight, kept=kept)
         return dx, dw
 
     @staticmethod
@@ -369,7 +416,17 @@ class linear_cross_entropy(Function):
     float32, without the logits in memory (see ops/_kernels.linear_cross_entropy): row by row [rows], or with a partition of the
     rows, as the flat batch's training sequences are one, the mean over each partition's labelled rows [P] (the reference takes
     such a loss a train partition: src/loquetier_src/models/mixed_llama.py:382-415).  x and w contiguous, of one 16-bit type.
-    Kept for the backward: the inputs and a float a row.  Its gradients cannot be differentiated again."""
+    Where x's gradient alone is wanted (a frozen vocabulary) the forward makes it but for the losses' own gradients, in the same sweep
+    over the vocabulary, and keeps it in float; with w's the backward makes the logits again.  Its gradients cannot be
+    differentiated again."""
+
+    @classmethod
+    def apply(cls, *args, **kwargs):
+        if cls is linear_cross_entropy and not kwargs and not torch._C._are_functorch_transforms_active():
+            out = kernel._host().linear_cross_entropy(*args)  # (plain calls; None: nothing was done)
+            if out is not None:
+                return out
+        return super().apply(*args, **kwargs)
 
     @staticmethod
     def forward(ctx: FunctionCtx, x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
@@ -379,15 +436,19 @@ class linear_cross_entropy(Function):
         means = weight = None
         if partition is not None:
             means, weight = (torch.empty(max(partition.numel() - 1, 0), **floats) for _ in range(2))
-        kernel.linear_cross_entropy(loss, lse, x, w, labels, partition, means, weight)
-        ctx.save_for_backward(x, w, labels, lse, partition, weight)
+        kept = None
+        if ctx.needs_input_grad[0] and not ctx.needs_input_grad[1]:
+            size = kernel.linear_cross_entropy_kept_size(x.size(0), x.size(1), w.size(0))
+            kept = torch.empty(size, dtype=torch.uint8, device=x.device)
+        kernel.linear_cross_entropy(loss, lse, x, w, labels, partition, means, weight, kept=kept)
+        ctx.save_for_backward(x, w, labels, loss, lse, partition, weight, kept)
         return loss if partition is None else means
 
     @staticmethod
     def backward(ctx: FunctionCtx, grad: torch.Tensor):
         if not (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]):
             return None, None, None, None
-        x, w, labels, lse, partition, weight = ctx.saved_tensors
-        dx, dw = _linear_cross_entropy_gradients.apply(grad, x, w, labels, lse, partition, weight, ctx.needs_input_grad[0],
+        x, w, labels, loss, lse, partition, weight, kept = ctx.saved_tensors
+        dx, dw = _linear_cross_entropy_gradients.apply(grad, x, w, labels, loss, lse, partition, weight, kept, ctx.needs_input_grad[0],
                                                        ctx.needs_input_grad[1])
         return dx, dw, None, None

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import struct
-from typing import Dict, Optional, Tuple
+from typing import Dict, Optional, Sequence, Tuple
 
 import torch
 
@@ -235,6 +235,16 @@ def put_ints(device: torch.device, words64, words32) -> Tuple[torch.Tensor, torc
             rc = _lib.load().smlm_put_words(buf.data_ptr(), data, len(data), _stream(dev))
         _lib.check(rc, "put_ints")
     return buf[:n64], buf[n64:].view(torch.int32)[:n32]
+
+
+def put_words(dst: torch.Tensor, data: bytes) -> None:
+    """The bytes (a multiple of 4, as many as dst holds) into a contiguous tensor on the device, without waiting for it."""
+    _check_input(dst, "dst")
+    if len(data) != dst.numel() * dst.element_size() or len(data) % 4:
+        raise RuntimeError("dst must hold the words, whole ones")
+    with _on(dst.device):
+        rc = _lib.load().smlm_put_words(dst.data_ptr(), data, len(data), _stream(dst.device))
+    _lib.check(rc, "put_words")
 
 
 class SegmentPlan:
@@ -1307,7 +1317,155 @@ def paged_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v
     _lib.check(rc, "paged_attention")
 
 
-# ---- around a fine-tuning step: the loss over the vocabulary ------------------------------------------------------------
+# ---- around a fine-tuning step: the residual's addition with its norm, the loss over the vocabulary, the update --------------
+
+def add_rms_norm(output: Optional[torch.Tensor], rms_output: Optional[torch.Tensor], residual_output: Optional[torch.Tensor],
+                 input: torch.Tensor, residual: Optional[torch.Tensor], weight: torch.Tensor, epsilon: float,
+                 output8: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None) -> None:
+    """residual_output = input + residual, and of it the norm: output = residual_output * rms * weight, rms_output = 1 /
+    sqrt(mean(residual_output^2) + epsilon) per row (see include/smlm.h).  input, residual and outputs [rows, cols] fp16 or bf16,
+    weight [cols], rms_output float32 [rows, 1]; what is not wanted is None.  Outputs may be the inputs.
+
+    output8 (float8_e4m3fn [rows, cols]) is the norm in 8 bits, its values those of the norm divided by scale: float32 [rows, 1],
+    a row's largest over 448, or [rows, cols / 128], that of 128 columns each.  residual None: the norm of input."""
+    if _host().add_rms(output, rms_output, residual_output, input, residual, weight, epsilon, output8, scale):
+        return
+    for t, n in ((input, "input"), (weight, "weight")):
+        _check_input(t, n)
+    _check_dim(2, input, "input")
+    _check_dim(1, weight, "weight")
+    rows, cols = input.shape
+    dev = input.device
+    if input.dtype not in _DTYPE_CODE or cols % 8 != 0 or cols == 0:
+        raise RuntimeError(f"No suitable kernel. dtype={input.dtype} columns={cols}")
+    if weight.size(0) != cols:
+        raise RuntimeError("weight must have one entry per column of input")
+    _check_ints(dev, input.dtype, 1, weight=weight)
+    _check_ints(dev, input.dtype, 2, output=output, residual_output=residual_output, residual=residual)
+    for t, n in ((output, "output"), (residual_output, "residual_output"), (residual, "residual")):
+        if t is not None and t.shape != input.shape:
+            raise RuntimeError(f"{n} and input must have the same shape")
+    if residual is None and residual_output is not None:
+        raise RuntimeError("residual_output is the sum with a residual")
+    if output is None and output8 is None and residual_output is None:
+        raise RuntimeError("an output is needed")
+    _check_ints(dev, torch.float32, 2, rms_output=rms_output, scale=scale)
+    if rms_output is not None and tuple(rms_output.shape) != (rows, 1):
+        raise RuntimeError("rms_output must be [rows, 1]")
+    group = 0
+    if (output8 is None) != (scale is None):
+        raise RuntimeError("output8 and scale come together")
+    if output8 is not None:
+        _check_ints(dev, torch.float8_e4m3fn, 2, output8=output8)
+        if output8.shape != input.shape:
+            raise RuntimeError("output8 and input must have the same shape")
+        if scale.size(0) != rows or scale.size(1) not in (1, -(-cols // 128)) or (scale.size(1) != 1 and cols % 128):
+            raise RuntimeError("scale must be [rows, 1] or [rows, cols / 128]")
+        group = 0 if scale.size(1) == 1 else 128
+    with _on(dev):
+        rc = _lib.load().smlm_add_rms_norm_fwd(_ptr(output), _ptr(rms_output), _ptr(residual_output), _ptr(input), _ptr(residual),
+                                               _ptr(weight), _ptr(output8), _ptr(scale), group, rows, cols, float(epsilon),
+                                               _DTYPE_CODE[input.dtype], _stream(dev))
+    _lib.check(rc, "add_rms_norm")
+
+
+def add_rms_norm_backward(dh: torch.Tensor, dw: torch.Tensor, grad_output: torch.Tensor, grad_residual: Optional[torch.Tensor],
+                          h: torch.Tensor, w: torch.Tensor, rms: torch.Tensor, workspace: Optional[Workspace] = None) -> None:
+    """dh [rows, cols], the gradient of both of add_rms_norm's summands, and dw [cols], from the gradients of its outputs
+    (grad_residual: that of residual_output, None for none) and its saved sum h and rms.  dh may be either gradient."""
+    dev = h.device
+    for t, n in ((h, "h"), (w, "w")):
+        _check_input(t, n)
+    code = _dtype_code(h)
+    _check_ints(dev, h.dtype, 2, h=h, dh=dh, grad_output=grad_output, grad_residual=grad_residual)
+    _check_ints(dev, h.dtype, 1, w=w, dw=dw)
+    rows, cols = h.shape
+    for t, n in ((dh, "dh"), (grad_output, "grad_output"), (grad_residual, "grad_residual")):
+        if t is not None and t.shape != h.shape:
+            raise RuntimeError(f"{n} must match h")
+    if w.size(0) != cols or dw.size(0) != cols:
+        raise RuntimeError("w and dw must have one entry per column of h")
+    if rms.dtype != torch.float32 or rms.numel() != rows or rms.device != dev or not rms.is_contiguous():
+        raise RuntimeError("rms must be float32 with one entry per row")
+    if cols % 8 != 0 or cols == 0:
+        raise RuntimeError(f"No suitable kernel. dtype={h.dtype} columns={cols}")
+    if rows == 0:
+        dw.zero_()
+        return
+    with _on(dev):
+        ws = _workspace(dev, _lib.size_query("smlm_rms_norm_bwd_workspace_size", rows, cols), workspace)
+        rc = _lib.load().smlm_add_rms_norm_bwd(_ptr(dh), _ptr(dw), _ptr(grad_output), _ptr(grad_residual), _ptr(h), _ptr(w), _ptr(rms),
+                                               ws.data_ptr(), ws.numel(), rows, cols, code, _stream(dev))
+    _lib.check(rc, "add_rms_norm_backward")
+
+
+ADAMW_BLOCK = 256  # weights that share a scale of 8-bit states; tensors' states begin at multiples of it
+
+
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Tensor]], exp_avg: torch.Tensor,
+               exp_avg_sq: torch.Tensor, step: torch.Tensor, hyper: torch.Tensor, group: torch.Tensor,
+               avg_scale: Optional[torch.Tensor] = None, sq_scale: Optional[torch.Tensor] = None,
+               master: Optional[torch.Tensor] = None, workspace: Optional[Workspace] = None) -> None:
+    """One AdamW step of all params (contiguous, of one type: fp16, bf16 or float32) in place (see include/smlm.h for the
+    formulas).  grads: of the same type; None: that tensor stays as it is.  Nothing waits for the GPU, and nothing is kept.
+
+    exp_avg, exp_avg_sq: flat states, tensor after tensor, each filled up to a multiple of ADAMW_BLOCK with zeros: float32, or
+    float8_e4m3fn with avg_scale and sq_scale (float32, one for ADAMW_BLOCK weights), exp_avg_sq then the second average's root.
+    step int32 [tensors], counted on; group int32 [tensors]: rows of hyper float32 [groups, 5] (lr, beta1, beta2, eps, weight decay).
+    master: float32 weights, flat as the states, of which 16-bit params are the rounding (a weight that is not takes its
+    master's place)."""
+    if _host().adamw_step(params, grads, exp_avg, exp_avg_sq, step, hyper, group, avg_scale, sq_scale, master, workspace):
+        return
+    n = len(params)
+    if len(grads) != n:
+        raise RuntimeError("grads must have one entry per tensor")
+    _check_input(exp_avg, "exp_avg")
+    dev = exp_avg.device
+    eight = exp_avg.dtype == torch.float8_e4m3fn
+    _check_ints(dev, torch.float8_e4m3fn if eight else torch.float32, 1, exp_avg=exp_avg, exp_avg_sq=exp_avg_sq)
+    _check_ints(dev, torch.int32, 1, step=step, group=group)
+    _check_ints(dev, torch.float32, 2, hyper=hyper)
+    _check_ints(dev, torch.float32, 1, avg_scale=avg_scale, sq_scale=sq_scale, master=master)
+    if step.size(0) != n or group.size(0) != n or hyper.size(1) != 5:
+        raise RuntimeError("step and group must have one entry per tensor, hyper five columns")
+    if n == 0:
+        return
+    dt = params[0].dtype
+    code = _lib.SMLM_DTYPE_F32 if dt == torch.float32 else _DTYPE_CODE.get(dt)
+    if code is None or (dt == torch.float32 and master is not None):
+        raise RuntimeError(f"No suitable kernel. dtype={dt}" + (" with float weights beside it" if master is not None else ""))
+    where, at, sizes, blocks = (C.c_void_p * n)(), (C.c_void_p * n)(), (C.c_int64 * n)(), 0
+    for i, (p, g) in enumerate(zip(params, grads)):
+        if p.dtype != dt or p.device != dev or not p.is_contiguous():
+            raise RuntimeError(f"params must be contiguous, of one dtype and on {dev}")
+        if g is not None:
+            if g.dtype != dt or g.device != dev or g.shape != p.shape or not g.is_contiguous():
+                raise RuntimeError("a gradient must match its tensor, contiguous as it is")
+            at[i] = g.data_ptr()
+        size = p.numel()
+        where[i], sizes[i] = p.data_ptr(), size
+        blocks += (size + ADAMW_BLOCK - 1) // ADAMW_BLOCK
+    full = [p for p, size in zip(where, sizes) if size]
+    if len(set(full)) != len(full):
+        raise RuntimeError("a tensor is named twice")
+    for t, name in ((exp_avg, "exp_avg"), (exp_avg_sq, "exp_avg_sq"), (master, "master")):
+        if t is not None and t.size(0) != blocks * ADAMW_BLOCK:
+            raise RuntimeError(f"{name} must have {blocks * ADAMW_BLOCK} entries")
+    if eight != (avg_scale is not None) or eight != (sq_scale is not None):
+        raise RuntimeError("states in 8 bits come with scales, others without")
+    if eight and (avg_scale.size(0) != blocks or sq_scale.size(0) != blocks):
+        raise RuntimeError(f"avg_scale and sq_scale must have {blocks} entries")
+    a = _lib.AdamW(params=C.addressof(where), grads=C.addressof(at), sizes=C.addressof(sizes), step=step.data_ptr(),
+                   group=group.data_ptr(), hyper=_ptr(hyper), exp_avg=_ptr(exp_avg), exp_avg_sq=_ptr(exp_avg_sq),
+                   avg_scale=_ptr(avg_scale), sq_scale=_ptr(sq_scale), master=_ptr(master), n_tensors=n, n_groups=hyper.size(0),
+                   state_bits=8 if eight else 32, dtype=code)
+    with _on(dev):
+        ws = _workspace(dev, _lib.size_query("smlm_adamw_workspace_size", n), workspace)
+        rc = _lib.load().smlm_adamw_step(C.byref(a), ws.data_ptr(), ws.numel(), _stream(dev))
+    _lib.check(rc, "adamw_step")
+    # (autograd then knows that saved weights are no longer what they were)
+    torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None])
+
 
 def _loss_shapes(x, w, labels, partition):
     for t, n in ((x, "x"), (w, "w")):
@@ -1330,37 +1488,56 @@ def _loss_shapes(x, w, labels, partition):
     return dev, T, H, V, 0 if partition is None else partition.size(0) - 1
 
 
+def linear_cross_entropy_kept_size(rows: int, columns: int, vocabulary: int) -> int:
+    """Bytes of linear_cross_entropy's `kept`."""
+    return _lib.size_query("smlm_vocab_loss_workspace_size", int(rows), int(columns), int(vocabulary), 5)
+
+
+def _check_kept(kept, dev, T, H, V) -> None:
+    _check_ints(dev, torch.uint8, 1, kept=kept)
+    if kept is not None and kept.numel() < linear_cross_entropy_kept_size(T, H, V):
+        raise RuntimeError(f"kept must have {linear_cross_entropy_kept_size(T, H, V)} bytes")
+
+
 def linear_cross_entropy(loss: torch.Tensor, lse: torch.Tensor, x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
                          partition: Optional[torch.Tensor] = None, means: Optional[torch.Tensor] = None,
-                         weight: Optional[torch.Tensor] = None, workspace: Optional[Workspace] = None) -> None:
+                         weight: Optional[torch.Tensor] = None, workspace: Optional[Workspace] = None,
+                         kept: Optional[torch.Tensor] = None) -> None:
     """loss[t] = logsumexp(x[t] w^T) - x[t] . w[labels[t]] and the logsumexp itself, both float32 [rows], for rows x [rows, columns]
     and a vocabulary's matrix w [vocabulary, columns] (fp16 or bf16), without the logits in memory.  labels: int64 [rows]; one
     outside [0, vocabulary) is none, and its row's loss is 0.
 
     partition (int32 [P + 1]: rows partition[p] to partition[p + 1], not decreasing): means [P] becomes the mean loss of each partition's
-    labelled rows (0 where there are none) and weight [P] one over their number; rows outside every partition have no label."""
+    labelled rows (0 where there are none) and weight [P] one over their number; rows outside every partition have no label.
+
+    kept (uint8 [linear_cross_entropy_kept_size(...)]): filled with what linear_cross_entropy_backward makes dx of, at a product more
+    here and none there."""
     dev, T, H, V, P = _loss_shapes(x, w, labels, partition)
     code = _dtype_code(x)
+    _check_kept(kept, dev, T, H, V)
     _check_ints(dev, torch.float32, 1, loss=loss, lse=lse, means=means, weight=weight)
     if loss.size(0) != T or lse.size(0) != T:
         raise RuntimeError("loss and lse must have one entry per row")
     if P and (means is None or weight is None or means.size(0) != P or weight.size(0) != P):
         raise RuntimeError("means and weight must have one entry per partition")
     with _on(dev):
-        ws = _workspace(dev, _lib.size_query("smlm_vocab_loss_workspace_size", T, H, V, 0), workspace)
-        rc = _lib.load().smlm_vocab_loss_fwd(_ptr(loss), _ptr(lse), _ptr(means), _ptr(weight), _ptr(x), _ptr(w), _ptr(labels),
+        ws = _workspace(dev, _lib.size_query("smlm_vocab_loss_workspace_size", T, H, V, 0 if kept is None else 4), workspace)
+        rc = _lib.load().smlm_vocab_loss_fwd(_ptr(loss), _ptr(lse), _ptr(means), _ptr(weight), _ptr(kept),
+                                             0 if kept is None else kept.numel(), _ptr(x), _ptr(w), _ptr(labels),
                                              _ptr(partition) if P else None, P, ws.data_ptr(), ws.numel(), T, H, V, code, _stream(dev))
     _lib.check(rc, "linear_cross_entropy")
 
 
-def linear_cross_entropy_backward(dx: Optional[torch.Tensor], dw: Optional[torch.Tensor], grad: torch.Tensor, lse: torch.Tensor,
-                                  x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
+def linear_cross_entropy_backward(dx: Optional[torch.Tensor], dw: Optional[torch.Tensor], grad: torch.Tensor, loss: torch.Tensor,
+                                  lse: torch.Tensor, x: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
                                   partition: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
-                                  workspace: Optional[Workspace] = None) -> None:
+                                  workspace: Optional[Workspace] = None, kept: Optional[torch.Tensor] = None) -> None:
     """Gradients of linear_cross_entropy's losses (grad float32 [rows]) or, with partition, of its means (grad float32 [P]) by x and w;
-    either may be None.  lse, weight: the forward's.  Rows without a label, or with a gradient of 0, get zeros and cost nothing."""
+    either may be None.  loss, lse, weight: the forward's.  Rows without a label, or with a gradient of 0, get zeros.
+    kept: the forward's; dx alone then takes no product (with dw it is not read)."""
     dev, T, H, V, P = _loss_shapes(x, w, labels, partition)
     code = _dtype_code(x)
+    _check_kept(kept, dev, T, H, V)
     for d, like, n in ((dx, x, "dx"), (dw, w, "dw")):
         if d is not None:
             _check_ints(dev, x.dtype, 2, **{n: d})
@@ -1368,9 +1545,9 @@ def linear_cross_entropy_backward(dx: Optional[torch.Tensor], dw: Optional[torch
                 raise RuntimeError(f"{n} must match {n[1:]}")
     if dx is None and dw is None:
         raise RuntimeError("dx or dw is needed")
-    _check_ints(dev, torch.float32, 1, grad=grad, lse=lse, weight=weight)
-    if lse.size(0) != T or grad.size(0) != (T if partition is None else P):
-        raise RuntimeError("lse must have one entry per row, grad one for each loss")
+    _check_ints(dev, torch.float32, 1, grad=grad, loss=loss, lse=lse, weight=weight)
+    if loss.size(0) != T or lse.size(0) != T or grad.size(0) != (T if partition is None else P):
+        raise RuntimeError("loss and lse must have one entry per row, grad one for each loss")
     if partition is not None and (weight is None or weight.size(0) != P):
         raise RuntimeError("weight must have one entry per partition")
     if T == 0 or (partition is not None and P == 0):
@@ -1379,8 +1556,12 @@ def linear_cross_entropy_backward(dx: Optional[torch.Tensor], dw: Optional[torch
                 d.zero_()
         return
     with _on(dev):
+        if kept is not None and dw is None:
+            rc = _lib.load().smlm_vocab_loss_bwd_kept(_ptr(dx), _ptr(grad), kept.data_ptr(), kept.numel(), _ptr(w), _ptr(partition),
+                                                      _ptr(weight), P, T, H, V, code, _stream(dev))
+            return _lib.check(rc, "linear_cross_entropy_backward")
         what = (dx is not None) + 2 * (dw is not None)
         ws = _workspace(dev, _lib.size_query("smlm_vocab_loss_workspace_size", T, H, V, what), workspace)
-        rc = _lib.load().smlm_vocab_loss_bwd(_ptr(dx), _ptr(dw), _ptr(grad), _ptr(lse), _ptr(x), _ptr(w), _ptr(labels), _ptr(partition),
-                                             _ptr(weight), P, ws.data_ptr(), ws.numel(), T, H, V, code, _stream(dev))
+        rc = _lib.load().smlm_vocab_loss_bwd(_ptr(dx), _ptr(dw), _ptr(grad), _ptr(loss), _ptr(lse), _ptr(x), _ptr(w), _ptr(labels),
+                                             _ptr(partition), _ptr(weight), P, ws.data_ptr(), ws.numel(), T, H, V, code, _stream(dev))
     _lib.check(rc, "linear_cross_entropy_backward")

@@ -1,0 +1,161 @@
+"""AdamW over the weights of all adapters at once: one launch, and one for the call's tables by 144 tensors, where torch's
+optimizers run a chain of launches an adapter (the reference keeps a trainer, and so an optimizer, an adapter:
+src/loquetier_src/trainer_utils.py)."""
+from __future__ import annotations
+
+import struct
+from typing import Any, Callable, Dict, List, Optional, Tuple
+
+import torch
+
+from .ops import _kernels as kernel
+
+
+class _Set:
+    """The tensors of one type on one device: their flat states."""
+
+    def __init__(self, params: List[torch.Tensor], groups: List[int], bits: int, master: bool):
+        dev, dtype = params[0].device, params[0].dtype
+        self.params = params
+        blocks = sum(-(-p.numel() // kernel.ADAMW_BLOCK) for p in params)
+        n = blocks * kernel.ADAMW_BLOCK
+        state = torch.float8_e4m3fn if bits == 8 else torch.float32
+        zeros = lambda size, dt: torch.zeros(size, dtype=dt, device=dev)
+        self.tensors: Dict[str, Optional[torch.Tensor]] = dict(
+            exp_avg=zeros(n, torch.uint8).view(state) if bits == 8 else zeros(n, state),
+            exp_avg_sq=zeros(n, torch.uint8).view(state) if bits == 8 else zeros(n, state),
+            avg_scale=zeros(blocks, torch.float32) if bits == 8 else None,
+            sq_scale=zeros(blocks, torch.float32) if bits == 8 else None,
+            # (zeros are the rounding of no weight but 0: each one takes its place at the first step)
+            master=zeros(n, torch.float32) if master and dtype != torch.float32 else None,
+            step=zeros(len(params), torch.int32))
+        self.group = kernel.put_ints(dev, [], groups)[1]
+        self.workspace = kernel.Workspace(dev)
+
+    def span(self, i: int) -> Tuple[int, int]:
+        at = sum(-(-p.numel() // kernel.ADAMW_BLOCK) for p in self.params[:i]) * kernel.ADAMW_BLOCK
+        return at, at + self.params[i].numel()
+
+
+class AdamW(torch.optim.Optimizer):
+    """`AdamW(params, lr, betas, eps, weight_decay)` with decoupled weight decay, as torch.optim.AdamW's arguments: params
+    are tensors or groups of them (an adapter a group, say) on GPUs, fp16, bf16 or float32, contiguous, each in one group once.
+
+    state_bits 32: averages in float; 8: in e4m3 with a float scale each for 256 weights.  master: float weights beside 16-bit ones,
+    which are their rounding (small updates add up that a 16-bit weight would lose); a weight that somebody sets is taken over
+    at the next step.  A tensor without a gradient stays as it is, its average's age too, so adapters may take steps by turns.
+
+    Step counts live on the device, so `step` may be captured into a graph after one eager step; the groups' rates too: `step`
+    writes those that have changed, between replays `update_rates` does.  Nothing waits for the GPU."""
+
+    def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, state_bits: int = 32, master: bool = True):
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 8 or 32")
+        self.state_bits, self.master = state_bits, bool(master)
+        self._sets: List[_Set] = []
+        self._rates: Dict[torch.device, Tuple[tuple, torch.Tensor]] = {}
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def add_param_group(self, param_group: Dict[str, Any]) -> None:
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        lr, (b1, b2) = float(group["lr"]), group["betas"]
+        if lr < 0 or group["eps"] < 0 or group["weight_decay"] < 0 or not (0 <= b1 < 1 and 0 <= b2 < 1):
+            self.param_groups.pop()
+            raise ValueError("lr, eps and weight_decay must not be negative, betas lie in [0, 1)")
+
+    def _prepare(self) -> None:
+        """States of the tensors that have none yet."""
+        known = sum(len(s.params) for s in self._sets)
+        every = [(g, p) for g, group in enumerate(self.param_groups) for p in group["params"]]
+        if known == len(every):
+            return
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the states must be made before a graph is captured: run an eager step")
+        have = {id(p) for s in self._sets for p in s.params}
+        kinds: Dict[tuple, Tuple[list, list]] = {}
+        for g, p in every:
+            if id(p) in have:
+                continue
+            if not p.is_cuda or not p.is_contiguous() or p.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+                raise RuntimeError("No suitable kernel: parameters must be contiguous fp16, bf16 or float32 tensors on a GPU")
+            ps, gs = kinds.setdefault((p.device, p.dtype), ([], []))
+            ps.append(p), gs.append(g)
+        self._sets += [_Set(ps, gs, self.state_bits, self.master) for ps, gs in kinds.values()]
+
+    def update_rates(self) -> None:
+        """Writes the groups' lr, betas, eps and weight decay to the device where they have changed (step does so itself; a captured
+        step reads what is there at its replay)."""
+        self._prepare()
+        now = tuple((float(g["lr"]), float(g["betas"][0]), float(g["betas"][1]), float(g["eps"]), float(g["weight_decay"]))
+                    for g in self.param_groups)
+        for dev in {s.params[0].device for s in self._sets}:
+            was = self._rates.get(dev)
+            if was is not None and was[0] == now:
+                continue
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("rates changed while a graph is captured: call update_rates before")
+            words = struct.pack(f"{5 * len(now)}f", *[v for row in now for v in row])
+            table = was[1] if was is not None and was[1].size(0) == len(now) else torch.empty(len(now), 5, device=dev)
+            kernel.put_words(table, words)
+            self._rates[dev] = (now, table)
+
+    @torch.no_grad()
+    def step(self, closure: Optional[Callable[[], torch.Tensor]] = None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        self.update_rates()
+        for s in self._sets:
+            grads = [p.grad for p in s.params]
+            if any(g is not None and not g.is_contiguous() for g in grads):
+                grads = [g if g is None else g.contiguous() for g in grads]
+            if any(g is not None for g in grads):
+                t = s.tensors
+                kernel.adamw_step(s.params, grads, t["exp_avg"], t["exp_avg_sq"], t["step"], self._rates[s.params[0].device][1],
+                                  s.group, t["avg_scale"], t["sq_scale"], t["master"], s.workspace)
+        return loss
+
+    def state_of(self, param: torch.Tensor) -> Dict[str, torch.Tensor]:
+        """A tensor's step count and averages (and float weights), as float tensors of its shape."""
+        self._prepare()
+        for s in self._sets:
+            for i, p in enumerate(s.params):
+                if p is not param:
+                    continue
+                (a, b), t = s.span(i), s.tensors
+                first, last = a // kernel.ADAMW_BLOCK, -(-b // kernel.ADAMW_BLOCK)
+                values = lambda name, scale: (t[name][a:last * kernel.ADAMW_BLOCK].float() if scale is None else (
+                    t[name][a:last * kernel.ADAMW_BLOCK].view(-1, kernel.ADAMW_BLOCK).float()
+                    * scale[first:last, None]).flatten())[:b - a].view(p.shape)
+                out = dict(step=t["step"][i].clone(), exp_avg=values("exp_avg", t["avg_scale"]),
+                           exp_avg_sq=values("exp_avg_sq", t["sq_scale"]))
+                if self.state_bits == 8:
+                    out["exp_avg_sq"] = out["exp_avg_sq"].square()
+                if t["master"] is not None:
+                    out["master"] = t["master"][a:b].view(p.shape).clone()
+                return out
+        raise KeyError("not one of the optimizer's tensors")
+
+    def state_dict(self) -> Dict[str, Any]:
+        out = super().state_dict()
+        out["state"] = {"bits": self.state_bits,
+                        "sets": [{n: t if t is None else t.clone() for n, t in s.tensors.items()} for s in self._sets]}
+        return out
+
+    def load_state_dict(self, state_dict: Dict[str, Any]) -> None:
+        state = state_dict["state"]
+        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
+        if not state["sets"]:  # (saved before its first step)
+            self._sets = []
+            return
+        self._prepare()
+        shape = lambda tensors: {n: None if t is None else (t.dtype, tuple(t.shape)) for n, t in tensors.items()}
+        if state["bits"] != self.state_bits or [shape(s.tensors) for s in self._sets] != [shape(s) for s in state["sets"]]:
+            raise ValueError("the saved states are of other tensors, or of another number of bits")
+        for s, saved in zip(self._sets, state["sets"]):
+            for name, t in s.tensors.items():
+                if t is not None:
+                    t.copy_(saved[name])

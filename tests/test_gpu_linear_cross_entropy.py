@@ -87,6 +87,7 @@ def check(x, w, labels, partition=None, want_w=True, grad=None):
 def test_rows_and_gradients(T, H, V, dt):
     x, w, labels = make(T, H, V, dt, T + V)
     check(x, w, labels)
+    check(x, w, labels, want_w=False)  # (a frozen vocabulary: another route)
 
 
 @pytest.mark.parametrize("dt", [FP16, BF16])
@@ -99,7 +100,7 @@ def test_rows_without_labels(T, H, V, labelled, dt):
     a = x.detach().requires_grad_(True)
     out = linear_cross_entropy.apply(a, w, labels, edges)
     got = torch.autograd.grad(out, a, torch.ones_like(out))[0]
-    ref_out, ref = check(xz, w, labels, edges, grad=torch.ones_like(out))
+    ref_out, ref = check(xz, w, labels, edges, want_w=False, grad=torch.ones_like(out))
     assert torch.equal(out, ref_out) and torch.equal(got, ref[0])
     assert out[1] == 0 and not got[labels < 0].any()
 
@@ -137,12 +138,52 @@ def test_one_partitions_loss_alone():
     assert not dx[:200].any() and dx[200:].any()
 
 
-def test_frozen_head_and_frozen_rows():
+def test_frozen_rows_and_kept_sums():
     x, w, labels = make(100, 64, 300, BF16)
     a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
     both = torch.autograd.grad(linear_cross_entropy.apply(a, b, labels).sum(), (a, b))
-    assert torch.equal(torch.autograd.grad(linear_cross_entropy.apply(a, w, labels).sum(), a)[0], both[0])
     assert torch.equal(torch.autograd.grad(linear_cross_entropy.apply(x, b, labels).sum(), b)[0], both[1])
+    # the calls behind it: what the forward keeps serves several backwards, of any gradients
+    f = lambda n: torch.empty(n, device="cuda")
+    kept = torch.empty(K.linear_cross_entropy_kept_size(100, 64, 300), dtype=torch.uint8, device="cuda")
+    loss, lse, one, three, other = f(100), f(100), torch.empty_like(x), torch.empty_like(x), torch.empty_like(x)
+    K.linear_cross_entropy(loss, lse, x, w, labels, kept=kept)
+    g = torch.ones(100, device="cuda")
+    K.linear_cross_entropy_backward(one, None, g, loss, lse, x, w, labels, kept=kept)
+    K.linear_cross_entropy_backward(three, None, 4 * g, loss, lse, x, w, labels, kept=kept)
+    K.linear_cross_entropy_backward(other, None, g, loss, lse, x, w, labels)
+    assert torch.equal(three.float(), 4 * one.float()) and torch.equal(other, both[0])
+    # two routes, each within eps / 2 of sum |G w| <= 2 max |w| and eps / 2 of its own rounding
+    assert (other.float() - one.float()).abs().max() <= 4 * 2.0 ** -8 * 2 * w.float().abs().max()
+
+
+@pytest.mark.parametrize("dt", [FP16, BF16])
+def test_references_move_from_piece_to_piece(dt):
+    """Logits that grow along the vocabulary by far more than 16-bit exponents hold, so that every piece (128 MiB of exponentials) takes
+    the rows' reference along, in some rows; in others the first piece holds the largest."""
+    T, H, V = 600, 64, 250000
+    g = torch.Generator().manual_seed(0)
+    x, w = torch.randn(T, H, generator=g), 0.3 * torch.randn(V, H, generator=g)
+    x[:, 0], x[:, 1] = 1.0, 0.0
+    x[::3, 1] = 1.0
+    x[1::3, 1] = -0.25
+    w[:, 1] = torch.arange(V) * (300.0 / V)
+    labels = torch.randint(0, V, (T,), generator=g)
+    labels[::2] = torch.randint(V - 2000, V, (300,), generator=g)
+    x, w, labels = x.to(dt).cuda().requires_grad_(True), w.to(dt).cuda(), labels.cuda()
+    out = linear_cross_entropy.apply(x, w, labels)
+    dx, = torch.autograd.grad(out.sum(), x)
+    z = x.detach().double() @ w.double().t().contiguous()
+    lse = torch.logsumexp(z, 1)
+    at = torch.arange(T, device="cuda")
+    # (of the row's largest logits too: sums of 64 terms in float, some of 300)
+    assert ((out.double() - (lse - z[at, labels])).abs() <= 2e-5 + 1e-6 * (z[at, labels].abs() + lse.abs())).all()
+    P = torch.exp(z - lse[:, None])
+    exact = P @ w.double() - w.double()[labels]
+    eps = torch.finfo(dt).eps
+    # entries below 2^-28 of a row's largest (fp16) lose bits of a 2^-39th of it: V 2^-39 |w| at most
+    limit = (P @ w.double().abs()) * (eps / 2 + 1e-5) + exact.abs() * eps / 2 + V * 2.0 ** -39 * w.double().abs().amax(0) + 1e-6
+    assert ((dx.double() - exact).abs() <= limit).all()
 
 
 @pytest.mark.parametrize("dt", [FP16, BF16])
@@ -201,6 +242,36 @@ def test_large_logits():
     assert torch.isfinite(torch.autograd.grad(out.sum(), x)[0]).all()
 
 
+@pytest.mark.parametrize("dt", [FP16, BF16])
+def test_labels_that_are_nearly_certain(dt):
+    """Rows whose label has all but 2^-5 to 2^-40 of the probability: losses and gradients are exact relative to their size (the logits' own
+    error aside: 2e-6 of the largest |x||w|, which moves others / e by as much), and where others vanish they are 0."""
+    T, H, V = 72, 128, 400
+    x, w, labels = make(T, H, V, dt, 11, spread=1.0)
+    boost = torch.linspace(1, 40, T)[:, None].cuda()
+    x = (0.1 * x.float() + boost * w[labels].float()).to(dt)
+    for frozen in (True, False):
+        a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(not frozen)
+        out = linear_cross_entropy.apply(a, b, labels)
+        dx, = torch.autograd.grad(out.sum(), a)
+        z = x.double() @ w.double().t().contiguous()
+        at = torch.arange(T, device="cuda")
+        own = z[at, labels]
+        z[at, labels] = -float("inf")
+        others = torch.exp(z - own[:, None])
+        loss = torch.log1p(others.sum(1))
+        top = (x.double().norm(dim=1).max() * w.double().norm(dim=1).max()).item()
+        soft = 4e-6 * top + 4e-6
+        keep = loss > 1e-30
+        assert ((out.double() - loss).abs() <= loss * soft)[keep].all()
+        P = others / (1 + others.sum(1, keepdim=True))
+        exact = P @ w.double() - P.sum(1, keepdim=True) * w.double()[labels]
+        size = P @ w.double().abs() + P.sum(1, keepdim=True) * w.double()[labels].abs()
+        eps, f = torch.finfo(dt).eps, torch.finfo(dt)
+        limit = size * (eps / 2 + 2 * soft) + exact.abs() * eps / 2 + f.smallest_normal * f.eps
+        assert ((dx.double() - exact).abs() <= limit).all()
+
+
 def test_differences():
     """The gradient against central differences of the loss: x moves along a direction by powers of two that bf16 holds."""
     x, w, labels = make(8, 64, 200, BF16, 6)
@@ -224,11 +295,14 @@ def test_captured_and_replayed():
     ws = K.Workspace(x.device)
     f = lambda n: torch.empty(n, device="cuda")
     loss, lse, means, weight, dx, dw = f(300), f(300), f(2), f(2), torch.empty_like(x), torch.empty_like(w)
-    g = torch.ones(2, device="cuda")
+    g, dk = torch.ones(2, device="cuda"), torch.empty_like(x)
+    kept = torch.empty(K.linear_cross_entropy_kept_size(300, 128, 1000), dtype=torch.uint8, device="cuda")
 
     def step():
         K.linear_cross_entropy(loss, lse, x, w, labels, part, means, weight, ws)
-        K.linear_cross_entropy_backward(dx, dw, g, lse, x, w, labels, part, weight, ws)
+        K.linear_cross_entropy_backward(dx, dw, g, loss, lse, x, w, labels, part, weight, ws)
+        K.linear_cross_entropy(loss, lse, x, w, labels, part, means, weight, ws, kept)
+        K.linear_cross_entropy_backward(dk, None, g, loss, lse, x, w, labels, part, weight, ws, kept)
 
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
@@ -243,10 +317,10 @@ def test_captured_and_replayed():
         x.copy_(x2), w.copy_(w2), labels.copy_(l2)
         graph.replay()
         torch.cuda.synchronize()
-        got = [t.clone() for t in (means, dx, dw)]
+        got = [t.clone() for t in (means, dx, dw, dk)]
         step()
         torch.cuda.synchronize()
-        assert all(torch.equal(a, b) for a, b in zip(got, (means, dx, dw)))
+        assert all(torch.equal(a, b) for a, b in zip(got, (means, dx, dw, dk)))
         check(x, w, labels, part)
 
 
