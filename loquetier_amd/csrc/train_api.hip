@@ -14,8 +14,10 @@ int check_dtype(int dtype) { return dtype == SMLM_DTYPE_F16 || dtype == SMLM_DTY
 // ---- the loss over the vocabulary ----
 
 constexpr int kLossMaxDim = 1 << 22;           // H: a tile's rows stay inside a resource
-constexpr int64_t kLossPieceBytes = 128 << 20;  // of G at a time
-constexpr int kLossMostSplits = 64;
+#ifndef LPB
+#define LPB 512
+#endif
+constexpr int64_t kLossPieceBytes = (int64_t)LPB << 20;  // of G at a time
 
 int loss_check(int T, int H, int V, int dtype) {
   if (T < 0 || H <= 0 || V <= 0) return SMLM_ERR_ARG;
@@ -28,21 +30,33 @@ int loss_check(int T, int H, int V, int dtype) {
   return SMLM_OK;
 }
 bool loss_few(int T) { return T <= kLossFewRows; }
-// Vocabulary entries a piece: whole tiles.
+// Vocabulary entries a piece: whole tiles, as many in each.
 int loss_piece(int T, int V) {
-  const int64_t most = kLossPieceBytes / (2 * (int64_t)(T > 0 ? T : 1)) / kLossTileV * kLossTileV;
-  const int all = round_up(V, kLossTileV);
-  return most < kLossTileV ? kLossTileV : most < all ? (int)most : all;
+  const int64_t pieces = (2 * (int64_t)(T > 0 ? T : 1) * V + kLossPieceBytes - 1) / kLossPieceBytes;
+  const int64_t each = (V + pieces - 1) / pieces;
+  return (int)((each + kLossTileV - 1) / kLossTileV * kLossTileV);
 }
-int64_t loss_dx_floats(int T, int H) {
-  const int64_t one = (int64_t)T * H, tile = loss_few(T) ? kLossFewRows : kLossRows, cut = 256 * 256 * tile;
-  const int64_t split = cut < kLossMostSplits * one ? cut : kLossMostSplits * one;
-  return one > split ? one : split;
+int loss_stages(int T, int V) {
+  const int piece = loss_piece(T, V);
+  return ceil_div(piece < V ? piece : V, kGemmK);
+}
+// Parts of cut tiles, whatever the number of labelled rows; units of dx.
+int loss_parts(int T, int H, int stages, int* most_units) {
+  const bool few = loss_few(T);
+  int parts = 0, units = 0;
+  for (int r = 1; r <= ceil_div(T, few ? kLossFewRows : kLossRows); ++r) {
+    const LossCuts c = loss_cuts(r * ceil_div(H, 256), stages, few);
+    const int u = round_up(c.whole, 8) + round_up(c.rest * c.parts, 8);
+    parts = c.rest * c.parts > parts ? c.rest * c.parts : parts;
+    units = u > units ? u : units;
+  }
+  if (most_units) *most_units = units;
+  return parts;
 }
 
 struct LossSpace {
   LossRows rows;
-  float *part, *at_label, *dx;
+  float *part, *at_label, *dx, *cut;
   uint16_t* g;
   int pad, parts, piece;
 };
@@ -56,8 +70,12 @@ struct LossTaker {
     p = base ? reinterpret_cast<P*>(base + o) : nullptr;
   }
 };
+void loss_take_dx(LossTaker& k, int T, int H, int V, LossSpace* s) {
+  k.take(s->dx, 4 * (size_t)T * H);
+  k.take(s->cut, 4 * (size_t)loss_parts(T, H, loss_stages(T, V), nullptr) * 256 * (loss_few(T) ? kLossFewRows : kLossRows));
+}
 // What the forward keeps for the gradient of x: its sums, and what the fold needs.
-size_t loss_keep(void* base, int T, int H, LossSpace* s) {
+size_t loss_keep(void* base, int T, int H, int V, LossSpace* s) {
   LossTaker k{reinterpret_cast<char*>(base)};
   const size_t t = (size_t)T;
   k.take(s->rows.count, 256);
@@ -65,7 +83,7 @@ size_t loss_keep(void* base, int T, int H, LossSpace* s) {
   k.take(s->rows.label, 4 * t);
   k.take(s->rows.sum, 4 * t);
   k.take(s->rows.share, 4 * t);
-  k.take(s->dx, 4 * (size_t)loss_dx_floats(T, H));
+  loss_take_dx(k, T, H, V, s);
   return k.off;
 }
 // what: 0 the forward, 1 the backward with dx, 2 with dw, 3 with both, 4 the forward that keeps.
@@ -97,28 +115,25 @@ size_t loss_carve(void* base, int T, int H, int V, int what, LossSpace* s) {
     k.take(s->rows.lost, 4 * t);
   }
   if (what) k.take(s->g, 2 * t * s->piece);
-  if (what == 1 || what == 3) k.take(s->dx, 4 * (size_t)loss_dx_floats(T, H));
+  if (what == 1 || what == 3) loss_take_dx(k, T, H, V, s);
   return k.off;
 }
 
 dim3 loss_grid(int64_t units) { return dim3((unsigned)((units + 7) / 8 * 8)); }
 
-template <int MODE>
-int loss_logits(bool f16, bool few, dim3 grid, hipStream_t st, const LossTileArgs& a) {
-  const dim3 bl(256);
-  if (few)
-    return f16 ? launch(loss_logits_kernel<SMLM_DTYPE_F16, true, MODE>, grid, bl, st, a)
-               : launch(loss_logits_kernel<SMLM_DTYPE_BF16, true, MODE>, grid, bl, st, a);
-  return f16 ? launch(loss_logits_kernel<SMLM_DTYPE_F16, false, MODE>, grid, bl, st, a)
-             : launch(loss_logits_kernel<SMLM_DTYPE_BF16, false, MODE>, grid, bl, st, a);
+int loss_logits(int mode, bool f16, bool few, dim3 grid, hipStream_t st, const LossTileArgs& a) {
+  void (*const kernels[3][2][2])(LossTileArgs) = {  // by mode, rows and type
+      {{loss_logits_kernel<SMLM_DTYPE_F16, false, kLossSums>, loss_logits_kernel<SMLM_DTYPE_BF16, false, kLossSums>},
+       {loss_logits_kernel<SMLM_DTYPE_F16, true, kLossSums>, loss_logits_kernel<SMLM_DTYPE_BF16, true, kLossSums>}},
+      {{loss_logits_kernel<SMLM_DTYPE_F16, false, kLossSoft>, loss_logits_kernel<SMLM_DTYPE_BF16, false, kLossSoft>},
+       {loss_logits_kernel<SMLM_DTYPE_F16, true, kLossSoft>, loss_logits_kernel<SMLM_DTYPE_BF16, true, kLossSoft>}},
+      {{loss_logits_kernel<SMLM_DTYPE_F16, false, kLossGrad>, loss_logits_kernel<SMLM_DTYPE_BF16, false, kLossGrad>},
+       {loss_logits_kernel<SMLM_DTYPE_F16, true, kLossGrad>, loss_logits_kernel<SMLM_DTYPE_BF16, true, kLossGrad>}}};
+  return launch(kernels[mode][few][!f16], grid, dim3(256), st, a);
 }
 int loss_dx(bool f16, bool few, hipStream_t st, const LossTileArgs& a) {
-  const int tile = few ? kLossFewRows : kLossRows, h_tiles = ceil_div(a.H, 256);
-  int most = 0;  // units, whatever the number of labelled rows
-  for (int r = 1; r <= ceil_div(a.T, tile); ++r) {
-    const int u = r * h_tiles * loss_splits(r, h_tiles, a.most_splits);
-    if (u > most) most = u;
-  }
+  int most = 0;
+  loss_parts(a.T, a.H, a.stages, &most);
   const dim3 grid = loss_grid(most), bl(256);
   if (few)
     return f16 ? launch(loss_dx_kernel<SMLM_DTYPE_F16, true>, grid, bl, st, a) : launch(loss_dx_kernel<SMLM_DTYPE_BF16, true>, grid, bl, st, a);
@@ -133,7 +148,7 @@ SMLM_API int smlm_vocab_loss_workspace_size(int T, int H, int V, int what, size_
   if (!bytes || what < 0 || what > 5) return SMLM_ERR_ARG;
   if (int rc = loss_check(T, H, V, SMLM_DTYPE_F16)) return rc;
   LossSpace s{};
-  *bytes = what == 5 ? loss_keep(nullptr, T, H, &s) : loss_carve(nullptr, T, H, V, what, &s);
+  *bytes = what == 5 ? loss_keep(nullptr, T, H, V, &s) : loss_carve(nullptr, T, H, V, what, &s);
   return SMLM_OK;
 }
 
@@ -149,7 +164,7 @@ SMLM_API int smlm_vocab_loss_fwd(float* loss, float* lse, float* means, float* w
   hipStream_t st = (hipStream_t)stream;
   if (T > 0) {
     LossSpace s{};
-    if (kept && kept_bytes < loss_keep(kept, T, H, &s)) return SMLM_ERR_WORKSPACE;
+    if (kept && kept_bytes < loss_keep(kept, T, H, V, &s)) return SMLM_ERR_WORKSPACE;
     if (workspace_bytes < loss_carve(workspace, T, H, V, kept ? 4 : 0, &s)) return SMLM_ERR_WORKSPACE;
     const LossScanArgs sa{s.rows, labels, loss, lse, nullptr, P ? partition : nullptr, nullptr, T, V, P, 0, kept != nullptr};
     LOSS_TRY(launch(loss_scan_kernel<false>, dim3(1), dim3(kLossScanThreads), st, sa));
@@ -157,13 +172,13 @@ SMLM_API int smlm_vocab_loss_fwd(float* loss, float* lse, float* means, float* w
     LOSS_TRY(launch(loss_gather_kernel, dim3((unsigned)ceil_div(T, 4)), dim3(256), st, ga));
     LossTileArgs a{};
     a.rows = s.rows, a.x = ga.x, a.w = reinterpret_cast<const uint16_t*>(w), a.part = s.part, a.at_label = s.at_label;
-    a.g = s.g, a.dx = s.dx, a.T = T, a.H = H, a.V = V, a.pad = s.pad, a.ldg = s.piece, a.most_splits = kLossMostSplits, a.turned = 1;
+    a.g = s.g, a.dx = s.dx, a.T = T, a.H = H, a.V = V, a.pad = s.pad, a.ldg = s.piece, a.cut = s.cut, a.stages = loss_stages(T, V), a.turned = 1;
     const bool few = loss_few(T), f16 = dtype == SMLM_DTYPE_F16;
     for (int v0 = 0; v0 < V; v0 += s.piece) {
       a.v0 = v0, a.v1 = V - v0 < s.piece ? V : v0 + s.piece, a.add = v0 > 0;
       const int v_tiles = ceil_div(a.v1 - v0, kLossTileV), parts = v_tiles * (few ? 4 : 2);
       const dim3 grid = loss_grid((int64_t)ceil_div(T, few ? kLossFewRows : kLossRows) * v_tiles);
-      LOSS_TRY(kept ? loss_logits<kLossSoft>(f16, few, grid, st, a) : loss_logits<kLossSums>(f16, few, grid, st, a));
+      LOSS_TRY(loss_logits(kept ? kLossSoft : kLossSums, f16, few, grid, st, a));
       const LossRefsArgs ra{s.rows, s.part, s.at_label, loss, lse, parts, s.pad, v0 == 0, a.v1 == V,
                             kept && f16 ? kLossBias<SMLM_DTYPE_F16> : 0.0f};
       const dim3 rows16((unsigned)ceil_div(T, 16));
@@ -189,9 +204,9 @@ SMLM_API int smlm_vocab_loss_bwd_kept(void* dx, const float* grad, const void* k
   if (!dx || !grad || !kept || !w) return SMLM_ERR_ARG;
   if (!aligned16(dx) || !aligned16(kept) || !aligned16(w)) return SMLM_ERR_ALIGN;
   LossSpace s{};
-  if (kept_bytes < loss_keep(const_cast<void*>(kept), T, H, &s)) return SMLM_ERR_WORKSPACE;
-  const LossDxFoldArgs fa{s.rows, s.dx, reinterpret_cast<uint16_t*>(dx), reinterpret_cast<const uint16_t*>(w), T, H, loss_few(T),
-                          kLossMostSplits, grad, partition, weight, P};
+  if (kept_bytes < loss_keep(const_cast<void*>(kept), T, H, V, &s)) return SMLM_ERR_WORKSPACE;
+  const LossDxFoldArgs fa{s.rows, s.dx, s.cut, reinterpret_cast<uint16_t*>(dx), reinterpret_cast<const uint16_t*>(w), T, H, loss_few(T),
+                          loss_stages(T, V), grad, partition, weight, P};
   const dim3 grid((unsigned)ceil_div(T, 4)), bl(256);
   hipStream_t st = (hipStream_t)stream;
   return dtype == SMLM_DTYPE_F16 ? launch(loss_dx_fold_kernel<SMLM_DTYPE_F16, true>, grid, bl, st, fa)
@@ -216,13 +231,13 @@ SMLM_API int smlm_vocab_loss_bwd(void* dx, void* dw, const float* grad, const fl
   LOSS_TRY(launch(loss_gather_kernel, dim3((unsigned)ceil_div(T, 4)), dim3(256), st, ga));
   LossTileArgs a{};
   a.rows = s.rows, a.x = ga.x, a.w = reinterpret_cast<const uint16_t*>(w), a.g = s.g, a.dx = s.dx;
-  a.dw = reinterpret_cast<uint16_t*>(dw), a.T = T, a.H = H, a.V = V, a.ldg = s.piece, a.most_splits = kLossMostSplits;
+  a.dw = reinterpret_cast<uint16_t*>(dw), a.T = T, a.H = H, a.V = V, a.ldg = s.piece, a.cut = s.cut, a.stages = loss_stages(T, V);
   const int tile = few ? kLossFewRows : kLossRows, h_tiles = ceil_div(H, 256);
   const dim3 bl(256);
   for (int v0 = 0; v0 < V; v0 += s.piece) {
     a.v0 = v0, a.v1 = V - v0 < s.piece ? V : v0 + s.piece, a.add = v0 > 0;
     const int v_tiles = ceil_div(a.v1 - v0, kLossTileV);
-    LOSS_TRY(loss_logits<kLossGrad>(f16, few, loss_grid((int64_t)ceil_div(T, tile) * v_tiles), st, a));
+    LOSS_TRY(loss_logits(kLossGrad, f16, few, loss_grid((int64_t)ceil_div(T, tile) * v_tiles), st, a));
     if (dx) LOSS_TRY(loss_dx(f16, few, st, a));
     if (dw) {
       const dim3 gw = loss_grid((int64_t)h_tiles * v_tiles);
@@ -230,7 +245,7 @@ SMLM_API int smlm_vocab_loss_bwd(void* dx, void* dw, const float* grad, const fl
     }
   }
   if (!dx) return SMLM_OK;
-  const LossDxFoldArgs fa{s.rows, s.dx, reinterpret_cast<uint16_t*>(dx), a.w, T, H, few, kLossMostSplits, nullptr, nullptr, nullptr, 0};
+  const LossDxFoldArgs fa{s.rows, s.dx, s.cut, reinterpret_cast<uint16_t*>(dx), a.w, T, H, few, a.stages, nullptr, nullptr, nullptr, 0};
   const dim3 grid((unsigned)ceil_div(T, 4));
   return f16 ? launch(loss_dx_fold_kernel<SMLM_DTYPE_F16, false>, grid, bl, st, fa)
              : launch(loss_dx_fold_kernel<SMLM_DTYPE_BF16, false>, grid, bl, st, fa);

@@ -172,28 +172,38 @@ struct LossTileArgs {
   float* part;        // [parts][pad][2] a row's reference and sum of a part of the vocabulary (forward)
   float* at_label;    // [pad] (forward)
   uint16_t* g;        // [n, ldg] G, or the exponentials
-  float* dx;          // [splits][n, H]
+  float* dx;          // [n, H]: sums for dx
+  float* cut;         // [parts][tile]: those of tiles whose axis is cut
   uint16_t* dw;       // [V, H] (backward)
   int T, H, V, pad;
   int v0, v1, ldg;    // the piece of the vocabulary
-  int most_splits, add;  // add: to what is there of dx, turned (`turned`)
+  int stages, add;    // of a whole piece; add: to what is there of dx, turned (`turned`)
   int turned;
 };
 
 __device__ __forceinline__ const uint16_t* loss_x(const LossTileArgs& a, int n) { return n == a.T ? a.x : a.rows.x; }
 
-// Which tiles a workgroup takes: workgroups go to the eight XCDs in turn, and each XCD takes a run of the tiles, eight row tiles by
-// the next after another, so that its L2 holds what its 32 workgroups share (8 x 4 tiles: 12 operands' stages for 32 workgroups).
+// Which tiles a workgroup takes: workgroups go to the eight XCDs in turn, and each XCD takes a run of the tiles, four row tiles by
+// the next after another, so that its L2 holds what its 32 workgroups share.  (Eight row tiles: 1.16 PFLOP/s for 1.23 at 32000 x 4096 x
+// 4096, 1.11 for 1.26 at 8192 x 8192 x 8192; two: 1.17 and 1.10.)
+constexpr int kLossGroup = 4;
 struct LossUnit {
   int rows, other;
   bool any;
 };
+__device__ __forceinline__ LossUnit loss_tile(int u, int n_rows, int n_other) {
+  const int group = u / (kLossGroup * n_other), in = u - group * kLossGroup * n_other, wide = min(kLossGroup, n_rows - group * kLossGroup);
+  return {group * kLossGroup + in % wide, in / wide, true};
+}
+__device__ __forceinline__ int loss_tile_number(int rows, int other, int n_rows, int n_other) {
+  const int group = rows / kLossGroup, wide = min(kLossGroup, n_rows - group * kLossGroup);
+  return group * kLossGroup * n_other + other * wide + rows % kLossGroup;
+}
 __device__ __forceinline__ LossUnit loss_unit(int n_rows, int n_other) {
   const int units = n_rows * n_other, per = (units + 7) >> 3;
   const int local = (int)blockIdx.x >> 3, u = ((int)blockIdx.x & 7) * per + local;
   if (local >= per || u >= units) return {0, 0, false};
-  const int group = u / (8 * n_other), in = u - group * 8 * n_other, wide = min(8, n_rows - group * 8);
-  return {group * 8 + in % wide, in / wide, true};
+  return loss_tile(u, n_rows, n_other);
 }
 
 template <int IA, int JB>
@@ -234,6 +244,30 @@ __device__ __forceinline__ void loss_store(const f32x16 (&acc)[IA][JB], uint16_t
   }
 }
 
+// The same of sums whose operands both lie across: row 4 n + j of the wave's blocks, columns 4 m + i.
+template <int DT>
+__device__ __forceinline__ void loss_store_across(const f32x16 (&acc)[4][4], uint16_t* lds, uint16_t* out, int64_t ld, int rows, int cols) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int row = gemm_row<true, 4>(j, lane & 31);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int m = gemm_sum_row(e, lane);
+      u32x2 two;
+      two[0] = pack2<DT>(acc[0][j][e], acc[1][j][e]);
+      two[1] = pack2<DT>(acc[2][j][e], acc[3][j][e]);
+      *(u32x2*)(lds + row * 128 + (((m >> 1) ^ ((row >> 2) & 15)) << 3) + (m & 1) * 4) = two;
+    }
+  }
+#pragma unroll 4
+  for (int r0 = 0; r0 < 128; r0 += 4) {
+    const int row = r0 + (lane >> 4), piece = lane & 15;
+    const u32x4 v = *(const u32x4*)(lds + row * 128 + ((piece ^ ((row >> 2) & 15)) << 3));
+    if (row < rows && piece * 8 < cols) stg16(out + (int64_t)row * ld + piece * 8, v);
+  }
+}
+
 // Waits until nobody reads the stages and no load to them is on its way.
 __device__ __forceinline__ void loss_lds_free() {
   __builtin_amdgcn_s_waitcnt(0x0f70);
@@ -256,15 +290,15 @@ template <int DT, bool FEW, int MODE>
 __global__ __launch_bounds__(256, 1) void loss_logits_kernel(LossTileArgs a) {
   constexpr int WA = FEW ? 4 : 2, IA = FEW ? 2 : 4, WB = FEW ? 1 : 2, JB = FEW ? 2 : 4;
   typedef GemmShape<WA, IA, false, WB, JB, false> S;
-  __shared__ __align__(16) uint16_t lds[2 * S::kStage];
+  __shared__ __align__(16) uint16_t lds[kGemmStages * S::kStage];
   const int n = uload(a.rows.count, 0);
   const LossUnit u = loss_unit((n + S::kB - 1) / S::kB, (a.v1 - a.v0 + kLossTileV - 1) / kLossTileV);
   if (!u.any) return;
   f32x16 acc[IA][JB];
   loss_zero(acc);
   const int first_v = a.v0 + u.other * kLossTileV, first_t = u.rows * S::kB;
-  gemm_tile<DT, WA, IA, false, WB, JB, false>(acc, lds, GemmOperand{a.w, a.H, a.V}, first_v,
-                                              GemmOperand{loss_x(a, n), a.H, n}, first_t, 0, a.H);
+  const GemmOperand w{a.w, a.H, a.V}, x{loss_x(a, n), a.H, n};
+  GemmTile<DT, WA, IA, false, WB, JB, false>::run(acc, lds, w, first_v, x, first_t, 0, a.H);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
   const int v = first_v + (wave / WB) * IA * 32, t = first_t + (wave % WB) * JB * 32 + (lane & 31);
   const bool ends = v + IA * 32 > a.v1;  // the vocabulary ends inside the wave's part
@@ -304,9 +338,9 @@ __global__ __launch_bounds__(256, 1) void loss_logits_kernel(LossTileArgs a) {
       for (int i = 0; i < IA; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, -to));
-          if (MODE == kLossSoft) acc[i][j][e] = x;
-          l += x;
+          const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], kLog2e, -to));
+          if (MODE == kLossSoft) acc[i][j][e] = y;
+          l += y;
         }
       l += __shfl_xor(l, 32, kWaveSize);
       if (tj < n && h == 0) {
@@ -341,12 +375,21 @@ __global__ __launch_bounds__(256, 1) void loss_logits_kernel(LossTileArgs a) {
   }
 }
 
-// How many parts the vocabulary's axis of dx is cut into: as many as leave no compute unit without a tile.
-__device__ __host__ __forceinline__ int loss_splits(int row_tiles, int h_tiles, int most) {
-  const int tiles = row_tiles * h_tiles;
-  if (tiles <= 0) return 1;
-  const int s = 256 / tiles;
-  return s < 1 ? 1 : s > most ? most : s;
+// The tiles of dx that fill whole rounds of the compute units take the vocabulary's axis whole; of the others it is cut into as many
+// parts as take the least time: rounds of a part's stages, and what a part costs to write and add up (a tile of floats, both ways at
+// HBM's rate: a 17th of a stage each).  Whatever the piece, the cuts are those of a whole one.
+struct LossCuts {
+  int whole, parts, rest;  // tiles that are whole; parts of each other; their number
+};
+constexpr int kLossMostParts = 512;
+__host__ __device__ __forceinline__ LossCuts loss_cuts(int tiles, int stages, bool few) {
+  const int slots = few ? 512 : 256, rest = tiles % slots;
+  int best = 1, least = 0x7fffffff;
+  for (int s = 1; s <= 64 && s <= stages && (s == 1 || rest * s <= kLossMostParts); ++s) {
+    const int cost = (rest * s + slots - 1) / slots * ((stages + s - 1) / s) * 64 + rest * s * (few ? 1 : 4);
+    if (cost < least) least = cost, best = s;
+  }
+  return best == 1 ? LossCuts{tiles, 1, 0} : LossCuts{tiles - rest, best, rest};
 }
 
 // dx's sums over a piece of the vocabulary (added to what is there already with `add`), in float.
@@ -354,44 +397,68 @@ template <int DT, bool FEW>
 __global__ __launch_bounds__(256, 1) void loss_dx_kernel(LossTileArgs a) {
   constexpr int WA = FEW ? 4 : 2, IA = FEW ? 2 : 4, WB = FEW ? 1 : 2, JB = FEW ? 2 : 4;
   typedef GemmShape<WA, IA, true, WB, JB, false> S;
-  __shared__ __align__(16) uint16_t lds[2 * S::kStage];
+  typedef float sums __attribute__((ext_vector_type(IA)));
+  __shared__ __align__(16) uint16_t lds[kGemmStages * S::kStage];
   const int n = uload(a.rows.count, 0);
   const int row_tiles = (n + S::kB - 1) / S::kB, h_tiles = (a.H + S::kA - 1) / S::kA;
-  const int splits = loss_splits(row_tiles, h_tiles, a.most_splits);
-  const LossUnit u = loss_unit(row_tiles, h_tiles * splits);
-  if (!u.any) return;
-  const int split = u.other / h_tiles, first_h = (u.other - split * h_tiles) * S::kA, first_t = u.rows * S::kB;
-  const int stages = (a.v1 - a.v0 + kGemmK - 1) / kGemmK, each = (stages + splits - 1) / splits;
-  const int k0 = min(split * each, stages) * kGemmK, k1 = min((split + 1) * each, stages) * kGemmK;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
-  float* out = a.dx + (int64_t)split * n * a.H;
-  const int hh = first_h + (wave / WB) * IA * 32 + 4 * h, t = first_t + (wave % WB) * JB * 32 + (lane & 31);
+  const LossCuts cuts = loss_cuts(row_tiles * h_tiles, a.stages, FEW);
+  // (each XCD takes its share of the whole tiles, then of the parts)
+  const int xcd = (int)blockIdx.x & 7, whole = (cuts.whole + 7) >> 3, parts = (cuts.rest * cuts.parts + 7) >> 3;
+  int local = (int)blockIdx.x >> 3, tile, part = 0, at = -1;
+  if (local < whole) {
+    tile = xcd * whole + local;
+    if (tile >= cuts.whole) return;
+  } else {
+    local -= whole;
+    const int p = xcd * parts + local;
+    if (local >= parts || p >= cuts.rest * cuts.parts) return;
+    part = p / cuts.rest;
+    at = p - part * cuts.rest;
+    tile = cuts.whole + at;
+    at = at * cuts.parts + part;
+  }
+  const LossUnit u = loss_tile(tile, row_tiles, h_tiles);
+  const int first_h = u.other * S::kA, first_t = u.rows * S::kB, cols = a.v1 - a.v0;
+  const int each = at < 0 ? a.stages : (a.stages + cuts.parts - 1) / cuts.parts;
+  const int k0 = min(part * each * kGemmK, cols), k1 = min((part + 1) * each * kGemmK, cols);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  // (a cut tile's sums lie as a tile by itself)
+  const int ld = at < 0 ? a.H : S::kA;
+  float* out = at < 0 ? a.dx + (int64_t)first_t * a.H + first_h : a.cut + (int64_t)at * S::kA * S::kB;
+  const int rows = n - first_t, wide = a.H - first_h;
+  const int row0 = (wave % WB) * JB * 32 + (lane & 31), col0 = (wave / WB) * IA * 32;
   f32x16 acc[IA][JB];
   loss_zero(acc);
   if (a.add) {
 #pragma unroll
-    for (int j = 0; j < JB; ++j)
+    for (int j = 0; j < JB; ++j) {
+      const int row = row0 + j * 32;
+      const float turn = a.turned && row < rows ? a.rows.turn[first_t + row] : 1.0f;
 #pragma unroll
-      for (int i = 0; i < IA; ++i)
+      for (int e = 0; e < 16; ++e) {
+        const int col = col0 + IA * gemm_sum_row(e, lane);
+        if (row < rows && col < wide) {
+          const sums v = *(const SMLM_GLOBAL sums*)(out + (int64_t)row * ld + col) * turn;
 #pragma unroll
-        for (int e = 0; e < 16; e += 4)
-          if (t + j * 32 < n && hh + i * 32 + 2 * e < a.H) {
-            f32x4 v = ldg_f4(out + (int64_t)(t + j * 32) * a.H + hh + i * 32 + 2 * e);
-            if (a.turned) v *= a.rows.turn[t + j * 32];
-            acc[i][j][e] = v[0], acc[i][j][e + 1] = v[1], acc[i][j][e + 2] = v[2], acc[i][j][e + 3] = v[3];
-          }
+          for (int i = 0; i < IA; ++i) acc[i][j][e] = v[i];
+        }
+      }
+    }
   }
-  gemm_tile<DT, WA, IA, true, WB, JB, false>(acc, lds, GemmOperand{a.w + (int64_t)a.v0 * a.H, a.H, a.V - a.v0}, first_h,
+  GemmTile<DT, WA, IA, true, WB, JB, false>::run(acc, lds, GemmOperand{a.w + (int64_t)a.v0 * a.H, a.H, a.V - a.v0}, first_h,
                                              GemmOperand{a.g, a.ldg, n}, first_t, k0, k1);
 #pragma unroll
-  for (int j = 0; j < JB; ++j)
+  for (int j = 0; j < JB; ++j) {
+    const int row = row0 + j * 32;
 #pragma unroll
-    for (int i = 0; i < IA; ++i)
+    for (int e = 0; e < 16; ++e) {
+      const int col = col0 + IA * gemm_sum_row(e, lane);
+      sums v;
 #pragma unroll
-      for (int e = 0; e < 16; e += 4)
-        if (t + j * 32 < n && hh + i * 32 + 2 * e < a.H)
-          *(SMLM_GLOBAL f32x4*)(out + (int64_t)(t + j * 32) * a.H + hh + i * 32 + 2 * e) =
-              f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+      for (int i = 0; i < IA; ++i) v[i] = acc[i][j][e];
+      if (row < rows && col < wide) *(SMLM_GLOBAL sums*)(out + (int64_t)row * ld + col) = v;
+    }
+  }
 }
 
 // dw's rows of a piece of the vocabulary.
@@ -399,14 +466,14 @@ template <int DT>
 __global__ __launch_bounds__(256, 1) void loss_dw_kernel(LossTileArgs a) {
   constexpr int WA = 2, IA = 4, WB = 2, JB = 4;
   typedef GemmShape<WA, IA, true, WB, JB, true> S;
-  __shared__ __align__(16) uint16_t lds[2 * S::kStage];
+  __shared__ __align__(16) uint16_t lds[kGemmStages * S::kStage];
   const int n = uload(a.rows.count, 0);
   const LossUnit u = loss_unit((a.H + S::kA - 1) / S::kA, (a.v1 - a.v0 + S::kB - 1) / S::kB);
   if (!u.any) return;
   f32x16 acc[IA][JB];
   loss_zero(acc);
   const int first_h = u.rows * S::kA, first_v = u.other * S::kB;
-  gemm_tile<DT, WA, IA, true, WB, JB, true>(acc, lds, GemmOperand{loss_x(a, n), a.H, n}, first_h, GemmOperand{a.g, a.ldg, n},
+  GemmTile<DT, WA, IA, true, WB, JB, true>::run(acc, lds, GemmOperand{loss_x(a, n), a.H, n}, first_h, GemmOperand{a.g, a.ldg, n},
                                             first_v, 0, n);
   const float unit = uload(a.rows.unit, 0);
 #pragma unroll
@@ -416,7 +483,7 @@ __global__ __launch_bounds__(256, 1) void loss_dw_kernel(LossTileArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hh = first_h + (wave / WB) * IA * 32, v = a.v0 + first_v + (wave % WB) * JB * 32;
   loss_lds_free();
-  loss_store<DT>(acc, lds + wave * IA * JB * 1024, a.dw + (int64_t)v * a.H + hh, a.H, a.v1 - v, a.H - hh);
+  loss_store_across<DT>(acc, lds + wave * IA * JB * 1024, a.dw + (int64_t)v * a.H + hh, a.H, a.v1 - v, a.H - hh);
 }
 
 struct LossRefsArgs {
@@ -544,10 +611,11 @@ __global__ __launch_bounds__(1024) void loss_means_kernel(LossMeansArgs a) {
 
 struct LossDxFoldArgs {
   LossRows rows;
-  const float* part;  // [splits][n, H]
+  const float* sums;  // [n, H]
+  const float* cut;   // [parts][tile]
   uint16_t* dx;       // [T, H]
   const uint16_t* w;  // [V, H]
-  int T, H, few, most_splits;
+  int T, H, few, stages;
   // of exponentials (KEPT): the rows' coefficients are found here
   const float* grad;         // [T], or [P]
   const int32_t* partition;  // [P + 1] or NULL
@@ -558,7 +626,8 @@ struct LossDxFoldArgs {
 template <int DT, bool KEPT>
 __global__ __launch_bounds__(256) void loss_dx_fold_kernel(LossDxFoldArgs a) {
   const int n = uload(a.rows.count, 0), lane = threadIdx.x & 63, tile = a.few ? kLossFewRows : kLossRows;
-  const int splits = loss_splits((n + tile - 1) / tile, (a.H + 255) / 256, a.most_splits);
+  const int row_tiles = (n + tile - 1) / tile, h_tiles = (a.H + 255) / 256;
+  const LossCuts cuts = loss_cuts(row_tiles * h_tiles, a.stages, a.few);
   const int t = (int)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= a.T) return;
   const int i = a.rows.number[t];
@@ -588,8 +657,10 @@ __global__ __launch_bounds__(256) void loss_dx_fold_kernel(LossDxFoldArgs a) {
     f32x4 lo = {0.f, 0.f, 0.f, 0.f}, hi = lo;
     float f[8];
     unpack8<DT>(ldg16(w + c), f);
-    for (int s = 0; s < splits; ++s) {
-      const float* p = a.part + ((int64_t)s * n + i) * a.H + c;
+    const int at = loss_tile_number(i / tile, c >> 8, row_tiles, h_tiles) - cuts.whole;
+    const float* p = at < 0 ? a.sums + (int64_t)i * a.H + c
+                            : a.cut + ((int64_t)at * cuts.parts * tile + i % tile) * 256 + (c & 255);
+    for (int s = 0; s < (at < 0 ? 1 : cuts.parts); ++s, p += tile * 256) {
       lo += ldg_f4(p);
       hi += ldg_f4(p + 4);
     }
