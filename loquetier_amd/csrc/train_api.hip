@@ -107,6 +107,7 @@ size_t loss_carve(void* base, int T, int H, int V, int what, LossSpace* s) {
     k.take(s->at_label, 4 * (size_t)s->pad);
     k.take(s->rows.ref, 4 * t);
     k.take(s->rows.turn, 4 * t);
+    k.take(s->rows.moved, 4 * (t / 16 + 1));
   } else {
     k.take(s->rows.number, 4 * t);
     k.take(s->rows.coef, 4 * t);
