@@ -29,7 +29,12 @@ int loss_check(int T, int H, int V, int dtype) {
     return SMLM_ERR_LIMIT;  // (workgroups)
   return SMLM_OK;
 }
-bool loss_few(int T) { return T <= kLossFewRows; }
+// Tiles of 64 rows, two workgroups a compute unit, where rows or tiles of 256 are few: 128 tiles leave half of the card idle.  us, tiles of
+// 256 rows / of 64, loss and gradient (4096 columns): 100 rows of 32000 entries (125 tiles) 235 / 193, 200 of 8000 (32) 169 / 115, 1000 of 8000
+// (128) 199 / 175; 1000 of 16000 (252) 282 / 310, 500 of 64000 (500) 576 / 713.
+bool loss_few(int T, int V) {
+  return T <= kLossFewRows || (int64_t)ceil_div(T, kLossRows) * ceil_div(V, kLossTileV) <= 128;
+}
 // Vocabulary entries a piece: whole tiles, as many in each.
 int loss_piece(int T, int V) {
   const int64_t pieces = (2 * (int64_t)(T > 0 ? T : 1) * V + kLossPieceBytes - 1) / kLossPieceBytes;
@@ -41,8 +46,7 @@ int loss_stages(int T, int V) {
   return ceil_div(piece < V ? piece : V, kGemmK);
 }
 // Parts of cut tiles, whatever the number of labelled rows; units of dx.
-int loss_parts(int T, int H, int stages, int* most_units) {
-  const bool few = loss_few(T);
+int loss_parts(int T, int H, int stages, bool few, int* most_units) {
   int parts = 0, units = 0;
   for (int r = 1; r <= ceil_div(T, few ? kLossFewRows : kLossRows); ++r) {
     const LossCuts c = loss_cuts(r * ceil_div(H, 256), stages, few);
@@ -72,7 +76,7 @@ struct LossTaker {
 };
 void loss_take_dx(LossTaker& k, int T, int H, int V, LossSpace* s) {
   k.take(s->dx, 4 * (size_t)T * H);
-  k.take(s->cut, 4 * (size_t)loss_parts(T, H, loss_stages(T, V), nullptr) * 256 * (loss_few(T) ? kLossFewRows : kLossRows));
+  k.take(s->cut, 4 * (size_t)loss_parts(T, H, loss_stages(T, V), loss_few(T, V), nullptr) * 256 * (loss_few(T, V) ? kLossFewRows : kLossRows));
 }
 // What the forward keeps for the gradient of x: its sums, and what the fold needs.
 size_t loss_keep(void* base, int T, int H, int V, LossSpace* s) {
@@ -101,7 +105,7 @@ size_t loss_carve(void* base, int T, int H, int V, int what, LossSpace* s) {
   k.take(s->rows.x, 2 * t * H);
   s->pad = round_up(T, 64);
   s->piece = what == 0 ? round_up(V, kLossTileV) : loss_piece(T, V);
-  s->parts = s->piece / kLossTileV * (loss_few(T) ? 4 : 2);
+  s->parts = s->piece / kLossTileV * (loss_few(T, V) ? 4 : 2);
   if (what == 0 || what == 4) {
     k.take(s->part, 8 * (size_t)s->parts * s->pad);
     k.take(s->at_label, 4 * (size_t)s->pad);
@@ -134,7 +138,7 @@ int loss_logits(int mode, bool f16, bool few, dim3 grid, hipStream_t st, const L
 }
 int loss_dx(bool f16, bool few, hipStream_t st, const LossTileArgs& a) {
   int most = 0;
-  loss_parts(a.T, a.H, a.stages, &most);
+  loss_parts(a.T, a.H, a.stages, few, &most);
   const dim3 grid = loss_grid(most), bl(256);
   if (few)
     return f16 ? launch(loss_dx_kernel<SMLM_DTYPE_F16, true>, grid, bl, st, a) : launch(loss_dx_kernel<SMLM_DTYPE_BF16, true>, grid, bl, st, a);
@@ -174,7 +178,7 @@ SMLM_API int smlm_vocab_loss_fwd(float* loss, float* lse, float* means, float* w
     LossTileArgs a{};
     a.rows = s.rows, a.x = ga.x, a.w = reinterpret_cast<const uint16_t*>(w), a.part = s.part, a.at_label = s.at_label;
     a.g = s.g, a.dx = s.dx, a.T = T, a.H = H, a.V = V, a.pad = s.pad, a.ldg = s.piece, a.cut = s.cut, a.stages = loss_stages(T, V), a.turned = 1;
-    const bool few = loss_few(T), f16 = dtype == SMLM_DTYPE_F16;
+    const bool few = loss_few(T, V), f16 = dtype == SMLM_DTYPE_F16;
     for (int v0 = 0; v0 < V; v0 += s.piece) {
       a.v0 = v0, a.v1 = V - v0 < s.piece ? V : v0 + s.piece, a.add = v0 > 0;
       const int v_tiles = ceil_div(a.v1 - v0, kLossTileV), parts = v_tiles * (few ? 4 : 2);
@@ -206,7 +210,7 @@ SMLM_API int smlm_vocab_loss_bwd_kept(void* dx, const float* grad, const void* k
   if (!aligned16(dx) || !aligned16(kept) || !aligned16(w)) return SMLM_ERR_ALIGN;
   LossSpace s{};
   if (kept_bytes < loss_keep(const_cast<void*>(kept), T, H, V, &s)) return SMLM_ERR_WORKSPACE;
-  const LossDxFoldArgs fa{s.rows, s.dx, s.cut, reinterpret_cast<uint16_t*>(dx), reinterpret_cast<const uint16_t*>(w), T, H, loss_few(T),
+  const LossDxFoldArgs fa{s.rows, s.dx, s.cut, reinterpret_cast<uint16_t*>(dx), reinterpret_cast<const uint16_t*>(w), T, H, loss_few(T, V),
                           loss_stages(T, V), grad, partition, weight, P};
   const dim3 grid((unsigned)ceil_div(T, 4)), bl(256);
   hipStream_t st = (hipStream_t)stream;
@@ -225,7 +229,7 @@ SMLM_API int smlm_vocab_loss_bwd(void* dx, void* dw, const float* grad, const fl
   LossSpace s{};
   if (workspace_bytes < loss_carve(workspace, T, H, V, (dx ? 1 : 0) | (dw ? 2 : 0), &s)) return SMLM_ERR_WORKSPACE;
   hipStream_t st = (hipStream_t)stream;
-  const bool f16 = dtype == SMLM_DTYPE_F16, few = loss_few(T);
+  const bool f16 = dtype == SMLM_DTYPE_F16, few = loss_few(T, V);
   const LossScanArgs sa{s.rows, labels, const_cast<float*>(loss), const_cast<float*>(lse), grad, partition, weight, T, V, P, f16, 1};
   LOSS_TRY(launch(loss_scan_kernel<true>, dim3(1), dim3(kLossScanThreads), st, sa));
   const LossGatherArgs ga{s.rows, reinterpret_cast<const uint16_t*>(x), T, H};

@@ -35,7 +35,7 @@ namespace smlm {
 
 constexpr int kLossTileV = 256;   // vocabulary entries a workgroup
 constexpr int kLossRows = 256;    // rows a workgroup where there are many
-constexpr int kLossFewRows = 64;  // ... and where there are few (kLossFew)
+constexpr int kLossFewRows = 64;  // ... and where rows or tiles are few (FEW)
 constexpr int kLossScanThreads = 1024;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -288,7 +288,7 @@ constexpr float kLossAbove = DT == SMLM_DTYPE_F16 ? 0.0f : 60.0f;
 template <int DT>
 constexpr float kLossBias = DT == SMLM_DTYPE_F16 ? 15.0f : 0.0f;  // fp16 entries are 2^15 times as large, and so are their sums
 
-// The logits' tiles.  FEW: one tile of kLossFewRows rows holds all of them.
+// The logits' tiles.
 template <int DT, bool FEW, int MODE>
 __global__ __launch_bounds__(256, FEW ? 2 : 1) void loss_logits_kernel(LossTileArgs a) {
   constexpr int WA = FEW ? 4 : 2, IA = FEW ? 2 : 4, WB = FEW ? 1 : 2, JB = FEW ? 2 : 4;

@@ -83,7 +83,9 @@ def check(x, w, labels, partition=None, want_w=True, grad=None):
 
 @pytest.mark.parametrize("dt", [FP16, BF16])
 @pytest.mark.parametrize("T,H,V", [(1, 64, 100), (1, 8, 1), (3, 72, 257), (33, 512, 2000), (64, 128, 300), (65, 128, 300), (130, 200, 1023),
-                                   (256, 64, 256), (257, 264, 513), (300, 1032, 777), (600, 256, 4097)])
+                                   (256, 64, 256), (257, 264, 513), (300, 1032, 777), (600, 256, 4097),
+                                   # (tiles of 256 rows: enough of them)
+                                   (513, 200, 20000), (1300, 136, 6000), (257, 8, 33001)])
 def test_rows_and_gradients(T, H, V, dt):
     x, w, labels = make(T, H, V, dt, T + V)
     check(x, w, labels)
