@@ -301,7 +301,14 @@ __global__ __launch_bounds__(256, FEW ? 2 : 1) void loss_logits_kernel(LossTileA
   loss_zero(acc);
   const int first_v = a.v0 + u.other * kLossTileV, first_t = u.rows * S::kB;
   const GemmOperand w{a.w, a.H, a.V}, x{loss_x(a, n), a.H, n};
-  GemmTile<DT, WA, IA, false, WB, JB, false>::run(acc, lds, w, first_v, x, first_t, 0, a.H);
+  // Where w comes from HBM at its rate (few rows), neighbouring workgroups begin at different columns: rows of w are often a multiple of
+  // 4 KiB apart, and all workgroups at one column meet in few channels.  (200 rows against 128256 of 4096: 286 us, 254 so; with many
+  // rows x is what workgroups at one column share.)
+  const int row_tiles = (n + S::kB - 1) / S::kB;
+  const int turn = row_tiles * S::kB <= 256 ? (u.other & 15) * (a.H >> 4) / kGemmK * kGemmK : 0;
+#pragma unroll 1
+  for (int s = 0; s < 2; ++s)
+    GemmTile<DT, WA, IA, false, WB, JB, false>::run(acc, lds, w, first_v, x, first_t, s ? 0 : turn, s ? turn : a.H);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
   const int v = first_v + (wave / WB) * IA * 32, t = first_t + (wave % WB) * JB * 32 + (lane & 31);
   const bool ends = v + IA * 32 > a.v1;  // the vocabulary ends inside the wave's part
