@@ -17,16 +17,16 @@
 // multiply-add, divisions and roots rounded correctly): a code's step is 2^24 times a float's, so the same step written in tensor
 // expressions gives the same codes, not others here and there.
 //
-// Bound by HBM: 22 to 30 bytes an element with float states and 16-bit weights, 10 to 18 with 8-bit ones.  A wave takes four blocks
-// of 256 in a row, all their loads on their way before the first is used; tables of a call travel in a launch's arguments, as
-// put_words_kernel's do.
+// Bound by HBM: 22 to 30 bytes an element with float states and 16-bit weights, 10 to 18 with 8-bit ones.  A wave takes a block of 256:
+// few registers, so many waves' loads are on their way.  (Four blocks a wave with all their loads ahead, two, one, us: 80 million
+// bf16 weights with float ones, float states 455, 439, 435 (5.5 TB/s); e4m3 states 343, 286, 271 (5.3 TB/s).)  The tables of a call
+// travel in launches' arguments, as put_words_kernel's do.
 #pragma once
 #include "add_rms_norm.hpp"
 
 namespace smlm {
 
 constexpr int kAdamBlock = 256;  // elements that share a scale
-constexpr int kAdamRun = 4;      // blocks a wave takes
 constexpr int kAdamF32 = 2;      // (element type of weights, after SMLM_DTYPE_*)
 
 // What a step needs of a tensor; 64 bytes, read by a wave at once.
@@ -159,6 +159,13 @@ __device__ __forceinline__ f32x4 adam_from8(uint32_t c, float s) {
   return f32x4{a[0] * s, a[1] * s, b[0] * s, b[1] * s};
 }
 
+// x / s, correctly rounded, from the correctly rounded inv = 1 / s: the remainder of the first guess corrects it (Markstein's
+// theorem; x / s is at most 448 and s is normal).  s 0 with inv 0: 0, and NaN of a NaN.
+__device__ __forceinline__ float adam_divide(float x, float s, float inv) {
+  const float q = x * inv;
+  return __builtin_fmaf(__builtin_fmaf(-q, s, x), inv, q);
+}
+
 // The last tensor that begins at block b or before it (empty ones begin where the next does): 64 guesses a round.
 __device__ __forceinline__ int adam_find(const AdamTensor* table, int n, uint32_t b, int lane) {
   int lo = 0, hi = n;  // table[lo].first <= b; the answer lies in [lo, hi)
@@ -176,85 +183,57 @@ template <int PT, bool EIGHT, bool MASTER>
 __global__ __launch_bounds__(256) void adam_kernel(AdamArgs a) {
 #pragma clang fp contract(off)
   const int lane = threadIdx.x & 63;
-  const int64_t b0 = ((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kAdamRun;
-  if (b0 >= a.blocks) return;
-  int ti = __builtin_amdgcn_readfirstlane(adam_find(a.table, a.n_tensors, (uint32_t)b0, lane));
-  f32x4 p[kAdamRun], g[kAdamRun], w[kAdamRun], m[kAdamRun], v[kAdamRun];
-  uint32_t mc[kAdamRun], vc[kAdamRun];
-  float ms[kAdamRun], vs[kAdamRun];
-  int tensor[kAdamRun], left[kAdamRun];
+  const int64_t b = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (b >= a.blocks) return;
+  const AdamTensor* t = a.table + __builtin_amdgcn_readfirstlane(adam_find(a.table, a.n_tensors, (uint32_t)b, lane));
+  if (!t->g) return;
+  const int64_t in = (b - t->first) * kAdamBlock + lane * 4, at = b * kAdamBlock + lane * 4, rest = t->n - in;
+  const int left = rest >= 4 ? 4 : rest > 0 ? (int)rest : 0;
+  f32x4 m, v, w, r, p = adam_load<PT>(t->p, in, left, t->plain);
+  const f32x4 g = adam_load<PT>(t->g, in, left, t->plain);
+  if (MASTER) w = *(const SMLM_GLOBAL f32x4*)(a.master + at);
+  if (EIGHT) {
+    m = adam_from8(*((const SMLM_GLOBAL uint32_t*)a.m + (at >> 2)), *((const SMLM_GLOBAL float*)a.m_scale + b));
+    v = adam_from8(*((const SMLM_GLOBAL uint32_t*)a.v + (at >> 2)), *((const SMLM_GLOBAL float*)a.v_scale + b));
+    v *= v;
+  } else {
+    m = *(const SMLM_GLOBAL f32x4*)((const float*)a.m + at);
+    v = *(const SMLM_GLOBAL f32x4*)((const float*)a.v + at);
+  }
+  if (MASTER) {
+    const f32x4 rounded = adam_round<PT>(w);
 #pragma unroll
-  for (int u = 0; u < kAdamRun; ++u) {
-    const int64_t b = b0 + u;
-    left[u] = 0;
-    if (b >= a.blocks) continue;
-    while (ti + 1 < a.n_tensors && a.table[ti + 1].first <= (uint32_t)b) ti = __builtin_amdgcn_readfirstlane(ti + 1);
-    tensor[u] = ti;
-    const AdamTensor* t = a.table + ti;
-    if (!t->g) continue;
-    const int64_t in = (b - t->first) * kAdamBlock + lane * 4, rest = t->n - in;
-    left[u] = rest >= 4 ? 4 : rest > 0 ? (int)rest : 0;
-    p[u] = adam_load<PT>(t->p, in, left[u], t->plain);
-    g[u] = adam_load<PT>(t->g, in, left[u], t->plain);
-    const int64_t at = b * kAdamBlock + lane * 4;
-    if (MASTER) w[u] = *(const SMLM_GLOBAL f32x4*)(a.master + at);
-    if (EIGHT) {
-      mc[u] = *((const SMLM_GLOBAL uint32_t*)a.m + (at >> 2));
-      vc[u] = *((const SMLM_GLOBAL uint32_t*)a.v + (at >> 2));
-      ms[u] = *((const SMLM_GLOBAL float*)a.m_scale + b);
-      vs[u] = *((const SMLM_GLOBAL float*)a.v_scale + b);
-    } else {
-      m[u] = *(const SMLM_GLOBAL f32x4*)((const float*)a.m + at);
-      v[u] = *(const SMLM_GLOBAL f32x4*)((const float*)a.v + at);
-    }
+    for (int e = 0; e < 4; ++e) p[e] = rounded[e] == p[e] ? w[e] : p[e];
   }
 #pragma unroll
-  for (int u = 0; u < kAdamRun; ++u) {
-    const int64_t b = b0 + u;
-    if (b >= a.blocks) continue;
-    const AdamTensor* t = a.table + tensor[u];
-    if (!t->g) continue;
-    const int64_t at = b * kAdamBlock + lane * 4, in = (b - t->first) * kAdamBlock + lane * 4;
-    if (EIGHT) {
-      m[u] = adam_from8(mc[u], ms[u]);
-      v[u] = adam_from8(vc[u], vs[u]);
-      v[u] *= v[u];
-    }
-    f32x4 r;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float x = p[u][e];
-      const float gr = g[u][e];
-      if (MASTER) x = adam_round<PT>(w[u])[e] == x ? w[u][e] : x;
-      m[u][e] = t->b1 * m[u][e] + t->nb1 * gr;
-      v[u][e] = t->b2 * v[u][e] + t->nb2 * gr * gr;
-      r[e] = EIGHT ? sqrtf(v[u][e]) : __builtin_amdgcn_sqrtf(v[u][e]);
-      x -= t->decay * x;
-      p[u][e] = x - t->size * m[u][e] * __builtin_amdgcn_rcpf(r[e] * t->root + t->eps);
-      if (e >= left[u]) m[u][e] = v[u][e] = r[e] = p[u][e] = 0.0f;  // (past the tensor's end: zeros, as the states began)
-    }
-    adam_store<PT>(t->p, in, left[u], t->plain, p[u]);
-    if (MASTER) *(SMLM_GLOBAL f32x4*)(a.master + at) = p[u];
-    if (EIGHT) {
-      float most_m = 0.0f, most_r = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) most_m = max_or_nan(most_m, fabsf(m[u][e])), most_r = max_or_nan(most_r, r[e]);
-      float mi, ri;
-      const float sm = scale8(wave_max(most_m), mi), sr = scale8(wave_max(most_r), ri);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        m[u][e] = mi == 0.0f ? m[u][e] * 0.0f : m[u][e] / sm;  // (0 of 0; of a NaN, NaN)
-        const float q = ri == 0.0f ? r[e] * 0.0f : r[e] / sr;
-        r[e] = r[e] > 0.0f && q < 0x1p-9f && ri != 0.0f ? 0x1p-9f : q;
-      }
-      *((SMLM_GLOBAL uint32_t*)a.m + (at >> 2)) = pack8(m[u][0], m[u][1], m[u][2], m[u][3]);
-      *((SMLM_GLOBAL uint32_t*)a.v + (at >> 2)) = pack8(r[0], r[1], r[2], r[3]);
-      if (lane == 0) a.m_scale[b] = sm, a.v_scale[b] = sr;
-    } else {
-      *(SMLM_GLOBAL f32x4*)((float*)a.m + at) = m[u];
-      *(SMLM_GLOBAL f32x4*)((float*)a.v + at) = v[u];
-    }
+  for (int e = 0; e < 4; ++e) {
+    m[e] = t->b1 * m[e] + t->nb1 * g[e];
+    v[e] = t->b2 * v[e] + t->nb2 * g[e] * g[e];
+    r[e] = EIGHT ? sqrtf(v[e]) : __builtin_amdgcn_sqrtf(v[e]);
+    p[e] -= t->decay * p[e];
+    p[e] -= t->size * m[e] * __builtin_amdgcn_rcpf(r[e] * t->root + t->eps);
+    if (e >= left) m[e] = v[e] = r[e] = p[e] = 0.0f;  // (past the tensor's end: zeros, as the states began)
   }
+  adam_store<PT>(t->p, in, left, t->plain, p);
+  if (MASTER) *(SMLM_GLOBAL f32x4*)(a.master + at) = p;
+  if (!EIGHT) {
+    *(SMLM_GLOBAL f32x4*)((float*)a.m + at) = m;
+    *(SMLM_GLOBAL f32x4*)((float*)a.v + at) = v;
+    return;
+  }
+  float most_m = 0.0f, most_r = 0.0f, mi, ri;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) most_m = max_or_nan(most_m, fabsf(m[e])), most_r = max_or_nan(most_r, r[e]);
+  const float sm = scale8(wave_max(most_m), mi), sr = scale8(wave_max(most_r), ri);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    m[e] = adam_divide(m[e], sm, mi);
+    const float q = adam_divide(r[e], sr, ri);
+    r[e] = r[e] > 0.0f && q < 0x1p-9f && ri != 0.0f ? 0x1p-9f : q;
+  }
+  *((SMLM_GLOBAL uint32_t*)a.m + (at >> 2)) = pack8(m[0], m[1], m[2], m[3]);
+  *((SMLM_GLOBAL uint32_t*)a.v + (at >> 2)) = pack8(r[0], r[1], r[2], r[3]);
+  if (lane == 0) a.m_scale[b] = sm, a.v_scale[b] = sr;
 }
 
 }  // namespace smlm

@@ -14,10 +14,7 @@ int check_dtype(int dtype) { return dtype == SMLM_DTYPE_F16 || dtype == SMLM_DTY
 // ---- the loss over the vocabulary ----
 
 constexpr int kLossMaxDim = 1 << 22;           // H: a tile's rows stay inside a resource
-#ifndef LPB
-#define LPB 512
-#endif
-constexpr int64_t kLossPieceBytes = (int64_t)LPB << 20;  // of G at a time
+constexpr int64_t kLossPieceBytes = (int64_t)512 << 20;  // of exponentials, or of G, at a time
 
 int loss_check(int T, int H, int V, int dtype) {
   if (T < 0 || H <= 0 || V <= 0) return SMLM_ERR_ARG;
@@ -361,7 +358,7 @@ SMLM_API int smlm_adamw_step(const smlm_adamw* p, void* workspace, size_t worksp
     if (p->sizes[i] > 0 && !p->params[i]) return SMLM_ERR_ARG;
     blocks += (p->sizes[i] + kAdamBlock - 1) / kAdamBlock;
   }
-  if (blocks > ((int64_t)1 << 32) - 64) return SMLM_ERR_LIMIT;
+  if (blocks > ((int64_t)1 << 32) - 64) return SMLM_ERR_LIMIT;  // (and so are the workgroups, four blocks each)
   if (blocks > 0 && (!p->exp_avg || !p->exp_avg_sq || (eight && (!p->avg_scale || !p->sq_scale)))) return SMLM_ERR_ARG;
   if (!aligned16(p->exp_avg) || !aligned16(p->exp_avg_sq) || !aligned16(p->master) || !aligned16(workspace)) return SMLM_ERR_ALIGN;
   if (workspace_bytes < (size_t)p->n_tensors * sizeof(AdamTensor)) return SMLM_ERR_WORKSPACE;
@@ -378,7 +375,7 @@ SMLM_API int smlm_adamw_step(const smlm_adamw* p, void* workspace, size_t worksp
   }
   if (blocks == 0) return SMLM_OK;
   const AdamArgs a{table, p->exp_avg, p->exp_avg_sq, p->avg_scale, p->sq_scale, p->master, p->n_tensors, blocks};
-  const dim3 grid((unsigned)((blocks + 4 * kAdamRun - 1) / (4 * kAdamRun)));
+  const dim3 grid((unsigned)((blocks + 3) / 4));
   if (f32) return launch_adam<kAdamF32>(eight, false, grid, st, a);
   return p->dtype == SMLM_DTYPE_F16 ? launch_adam<SMLM_DTYPE_F16>(eight, p->master != nullptr, grid, st, a)
                                     : launch_adam<SMLM_DTYPE_BF16>(eight, p->master != nullptr, grid, st, a);
