@@ -148,7 +148,7 @@ struct LinearCrossEntropy : public Function<LinearCrossEntropy> {
     const Tensor mem = bytes(need, x);
     check(lib.loss_fwd((float*)loss.data_ptr(), (float*)lse.data_ptr(), P ? (float*)means.data_ptr() : nullptr,
                        P ? (float*)weight.data_ptr() : nullptr, keep ? kept.data_ptr() : nullptr, keep, x.data_ptr(), w.data_ptr(), (const int64_t*)labels.data_ptr(),
-                       P ? (const int32_t*)partition->data_ptr() : nullptr, P, mem.data_ptr(), need, T, H, V, dtype_code(x), stream(x)),
+                       partition ? (const int32_t*)partition->data_ptr() : nullptr, P, mem.data_ptr(), need, T, H, V, dtype_code(x), stream(x)),
           "linear_cross_entropy");
     ctx->save_for_backward({x, w, labels, loss, lse, partition ? *partition : Tensor(), weight, kept});
     ctx->saved_data["partitioned"] = (bool)partition;

@@ -14,7 +14,10 @@ int check_dtype(int dtype) { return dtype == SMLM_DTYPE_F16 || dtype == SMLM_DTY
 // ---- the loss over the vocabulary ----
 
 constexpr int kLossMaxDim = 1 << 22;           // H: a tile's rows stay inside a resource
-constexpr int64_t kLossPieceBytes = (int64_t)512 << 20;  // of exponentials, or of G, at a time
+// Of exponentials, or of G, at a time: every piece ends the grid twice and adds to dx's sums.  Loss and dx, us, pieces of 128 / 256 / 512 / 1024
+// MiB (4096 columns): 4096 rows of 128256 entries 7839 / 7347 / 7246 / 7179, 8192 rows 16225 / 15208 / 14607 / 14479, 8192 of 32000 4070 / 3806 /
+// 3698 / 3698 (one piece from 512 on).
+constexpr int64_t kLossPieceBytes = (int64_t)512 << 20;
 
 int loss_check(int T, int H, int V, int dtype) {
   if (T < 0 || H <= 0 || V <= 0) return SMLM_ERR_ARG;
@@ -168,7 +171,7 @@ SMLM_API int smlm_vocab_loss_fwd(float* loss, float* lse, float* means, float* w
     LossSpace s{};
     if (kept && kept_bytes < loss_keep(kept, T, H, V, &s)) return SMLM_ERR_WORKSPACE;
     if (workspace_bytes < loss_carve(workspace, T, H, V, kept ? 4 : 0, &s)) return SMLM_ERR_WORKSPACE;
-    const LossScanArgs sa{s.rows, labels, loss, lse, nullptr, P ? partition : nullptr, nullptr, T, V, P, 0, kept != nullptr};
+    const LossScanArgs sa{s.rows, labels, loss, lse, nullptr, partition, nullptr, T, V, P, 0, kept != nullptr};
     LOSS_TRY(launch(loss_scan_kernel<false>, dim3(1), dim3(kLossScanThreads), st, sa));
     const LossGatherArgs ga{s.rows, reinterpret_cast<const uint16_t*>(x), T, H};
     LOSS_TRY(launch(loss_gather_kernel, dim3((unsigned)ceil_div(T, 4)), dim3(256), st, ga));
@@ -265,7 +268,13 @@ int launch_add_rms(hipStream_t st, const AddRmsArgs& a) {
     const dim3 grid((unsigned)a.rows);
     return a.cols <= 8192 ? launch(add_rms_kernel<DT, 4, 4>, grid, bl, st, a) : launch(add_rms_kernel<DT, 4, 8>, grid, bl, st, a);
   }
-  if (a.rows <= 1024 && a.cols > 1024) return launch(add_rms_kernel<DT, 4, 2>, dim3((unsigned)a.rows), bl, st, a);
+  // Four waves a row of more than 1024 columns where rows are few.  us, a wave a row / four, 2048 columns: 1 row 2.28 / 1.95, 256 3.36 / 2.89,
+  // 512 3.73 / 3.36, 1024 4.23 / 4.30, 2048 6.7 / 7.3; 4096 columns: 1 row 3.03 / 2.16, 256 4.73 / 3.39, 512 4.95 / 5.15, 1024 6.7 / 7.4.  (1024
+  // columns: 8 rows 2.21 / 2.20, 256 2.35 / 2.70.)
+  if (a.cols > 1024 && (int64_t)a.rows * a.cols <= (1 << 20)) {
+    const dim3 grid((unsigned)a.rows);
+    return a.cols <= 2048 ? launch(add_rms_kernel<DT, 4, 1>, grid, bl, st, a) : launch(add_rms_kernel<DT, 4, 2>, grid, bl, st, a);
+  }
   const dim3 grid((unsigned)ceil_div(a.rows, 4));
   if (a.cols <= 512) return launch(add_rms_kernel<DT, 1, 1>, grid, bl, st, a);
   if (a.cols <= 1024) return launch(add_rms_kernel<DT, 1, 2>, grid, bl, st, a);

@@ -1524,7 +1524,7 @@ def linear_cross_entropy(loss: torch.Tensor, lse: torch.Tensor, x: torch.Tensor,
         ws = _workspace(dev, _lib.size_query("smlm_vocab_loss_workspace_size", T, H, V, 0 if kept is None else 4), workspace)
         rc = _lib.load().smlm_vocab_loss_fwd(_ptr(loss), _ptr(lse), _ptr(means), _ptr(weight), _ptr(kept),
                                              0 if kept is None else kept.numel(), _ptr(x), _ptr(w), _ptr(labels),
-                                             _ptr(partition) if P else None, P, ws.data_ptr(), ws.numel(), T, H, V, code, _stream(dev))
+                                             _ptr(partition), P, ws.data_ptr(), ws.numel(), T, H, V, code, _stream(dev))
     _lib.check(rc, "linear_cross_entropy")
 
 

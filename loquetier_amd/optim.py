@@ -54,7 +54,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("state_bits must be 8 or 32")
         self.state_bits, self.master = state_bits, bool(master)
         self._sets: List[_Set] = []
-        self._rates: Dict[torch.device, Tuple[tuple, torch.Tensor]] = {}
+        # what was written, and the tables: the newest, and smaller ones that a captured step may read
+        self._rates: Dict[torch.device, Tuple[tuple, List[torch.Tensor]]] = {}
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def add_param_group(self, param_group: Dict[str, Any]) -> None:
@@ -96,10 +97,12 @@ class AdamW(torch.optim.Optimizer):
                 continue
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("rates changed while a graph is captured: call update_rates before")
-            words = struct.pack(f"{5 * len(now)}f", *[v for row in now for v in row])
-            table = was[1] if was is not None and was[1].size(0) == len(now) else torch.empty(len(now), 5, device=dev)
-            kernel.put_words(table, words)
-            self._rates[dev] = (now, table)
+            tables = was[1] if was is not None else []
+            if not tables or tables[-1].size(0) != len(now):
+                tables.append(torch.empty(len(now), 5, device=dev))
+            for table in tables:
+                kernel.put_words(table, struct.pack(f"{table.numel()}f", *[v for row in now[:table.size(0)] for v in row]))
+            self._rates[dev] = (now, tables)
 
     @torch.no_grad()
     def step(self, closure: Optional[Callable[[], torch.Tensor]] = None):
@@ -114,12 +117,12 @@ class AdamW(torch.optim.Optimizer):
                 grads = [g if g is None else g.contiguous() for g in grads]
             if any(g is not None for g in grads):
                 t = s.tensors
-                kernel.adamw_step(s.params, grads, t["exp_avg"], t["exp_avg_sq"], t["step"], self._rates[s.params[0].device][1],
+                kernel.adamw_step(s.params, grads, t["exp_avg"], t["exp_avg_sq"], t["step"], self._rates[s.params[0].device][1][-1],
                                   s.group, t["avg_scale"], t["sq_scale"], t["master"], s.workspace)
         return loss
 
     def state_of(self, param: torch.Tensor) -> Dict[str, torch.Tensor]:
-        """A tensor's step count and averages (and float weights), as float tensors of its shape."""
+        """Copies of a tensor's step count and averages (and float weights), float tensors of its shape."""
         self._prepare()
         for s in self._sets:
             for i, p in enumerate(s.params):
@@ -127,7 +130,7 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 (a, b), t = s.span(i), s.tensors
                 first, last = a // kernel.ADAMW_BLOCK, -(-b // kernel.ADAMW_BLOCK)
-                values = lambda name, scale: (t[name][a:last * kernel.ADAMW_BLOCK].float() if scale is None else (
+                values = lambda name, scale: (t[name][a:last * kernel.ADAMW_BLOCK].clone() if scale is None else (
                     t[name][a:last * kernel.ADAMW_BLOCK].view(-1, kernel.ADAMW_BLOCK).float()
                     * scale[first:last, None]).flatten())[:b - a].view(p.shape)
                 out = dict(step=t["step"][i].clone(), exp_avg=values("exp_avg", t["avg_scale"]),
@@ -149,7 +152,10 @@ class AdamW(torch.optim.Optimizer):
         state = state_dict["state"]
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         if not state["sets"]:  # (saved before its first step)
-            self._sets = []
+            for s in self._sets:
+                for t in s.tensors.values():
+                    if t is not None:
+                        t.view(torch.uint8).zero_()
             return
         self._prepare()
         shape = lambda tensors: {n: None if t is None else (t.dtype, tuple(t.shape)) for n, t in tensors.items()}

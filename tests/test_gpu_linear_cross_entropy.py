@@ -160,10 +160,11 @@ def test_frozen_rows_and_kept_sums():
 
 
 @pytest.mark.parametrize("dt", [FP16, BF16])
-def test_references_move_from_piece_to_piece(dt):
-    """Logits that grow along the vocabulary by far more than 16-bit exponents hold, so that every piece (128 MiB of exponentials) takes
-    the rows' reference along, in some rows; in others the first piece holds the largest."""
-    T, H, V = 600, 64, 250000
+@pytest.mark.parametrize("T", [600, 2400])
+def test_references_move_from_piece_to_piece(T, dt):
+    """Logits that grow along the vocabulary by far more than 16-bit exponents hold, so that every tile, and every piece (512 MiB of
+    exponentials: one, three), takes the rows' reference along, in some rows; in others the first holds the largest."""
+    H, V = 64, 250000
     g = torch.Generator().manual_seed(0)
     x, w = torch.randn(T, H, generator=g), 0.3 * torch.randn(V, H, generator=g)
     x[:, 0], x[:, 1] = 1.0, 0.0
@@ -171,7 +172,7 @@ def test_references_move_from_piece_to_piece(dt):
     x[1::3, 1] = -0.25
     w[:, 1] = torch.arange(V) * (300.0 / V)
     labels = torch.randint(0, V, (T,), generator=g)
-    labels[::2] = torch.randint(V - 2000, V, (300,), generator=g)
+    labels[::2] = torch.randint(V - 2000, V, (T // 2,), generator=g)
     x, w, labels = x.to(dt).cuda().requires_grad_(True), w.to(dt).cuda(), labels.cuda()
     out = linear_cross_entropy.apply(x, w, labels)
     dx, = torch.autograd.grad(out.sum(), x)
@@ -189,9 +190,9 @@ def test_references_move_from_piece_to_piece(dt):
 
 
 @pytest.mark.parametrize("dt", [FP16, BF16])
-def test_pieces_of_the_vocabulary(dt):
-    """G of more than one piece (128 MiB of it at a time)."""
-    T, V = 700, 100001
+@pytest.mark.parametrize("T,V", [(700, 100001), (2200, 300001)])
+def test_pieces_of_the_vocabulary(T, V, dt):
+    """G of one piece and of three (512 MiB of it at a time)."""
     x, w, labels = make(T, 64, V, dt, 5)
     x = x.requires_grad_(True)
     w = w.requires_grad_(True)
@@ -207,6 +208,85 @@ def test_pieces_of_the_vocabulary(dt):
     for got, a, b in ((dx, G, w.detach().double()), (dw, G.t().contiguous(), x.detach().double())):
         exact, bound = a @ b, a.abs() @ b.abs()
         assert ((got.double() - exact).abs() <= bound * (eps / 2 + 1e-5) + exact.abs() * eps / 2 + 1e-7).all()
+
+
+def test_no_partition_at_all():
+    """An edge alone: no row lies in a partition."""
+    x, w, labels = make(70, 64, 300, BF16)
+    part = torch.tensor([0], dtype=torch.int32, device="cuda")
+    loss, lse = torch.full((70,), 7.0, device="cuda"), torch.full((70,), 7.0, device="cuda")
+    K.linear_cross_entropy(loss, lse, x, w, labels, part)
+    assert not loss.any() and not lse.any()
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    out = linear_cross_entropy.apply(x, w, labels, part)
+    dx, dw = torch.autograd.grad(out.sum(), (x, w))
+    assert out.shape == (0,) and not dx.any() and not dw.any()
+
+
+def test_offsets_past_32_bits():
+    """A vocabulary's matrix of more than 4 GiB in one piece, and rows of more than 4 GiB, against products of chunks in float32."""
+    for T, H, V in ((300, 8192, 290000), (290000, 8192, 300)):
+        g = torch.Generator(device="cuda").manual_seed(T)
+        x = (torch.randn(T, H, generator=g, device="cuda", dtype=BF16)).requires_grad_(True)
+        w = (torch.randn(V, H, generator=g, device="cuda", dtype=BF16) * (1.0 / 64)).requires_grad_(True)
+        labels = torch.randint(0, V, (T,), generator=g, device="cuda")
+        out = linear_cross_entropy.apply(x, w, labels)
+        dx, dw = torch.autograd.grad(out.sum(), (x, w))
+        frozen, = torch.autograd.grad(linear_cross_entropy.apply(x, w.detach(), labels).sum(), x)
+        xd, wd = x.detach(), w.detach()
+        for rows in (slice(0, 40), slice(T - 40, T)):  # (whole rows of the gradient of x)
+            xr = xd[rows].float()
+            z = torch.cat([xr @ wd[i:i + 20000].float().t() for i in range(0, V, 20000)], 1)
+            lse = torch.logsumexp(z, 1)
+            at = torch.arange(40, device="cuda")
+            # (logits of size 1.4 sqrt(2): sums of 8192 products, 8192 2^-24 of |x||w| at most and both sides' error far less)
+            assert (out[rows] - (lse - z[at, labels[rows]])).abs().max() < 1e-3
+            G = torch.exp(z - lse[:, None])
+            G[at, labels[rows]] -= 1
+            exact = sum(G[:, i:i + 20000] @ wd[i:i + 20000].float() for i in range(0, V, 20000))
+            # |error| <= sum |G w| eps / 2 and its own rounding, and of exp(z - lse) 1e-3 of sum |p w|
+            bound = sum(G[:, i:i + 20000].abs() @ wd[i:i + 20000].float().abs() for i in range(0, V, 20000))
+            for got in (dx, frozen):
+                assert ((got[rows].float() - exact).abs() <= bound * (2.0 ** -8 + 1e-3) + exact.abs() * 2.0 ** -8 + 1e-6).all()
+        lse = torch.empty(T, device="cuda")
+        K.linear_cross_entropy(torch.empty_like(lse), lse, xd, wd, labels)
+        for cols in (slice(0, 40), slice(V - 40, V)):  # (whole rows of the gradient of w)
+            at = torch.arange(cols.start, cols.stop, device="cuda")
+            exact = bound = 0.0
+            for i in range(0, T, 20000):
+                xr = xd[i:i + 20000].float()
+                G = torch.exp(xr @ wd[cols].float().t() - lse[i:i + 20000, None]) - (labels[i:i + 20000, None] == at).float()
+                exact, bound = exact + G.t().contiguous() @ xr, bound + G.abs().t().contiguous() @ xr.abs()
+            assert ((dw[cols].float() - exact).abs() <= bound * (2.0 ** -8 + 1e-3) + exact.abs() * 2.0 ** -8 + 1e-6).all()
+
+
+def test_old_bytes_of_the_workspace():
+    """Nothing is read of a workspace, or of what is kept, before it is written."""
+    for T, H, V, labelled in ((70, 136, 300, 0.5), (700, 264, 1000, 0.7), (513, 200, 20000, 0.9)):
+        x, w, labels = make(T, H, V, BF16, 4, labelled)
+        got = []
+        for byte in (0, 255):
+            f = lambda *s: torch.empty(*s, device="cuda")
+            mem = lambda what: torch.full((K._lib.size_query("smlm_vocab_loss_workspace_size", T, H, V, what),), byte, dtype=torch.uint8, device="cuda")
+            L, st = K._lib.load(), torch.cuda.current_stream().cuda_stream
+            loss, lse, alone, lone_lse, g = f(T), f(T), f(T), f(T), torch.ones(T, device="cuda")
+            dx, dw, dx_alone, dx_kept = (torch.empty_like(t) for t in (x, w, x, x))
+            kept, ws = mem(5), mem(4)
+            p = lambda t: t.data_ptr()
+            rc = L.smlm_vocab_loss_fwd(p(loss), p(lse), None, None, p(kept), kept.numel(), p(x), p(w), p(labels), None, 0, p(ws), ws.numel(),
+                                       T, H, V, 1, st)
+            rc |= L.smlm_vocab_loss_bwd_kept(p(dx_kept), p(g), p(kept), kept.numel(), p(w), None, None, 0, T, H, V, 1, st)
+            w0, w3, w1 = mem(0), mem(3), mem(1)
+            rc |= L.smlm_vocab_loss_fwd(p(alone), p(lone_lse), None, None, None, 0, p(x), p(w), p(labels), None, 0, p(w0), w0.numel(),
+                                        T, H, V, 1, st)
+            rc |= L.smlm_vocab_loss_bwd(p(dx), p(dw), p(g), p(loss), p(lse), p(x), p(w), p(labels), None, None, 0, p(w3), w3.numel(),
+                                        T, H, V, 1, st)
+            rc |= L.smlm_vocab_loss_bwd(p(dx_alone), None, p(g), p(loss), p(lse), p(x), p(w), p(labels), None, None, 0, p(w1), w1.numel(),
+                                        T, H, V, 1, st)
+            assert rc == 0
+            got.append([loss, lse, alone, lone_lse, dx, dw, dx_alone, dx_kept])
+        for a, b in zip(*got):
+            assert torch.isfinite(a).all() and torch.equal(a, b)
 
 
 def test_small_gradients_in_fp16():
