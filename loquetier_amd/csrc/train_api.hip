@@ -78,6 +78,7 @@ void loss_take_dx(LossTaker& k, int T, int H, int V, LossSpace* s) {
   k.take(s->dx, 4 * (size_t)T * H);
   k.take(s->cut, 4 * (size_t)loss_parts(T, H, loss_stages(T, V), loss_few(T, V), nullptr) * 256 * (loss_few(T, V) ? kLossFewRows : kLossRows));
 }
+bool loss_twice(int T, int what) { return T <= kLossTwice && (what == 2 || what == 3); }
 // What the forward keeps for the gradient of x: its sums, and what the fold needs.
 size_t loss_keep(void* base, int T, int H, int V, LossSpace* s) {
   LossTaker k{reinterpret_cast<char*>(base)};
@@ -102,7 +103,8 @@ size_t loss_carve(void* base, int T, int H, int V, int what, LossSpace* s) {
     k.take(s->rows.share, 4 * t);
   }
   k.take(s->rows.row, 4 * t);
-  k.take(s->rows.x, 2 * t * H);
+  const size_t twice = loss_twice(T, what) ? 2 * kLossTwice : t;  // rows of x and G
+  k.take(s->rows.x, 2 * twice * H);
   s->pad = round_up(T, 64);
   s->piece = what == 0 ? round_up(V, kLossTileV) : loss_piece(T, V);
   s->parts = s->piece / kLossTileV * (loss_few(T, V) ? 4 : 2);
@@ -119,7 +121,7 @@ size_t loss_carve(void* base, int T, int H, int V, int what, LossSpace* s) {
     k.take(s->rows.own, 4 * t);
     k.take(s->rows.lost, 4 * t);
   }
-  if (what) k.take(s->g, 2 * t * s->piece);
+  if (what) k.take(s->g, 2 * twice * s->piece);
   if (what == 1 || what == 3) loss_take_dx(k, T, H, V, s);
   return k.off;
 }
@@ -173,7 +175,7 @@ SMLM_API int smlm_vocab_loss_fwd(float* loss, float* lse, float* means, float* w
     if (workspace_bytes < loss_carve(workspace, T, H, V, kept ? 4 : 0, &s)) return SMLM_ERR_WORKSPACE;
     const LossScanArgs sa{s.rows, labels, loss, lse, nullptr, partition, nullptr, T, V, P, 0, kept != nullptr};
     LOSS_TRY(launch(loss_scan_kernel<false>, dim3(1), dim3(kLossScanThreads), st, sa));
-    const LossGatherArgs ga{s.rows, reinterpret_cast<const uint16_t*>(x), T, H};
+    const LossGatherArgs ga{s.rows, reinterpret_cast<const uint16_t*>(x), T, H, 0};
     LOSS_TRY(launch(loss_gather_kernel, dim3((unsigned)ceil_div(T, 4)), dim3(256), st, ga));
     LossTileArgs a{};
     a.rows = s.rows, a.x = ga.x, a.w = reinterpret_cast<const uint16_t*>(w), a.part = s.part, a.at_label = s.at_label;
@@ -232,9 +234,11 @@ SMLM_API int smlm_vocab_loss_bwd(void* dx, void* dw, const float* grad, const fl
   const bool f16 = dtype == SMLM_DTYPE_F16, few = loss_few(T, V);
   const LossScanArgs sa{s.rows, labels, const_cast<float*>(loss), const_cast<float*>(lse), grad, partition, weight, T, V, P, f16, 1};
   LOSS_TRY(launch(loss_scan_kernel<true>, dim3(1), dim3(kLossScanThreads), st, sa));
-  const LossGatherArgs ga{s.rows, reinterpret_cast<const uint16_t*>(x), T, H};
-  LOSS_TRY(launch(loss_gather_kernel, dim3((unsigned)ceil_div(T, 4)), dim3(256), st, ga));
+  const int twice = loss_twice(T, (dx ? 1 : 0) | (dw ? 2 : 0));
+  const LossGatherArgs ga{s.rows, reinterpret_cast<const uint16_t*>(x), T, H, twice};
+  LOSS_TRY(launch(loss_gather_kernel, dim3((unsigned)ceil_div(twice ? 2 * kLossTwice : T, 4)), dim3(256), st, ga));
   LossTileArgs a{};
+  a.twice = twice;
   a.rows = s.rows, a.x = ga.x, a.w = reinterpret_cast<const uint16_t*>(w), a.g = s.g, a.dx = s.dx;
   a.dw = reinterpret_cast<uint16_t*>(dw), a.T = T, a.H = H, a.V = V, a.ldg = s.piece, a.cut = s.cut, a.stages = loss_stages(T, V);
   const int tile = few ? kLossFewRows : kLossRows, h_tiles = ceil_div(H, 256);

@@ -55,7 +55,7 @@ struct LossRows {
   float* share;      // [T] in the end: the part of them that is not the label's
   float* turn;       // [T] what the sums so far are multiplied with
   int32_t* moved;    // [T / 16] whether anything of sixteen rows' entries is to be turned
-  uint16_t* x;       // [n, H] the rows side by side, unless n == T
+  uint16_t* x;       // [n, H] the rows side by side, unless n == T; [64, H] where G is held twice
 };
 
 struct LossScanArgs {
@@ -150,18 +150,31 @@ __global__ __launch_bounds__(kLossScanThreads) void loss_scan_kernel(LossScanArg
   }
 }
 
+// Up to 32 rows, where dw is made: G is held as its rounding (rows 0 to 31 of 64) and what that took (32 to 63), both against the same rows of
+// x.  In dw a row of w meets one entry of size c, its label's, and rounding is one relative error of all its columns, of all a
+// partition's labels even; in a sum of many rows such errors are of random sign, here they would be the result's: 7 rows of 5304 columns
+// in fp16 3.2e-4 off for the 2.1e-4 of the output's own rounding.  The second half of a tile of 64 rows, and of a stage of
+// 64, is empty otherwise, so it costs nothing.
+constexpr int kLossTwice = 32;
+
 struct LossGatherArgs {
   LossRows rows;
   const uint16_t* x;
-  int T, H;
+  int T, H, twice;
 };
 // A wave a row.
 __global__ __launch_bounds__(256) void loss_gather_kernel(LossGatherArgs a) {
   const int n = uload(a.rows.count, 0), lane = threadIdx.x & 63;
-  if (n == a.T) return;
-  for (int i = (int)blockIdx.x * 4 + (threadIdx.x >> 6); i < n; i += (int)gridDim.x * 4) {
-    const uint16_t* from = a.x + (int64_t)a.rows.row[i] * a.H;
+  if (n == a.T && !a.twice) return;
+  for (int i = (int)blockIdx.x * 4 + (threadIdx.x >> 6); i < (a.twice ? 2 * kLossTwice : n); i += (int)gridDim.x * 4) {
+    const int at = a.twice ? i & (kLossTwice - 1) : i;
     uint16_t* to = a.rows.x + (int64_t)i * a.H;
+    if (at >= n) {
+      const u32x4 zero = {0u, 0u, 0u, 0u};
+      for (int c = lane * 8; c < a.H; c += 512) stg16(to + c, zero);
+      continue;
+    }
+    const uint16_t* from = a.x + (int64_t)a.rows.row[at] * a.H;
     for (int c = lane * 8; c < a.H; c += 512) stg16(to + c, ldg16(from + c));
   }
 }
@@ -180,6 +193,7 @@ struct LossTileArgs {
   int v0, v1, ldg;    // the piece of the vocabulary
   int stages, add;    // of a whole piece; add: to what is there of dx, turned (`turned`)
   int turned;
+  int twice;          // G is held twice (backward, up to kLossTwice rows)
 };
 
 __device__ __forceinline__ const uint16_t* loss_x(const LossTileArgs& a, int n) { return n == a.T ? a.x : a.rows.x; }
@@ -377,12 +391,24 @@ __global__ __launch_bounds__(256, FEW ? 2 : 1) void loss_logits_kernel(LossTileA
             }
         if (here && tj < n) a.rows.lost[tj] = lost;
       }
+      if (FEW && a.twice) {  // (the tile's first 32 rows are all: what lies in the others is made of them)
+#pragma unroll
+        for (int i = 0; i < IA; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float y = tj < n ? acc[i][0][e] : 0.0f;
+            const float took = y - Num<DT>::lo(pack2<DT>(y, 0.0f));
+            acc[i][0][e] = y, acc[i][JB - 1][e] = fabsf(took) < INFINITY ? took : 0.0f;  // (infinities stay what they are)
+          }
+        break;
+      }
     }
   }
   if (MODE != kLossSums) {
     loss_lds_free();
     const int row = first_t + (wave % WB) * JB * 32;
-    loss_store<DT>(acc, lds + wave * IA * JB * 1024, a.g + (int64_t)row * a.ldg + (v - a.v0), a.ldg, n - row, IA * 32);
+    loss_store<DT>(acc, lds + wave * IA * JB * 1024, a.g + (int64_t)row * a.ldg + (v - a.v0), a.ldg,
+                   FEW && MODE == kLossGrad && a.twice ? 2 * kLossTwice : n - row, IA * 32);
   }
 }
 
@@ -478,14 +504,14 @@ __global__ __launch_bounds__(256, 1) void loss_dw_kernel(LossTileArgs a) {
   constexpr int WA = 2, IA = 4, WB = 2, JB = 4;
   typedef GemmShape<WA, IA, true, WB, JB, true> S;
   __shared__ __align__(16) uint16_t lds[kGemmStages * S::kStage];
-  const int n = uload(a.rows.count, 0);
+  const int rows = uload(a.rows.count, 0), n = a.twice && rows ? 2 * kLossTwice : rows;
   const LossUnit u = loss_unit((a.H + S::kA - 1) / S::kA, (a.v1 - a.v0 + S::kB - 1) / S::kB);
   if (!u.any) return;
   f32x16 acc[IA][JB];
   loss_zero(acc);
   const int first_h = u.rows * S::kA, first_v = u.other * S::kB;
-  GemmTile<DT, WA, IA, true, WB, JB, true>::run(acc, lds, GemmOperand{loss_x(a, n), a.H, n}, first_h, GemmOperand{a.g, a.ldg, n},
-                                            first_v, 0, n);
+  GemmTile<DT, WA, IA, true, WB, JB, true>::run(acc, lds, GemmOperand{a.twice ? a.rows.x : loss_x(a, n), a.H, n}, first_h,
+                                            GemmOperand{a.g, a.ldg, n}, first_v, 0, n);
   const float unit = uload(a.rows.unit, 0);
 #pragma unroll
   for (int i = 0; i < IA; ++i)

@@ -210,6 +210,37 @@ def test_pieces_of_the_vocabulary(T, V, dt):
         assert ((got.double() - exact).abs() <= bound * (eps / 2 + 1e-5) + exact.abs() * eps / 2 + 1e-7).all()
 
 
+@pytest.mark.parametrize("dt", [FP16, BF16])
+@pytest.mark.parametrize("T,H,V,labelled", [(1, 64, 100, 1.0), (7, 1304, 805, 1.0), (32, 264, 1000, 1.0), (32, 264, 1000, 0.6), (9, 104, 156, 0.5)])
+def test_few_rows_keep_what_rounding_takes(T, H, V, labelled, dt):
+    """The vocabulary's gradient of up to 32 rows: entries of G are held in two numbers, off by (eps / 2)^2, so that the result's own
+    rounding is what is left (and the logits' error, of p)."""
+    x, w, labels = make(T, H, V, dt, T + H, labelled)
+    part = torch.tensor([0, T // 3, T - T // 4, T], dtype=torch.int32, device="cuda")
+    grad = torch.tensor([1.3, 0.7, 1.1], device="cuda")
+    w = w.requires_grad_(True)
+    out = linear_cross_entropy.apply(x, w, labels, part)
+    dw, = torch.autograd.grad(out, w, grad)
+    c = torch.zeros(T, dtype=torch.float64)
+    for p, (a, b) in enumerate(zip(part.tolist(), part.tolist()[1:])):
+        c[a:b] = grad.double().cpu()[p] / max(1, int((labels[a:b] >= 0).sum()))
+    _, _, _, exact, _, (bound, soft) = want(x, w.detach(), labels, c)
+    eps = torch.finfo(dt).eps
+    top = float(x.float().norm(dim=1).max() * w.detach().float().norm(dim=1).max())
+    limit = exact.abs() * eps / 2 + bound * (eps * eps / 4 + 4 * 2.0 ** -24) + soft * (2e-6 * top + 1e-6) + 1e-7 * bound.max()
+    limit += torch.finfo(dt).smallest_normal * eps
+    assert ((dw.double().cpu() - exact).abs() <= limit).all()
+
+
+def test_few_rows_of_infinite_gradients():
+    x, w, labels = make(3, 64, 100, BF16)
+    w = w.requires_grad_(True)
+    out = linear_cross_entropy.apply(x, w, labels)
+    dw, = torch.autograd.grad(out, w, torch.tensor([1.0, float("inf"), 1.0], device="cuda"))
+    at = labels[1]
+    assert torch.equal(dw[at], torch.where(x[1] > 0, -float("inf"), float("inf")).to(BF16))
+
+
 def test_no_partition_at_all():
     """An edge alone: no row lies in a partition."""
     x, w, labels = make(70, 64, 300, BF16)
