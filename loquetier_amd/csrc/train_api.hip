@@ -103,8 +103,8 @@ size_t loss_carve(void* base, int T, int H, int V, int what, LossSpace* s) {
     k.take(s->rows.share, 4 * t);
   }
   k.take(s->rows.row, 4 * t);
-  const size_t twice = loss_twice(T, what) ? 2 * kLossTwice : t;  // rows of x and G
-  k.take(s->rows.x, 2 * twice * H);
+  const size_t twice = loss_twice(T, what) ? 2 * kLossTwice : t;  // rows of y and G
+  k.take(s->rows.x, 2 * t * H);
   s->pad = round_up(T, 64);
   s->piece = what == 0 ? round_up(V, kLossTileV) : loss_piece(T, V);
   s->parts = s->piece / kLossTileV * (loss_few(T, V) ? 4 : 2);
@@ -120,6 +120,8 @@ size_t loss_carve(void* base, int T, int H, int V, int what, LossSpace* s) {
     k.take(s->rows.lse2, 4 * t);
     k.take(s->rows.own, 4 * t);
     k.take(s->rows.lost, 4 * t);
+    k.take(s->rows.rest, 4 * t);
+    if (what & 2) k.take(s->rows.y, 2 * twice * H);
   }
   if (what) k.take(s->g, 2 * twice * s->piece);
   if (what == 1 || what == 3) loss_take_dx(k, T, H, V, s);
@@ -137,6 +139,10 @@ int loss_logits(int mode, bool f16, bool few, dim3 grid, hipStream_t st, const L
       {{loss_logits_kernel<SMLM_DTYPE_F16, false, kLossGrad>, loss_logits_kernel<SMLM_DTYPE_BF16, false, kLossGrad>},
        {loss_logits_kernel<SMLM_DTYPE_F16, true, kLossGrad>, loss_logits_kernel<SMLM_DTYPE_BF16, true, kLossGrad>}}};
   return launch(kernels[mode][few][!f16], grid, dim3(256), st, a);
+}
+int loss_gather(bool f16, int rows, hipStream_t st, const LossGatherArgs& a) {
+  const dim3 grid((unsigned)ceil_div(rows, 4)), bl(256);
+  return f16 ? launch(loss_gather_kernel<SMLM_DTYPE_F16>, grid, bl, st, a) : launch(loss_gather_kernel<SMLM_DTYPE_BF16>, grid, bl, st, a);
 }
 int loss_dx(bool f16, bool few, hipStream_t st, const LossTileArgs& a) {
   int most = 0;
@@ -176,7 +182,7 @@ SMLM_API int smlm_vocab_loss_fwd(float* loss, float* lse, float* means, float* w
     const LossScanArgs sa{s.rows, labels, loss, lse, nullptr, partition, nullptr, T, V, P, 0, kept != nullptr};
     LOSS_TRY(launch(loss_scan_kernel<false>, dim3(1), dim3(kLossScanThreads), st, sa));
     const LossGatherArgs ga{s.rows, reinterpret_cast<const uint16_t*>(x), T, H, 0};
-    LOSS_TRY(launch(loss_gather_kernel, dim3((unsigned)ceil_div(T, 4)), dim3(256), st, ga));
+    LOSS_TRY(loss_gather(dtype == SMLM_DTYPE_F16, T, st, ga));
     LossTileArgs a{};
     a.rows = s.rows, a.x = ga.x, a.w = reinterpret_cast<const uint16_t*>(w), a.part = s.part, a.at_label = s.at_label;
     a.g = s.g, a.dx = s.dx, a.T = T, a.H = H, a.V = V, a.pad = s.pad, a.ldg = s.piece, a.cut = s.cut, a.stages = loss_stages(T, V), a.turned = 1;
@@ -232,11 +238,13 @@ SMLM_API int smlm_vocab_loss_bwd(void* dx, void* dw, const float* grad, const fl
   if (workspace_bytes < loss_carve(workspace, T, H, V, (dx ? 1 : 0) | (dw ? 2 : 0), &s)) return SMLM_ERR_WORKSPACE;
   hipStream_t st = (hipStream_t)stream;
   const bool f16 = dtype == SMLM_DTYPE_F16, few = loss_few(T, V);
+  const int twice = loss_twice(T, (dx ? 1 : 0) | (dw ? 2 : 0));
+  if (!dw || !partition || twice) s.rows.rest = nullptr;  // (twice: nothing is lost that it would save)
+  if (!s.rows.rest && !twice) s.rows.y = nullptr;
   const LossScanArgs sa{s.rows, labels, const_cast<float*>(loss), const_cast<float*>(lse), grad, partition, weight, T, V, P, f16, 1};
   LOSS_TRY(launch(loss_scan_kernel<true>, dim3(1), dim3(kLossScanThreads), st, sa));
-  const int twice = loss_twice(T, (dx ? 1 : 0) | (dw ? 2 : 0));
   const LossGatherArgs ga{s.rows, reinterpret_cast<const uint16_t*>(x), T, H, twice};
-  LOSS_TRY(launch(loss_gather_kernel, dim3((unsigned)ceil_div(twice ? 2 * kLossTwice : T, 4)), dim3(256), st, ga));
+  LOSS_TRY(loss_gather(f16, twice ? 2 * kLossTwice : T, st, ga));
   LossTileArgs a{};
   a.twice = twice;
   a.rows = s.rows, a.x = ga.x, a.w = reinterpret_cast<const uint16_t*>(w), a.g = s.g, a.dx = s.dx;

@@ -24,8 +24,8 @@
 // float: where a label is nearly certain nothing cancels, and the gradient is as exact, relative to its size, as anywhere.
 //
 // Rounding to 16 bits: half a step of each entry, as any product of 16-bit operands has it (of G at the label too, where dw is
-// wanted: what dx loses by it is given back in float).  fp16 entries are held 2^15 times as large (G relative to the largest |c|):
-// probabilities of a large vocabulary lie below fp16's normal numbers.
+// wanted: what dx loses by it is given back in float).  fp16 entries are held 2^15 times as large: probabilities of a large vocabulary lie
+// below fp16's normal numbers.  G is held relative to the largest |c|, in fp16 as 2^14.
 #pragma once
 #include "gemm_tile.hpp"
 #include "rms_norm.hpp"
@@ -45,7 +45,8 @@ struct LossRows {
   int32_t* row;      // [T] row of the batch
   int32_t* label;    // [T]
   int32_t* number;   // [T] of a row of the batch, -1: none (backward)
-  float* coef;       // [T] c, in fp16 relative to `unit` (backward)
+  float* coef;       // [T] c relative to `unit`, or a power of two (backward)
+  float* rest;       // [T] what c is of coef, in [0.5, 1], or NULL: all 1 (backward)
   float* lse2;       // [T] lse in powers of two (backward)
   float* own;        // [T] exp(-loss) - 1 (backward)
   float* lost;       // [T] what rounding took from G at the label (backward)
@@ -55,7 +56,8 @@ struct LossRows {
   float* share;      // [T] in the end: the part of them that is not the label's
   float* turn;       // [T] what the sums so far are multiplied with
   int32_t* moved;    // [T / 16] whether anything of sixteen rows' entries is to be turned
-  uint16_t* x;       // [n, H] the rows side by side, unless n == T; [64, H] where G is held twice
+  uint16_t* x;       // [n, H] the rows side by side, unless n == T
+  uint16_t* y;       // [n, H], or [64, H] where G is held twice: the rows (times `rest`), for dw (backward; NULL: x will do)
 };
 
 struct LossScanArgs {
@@ -143,10 +145,20 @@ __global__ __launch_bounds__(kLossScanThreads) void loss_scan_kernel(LossScanArg
     if (lane == 0) most[wave] = top;
     __syncthreads();
     for (int w = 0; w < kLossScanThreads / 64; ++w) top = fmaxf(top, most[w]);
-    const bool turn = a.f16 && top > 0.0f;
-    if (threadIdx.x == 0) a.to.unit[0] = turn ? top * 0x1p-15f : 1.0f;
-    if (turn)  // (dividing first: neither quotient nor product leaves the floats)
-      for (int i = threadIdx.x; i < before; i += kLossScanThreads) a.to.coef[i] = a.to.coef[i] / top * 0x1p15f;
+    const bool turn = top > 0.0f;
+    const float up = a.f16 ? 0x1p14f : 1.0f;  // (fp16: out of the subnormal numbers)
+    if (threadIdx.x == 0) a.to.unit[0] = turn ? top / up : 1.0f;
+    for (int i = threadIdx.x; i < before; i += kLossScanThreads) {
+      float c = a.to.coef[i];
+      if (turn) c = c / top * up;  // (dividing first: neither quotient nor product leaves the floats)
+      if (a.to.rest) {
+        const float two = 2.0f * __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, c) & 0xff800000u);
+        const bool plain = !(fabsf(c) < INFINITY) || two == 0.0f;
+        a.to.rest[i] = plain ? 1.0f : c / two;
+        c = plain ? c : two;
+      }
+      a.to.coef[i] = c;
+    }
   }
 }
 
@@ -157,25 +169,35 @@ __global__ __launch_bounds__(kLossScanThreads) void loss_scan_kernel(LossScanArg
 // 64, is empty otherwise, so it costs nothing.
 constexpr int kLossTwice = 32;
 
+// Of a partition's rows c is one number, and its rounding at their labels, where G is nearly -c, would be one error of all of them: in dw up to
+// 2.6 times the output's own rounding (bf16, 300 rows in two partitions).  So coef is the power of two above c, and dw's other operand, the rows,
+// is multiplied with the rest, c / coef, and rounded: errors of random sign, none for the partition of the largest c.  dx takes the rest in float.
 struct LossGatherArgs {
   LossRows rows;
   const uint16_t* x;
   int T, H, twice;
 };
 // A wave a row.
+template <int DT>
 __global__ __launch_bounds__(256) void loss_gather_kernel(LossGatherArgs a) {
-  const int n = uload(a.rows.count, 0), lane = threadIdx.x & 63;
-  if (n == a.T && !a.twice) return;
-  for (int i = (int)blockIdx.x * 4 + (threadIdx.x >> 6); i < (a.twice ? 2 * kLossTwice : n); i += (int)gridDim.x * 4) {
+  const int n = uload(a.rows.count, 0), lane = threadIdx.x & 63, all = a.twice ? 2 * kLossTwice : n;
+  if (n == a.T && !a.rows.y) return;
+  for (int i = (int)blockIdx.x * 4 + (threadIdx.x >> 6); i < all; i += (int)gridDim.x * 4) {
     const int at = a.twice ? i & (kLossTwice - 1) : i;
-    uint16_t* to = a.rows.x + (int64_t)i * a.H;
-    if (at >= n) {
-      const u32x4 zero = {0u, 0u, 0u, 0u};
-      for (int c = lane * 8; c < a.H; c += 512) stg16(to + c, zero);
-      continue;
+    const bool none = at >= n;
+    const uint16_t* from = a.x + (none ? 0 : (int64_t)a.rows.row[at] * a.H);
+    const float rest = none || !a.rows.rest ? 1.0f : a.rows.rest[at];
+    for (int c = lane * 8; c < a.H; c += 512) {
+      u32x4 v = {0u, 0u, 0u, 0u};
+      if (!none) v = ldg16(from + c);
+      if (n != a.T && i < n) stg16(a.rows.x + (int64_t)i * a.H + c, v);
+      if (!a.rows.y) continue;
+      float f[8];
+      unpack8<DT>(v, f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = pack2<DT>(f[2 * e] * rest, f[2 * e + 1] * rest);
+      stg16(a.rows.y + (int64_t)i * a.H + c, v);
     }
-    const uint16_t* from = a.x + (int64_t)a.rows.row[at] * a.H;
-    for (int c = lane * 8; c < a.H; c += 512) stg16(to + c, ldg16(from + c));
   }
 }
 
@@ -510,7 +532,7 @@ __global__ __launch_bounds__(256, 1) void loss_dw_kernel(LossTileArgs a) {
   f32x16 acc[IA][JB];
   loss_zero(acc);
   const int first_h = u.rows * S::kA, first_v = u.other * S::kB;
-  GemmTile<DT, WA, IA, true, WB, JB, true>::run(acc, lds, GemmOperand{a.twice ? a.rows.x : loss_x(a, n), a.H, n}, first_h,
+  GemmTile<DT, WA, IA, true, WB, JB, true>::run(acc, lds, GemmOperand{a.rows.y ? a.rows.y : loss_x(a, n), a.H, n}, first_h,
                                             GemmOperand{a.g, a.ldg, n}, first_v, 0, n);
   const float unit = uload(a.rows.unit, 0);
 #pragma unroll
@@ -693,7 +715,7 @@ __global__ __launch_bounds__(256) void loss_dx_fold_kernel(LossDxFoldArgs a) {
     by = c * a.rows.sum[i], label = -c * a.rows.share[i];
     none = c == 0.0f;  // (nothing hangs on this row)
   } else if (i >= 0) {
-    by = a.rows.unit[0], label = a.rows.lost[i] * by;
+    by = a.rows.unit[0] * (a.rows.rest ? a.rows.rest[i] : 1.0f), label = a.rows.lost[i] * by;
   }
   if (none) {
     const u32x4 zero = {0u, 0u, 0u, 0u};

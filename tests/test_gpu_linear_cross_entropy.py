@@ -6,7 +6,8 @@ here far less (errors of random sign); 2e-6 of the largest |x||w| covers them, a
 to 1e-5 of it.  An entry G = c (p - [label]) has p = exp(z - lse): off by p times the logits' error, and by some steps of a float
 of the exponential and the logarithm (v_exp_f32 and v_log_f32, 2^-23 each; 1e-6 in all) - of p, not of G, which is near 0 where a label is
 nearly certain.  It is then rounded to 16 bits, at most eps / 2 of |G|, multiplied in float, and the result is rounded once more:
-|error| <= sum |G w| eps / 2 + sum |c p w| (2e-6 |x||w| + 1e-6) + |dx| eps / 2, and a float's rounding of the sums, 1e-7 of their largest."""
+|error| <= sum |G w| eps / 2 + sum |c p w| (2e-6 |x||w| + 1e-6) + |dx| eps / 2, and a float's rounding of the sums, 1e-7 of their largest.
+With partitions the rows are rounded once more for dw, times what c is of a power of two: sum |G x| eps / 2 again."""
 import math
 
 import pytest
@@ -45,9 +46,9 @@ def want(x, w, labels, c):
     return loss, torch.where(ok, lse, 0), G @ w, G.t() @ x, bx, bw
 
 
-def close(got, exact, bounds, eps, top):
+def close(got, exact, bounds, eps, top, roundings=1):
     off, (bound, soft) = (got.double().cpu() - exact).abs(), bounds
-    limit = bound * eps / 2 + soft * (2e-6 * top + 1e-6) + exact.abs() * eps / 2 + 1e-7 * bound.max()
+    limit = roundings * bound * eps / 2 + soft * (2e-6 * top + 1e-6) + exact.abs() * eps / 2 + 1e-7 * bound.max()
     limit += torch.finfo(got.dtype).smallest_normal * eps  # (a step of the subnormal numbers)
     assert torch.isfinite(got).all()
     assert (off <= limit).all(), (off / limit).max()
@@ -77,7 +78,7 @@ def check(x, w, labels, partition=None, want_w=True, grad=None):
     eps = torch.finfo(x.dtype).eps
     close(grads[0], dx, bx, eps, top)
     if want_w:
-        close(grads[1], dw, bw, eps, top)
+        close(grads[1], dw, bw, eps, top, 1 if partition is None else 2)
     return out, grads
 
 
@@ -230,6 +231,23 @@ def test_few_rows_keep_what_rounding_takes(T, H, V, labelled, dt):
     limit = exact.abs() * eps / 2 + bound * (eps * eps / 4 + 4 * 2.0 ** -24) + soft * (2e-6 * top + 1e-6) + 1e-7 * bound.max()
     limit += torch.finfo(dt).smallest_normal * eps
     assert ((dw.double().cpu() - exact).abs() <= limit).all()
+
+
+@pytest.mark.parametrize("dt", [FP16, BF16])
+def test_a_partitions_rows_do_not_share_an_error(dt):
+    """c of the second partition lies half a step above a 16-bit number, and so would G, nearly -c, at all its labels: an error of eps / 2 of
+    almost all of the gradient.  As it is, the rows times c's part of a power of two are rounded, and the result: each uniform in half a
+    step, (eps / 2)^2 / 3 at most in the mean square; the other entries of G (a 100th of the squares here) add theirs."""
+    T, V, eps = 300, 20000, torch.finfo(dt).eps
+    x, w, labels = make(T, 256, V, dt, 9, spread=0.5)
+    w = w.requires_grad_(True)
+    part = torch.tensor([0, 20, 300], dtype=torch.int32, device="cuda")
+    out = linear_cross_entropy.apply(x, w, labels, part)
+    dw, = torch.autograd.grad(out, w, torch.tensor([40.0, 280 * (1 + eps / 2)], device="cuda"))
+    c = torch.full((T,), 1 + eps / 2, dtype=torch.float64)
+    c[:20] = 2.0
+    exact = want(x, w.detach(), labels, c)[3]
+    assert (dw.double().cpu() - exact).norm() <= 1.1 * math.sqrt(2 / 3) * eps / 2 * exact.norm()
 
 
 def test_few_rows_of_infinite_gradients():
