@@ -26,6 +26,10 @@
 // Rounding to 16 bits: half a step of each entry, as any product of 16-bit operands has it (of G at the label too, where dw is
 // wanted: what dx loses by it is given back in float).  fp16 entries are held 2^15 times as large: probabilities of a large vocabulary lie
 // below fp16's normal numbers.  G is held relative to the largest |c|, in fp16 as 2^14.
+//
+// Measured, us (4096 columns; PFLOP/s): 4099 rows of 128256 entries, bf16, logits with exponentials 4020 (1.07), dx 3920 (1.10), fold 65; 2458
+// labelled rows of 4096, 32000 entries, 636 (1.01), 702 (0.92), 30; 2048 rows of 32000, fp16, logits 499 (1.07), again for G 501,
+// dx 527 (1.02), dw 583 (0.92); 200 rows of 128256 the loss alone 254 to 270 (4.1 to 3.9 TB/s of w).  Power bounds the products: 1.75 with zeros.
 #pragma once
 #include "gemm_tile.hpp"
 #include "rms_norm.hpp"
@@ -170,7 +174,7 @@ __global__ __launch_bounds__(kLossScanThreads) void loss_scan_kernel(LossScanArg
 constexpr int kLossTwice = 32;
 
 // Of a partition's rows c is one number, and its rounding at their labels, where G is nearly -c, would be one error of all of them: in dw up to
-// 2.6 times the output's own rounding (bf16, 300 rows in two partitions).  So coef is the power of two above c, and dw's other operand, the rows,
+// eps / 2, where the output's own rounding is 0.41 of that in the mean square.  So coef is the power of two above c, and dw's other operand, the rows,
 // is multiplied with the rest, c / coef, and rounded: errors of random sign, none for the partition of the largest c.  dx takes the rest in float.
 struct LossGatherArgs {
   LossRows rows;

@@ -2,7 +2,8 @@
 `BatchLenInfo` (row layout of the flat batch) and the `add_lora` autograd
 Function, with the reference's positional arguments and `None`-padded backward
 tuple, running on the HIP kernels; the `rms_norm` autograd Function
-(kernel_utils.py:149-176); and `qk_norm_rope`, the same for queries and keys by head with their rotation.
+(kernel_utils.py:149-176); `qk_norm_rope`, the same for queries and keys by head with their rotation;
+`add_rms_norm`, the norm with the residual's addition; and `linear_cross_entropy`, the loss over the vocabulary.
 """
 from __future__ import annotations
 

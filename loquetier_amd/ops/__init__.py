@@ -1,4 +1,4 @@
-"""Operator namespace mirroring `loquetier.ops` for the SMLM path and the cache's calls.
+"""Operator namespace mirroring `loquetier.ops` for the SMLM path, the cache's calls and those around a fine-tuning step.
 
 A reference checkout switches to these kernels by replacing
 `from loquetier.ops import _kernels as kernel`
