@@ -23,6 +23,7 @@
 // travel in launches' arguments, as put_words_kernel's do.
 #pragma once
 #include "add_rms_norm.hpp"
+#include "wave_scan.hpp"
 
 namespace smlm {
 
@@ -58,33 +59,38 @@ struct AdamBeginArgs {
 // A thread a tensor.  1 - b^t in 64 bits: near b = 1 a float's would lose it.
 template <int N>
 __global__ __launch_bounds__(256) void adam_begin_kernel(AdamBeginArgs<N> a) {
-  __shared__ uint32_t blocks[N];
-  for (int i = threadIdx.x; i < a.n; i += 256)
-    blocks[i] = (uint32_t)(((a.entry[i].n & INT64_MAX) + kAdamBlock - 1) / kAdamBlock);
+  static_assert(N <= 256, "a thread each");
+  __shared__ uint32_t sums[4];
+  const int i = threadIdx.x, wave = i >> 6;
+  const bool here = i < a.n;
+  const AdamEntry entry = here ? a.entry[i] : AdamEntry{0, 0, 0};
+  const int group = here ? a.group[a.at + i] : -1;
+  int step = here ? a.step[a.at + i] : 0;
+  const bool known = group >= 0 && group < a.n_groups;
+  float h[5];
+#pragma unroll
+  for (int e = 0; e < 5; ++e) h[e] = known ? a.hyper[5 * group + e] : 0.0f;
+  const uint32_t mine = (uint32_t)(((entry.n & INT64_MAX) + kAdamBlock - 1) / kAdamBlock);
+  const uint32_t upto = (uint32_t)wave_scan((int)mine);
+  if ((i & 63) == 63) sums[wave] = upto;
   __syncthreads();
-  for (int i = threadIdx.x; i < a.n; i += 256) {
-    AdamTensor t;
-    t.p = a.entry[i].p, t.g = a.entry[i].g, t.n = a.entry[i].n & INT64_MAX, t.plain = a.entry[i].n < 0;
-    uint32_t first = (uint32_t)a.first;
-    for (int j = 0; j < i; ++j) first += blocks[j];
-    t.first = first;
-    const int group = a.group[a.at + i];
-    int step = a.step[a.at + i];
-    if (group < 0 || group >= a.n_groups) t.g = 0;
-    if (t.g) {
-      a.step[a.at + i] = ++step;
-      const float* h = a.hyper + 5 * group;
-      const double lr = h[0], b1 = h[1], b2 = h[2];
-      double p1 = 1.0, p2 = 1.0, q1 = b1, q2 = b2;
-      for (int s = step > 0 ? step : 0; s; s >>= 1, q1 *= q1, q2 *= q2)
-        if (s & 1) p1 *= q1, p2 *= q2;
-      t.b1 = h[1], t.nb1 = (float)(1.0 - b1), t.b2 = h[2], t.nb2 = (float)(1.0 - b2);
-      t.size = (float)(lr / (1.0 - p1)), t.root = (float)(1.0 / sqrt(1.0 - p2)), t.eps = h[3], t.decay = (float)(lr * (double)h[4]);
-    } else {
-      t.b1 = t.nb1 = t.b2 = t.nb2 = t.size = t.root = t.eps = t.decay = 0.0f;
-    }
-    a.table[a.at + i] = t;
+  if (!here) return;
+  AdamTensor t;
+  t.first = (uint32_t)a.first + upto - mine;
+  for (int w = 0; w < wave; ++w) t.first += sums[w];
+  t.p = entry.p, t.g = known ? entry.g : 0, t.n = entry.n & INT64_MAX, t.plain = entry.n < 0;
+  if (t.g) {
+    a.step[a.at + i] = ++step;
+    const double lr = h[0], b1 = h[1], b2 = h[2];
+    double p1 = 1.0, p2 = 1.0, q1 = b1, q2 = b2;
+    for (int s = step > 0 ? step : 0; s; s >>= 1, q1 *= q1, q2 *= q2)
+      if (s & 1) p1 *= q1, p2 *= q2;
+    t.b1 = h[1], t.nb1 = (float)(1.0 - b1), t.b2 = h[2], t.nb2 = (float)(1.0 - b2);
+    t.size = (float)(lr / (1.0 - p1)), t.root = (float)(1.0 / sqrt(1.0 - p2)), t.eps = h[3], t.decay = (float)(lr * (double)h[4]);
+  } else {
+    t.b1 = t.nb1 = t.b2 = t.nb2 = t.size = t.root = t.eps = t.decay = 0.0f;
   }
+  a.table[a.at + i] = t;
 }
 
 struct AdamArgs {

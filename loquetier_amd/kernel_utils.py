@@ -427,6 +427,8 @@ class linear_cross_entropy(Function):
             out = kernel._host().linear_cross_entropy(*args)  # (plain calls; None: nothing was done)
             if out is not None:
                 return out
+            if not torch.is_grad_enabled() and args and isinstance(args[0], torch.Tensor):
+                args = (args[0].detach(), *args[1:])  # (nothing is kept for a gradient that nobody will ask for)
         return super().apply(*args, **kwargs)
 
     @staticmethod
