@@ -165,13 +165,6 @@ __device__ __forceinline__ f32x4 adam_from8(uint32_t c, float s) {
   return f32x4{a[0] * s, a[1] * s, b[0] * s, b[1] * s};
 }
 
-// x / s, correctly rounded, from the correctly rounded inv = 1 / s: the remainder of the first guess corrects it (Markstein's
-// theorem; x / s is at most 448 and s is normal).  s 0 with inv 0: 0, and NaN of a NaN.
-__device__ __forceinline__ float adam_divide(float x, float s, float inv) {
-  const float q = x * inv;
-  return __builtin_fmaf(__builtin_fmaf(-q, s, x), inv, q);
-}
-
 // The last tensor that begins at block b or before it (empty ones begin where the next does): 64 guesses a round.
 __device__ __forceinline__ int adam_find(const AdamTensor* table, int n, uint32_t b, int lane) {
   int lo = 0, hi = n;  // table[lo].first <= b; the answer lies in [lo, hi)
@@ -227,14 +220,14 @@ __global__ __launch_bounds__(256) void adam_kernel(AdamArgs a) {
     *(SMLM_GLOBAL f32x4*)((float*)a.v + at) = v;
     return;
   }
-  float most_m = 0.0f, most_r = 0.0f, mi, ri;
+  float most_m = 0.0f, most_r = 0.0f, mb, mi, rb, ri;
 #pragma unroll
   for (int e = 0; e < 4; ++e) most_m = max_or_nan(most_m, fabsf(m[e])), most_r = max_or_nan(most_r, r[e]);
-  const float sm = scale8(wave_max(most_m), mi), sr = scale8(wave_max(most_r), ri);
+  const float sm = scale8(wave_max(most_m), mb, mi), sr = scale8(wave_max(most_r), rb, ri);
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    m[e] = adam_divide(m[e], sm, mi);
-    const float q = adam_divide(r[e], sr, ri);
+    m[e] = divide8(m[e], mb, mi);
+    const float q = divide8(r[e], rb, ri);
     r[e] = r[e] > 0.0f && q < 0x1p-9f && ri != 0.0f ? 0x1p-9f : q;
   }
   *((SMLM_GLOBAL uint32_t*)a.m + (at >> 2)) = pack8(m[0], m[1], m[2], m[3]);

@@ -4,8 +4,9 @@
 //   h = round16(x + residual),  y = h w / sqrt(mean h^2 + eps),  out = round16(y),  out8 = e4m3(y / scale),  scale = max |y| / 448
 //
 // by row or by 128 columns.  The norm is of h as it is stored, as a norm launched on the stored sum would have it, so the residual
-// stream and the backward see the same h.  y is rounded once for each of its forms.  448 is the largest e4m3, so the largest of a
-// group becomes it; a group whose scale is below the normal floats is zeros with a scale of 0.  Infinities and NaN make the scale NaN.
+// stream and the backward see the same h.  y is rounded once for each of its forms: y / scale is the correctly rounded quotient (a product
+// with 1 / scale is not, and of 8.65 million codes 248 were the neighbour of the quotient's).  448 is the largest e4m3, so the largest of a
+// group becomes it; a group whose scale is below the normal floats is zeros with a scale of 0.  An infinite y makes the scale infinite, NaN makes it NaN.
 //
 // Bound by HBM: 4 bytes read and 4 written an element, 5 with the 8-bit form.  A row stays in registers from its sum to its last
 // output.  The backward is rms_norm.hpp's, to which the gradient that reaches h through the residual is added.  (4096 columns: 4096
@@ -49,12 +50,20 @@ __device__ __forceinline__ float wave_max(float x) {
   auto lane = [&](int l) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l)); };
   return max_or_nan(max_or_nan(lane(0), lane(16)), max_or_nan(lane(32), lane(48)));
 }
-// A group's scale from its largest value, and what its values are multiplied with.
-__device__ __forceinline__ float scale8(float most, float& inv) {
+// A group's scale from its largest value, and what its values are divided by: that, and one over it (0 and 0 of an infinite scale: finite
+// values become 0).
+__device__ __forceinline__ float scale8(float most, float& by, float& inv) {
   float s = most * (1.0f / kMostE4m3);
   if (s < 0x1p-126f) s = 0.0f;
   inv = s == 0.0f ? 0.0f : 1.0f / s;
+  by = s < INFINITY ? s : 0.0f;
   return s;
+}
+// x / s, correctly rounded, from the correctly rounded inv = 1 / s: the remainder of the first guess corrects it (Markstein's
+// theorem; x / s is at most 448 and s is normal).  s 0 with inv 0: 0, and NaN of an infinity or NaN.
+__device__ __forceinline__ float divide8(float x, float s, float inv) {
+  const float q = x * inv;
+  return __builtin_fmaf(__builtin_fmaf(-q, s, x), inv, q);
 }
 __device__ __forceinline__ uint32_t pack8(float a, float b, float c, float d) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false), true);
@@ -112,7 +121,7 @@ __global__ __launch_bounds__(256) void add_rms_kernel(AddRmsArgs a) {
   }
   const float rms = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
   if (a.rms && lane == 0 && sub == 0) a.rms[row] = rms;
-  float inv = 0.0f;
+  float by = 0.0f, inv = 0.0f;
   if (a.out8 && !a.grouped) {
     float most = 0.0f;
 #pragma unroll
@@ -130,7 +139,7 @@ __global__ __launch_bounds__(256) void add_rms_kernel(AddRmsArgs a) {
       __syncthreads();
       most = max_or_nan(max_or_nan(part[1][0], part[1][1]), max_or_nan(part[1][2], part[1][3]));
     }
-    const float s = scale8(most, inv);
+    const float s = scale8(most, by, inv);
     if (lane == 0 && sub == 0) a.scale[row] = s;
   }
 #pragma unroll
@@ -151,12 +160,13 @@ __global__ __launch_bounds__(256) void add_rms_kernel(AddRmsArgs a) {
         float m = 0.0f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) m = max_or_nan(m, fabsf(f[e]));
-        const float s = scale8(row_max16(m), inv);
+        const float s = scale8(row_max16(m), by, inv);
         if (ok[i] && (lane & 15) == 0) a.scale[(int64_t)row * (a.cols >> 7) + (col[i] >> 7)] = s;
       }
       if (ok[i]) {
-        const u32x2 o = {pack8(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
-                         pack8(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv)};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = divide8(f[e], by, inv);
+        const u32x2 o = {pack8(f[0], f[1], f[2], f[3]), pack8(f[4], f[5], f[6], f[7])};
         __builtin_nontemporal_store(o, (SMLM_GLOBAL u32x2*)(a.out8 + at + col[i]));
       }
     }
@@ -202,7 +212,7 @@ __global__ __launch_bounds__(256) void add_rms_wide_kernel(AddRmsArgs a) {
     ss = block_sum_f32(ss, red4);
     const float rms = 1.0f / sqrtf(ss / (float)a.cols + a.eps);
     if (a.rms && threadIdx.x == 0) a.rms[row] = rms;
-    float inv = 0.0f;
+    float by = 0.0f, inv = 0.0f;
     if (a.out8 && !a.grouped) {
       float most = 0.0f;
       for (int col = threadIdx.x * 8; col < a.cols; col += 256 * 8) {
@@ -216,7 +226,7 @@ __global__ __launch_bounds__(256) void add_rms_wide_kernel(AddRmsArgs a) {
       __syncthreads();
       if ((threadIdx.x & 63) == 0) red4[threadIdx.x >> 6] = most;
       __syncthreads();
-      const float s = scale8(max_or_nan(max_or_nan(red4[0], red4[1]), max_or_nan(red4[2], red4[3])), inv);
+      const float s = scale8(max_or_nan(max_or_nan(red4[0], red4[1]), max_or_nan(red4[2], red4[3])), by, inv);
       if (threadIdx.x == 0) a.scale[row] = s;
     }
     for (int c0 = 0; c0 < a.cols; c0 += 256 * 8) {  // (all lanes stay: groups of sixteen of them meet)
@@ -227,23 +237,25 @@ __global__ __launch_bounds__(256) void add_rms_wide_kernel(AddRmsArgs a) {
       unpack8<DT>(ldg16(a.w + col), g);
 #pragma unroll
       for (int e = 0; e < 8; ++e) f[e] = f[e] * rms * g[e];
-      if (a.out8) {
-        if (a.grouped) {
-          float m = 0.0f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) m = max_or_nan(m, fabsf(f[e]));
-          const float s = scale8(row_max16(m), inv);
-          if (ok && (threadIdx.x & 15) == 0) a.scale[(int64_t)row * (a.cols >> 7) + (col >> 7)] = s;
-        }
-        if (ok)
-          *(SMLM_GLOBAL u32x2*)(a.out8 + at + col) = u32x2{pack8(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
-                                                           pack8(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv)};
-      }
       if (a.out && ok) {
         u32x4 o;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = pack2<DT>(f[2 * e], f[2 * e + 1]);
         stg16(a.out + at + col, o);
+      }
+      if (a.out8) {
+        if (a.grouped) {
+          float m = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) m = max_or_nan(m, fabsf(f[e]));
+          const float s = scale8(row_max16(m), by, inv);
+          if (ok && (threadIdx.x & 15) == 0) a.scale[(int64_t)row * (a.cols >> 7) + (col >> 7)] = s;
+        }
+        if (ok) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = divide8(f[e], by, inv);
+          *(SMLM_GLOBAL u32x2*)(a.out8 + at + col) = u32x2{pack8(f[0], f[1], f[2], f[3]), pack8(f[4], f[5], f[6], f[7])};
+        }
       }
     }
   }

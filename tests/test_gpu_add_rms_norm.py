@@ -230,3 +230,28 @@ def test_refusals():
     y = x[:, :136].contiguous()
     with pytest.raises(RuntimeError, match="scale must be"):
         K.add_rms_norm(e(8, 136), None, None, y, None, w[:136], EPS, e(8, 136, dt=F8), e(8, 2, dt=torch.float32))
+
+
+@pytest.mark.parametrize("rows,cols,group", [(2112, 4096, 128), (2112, 4096, 4096), (16000, 512, 128), (300, 20480, 128), (300, 20480, 20480)])
+@pytest.mark.parametrize("dt", [FP16, BF16])
+def test_codes_are_those_of_the_quotients(rows, cols, group, dt):
+    """The 8-bit values are the rounding of the correctly rounded y / scale (a product with 1 / scale is off by more, and between two codes takes
+    the other one), so the norm in tensor expressions gives the same codes: of the kernel's own h, rms and scales, bit for bit."""
+    x, residual, w = make(rows, cols, dt, rows + group)
+    h, rms, scale = torch.empty_like(x), torch.empty(rows, 1, device="cuda"), torch.empty(rows, cols // group, device="cuda")
+    out8 = torch.empty(rows, cols, dtype=F8, device="cuda")
+    K.add_rms_norm(None, rms, h, x, residual, w, EPS, out8, scale)
+    y = (h.float() * rms * w.float()).unflatten(1, (-1, group))
+    assert torch.equal((y / scale[..., None]).flatten(1).to(F8).float(), out8.float())
+
+
+def test_an_infinite_norm_leaves_its_groups_other_codes():
+    x = torch.ones(2, 256, dtype=BF16, device="cuda")
+    w = torch.ones(256, dtype=BF16, device="cuda")
+    x[0, :128] = 0
+    x[0, 3], w[3] = 8.0, 3e38  # (y overflows there)
+    out8, scale = torch.empty(2, 256, dtype=F8, device="cuda"), torch.empty(2, 2, device="cuda")
+    K.add_rms_norm(None, None, None, x, None, w, EPS, out8, scale)
+    codes = out8.float()
+    assert scale[0, 0] == float("inf") and torch.isnan(codes[0, 3]) and not codes[0, :128][torch.arange(128) != 3].any()
+    assert torch.isfinite(scale[:, 1]).all() and torch.isfinite(codes[:, 128:]).all()
