@@ -618,6 +618,8 @@ __global__ __launch_bounds__(256) void loss_refs_kernel(LossRefsArgs a) {
     loss = (__builtin_amdgcn_logf(all) - x) * kLn2;
     over = 1.0f / all, share = l / all;
   }
+  // what an infinity is divided by itself, or NaN: nothing but z may tell
+  if (!(z < INFINITY) || (z == -INFINITY && m == -INFINITY)) loss = over = share = NAN;
   const int row = a.rows.row[t];
   a.loss[row] = loss, a.lse[row] = z + loss;
   a.rows.sum[t] = over, a.rows.share[t] = share;

@@ -502,3 +502,36 @@ def test_refusals():
                       (dict(partition=part[:0]), "partition"), (dict(w=w[:0]), "No suitable kernel")):
         with pytest.raises(RuntimeError, match=text):
             ok(**bad)
+
+
+def at_the_label(x, w, labels, row, value, rest=0.0):
+    """Makes value the row's logit at its label, and rest (0: finite ones) all its others; other rows keep theirs."""
+    x[:, 0], w[:, 0] = 0, math.copysign(1.0, rest) if rest else 0
+    big = 1e30 if x.dtype == BF16 and not rest else float("inf")  # (1e30 1e30 is an infinity; fp16's largest numbers make none)
+    x[row, 0], w[labels[row], 0] = big, math.copysign(1e30 if big < math.inf else 1.0, value)
+
+
+@pytest.mark.parametrize("frozen", [True, False])
+@pytest.mark.parametrize("T,V", [(70, 300), (20, 300), (600, 20000)])
+@pytest.mark.parametrize("dt,rest", [(BF16, 0.0), (BF16, -math.inf), (FP16, -math.inf)])
+def test_a_label_of_infinite_probability(T, V, frozen, dt, rest):
+    """The label's logit is +infinity, the others are finite or -infinity: a softmax divides infinity by infinity, and the row's loss and
+    gradient are NaN as its."""
+    x, w, labels = make(T, 64, V, dt, 12)
+    at_the_label(x, w, labels, 5, math.inf, rest)
+    others = torch.arange(T, device="cuda") != 5
+    x, w = x.requires_grad_(True), w.requires_grad_(not frozen)
+    out = linear_cross_entropy.apply(x, w, labels)
+    assert torch.isnan(out[5]) and torch.isfinite(out[others]).all()
+    assert torch.isnan(linear_cross_entropy.apply(x.detach(), w.detach(), labels)[5])
+    dx, = torch.autograd.grad(out.sum(), x)
+    assert torch.isnan(dx[5]).any() and torch.isfinite(dx[others]).all()
+
+
+def test_one_entry_that_is_no_number():
+    """A vocabulary of one entry: no other logit says that the label's is NaN or an infinity."""
+    x, w, labels = make(6, 64, 1, BF16, 2)
+    x[1], x[2, 0], w[0, 0] = float("nan"), float("inf"), 1.0
+    x[3, 0] = -float("inf")
+    out = linear_cross_entropy.apply(x, w, labels)
+    assert torch.isnan(out[1:4]).all() and not out[0].any() and not out[4:].any()
