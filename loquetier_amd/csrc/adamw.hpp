@@ -14,8 +14,8 @@
 // rounding (it was loaded, or set by someone) takes its place.
 //
 // What decides the 8-bit codes is computed as the formulas stand, operation by operation with each one's own rounding (no fused
-// multiply-add, divisions and roots rounded correctly): a code's step is 2^24 times a float's, so the same step written in tensor
-// expressions gives the same codes, not others here and there.
+// multiply-add, quotients rounded correctly, the root a sqrtf, which is not always the nearest float): a code's step is 2^20 times a float's, so the
+// same step written in tensor expressions on this card gives the same codes and scales, not others here and there.
 //
 // Bound by HBM: 22 to 30 bytes an element with float states and 16-bit weights, 10 to 18 with 8-bit ones.  A wave takes a block of 256:
 // few registers, so many waves' loads are on their way.  (Four blocks a wave with all their loads ahead, two, one, us: 80 million

@@ -319,3 +319,24 @@ def test_refusals():
     opt.param_groups[0]["params"][0].grad = torch.zeros(4)
     with pytest.raises(RuntimeError, match="No suitable kernel"):
         opt.step()
+
+
+@pytest.mark.parametrize("dt,master", [(BF16, True), (FP16, False), (F32, False)])
+def test_codes_are_those_of_the_tensor_expressions(dt, master):
+    """8-bit states, bit for bit: each operation of the averages is rounded by itself, as tensor expressions round it, so no code is its
+    neighbour.  Products, sums and quotients are the host's (IEEE), the root is that of tensors on the GPU (sqrtf, which may be a float's step off)."""
+    p = Problem([70000, 300, 5, 1 << 20], dt, 8, master, 17)
+    f = lambda t: t.float().cpu().view(-1, B)
+    m, v = f(p.m) * p.ms.cpu()[:, None], (f(p.v) * p.vs.cpu()[:, None]).square()
+    flat = torch.cat([torch.nn.functional.pad(g.float().cpu(), (0, -g.numel() % B)) for g in p.grads]).view(-1, B)
+    of = torch.arange(4).repeat_interleave(torch.tensor(p.blocks)) % 2
+    b1, b2 = p.hyper.cpu()[of, 1:3].unbind(1)
+    n1, n2 = ((1 - b.double()).float()[:, None] for b in (b1, b2))
+    m = b1[:, None] * m + n1 * flat
+    r = (b2[:, None] * v + n2 * flat * flat).cuda().sqrt().cpu()
+    p.run()
+    for got, scale, exact, least in ((p.m, p.ms, m, 0.0), (p.v, p.vs, r, 2.0 ** -9)):
+        s = exact.abs().amax(1) * torch.tensor(1 / 448)  # (a float's 1 / 448)
+        assert torch.equal(scale.cpu(), s)
+        q = exact / torch.where(s > 0, s, 1)[:, None]
+        assert torch.equal(f(got), torch.where((exact > 0) & (q < least), least, q).to(F8).float())
