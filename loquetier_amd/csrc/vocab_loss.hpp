@@ -608,20 +608,20 @@ __global__ __launch_bounds__(256) void loss_refs_kernel(LossRefsArgs a) {
   if (!a.last) return;
   // e = 2^x, in the sums' units; on the side where neither overflows
   const float z = a.at_label[t], x = (m == -INFINITY ? INFINITY : __builtin_fmaf(z, kLog2e, -m)) + a.bias;
-  float loss, over, share;
+  float loss, lse, over, share;
   if (x >= 0.0f) {
     const float e = __builtin_amdgcn_exp2f(-x), y = l * e;
     loss = y < 0x1p-10f ? y * (1.0f - y * (0.5f - y * (1.0f / 3.0f))) : __builtin_amdgcn_logf(1.0f + y) * kLn2;
-    over = e / (1.0f + y), share = y / (1.0f + y);
+    over = e / (1.0f + y), share = y / (1.0f + y), lse = z + loss;
   } else {
     const float all = l + __builtin_amdgcn_exp2f(x);
     loss = (__builtin_amdgcn_logf(all) - x) * kLn2;
-    over = 1.0f / all, share = l / all;
+    over = 1.0f / all, share = l / all, lse = (m - a.bias + __builtin_amdgcn_logf(all)) * kLn2;  // (not of z, which may be far below)
   }
   // what an infinity is divided by itself, or NaN: nothing but z may tell
   if (!(z < INFINITY) || (z == -INFINITY && m == -INFINITY)) loss = over = share = NAN;
   const int row = a.rows.row[t];
-  a.loss[row] = loss, a.lse[row] = z + loss;
+  a.loss[row] = loss, a.lse[row] = lse;
   a.rows.sum[t] = over, a.rows.share[t] = share;
 }
 

@@ -535,3 +535,45 @@ def test_one_entry_that_is_no_number():
     x[3, 0] = -float("inf")
     out = linear_cross_entropy.apply(x, w, labels)
     assert torch.isnan(out[1:4]).all() and not out[0].any() and not out[4:].any()
+
+
+@pytest.mark.parametrize("dt", [FP16, BF16])
+@pytest.mark.parametrize("T,V", [(70, 300), (20, 300), (600, 20000)])
+def test_a_label_far_below_the_others(T, V, dt):
+    """The label's logit is near -2^20: the logsumexp is of the others and as exact as theirs (2e-6 of |x||w| without the label's column; exponentials,
+    sum and logarithm 2e-6 and 2^-22 of it), where loss + z would be off by a float's step of 2^20; so are the gradients of both routes."""
+    x, w, labels = make(T, 64, V, dt, 13)
+    x[:, 0], w[:, 0] = 0, 0
+    top = (x.double().norm(dim=1).max() * w.double().norm(dim=1).max()).item()
+    x[5, 0], w[labels[5], 0] = 1024, -1024
+    z = x.double() @ w.double().t().contiguous()
+    exact = torch.logsumexp(z, 1)
+    for kept in (None, torch.empty(K.linear_cross_entropy_kept_size(T, 64, V), dtype=torch.uint8, device="cuda")):
+        loss, lse = torch.empty(T, device="cuda"), torch.empty(T, device="cuda")
+        K.linear_cross_entropy(loss, lse, x, w, labels, kept=kept)
+        assert (lse.double() - exact)[5].abs() <= 2e-6 * top + 2e-6 + 2.0 ** -22 * exact[5].abs()
+        assert (loss.double() - (exact - z[torch.arange(T), labels]))[5].abs() <= 2.0 ** -3 + 1e-3  # (a float's step of 2^20, and the logits)
+    check(x, w, labels)
+    check(x, w, labels, want_w=False)
+
+
+@pytest.mark.parametrize("T,V", [(70, 300), (20, 300), (600, 20000)])
+def test_a_label_of_no_probability(T, V):
+    """The label's logit is -infinity: the loss is infinite, the logsumexp that of the others, and the gradient finite: it pulls with all its
+    weight.  Both routes."""
+    x, w, labels = make(T, 64, V, BF16, 14)
+    at_the_label(x, w, labels, 5, -math.inf)
+    z = x.double() @ w.double().t().contiguous()
+    z[5, labels[5]] = -math.inf
+    loss, lse = torch.empty(T, device="cuda"), torch.empty(T, device="cuda")
+    K.linear_cross_entropy(loss, lse, x, w, labels)
+    assert loss[5] == math.inf and (lse.double() - torch.logsumexp(z, 1)).abs().max() <= 1e-4
+    P = torch.softmax(z, 1)
+    exact = (P @ w.double() - w.double()[labels])[5]
+    for frozen in (True, False):
+        a = x.clone().requires_grad_(True)
+        out = linear_cross_entropy.apply(a, w.clone().requires_grad_(not frozen), labels)
+        dx, = torch.autograd.grad(out, a, torch.ones_like(out))
+        # |error| <= sum |G w| eps / 2 and its own rounding; 1e-4 of p by the logits
+        limit = (P[5] @ w.double().abs() + w.double()[labels[5]].abs()) * 2.0 ** -8 * 1.02 + exact.abs() * 2.0 ** -8
+        assert ((dx[5].double() - exact).abs() <= limit).all()
