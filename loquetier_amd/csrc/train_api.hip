@@ -35,9 +35,10 @@ int loss_check(int T, int H, int V, int dtype) {
 bool loss_few(int T, int V) {
   return T <= kLossFewRows || (int64_t)ceil_div(T, kLossRows) * ceil_div(V, kLossTileV) <= 128;
 }
-// Vocabulary entries a piece: whole tiles, as many in each.
+// Vocabulary entries a piece: whole tiles, as many in each.  Of up to 64 rows as of 64, which is what G has where it is held twice, and what a
+// tile has: 256 of a piece's rows then lie within 2^32 bytes, as gemm_tile's offsets have it.
 int loss_piece(int T, int V) {
-  const int64_t pieces = (2 * (int64_t)(T > 0 ? T : 1) * V + kLossPieceBytes - 1) / kLossPieceBytes;
+  const int64_t rows = T > 2 * kLossTwice ? T : 2 * kLossTwice, pieces = (2 * rows * V + kLossPieceBytes - 1) / kLossPieceBytes;
   const int64_t each = (V + pieces - 1) / pieces;
   return (int)((each + kLossTileV - 1) / kLossTileV * kLossTileV);
 }

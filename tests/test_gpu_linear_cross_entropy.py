@@ -579,3 +579,32 @@ def test_a_label_of_no_probability(T, V):
         # |error| <= sum |G w| eps / 2 and its own rounding; 1e-4 of p by the logits
         limit = (P[5] @ w.double().abs() + w.double()[labels[5]].abs()) * 2.0 ** -8 * 1.02 + exact.abs() * 2.0 ** -8
         assert ((dx[5].double() - exact).abs() <= limit).all()
+
+
+@pytest.mark.parametrize("T", [4, 40])
+def test_few_rows_of_a_vocabulary_past_32_bits(T):
+    """G of few rows is held in 64, each of 2^27 bytes if it were one piece: past 2^32 bytes the second half would be the first's again."""
+    V = (1 << 26) + 5
+    g = torch.Generator(device="cuda").manual_seed(T)
+    x = torch.randn(T, 8, generator=g, device="cuda", dtype=BF16).requires_grad_(True)
+    w = torch.randn(V, 8, generator=g, device="cuda", dtype=BF16).requires_grad_(True)
+    labels = torch.randint(0, V, (T,), generator=g, device="cuda")
+    labels[0], labels[1] = V - 1, 0
+    out = linear_cross_entropy.apply(x, w, labels)
+    dx, dw = torch.autograd.grad(out.sum(), (x, w))
+    step, xd, wd = 1 << 22, x.detach().float(), w.detach()
+    lse = torch.logsumexp(torch.stack([torch.logsumexp(xd @ wd[i:i + step].float().t().contiguous(), 1) for i in range(0, V, step)]), 0)
+    at = (xd * wd[labels].float()).sum(1)
+    assert (out.detach() - (lse - at)).abs().max() < 1e-4
+    exact_dx = bound_dx = 0.0
+    eps = 2.0 ** -7
+    for i in range(0, V, step):
+        wi = wd[i:i + step].float()
+        G = torch.exp(xd @ wi.t().contiguous() - lse[:, None])
+        here = ((labels >= i) & (labels < i + wi.shape[0])).nonzero()[:, 0]
+        G[here, labels[here] - i] -= 1
+        exact_dx, bound_dx = exact_dx + G.double() @ wi.double(), bound_dx + G.abs().double() @ wi.abs().double()
+        exact, bound = G.t().contiguous() @ xd, G.abs().t().contiguous() @ xd.abs()
+        # |error| <= sum |G x| eps / 2 and eps / 2 of the result, and 1e-4 of p by the logits
+        assert ((dw[i:i + step].float() - exact).abs() <= bound * (eps / 2 + 2e-4) + exact.abs() * eps / 2 + 1e-12).all(), i
+    assert ((dx.double() - exact_dx).abs() <= bound_dx * (eps / 2 + 2e-4) + exact_dx.abs() * eps / 2 + 1e-6).all()

@@ -88,6 +88,18 @@ def test_loss_sizes(L):
     assert all(size(4, 64, 100, what, C.byref(n)) == 0 and n.value > 0 for what in range(6))
 
 
+@pytest.mark.parametrize("T", [1, 4, 32, 33, 64, 65, 300])
+@pytest.mark.parametrize("V", [1 << 22, (1 << 22) + 1, 1 << 26, 1 << 28])
+def test_loss_pieces_fit_their_offsets(L, T, V):
+    """Exponentials and G live 512 MiB at a time (a tile more of the vocabulary at most), also where G of few rows is held twice, in 64 rows: rows
+    are found by offsets of 32 bits."""
+    n = C.c_size_t()
+    # (beside them a few numbers a row; with the rows' gradient up to 512 partial tiles of 256 x 256 floats)
+    for what, besides in ((2, 1 << 20), (1, 130 << 20), (3, 130 << 20)):
+        assert L.smlm_vocab_loss_workspace_size(T, 8, V, what, C.byref(n)) == 0
+        assert n.value <= (512 << 20) + 2 * 256 * max(T, 64) + besides
+
+
 def adam(L, n=2, workspace=A, room=LOTS, sizes=(10, 300), params=(A, A + 1024), **change):
     where, at, count = (C.c_void_p * n)(*params[:n]), (C.c_void_p * n)(*([A] * n)), (C.c_int64 * n)(*sizes[:n])
     a = lib.AdamW(params=C.addressof(where), grads=C.addressof(at), sizes=C.addressof(count), step=A, group=A, hyper=A, exp_avg=A,
