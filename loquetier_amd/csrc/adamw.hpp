@@ -99,8 +99,10 @@ struct AdamArgs {
   float *m_scale, *v_scale;  // [blocks] (8 bits)
   float* master;             // [blocks * 256] or NULL
   int n_tensors;
-  int64_t blocks;
+  int64_t from, blocks;    // the launch's first block; all blocks
 };
+// Workgroups a launch: from 2^32 threads on HIP drops what is over, and a card's memory holds more blocks.
+constexpr int64_t kAdamGroups = 1 << 22;
 
 typedef float f32x2_adam __attribute__((ext_vector_type(2)));
 
@@ -182,7 +184,7 @@ template <int PT, bool EIGHT, bool MASTER>
 __global__ __launch_bounds__(256) void adam_kernel(AdamArgs a) {
 #pragma clang fp contract(off)
   const int lane = threadIdx.x & 63;
-  const int64_t b = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t b = a.from + (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (b >= a.blocks) return;
   const AdamTensor* t = a.table + __builtin_amdgcn_readfirstlane(adam_find(a.table, a.n_tensors, (uint32_t)b, lane));
   if (!t->g) return;

@@ -380,7 +380,7 @@ SMLM_API int smlm_adamw_step(const smlm_adamw* p, void* workspace, size_t worksp
     if (p->sizes[i] > 0 && !p->params[i]) return SMLM_ERR_ARG;
     blocks += (p->sizes[i] + kAdamBlock - 1) / kAdamBlock;
   }
-  if (blocks > ((int64_t)1 << 32) - 64) return SMLM_ERR_LIMIT;  // (and so are the workgroups, four blocks each)
+  if (blocks > ((int64_t)1 << 32) - 64) return SMLM_ERR_LIMIT;
   if (blocks > 0 && (!p->exp_avg || !p->exp_avg_sq || (eight && (!p->avg_scale || !p->sq_scale)))) return SMLM_ERR_ARG;
   if (!aligned16(p->exp_avg) || !aligned16(p->exp_avg_sq) || !aligned16(p->master) || !aligned16(workspace)) return SMLM_ERR_ALIGN;
   if (workspace_bytes < (size_t)p->n_tensors * sizeof(AdamTensor)) return SMLM_ERR_WORKSPACE;
@@ -396,9 +396,14 @@ SMLM_API int smlm_adamw_step(const smlm_adamw* p, void* workspace, size_t worksp
     at += n;
   }
   if (blocks == 0) return SMLM_OK;
-  const AdamArgs a{table, p->exp_avg, p->exp_avg_sq, p->avg_scale, p->sq_scale, p->master, p->n_tensors, blocks};
-  const dim3 grid((unsigned)((blocks + 3) / 4));
-  if (f32) return launch_adam<kAdamF32>(eight, false, grid, st, a);
-  return p->dtype == SMLM_DTYPE_F16 ? launch_adam<SMLM_DTYPE_F16>(eight, p->master != nullptr, grid, st, a)
-                                    : launch_adam<SMLM_DTYPE_BF16>(eight, p->master != nullptr, grid, st, a);
+  for (int64_t from = 0; from < blocks; from += kAdamGroups * 4) {
+    const int64_t here = blocks - from < kAdamGroups * 4 ? blocks - from : kAdamGroups * 4;
+    const AdamArgs a{table, p->exp_avg, p->exp_avg_sq, p->avg_scale, p->sq_scale, p->master, p->n_tensors, from, blocks};
+    const dim3 grid((unsigned)((here + 3) / 4));
+    const int rc = f32 ? launch_adam<kAdamF32>(eight, false, grid, st, a)
+                   : p->dtype == SMLM_DTYPE_F16 ? launch_adam<SMLM_DTYPE_F16>(eight, p->master != nullptr, grid, st, a)
+                                                : launch_adam<SMLM_DTYPE_BF16>(eight, p->master != nullptr, grid, st, a);
+    if (rc) return rc;
+  }
+  return SMLM_OK;
 }

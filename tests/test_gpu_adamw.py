@@ -340,3 +340,25 @@ def test_codes_are_those_of_the_tensor_expressions(dt, master):
         assert torch.equal(scale.cpu(), s)
         q = exact / torch.where(s > 0, s, 1)[:, None]
         assert torch.equal(f(got), torch.where((exact > 0) & (q < least), least, q).to(F8).float())
+
+
+def test_more_blocks_than_a_launch_takes():
+    """2^34 weights, 2^26 blocks of a wave each: more threads than HIP launches at once.  (100 GB; mostly zeros, which stay.)"""
+    torch.cuda.empty_cache()
+    n = (1 << 34) + 300
+    if torch.cuda.mem_get_info()[0] < n * 6.2 + (1 << 33):
+        pytest.skip("needs 115 GB")
+    blocks = -(-n // B)
+    zeros = lambda k, dt: torch.zeros(k, dtype=torch.uint8 if dt == F8 else dt, device="cuda").view(dt)
+    w, g, m, v = zeros(n, BF16), zeros(n, BF16), zeros(blocks * B, F8), zeros(blocks * B, F8)
+    ms, vs = zeros(blocks, F32), zeros(blocks, F32)
+    at = torch.tensor([0, 1 << 32, (1 << 33) - 1, (1 << 34) - 1, n - 1], device="cuda")
+    w[at], g[at] = 1.0, torch.tensor([1.0, -1.0, 2.0, 1.0, -1.0], dtype=BF16, device="cuda")
+    step, group = zeros(1, torch.int32), zeros(1, torch.int32)
+    K.adamw_step([w], [g], m, v, step, torch.tensor([[0.125, 0.9, 0.999, 1e-8, 0.0]], device="cuda"), group, ms, vs)
+    assert step.item() == 1
+    # (a first step is lr, up to 1e-6 of it: 1 -+ 0.125 to half a step of bf16)
+    want = torch.tensor([0.875, 1.125, 0.875, 0.875, 1.125], device="cuda")
+    assert ((w[at].float() - want).abs() <= 2.0 ** -8 * want).all()
+    assert sum(int(w[i:i + (1 << 30)].count_nonzero()) for i in range(0, n, 1 << 30)) == 5
+    assert ((ms[at // B] * 448 - 0.1 * g[at].abs().float()).abs() < 1e-6).all() and int(ms.count_nonzero()) == 5
