@@ -273,6 +273,8 @@ SMLM_API int smlm_vocab_loss_bwd(void* dx, void* dw, const float* grad, const fl
 
 namespace {
 
+constexpr int kAddRmsRows = 1 << 22;  // a launch, a workgroup each at most: from 2^32 threads on HIP drops what is over
+
 template <int DT>
 int launch_add_rms(hipStream_t st, const AddRmsArgs& a) {
   const dim3 bl(256);
@@ -306,11 +308,22 @@ SMLM_API int smlm_add_rms_norm_fwd(void* out, float* rms, void* h, const void* x
   if (!x || !w) return SMLM_ERR_ARG;
   if (!aligned16(out) || !aligned16(h) || !aligned16(x) || !aligned16(residual) || !aligned16(w) || !aligned16(out8))
     return SMLM_ERR_ALIGN;
-  const AddRmsArgs a{reinterpret_cast<uint16_t*>(out), rms, reinterpret_cast<uint16_t*>(h), reinterpret_cast<const uint16_t*>(x),
-                     reinterpret_cast<const uint16_t*>(residual), reinterpret_cast<const uint16_t*>(w),
-                     reinterpret_cast<uint8_t*>(out8), scale, rows, cols, group == 128, eps};
+  AddRmsArgs a{reinterpret_cast<uint16_t*>(out), rms, reinterpret_cast<uint16_t*>(h), reinterpret_cast<const uint16_t*>(x),
+               reinterpret_cast<const uint16_t*>(residual), reinterpret_cast<const uint16_t*>(w),
+               reinterpret_cast<uint8_t*>(out8), scale, rows, cols, group == 128, eps};
   hipStream_t st = (hipStream_t)stream;
-  return dtype == SMLM_DTYPE_F16 ? launch_add_rms<SMLM_DTYPE_F16>(st, a) : launch_add_rms<SMLM_DTYPE_BF16>(st, a);
+  for (int from = 0;; from += kAddRmsRows) {
+    a.rows = rows - from < kAddRmsRows ? rows - from : kAddRmsRows;
+    const int rc = dtype == SMLM_DTYPE_F16 ? launch_add_rms<SMLM_DTYPE_F16>(st, a) : launch_add_rms<SMLM_DTYPE_BF16>(st, a);
+    if (rc || rows - from <= kAddRmsRows) return rc;
+    const int64_t n = (int64_t)kAddRmsRows * cols;
+    a.x += n;
+    if (out) a.out += n;
+    if (rms) a.rms += kAddRmsRows;
+    if (h) a.h += n;
+    if (residual) a.residual += n;
+    if (out8) a.out8 += n, a.scale += group ? n / 128 : kAddRmsRows;
+  }
 }
 
 SMLM_API int smlm_add_rms_norm_bwd(void* dh, void* dw, const void* g, const void* gh, const void* h, const void* w, const float* rms,

@@ -255,3 +255,26 @@ def test_an_infinite_norm_leaves_its_groups_other_codes():
     codes = out8.float()
     assert scale[0, 0] == float("inf") and torch.isnan(codes[0, 3]) and not codes[0, :128][torch.arange(128) != 3].any()
     assert torch.isfinite(scale[:, 1]).all() and torch.isfinite(codes[:, 128:]).all()
+
+
+def test_more_rows_than_a_launch_takes():
+    """2^24 workgroups of 256 are more threads than HIP launches at once.  Rows repeat, so that a few tell of all."""
+    rows, cols = (1 << 26) + 5, 8
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < rows * cols * 8 + (1 << 33):
+        pytest.skip("needs the memory")
+    few = 1 << 12
+    x, residual, w = make(few, cols, BF16, 3)
+    want = [torch.empty_like(x), torch.empty(few, 1, device="cuda"), torch.empty_like(x)]
+    K.add_rms_norm(*want, x, residual, w, EPS)
+    x = x.repeat(-(-rows // few), 1)[:rows]
+    x[-1] = 1.0  # (the last row is its own)
+    residual = residual.repeat(-(-rows // few), 1)[:rows]
+    out, rms, h = torch.empty_like(x), torch.empty(rows, 1, device="cuda"), torch.empty_like(x)
+    K.add_rms_norm(out, rms, h, x, residual, w, EPS)
+    whole = rows // few * few
+    for got, one in zip((out, rms, h), want):
+        got = got[:whole].view(-1, *one.shape)
+        assert all(torch.allclose(got[i:i + 64].float(), one.float(), rtol=2e-2, atol=1e-6) for i in range(0, len(got), 64))
+    y, _ = norm64(total(x[-1:], residual[-1:]), w)
+    near(out[-1:], y, BF16)
