@@ -19,14 +19,19 @@ constexpr int kLossMaxDim = 1 << 22;           // H: a tile's rows stay inside a
 // 3698 / 3698 (one piece from 512 on).
 constexpr int64_t kLossPieceBytes = (int64_t)512 << 20;
 
+// From 2^32 threads a launch on HIP drops what is over.  Workgroups a launch, and what has a workgroup for 16 rows.  (Products of matrices that
+// fit a card have fewer tiles.)
+constexpr int kLossGroups = 1 << 22;
+constexpr int kLossMostRows = (1 << 28) - 16;
+
 int loss_check(int T, int H, int V, int dtype) {
   if (T < 0 || H <= 0 || V <= 0) return SMLM_ERR_ARG;
   if (int rc = check_dtype(dtype)) return rc;
   if (H & 7) return SMLM_ERR_ALIGN;
-  if (H > kLossMaxDim || T > (1 << 28) || V > (1 << 28)) return SMLM_ERR_LIMIT;
+  if (H > kLossMaxDim || T > kLossMostRows || V > (1 << 28)) return SMLM_ERR_LIMIT;
   if ((int64_t)ceil_div(T, kLossFewRows) * ceil_div(V, kLossTileV) > (1 << 30) ||
       (int64_t)ceil_div(H, 256) * ceil_div(V, kLossTileV) > (1 << 30))
-    return SMLM_ERR_LIMIT;  // (workgroups)
+    return SMLM_ERR_LIMIT;  // (tiles)
   return SMLM_OK;
 }
 // Tiles of 64 rows, two workgroups a compute unit, where rows or tiles of 256 are few: 128 tiles leave half of the card idle.  us, tiles of
@@ -41,6 +46,11 @@ int loss_piece(int T, int V) {
   const int64_t rows = T > 2 * kLossTwice ? T : 2 * kLossTwice, pieces = (2 * rows * V + kLossPieceBytes - 1) / kLossPieceBytes;
   const int64_t each = (V + pieces - 1) / pieces;
   return (int)((each + kLossTileV - 1) / kLossTileV * kLossTileV);
+}
+// The same where nothing is stored: all of it, or what a launch takes.
+int loss_sums_piece(int T, int V) {
+  const int most = kLossGroups / ceil_div(T > 0 ? T : 1, loss_few(T, V) ? kLossFewRows : kLossRows), tiles = ceil_div(V, kLossTileV);
+  return kLossTileV * (tiles < most ? tiles : most);
 }
 int loss_stages(int T, int V) {
   const int piece = loss_piece(T, V);
@@ -107,7 +117,7 @@ size_t loss_carve(void* base, int T, int H, int V, int what, LossSpace* s) {
   const size_t twice = loss_twice(T, what) ? 2 * kLossTwice : t;  // rows of y and G
   k.take(s->rows.x, 2 * t * H);
   s->pad = round_up(T, 64);
-  s->piece = what == 0 ? round_up(V, kLossTileV) : loss_piece(T, V);
+  s->piece = what == 0 ? loss_sums_piece(T, V) : loss_piece(T, V);
   s->parts = s->piece / kLossTileV * (loss_few(T, V) ? 4 : 2);
   if (what == 0 || what == 4) {
     k.take(s->part, 8 * (size_t)s->parts * s->pad);
@@ -142,7 +152,8 @@ int loss_logits(int mode, bool f16, bool few, dim3 grid, hipStream_t st, const L
   return launch(kernels[mode][few][!f16], grid, dim3(256), st, a);
 }
 int loss_gather(bool f16, int rows, hipStream_t st, const LossGatherArgs& a) {
-  const dim3 grid((unsigned)ceil_div(rows, 4)), bl(256);
+  const int groups = ceil_div(rows, 4);
+  const dim3 grid((unsigned)(groups < kLossGroups ? groups : kLossGroups)), bl(256);
   return f16 ? launch(loss_gather_kernel<SMLM_DTYPE_F16>, grid, bl, st, a) : launch(loss_gather_kernel<SMLM_DTYPE_BF16>, grid, bl, st, a);
 }
 int loss_dx(bool f16, bool few, hipStream_t st, const LossTileArgs& a) {
@@ -152,6 +163,17 @@ int loss_dx(bool f16, bool few, hipStream_t st, const LossTileArgs& a) {
   if (few)
     return f16 ? launch(loss_dx_kernel<SMLM_DTYPE_F16, true>, grid, bl, st, a) : launch(loss_dx_kernel<SMLM_DTYPE_BF16, true>, grid, bl, st, a);
   return f16 ? launch(loss_dx_kernel<SMLM_DTYPE_F16, false>, grid, bl, st, a) : launch(loss_dx_kernel<SMLM_DTYPE_BF16, false>, grid, bl, st, a);
+}
+template <bool KEPT>
+int loss_dx_fold(bool f16, hipStream_t st, LossDxFoldArgs a) {
+  for (; a.from < a.T; a.from += kLossGroups * 4) {
+    const int groups = ceil_div(a.T - a.from, 4);
+    const dim3 grid((unsigned)(groups < kLossGroups ? groups : kLossGroups)), bl(256);
+    const int rc = f16 ? launch(loss_dx_fold_kernel<SMLM_DTYPE_F16, KEPT>, grid, bl, st, a)
+                       : launch(loss_dx_fold_kernel<SMLM_DTYPE_BF16, KEPT>, grid, bl, st, a);
+    if (rc) return rc;
+  }
+  return SMLM_OK;
 }
 #define LOSS_TRY(call) \
   if (int rc = (call)) return rc
@@ -206,8 +228,11 @@ SMLM_API int smlm_vocab_loss_fwd(float* loss, float* lse, float* means, float* w
     }
   }
   if (P == 0) return SMLM_OK;
-  const LossMeansArgs ma{loss, labels, partition, means, weight, T, V};
-  return launch(loss_means_kernel, dim3((unsigned)P), dim3(1024), st, ma);
+  for (int from = 0; from < P; from += kLossGroups / 4) {  // (workgroups of 1024)
+    const LossMeansArgs ma{loss, labels, partition + from, means + from, weight + from, T, V};
+    LOSS_TRY(launch(loss_means_kernel, dim3((unsigned)(P - from < kLossGroups / 4 ? P - from : kLossGroups / 4)), dim3(1024), st, ma));
+  }
+  return SMLM_OK;
 }
 
 SMLM_API int smlm_vocab_loss_bwd_kept(void* dx, const float* grad, const void* kept, size_t kept_bytes, const void* w,
@@ -219,12 +244,9 @@ SMLM_API int smlm_vocab_loss_bwd_kept(void* dx, const float* grad, const void* k
   if (!aligned16(dx) || !aligned16(kept) || !aligned16(w)) return SMLM_ERR_ALIGN;
   LossSpace s{};
   if (kept_bytes < loss_keep(const_cast<void*>(kept), T, H, V, &s)) return SMLM_ERR_WORKSPACE;
-  const LossDxFoldArgs fa{s.rows, s.dx, s.cut, reinterpret_cast<uint16_t*>(dx), reinterpret_cast<const uint16_t*>(w), T, H, loss_few(T, V),
+  const LossDxFoldArgs fa{s.rows, s.dx, s.cut, reinterpret_cast<uint16_t*>(dx), reinterpret_cast<const uint16_t*>(w), 0, T, H, loss_few(T, V),
                           loss_stages(T, V), grad, partition, weight, P};
-  const dim3 grid((unsigned)ceil_div(T, 4)), bl(256);
-  hipStream_t st = (hipStream_t)stream;
-  return dtype == SMLM_DTYPE_F16 ? launch(loss_dx_fold_kernel<SMLM_DTYPE_F16, true>, grid, bl, st, fa)
-                                 : launch(loss_dx_fold_kernel<SMLM_DTYPE_BF16, true>, grid, bl, st, fa);
+  return loss_dx_fold<true>(dtype == SMLM_DTYPE_F16, (hipStream_t)stream, fa);
 }
 
 SMLM_API int smlm_vocab_loss_bwd(void* dx, void* dw, const float* grad, const float* loss, const float* lse, const void* x, const void* w,
@@ -263,10 +285,8 @@ SMLM_API int smlm_vocab_loss_bwd(void* dx, void* dw, const float* grad, const fl
     }
   }
   if (!dx) return SMLM_OK;
-  const LossDxFoldArgs fa{s.rows, s.dx, s.cut, reinterpret_cast<uint16_t*>(dx), a.w, T, H, few, a.stages, nullptr, nullptr, nullptr, 0};
-  const dim3 grid((unsigned)ceil_div(T, 4));
-  return f16 ? launch(loss_dx_fold_kernel<SMLM_DTYPE_F16, false>, grid, bl, st, fa)
-             : launch(loss_dx_fold_kernel<SMLM_DTYPE_BF16, false>, grid, bl, st, fa);
+  const LossDxFoldArgs fa{s.rows, s.dx, s.cut, reinterpret_cast<uint16_t*>(dx), a.w, 0, T, H, few, a.stages, nullptr, nullptr, nullptr, 0};
+  return loss_dx_fold<false>(f16, st, fa);
 }
 
 // ---- the residual's addition and its norm ----

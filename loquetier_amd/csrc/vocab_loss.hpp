@@ -186,7 +186,7 @@ template <int DT>
 __global__ __launch_bounds__(256) void loss_gather_kernel(LossGatherArgs a) {
   const int n = uload(a.rows.count, 0), lane = threadIdx.x & 63, all = a.twice ? 2 * kLossTwice : n;
   if (n == a.T && !a.rows.y) return;
-  for (int i = (int)blockIdx.x * 4 + (threadIdx.x >> 6); i < all; i += (int)gridDim.x * 4) {
+  for (int i = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6); i < all; i += (int)gridDim.x * 4) {
     const int at = a.twice ? i & (kLossTwice - 1) : i;
     const bool none = at >= n;
     const uint16_t* from = a.x + (none ? 0 : (int64_t)a.rows.row[at] * a.H);
@@ -691,7 +691,7 @@ struct LossDxFoldArgs {
   const float* cut;   // [parts][tile]
   uint16_t* dx;       // [T, H]
   const uint16_t* w;  // [V, H]
-  int T, H, few, stages;
+  int from, T, H, few, stages;  // from: the launch's first row
   // of exponentials (KEPT): the rows' coefficients are found here
   const float* grad;         // [T], or [P]
   const int32_t* partition;  // [P + 1] or NULL
@@ -704,7 +704,7 @@ __global__ __launch_bounds__(256) void loss_dx_fold_kernel(LossDxFoldArgs a) {
   const int n = uload(a.rows.count, 0), lane = threadIdx.x & 63, tile = a.few ? kLossFewRows : kLossRows;
   const int row_tiles = (n + tile - 1) / tile, h_tiles = (a.H + 255) / 256;
   const LossCuts cuts = loss_cuts(row_tiles * h_tiles, a.stages, a.few);
-  const int t = (int)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int t = a.from + (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6);
   if (t >= a.T) return;
   const int i = a.rows.number[t];
   uint16_t* to = a.dx + (int64_t)t * a.H;

@@ -608,3 +608,52 @@ def test_few_rows_of_a_vocabulary_past_32_bits(T):
         # |error| <= sum |G x| eps / 2 and eps / 2 of the result, and 1e-4 of p by the logits
         assert ((dw[i:i + step].float() - exact).abs() <= bound * (eps / 2 + 2e-4) + exact.abs() * eps / 2 + 1e-12).all(), i
     assert ((dx.double() - exact_dx).abs() <= bound_dx * (eps / 2 + 2e-4) + exact_dx.abs() * eps / 2 + 1e-6).all()
+
+
+def test_more_tiles_than_a_launch_takes():
+    """The losses alone of 2^20 rows against 2^20 entries, 2^24 tiles: more threads than HIP launches at once."""
+    T = V = 1 << 20
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x, w = (torch.randn(n, 8, generator=g, device="cuda", dtype=BF16) for n in (T, V))
+    labels = torch.randint(0, V, (T,), generator=g, device="cuda")
+    out = linear_cross_entropy.apply(x, w, labels)
+    for rows in (slice(0, 300), slice(T // 2, T // 2 + 300), slice(T - 300, T)):
+        z = x[rows].float() @ w.float().t().contiguous()
+        exact = torch.logsumexp(z, 1) - z[torch.arange(300), labels[rows]]
+        assert (out[rows] - exact).abs().max() < 1e-4  # (logits of size 8: 2e-6 of |x||w| and as much of a logsumexp in float)
+
+
+def test_more_rows_than_a_launch_takes():
+    """2^26 rows, four a workgroup of those that move rows and fold their gradients; every 2^12th has a label."""
+    T, V = (1 << 26) + 7, 40
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(T, 8, generator=g, device="cuda", dtype=BF16).requires_grad_(True)
+    w = torch.randn(V, 8, generator=g, device="cuda", dtype=BF16).requires_grad_(True)
+    labels = torch.full((T,), -100, device="cuda")
+    at = torch.arange(0, T, 1 << 12, device="cuda")
+    at[-1] = T - 1
+    labels[at] = torch.randint(0, V, at.shape, generator=g, device="cuda")
+    z = x.detach()[at].float() @ w.detach().float().t().contiguous()
+    G = torch.softmax(z, 1)
+    loss = torch.logsumexp(z, 1) - z[torch.arange(len(at)), labels[at]]
+    G[torch.arange(len(at)), labels[at]] -= 1
+    exact, bound = G @ w.detach().float(), G.abs() @ w.detach().float().abs()
+    for frozen in (True, False):
+        out = linear_cross_entropy.apply(x, w.detach() if frozen else w, labels)
+        dx = torch.autograd.grad(out.sum(), [x] if frozen else [x, w])[0]
+        assert (out.detach()[at] - loss).abs().max() < 1e-4 and int(out.count_nonzero()) == len(at)
+        assert ((dx[at].float() - exact).abs() <= bound * (2.0 ** -8 + 2e-4) + exact.abs() * 2.0 ** -8 + 1e-6).all()
+        assert int(dx.any(1).count_nonzero()) == len(at)
+
+
+def test_more_partitions_than_a_launch_takes():
+    """2^22 partitions of a row or none, a workgroup of 1024 each."""
+    T, P = 1 << 20, (1 << 22) + 9
+    x, w, labels = make(64, 8, 50, BF16, 3)
+    x, labels = x.repeat(T // 64, 1), labels.repeat(T // 64)
+    part = (torch.arange(P + 1, device="cuda") // 4).clamp(max=T).int()
+    rows = linear_cross_entropy.apply(x, w, labels)
+    means = linear_cross_entropy.apply(x, w, labels, part)
+    first = torch.arange(P, device="cuda") % 4 == 3
+    first &= torch.arange(P, device="cuda") // 4 < T
+    assert torch.equal(means[first], rows) and not means[~first].any()

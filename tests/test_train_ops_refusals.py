@@ -100,6 +100,12 @@ def test_loss_pieces_fit_their_offsets(L, T, V):
         assert n.value <= (512 << 20) + 2 * 256 * max(T, 64) + besides
 
 
+def test_loss_rows_that_no_launch_takes(L):
+    n = C.c_size_t()
+    for T, code in (((1 << 28) - 16, 0), ((1 << 28) - 15, LIMIT), (1 << 28, LIMIT)):  # (a workgroup for 16 rows: 2^32 threads are too many)
+        assert all(L.smlm_vocab_loss_workspace_size(T, 8, 50, what, C.byref(n)) == code for what in range(6))
+
+
 def adam(L, n=2, workspace=A, room=LOTS, sizes=(10, 300), params=(A, A + 1024), **change):
     where, at, count = (C.c_void_p * n)(*params[:n]), (C.c_void_p * n)(*([A] * n)), (C.c_int64 * n)(*sizes[:n])
     a = lib.AdamW(params=C.addressof(where), grads=C.addressof(at), sizes=C.addressof(count), step=A, group=A, hyper=A, exp_avg=A,
