@@ -17,7 +17,10 @@ class _Set:
     def __init__(self, params: List[torch.Tensor], groups: List[int], bits: int, master: bool):
         dev, dtype = params[0].device, params[0].dtype
         self.params = params
-        blocks = sum(-(-p.numel() // kernel.ADAMW_BLOCK) for p in params)
+        self.first = [0]  # each tensor's first block, and the end
+        for p in params:
+            self.first.append(self.first[-1] - (-p.numel() // kernel.ADAMW_BLOCK))
+        blocks = self.first[-1]
         n = blocks * kernel.ADAMW_BLOCK
         state = torch.float8_e4m3fn if bits == 8 else torch.float32
         zeros = lambda size, dt: torch.zeros(size, dtype=dt, device=dev)
@@ -32,9 +35,12 @@ class _Set:
         self.group = kernel.put_ints(dev, [], groups)[1]
         self.workspace = kernel.Workspace(dev)
 
-    def span(self, i: int) -> Tuple[int, int]:
-        at = sum(-(-p.numel() // kernel.ADAMW_BLOCK) for p in self.params[:i]) * kernel.ADAMW_BLOCK
-        return at, at + self.params[i].numel()
+    def parts(self, i: int) -> Dict[str, Optional[torch.Tensor]]:
+        """A tensor's share of the states, whole blocks."""
+        first, end = self.first[i:i + 2]
+        flat = slice(first * kernel.ADAMW_BLOCK, end * kernel.ADAMW_BLOCK)
+        of = dict(avg_scale=slice(first, end), sq_scale=slice(first, end), step=slice(i, i + 1))
+        return {n: None if t is None else t[of.get(n, flat)] for n, t in self.tensors.items()}
 
 
 class AdamW(torch.optim.Optimizer):
@@ -128,24 +134,39 @@ class AdamW(torch.optim.Optimizer):
             for i, p in enumerate(s.params):
                 if p is not param:
                     continue
-                (a, b), t = s.span(i), s.tensors
-                first, last = a // kernel.ADAMW_BLOCK, -(-b // kernel.ADAMW_BLOCK)
-                values = lambda name, scale: (t[name][a:last * kernel.ADAMW_BLOCK].clone() if scale is None else (
-                    t[name][a:last * kernel.ADAMW_BLOCK].view(-1, kernel.ADAMW_BLOCK).float()
-                    * scale[first:last, None]).flatten())[:b - a].view(p.shape)
-                out = dict(step=t["step"][i].clone(), exp_avg=values("exp_avg", t["avg_scale"]),
+                t = s.parts(i)
+                values = lambda name, scale: (t[name].clone() if scale is None else (
+                    t[name].view(-1, kernel.ADAMW_BLOCK).float() * scale[:, None]).flatten())[:p.numel()].view(p.shape)
+                out = dict(step=t["step"][0].clone(), exp_avg=values("exp_avg", t["avg_scale"]),
                            exp_avg_sq=values("exp_avg_sq", t["sq_scale"]))
                 if self.state_bits == 8:
                     out["exp_avg_sq"] = out["exp_avg_sq"].square()
                 if t["master"] is not None:
-                    out["master"] = t["master"][a:b].view(p.shape).clone()
+                    out["master"] = t["master"][:p.numel()].view(p.shape).clone()
                 return out
         raise KeyError("not one of the optimizer's tensors")
 
+    def _kinds(self) -> List[List[Tuple[_Set, int]]]:
+        """Where the tensors' states are, those of a type on a device together in the groups' order: as one set would hold them
+        if all had been there from the start."""
+        where = {id(p): (s, i) for s in self._sets for i, p in enumerate(s.params)}
+        kinds: Dict[tuple, List[Tuple[_Set, int]]] = {}
+        for group in self.param_groups:
+            for p in group["params"]:
+                if id(p) in where:
+                    kinds.setdefault((p.device, p.dtype), []).append(where[id(p)])
+        return list(kinds.values())
+
     def state_dict(self) -> Dict[str, Any]:
         out = super().state_dict()
-        out["state"] = {"bits": self.state_bits,
-                        "sets": [{n: t if t is None else t.clone() for n, t in s.tensors.items()} for s in self._sets]}
+        if self._sets:
+            self._prepare()  # (of a group that has joined since the last step too)
+        sets = []
+        for kind in self._kinds():
+            parts = [s.parts(i) for s, i in kind]
+            join = lambda ts: None if ts[0] is None else torch.cat([t.view(torch.uint8) for t in ts]).view(ts[0].dtype)
+            sets.append({n: join([p[n] for p in parts]) for n in parts[0]})
+        out["state"] = {"bits": self.state_bits, "sets": sets}
         return out
 
     def load_state_dict(self, state_dict: Dict[str, Any]) -> None:
@@ -158,10 +179,13 @@ class AdamW(torch.optim.Optimizer):
                         t.view(torch.uint8).zero_()
             return
         self._prepare()
+        kinds = [[s.parts(i) for s, i in kind] for kind in self._kinds()]
         shape = lambda tensors: {n: None if t is None else (t.dtype, tuple(t.shape)) for n, t in tensors.items()}
-        if state["bits"] != self.state_bits or [shape(s.tensors) for s in self._sets] != [shape(s) for s in state["sets"]]:
+        mine = [{n: None if t is None else (t.dtype, (sum(p[n].size(0) for p in parts),)) for n, t in parts[0].items()} for parts in kinds]
+        if state["bits"] != self.state_bits or mine != [shape(s) for s in state["sets"]]:
             raise ValueError("the saved states are of other tensors, or of another number of bits")
-        for s, saved in zip(self._sets, state["sets"]):
-            for name, t in s.tensors.items():
+        for parts, saved in zip(kinds, state["sets"]):
+            for name, t in saved.items():
                 if t is not None:
-                    t.copy_(saved[name])
+                    for part, of in zip(parts, t.split([p[name].size(0) for p in parts])):
+                        part[name].view(torch.uint8).copy_(of.view(torch.uint8))

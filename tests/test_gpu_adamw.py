@@ -362,3 +362,70 @@ def test_more_blocks_than_a_launch_takes():
     assert ((w[at].float() - want).abs() <= 2.0 ** -8 * want).all()
     assert sum(int(w[i:i + (1 << 30)].count_nonzero()) for i in range(0, n, 1 << 30)) == 5
     assert ((ms[at // B] * 448 - 0.1 * g[at].abs().float()).abs() < 1e-6).all() and int(ms.count_nonzero()) == 5
+
+
+def tensors(*sizes, dt=BF16, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(n, generator=g).to(dt).cuda().requires_grad_(True) for n in sizes]
+
+
+def take_step(opt, params, seed):
+    g = torch.Generator().manual_seed(seed)
+    for p in params:
+        p.grad = (torch.randn(p.shape, generator=g) * 1e-2).to(p.dtype).cuda()
+    opt.step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("master", [True, False])
+def test_saved_after_a_group_joined(bits, master):
+    """An adapter that joins while others train: the states go to and from an optimizer that has had all groups from the start, and one
+    whose groups joined as they did, and go on there bit for bit."""
+    a, c = tensors(300, 5, 1000), tensors(64, 700, dt=F32, seed=1)
+    new = lambda: AdamW([dict(params=a[:1] + c[:1], lr=1e-2)], lr=1e-3, state_bits=bits, master=master)
+    x = new()
+    take_step(x, a[:1] + c[:1], 1)
+    x.add_param_group(dict(params=a[1:2]))
+    take_step(x, a[:2] + c[:1], 2)
+    x.add_param_group(dict(params=[c[1], a[2]]))
+    take_step(x, a + c, 3)
+    saved = x.state_dict()
+    copies = []
+    for joins in (False, True):
+        b, d = ([t.detach().clone().requires_grad_(True) for t in ts] for ts in (a, c))
+        if joins:
+            y = AdamW([dict(params=b[:1] + d[:1], lr=1e-2)], lr=1e-3, state_bits=bits, master=master)
+            take_step(y, b[:1] + d[:1], 4)
+            y.add_param_group(dict(params=b[1:2]))
+            take_step(y, b[:1], 5)
+            y.add_param_group(dict(params=[d[1], b[2]]))
+            with torch.no_grad():
+                for p, q in zip(a + c, b + d):
+                    q.copy_(p)
+        else:
+            y = AdamW([dict(params=b[:1] + d[:1]), dict(params=b[1:2]), dict(params=[d[1], b[2]])], state_bits=bits, master=master)
+        y.load_state_dict(saved)
+        again = y.state_dict()
+        assert again["param_groups"] == saved["param_groups"]
+        for s, t in zip(saved["state"]["sets"], again["state"]["sets"]):
+            assert all(u is None and t[n] is None or torch.equal(u.view(torch.uint8), t[n].view(torch.uint8)) for n, u in s.items())
+        copies.append((y, b + d))
+    for i in range(4, 7):
+        take_step(x, a + c, i)
+        for y, ps in copies:
+            take_step(y, ps, i)
+    for y, ps in copies:
+        assert all(torch.equal(p, q) for p, q in zip(a + c, ps))
+        assert all(torch.equal(x.state_of(p)[n], y.state_of(q)[n]) for p, q in zip(a + c, ps) for n in x.state_of(p))
+
+
+def test_saved_before_a_joined_groups_first_step():
+    a = tensors(300, 500)
+    x = AdamW([dict(params=a[:1])])
+    take_step(x, a[:1], 1)
+    x.add_param_group(dict(params=a[1:]))
+    b = [t.detach().clone().requires_grad_(True) for t in a]
+    y = AdamW([dict(params=b[:1]), dict(params=b[1:])])
+    y.load_state_dict(x.state_dict())
+    take_step(x, a, 2), take_step(y, b, 2)
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and [int(y.state_of(q)["step"]) for q in b] == [2, 1]
