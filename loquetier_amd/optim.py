@@ -170,20 +170,23 @@ class AdamW(torch.optim.Optimizer):
         return out
 
     def load_state_dict(self, state_dict: Dict[str, Any]) -> None:
-        state = state_dict["state"]
+        """Takes over what `state_dict` gave; what is not of these tensors is refused before anything changes."""
+        state, kinds = state_dict["state"], []
+        if "sets" not in state:
+            raise ValueError("the saved states are not this optimizer's")
+        if state["sets"]:
+            self._prepare()
+            kinds = [[s.parts(i) for s, i in kind] for kind in self._kinds()]
+            shape = lambda tensors: {n: None if t is None else (t.dtype, tuple(t.shape)) for n, t in tensors.items()}
+            mine = [{n: None if t is None else (t.dtype, (sum(p[n].size(0) for p in parts),)) for n, t in parts[0].items()} for parts in kinds]
+            if state["bits"] != self.state_bits or mine != [shape(s) for s in state["sets"]]:
+                raise ValueError("the saved states are of other tensors, or of another number of bits")
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         if not state["sets"]:  # (saved before its first step)
             for s in self._sets:
                 for t in s.tensors.values():
                     if t is not None:
                         t.view(torch.uint8).zero_()
-            return
-        self._prepare()
-        kinds = [[s.parts(i) for s, i in kind] for kind in self._kinds()]
-        shape = lambda tensors: {n: None if t is None else (t.dtype, tuple(t.shape)) for n, t in tensors.items()}
-        mine = [{n: None if t is None else (t.dtype, (sum(p[n].size(0) for p in parts),)) for n, t in parts[0].items()} for parts in kinds]
-        if state["bits"] != self.state_bits or mine != [shape(s) for s in state["sets"]]:
-            raise ValueError("the saved states are of other tensors, or of another number of bits")
         for parts, saved in zip(kinds, state["sets"]):
             for name, t in saved.items():
                 if t is not None:

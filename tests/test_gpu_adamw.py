@@ -429,3 +429,25 @@ def test_saved_before_a_joined_groups_first_step():
     y.load_state_dict(x.state_dict())
     take_step(x, a, 2), take_step(y, b, 2)
     assert all(torch.equal(p, q) for p, q in zip(a, b)) and [int(y.state_of(q)["step"]) for q in b] == [2, 1]
+
+
+def test_a_refused_load_changes_nothing():
+    a = tensors(300, 500)
+    x = AdamW([dict(params=a[:1]), dict(params=a[1:], weight_decay=0.5)], lr=1e-2)
+    take_step(x, a, 1)
+    def other(sizes, groups, **kw):
+        b = tensors(*sizes)
+        y = AdamW([dict(params=[b[i] for i in g]) for g in groups], lr=0.5, **kw)
+        take_step(y, b, 2)
+        return y.state_dict()
+    b = tensors(300, 500)
+    theirs = torch.optim.AdamW([dict(params=b[:1]), dict(params=b[1:])], lr=0.5)
+    take_step(theirs, b, 3)
+    before = x.state_dict()
+    for bad in (other([300, 5000], [[0], [1]]), other([300, 500], [[0], [1]], state_bits=8), other([300, 500], [[0], [1]], master=False),
+                other([300, 500], [[0, 1]]), other([300], [[0]]), theirs.state_dict()):
+        with pytest.raises(ValueError):
+            x.load_state_dict(bad)
+        after = x.state_dict()
+        assert after["param_groups"] == before["param_groups"]
+        assert all(torch.equal(t, after["state"]["sets"][0][n]) for n, t in before["state"]["sets"][0].items() if t is not None)
