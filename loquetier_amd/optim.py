@@ -157,6 +157,9 @@ class AdamW(torch.optim.Optimizer):
                     kinds.setdefault((p.device, p.dtype), []).append(where[id(p)])
         return list(kinds.values())
 
+    def _shapes(self) -> List[List[Tuple[int, ...]]]:
+        return [[tuple(s.params[i].shape) for s, i in kind] for kind in self._kinds()]
+
     def state_dict(self) -> Dict[str, Any]:
         out = super().state_dict()
         if self._sets:
@@ -166,7 +169,7 @@ class AdamW(torch.optim.Optimizer):
             parts = [s.parts(i) for s, i in kind]
             join = lambda ts: None if ts[0] is None else torch.cat([t.view(torch.uint8) for t in ts]).view(ts[0].dtype)
             sets.append({n: join([p[n] for p in parts]) for n in parts[0]})
-        out["state"] = {"bits": self.state_bits, "sets": sets}
+        out["state"] = {"bits": self.state_bits, "sets": sets, "shapes": self._shapes()}
         return out
 
     def load_state_dict(self, state_dict: Dict[str, Any]) -> None:
@@ -179,7 +182,9 @@ class AdamW(torch.optim.Optimizer):
             kinds = [[s.parts(i) for s, i in kind] for kind in self._kinds()]
             shape = lambda tensors: {n: None if t is None else (t.dtype, tuple(t.shape)) for n, t in tensors.items()}
             mine = [{n: None if t is None else (t.dtype, (sum(p[n].size(0) for p in parts),)) for n, t in parts[0].items()} for parts in kinds]
-            if state["bits"] != self.state_bits or mine != [shape(s) for s in state["sets"]]:
+            if (state["bits"] != self.state_bits or mine != [shape(s) for s in state["sets"]] or
+                    # (tensors of other sizes may fill as many blocks; states without shapes are of an older program)
+                    state.get("shapes", self._shapes()) != self._shapes()):
                 raise ValueError("the saved states are of other tensors, or of another number of bits")
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
         if not state["sets"]:  # (saved before its first step)

@@ -451,3 +451,22 @@ def test_a_refused_load_changes_nothing():
         after = x.state_dict()
         assert after["param_groups"] == before["param_groups"]
         assert all(torch.equal(t, after["state"]["sets"][0][n]) for n, t in before["state"]["sets"][0].items() if t is not None)
+
+
+def test_states_of_tensors_of_other_shapes(tmp_path):
+    """Tensors that fill as many blocks in all as the saved ones are others all the same; what is saved goes through a file and the host."""
+    a = tensors(300, 200)
+    x = AdamW(a, state_bits=8)
+    take_step(x, a, 1)
+    for sizes in ((200, 300), (301, 200), ((30, 10), 200)):
+        with pytest.raises(ValueError, match="other tensors"):
+            AdamW([torch.zeros(n, dtype=BF16, device="cuda").requires_grad_(True) for n in sizes], state_bits=8).load_state_dict(x.state_dict())
+    torch.save(x.state_dict(), tmp_path / "state")
+    saved = torch.load(tmp_path / "state", map_location="cpu", weights_only=True)
+    b = [t.detach().clone().requires_grad_(True) for t in a]
+    y = AdamW(b, state_bits=8)
+    y.load_state_dict(saved)
+    take_step(x, a, 2), take_step(y, b, 2)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    del saved["state"]["shapes"]  # (as they were saved without)
+    AdamW(b, state_bits=8).load_state_dict(saved)
