@@ -35,6 +35,16 @@ class _Set:
         self.group = kernel.put_ints(dev, [], groups)[1]
         self.workspace = kernel.Workspace(dev)
 
+    def __getstate__(self) -> Dict[str, Any]:
+        # (the workspace is for the steps captured here; torch pickles no tensors of 8-bit floats, so they go as bytes)
+        tensors = {n: t if t is None or t.dtype != torch.float8_e4m3fn else t.view(torch.uint8) for n, t in self.tensors.items()}
+        return dict({n: v for n, v in self.__dict__.items() if n != "workspace"}, tensors=tensors)
+
+    def __setstate__(self, state: Dict[str, Any]) -> None:
+        self.__dict__.update(state)
+        self.tensors = {n: t if t is None or t.dtype != torch.uint8 else t.view(torch.float8_e4m3fn) for n, t in self.tensors.items()}
+        self.workspace = kernel.Workspace(self.group.device)
+
     def parts(self, i: int) -> Dict[str, Optional[torch.Tensor]]:
         """A tensor's share of the states, whole blocks."""
         first, end = self.first[i:i + 2]
@@ -63,6 +73,14 @@ class AdamW(torch.optim.Optimizer):
         # what was written, and the tables: the newest, and smaller ones that a captured step may read
         self._rates: Dict[torch.device, Tuple[tuple, List[torch.Tensor]]] = {}
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def __getstate__(self) -> Dict[str, Any]:
+        return dict(super().__getstate__(), state_bits=self.state_bits, master=self.master, _sets=self._sets)
+
+    def __setstate__(self, state: Dict[str, Any]) -> None:
+        super().__setstate__(state)
+        if "_sets" in state:  # (a copy, or what was pickled: the rates' tables are for the steps captured here)
+            self._rates = {}
 
     def add_param_group(self, param_group: Dict[str, Any]) -> None:
         super().add_param_group(param_group)

@@ -4,7 +4,9 @@ Tolerances.  Averages: two products and a sum in float, 3 x 2^-24 of the summand
 root, two products, a reciprocal (v_rcp_f32 and v_sqrt_f32: 2^-23 each), a sum: 1e-6 of the update, and 2^-23 of the weight for the two subtractions;
 16-bit weights are rounded once more, eps / 2.  8 bits: values relative to the block's scale, rounded to 2^-4 of the value or 2^-10 of the
 scale below the normal numbers."""
+import copy
 import math
+import pickle
 
 import pytest
 import torch
@@ -470,3 +472,24 @@ def test_states_of_tensors_of_other_shapes(tmp_path):
     assert all(torch.equal(p, q) for p, q in zip(a, b))
     del saved["state"]["shapes"]  # (as they were saved without)
     AdamW(b, state_bits=8).load_state_dict(saved)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("again", [copy.deepcopy, lambda pair: pickle.loads(pickle.dumps(pair))], ids=["copied", "pickled"])
+def test_copies_go_on_alone(bits, again):
+    a = tensors(300, 500)
+    x = AdamW([dict(params=a[:1], lr=1e-2)], state_bits=bits)
+    take_step(x, a[:1], 1)
+    x.add_param_group(dict(params=a[1:]))
+    take_step(x, a, 2)
+    y, b = again((x, a))
+    assert all(p is q for p, q in zip(b, [p for g in y.param_groups for p in g["params"]]))
+    before = x.state_dict()["state"]["sets"][0]
+    take_step(y, b, 3)
+    assert all(torch.equal(t.view(torch.uint8), before[n].view(torch.uint8))
+               for n, t in x.state_dict()["state"]["sets"][0].items() if t is not None)
+    take_step(x, a, 3)
+    x.param_groups[0]["lr"] = y.param_groups[0]["lr"] = 1e-3
+    take_step(x, a, 4), take_step(y, b, 4)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    assert all(torch.equal(x.state_of(p)[n], y.state_of(q)[n]) for p, q in zip(a, b) for n in x.state_of(p))
