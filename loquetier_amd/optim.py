@@ -32,8 +32,14 @@ class _Set:
             # (zeros are the rounding of no weight but 0: each one takes its place at the first step)
             master=zeros(n, torch.float32) if master and dtype != torch.float32 else None,
             step=zeros(len(params), torch.int32))
-        self.group = kernel.put_ints(dev, [], groups)[1]
+        self.groups, self.group = groups, kernel.put_ints(dev, [], groups)[1]
         self.workspace = kernel.Workspace(dev)
+
+    def regroup(self, groups: List[int]) -> None:
+        """Other groups of the tensors (-1: none, and the tensor stays as it is), in the place that captured steps read."""
+        if groups != self.groups:
+            kernel.put_words(self.group, struct.pack(f"{len(groups)}i", *groups))
+            self.groups = groups
 
     def __getstate__(self) -> Dict[str, Any]:
         # (the workspace is for the steps captured here; torch pickles no tensors of 8-bit floats, so they go as bytes)
@@ -59,7 +65,8 @@ class AdamW(torch.optim.Optimizer):
 
     state_bits 32: averages in float; 8: in e4m3 with a float scale each for 256 weights.  master: float weights beside 16-bit ones,
     which are their rounding (small updates add up that a 16-bit weight would lose); a weight that somebody sets is taken over
-    at the next step.  A tensor without a gradient stays as it is, its average's age too, so adapters may take steps by turns.
+    at the next step.  A tensor without a gradient stays as it is, its average's age too, so adapters may take steps by turns; one whose
+    group is taken out of `param_groups` stays too, and goes on if it comes back.
 
     Step counts live on the device, so `step` may be captured into a graph after one eager step; the groups' rates too: `step`
     writes those that have changed, between replays `update_rates` does.  Nothing waits for the GPU."""
@@ -70,6 +77,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("state_bits must be 8 or 32")
         self.state_bits, self.master = state_bits, bool(master)
         self._sets: List[_Set] = []
+        self._order: List[Tuple[int, int]] = []  # the tensors' groups and ids, as the sets have them
         # what was written, and the tables: the newest, and smaller ones that a captured step may read
         self._rates: Dict[torch.device, Tuple[tuple, List[torch.Tensor]]] = {}
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
@@ -80,7 +88,7 @@ class AdamW(torch.optim.Optimizer):
     def __setstate__(self, state: Dict[str, Any]) -> None:
         super().__setstate__(state)
         if "_sets" in state:  # (a copy, or what was pickled: the rates' tables are for the steps captured here)
-            self._rates = {}
+            self._rates, self._order = {}, []
 
     def add_param_group(self, param_group: Dict[str, Any]) -> None:
         super().add_param_group(param_group)
@@ -91,23 +99,27 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("lr, eps and weight_decay must not be negative, betas lie in [0, 1)")
 
     def _prepare(self) -> None:
-        """States of the tensors that have none yet."""
-        known = sum(len(s.params) for s in self._sets)
-        every = [(g, p) for g, group in enumerate(self.param_groups) for p in group["params"]]
-        if known == len(every):
+        """States of the tensors that have none yet, and the groups of those that have."""
+        every = [(g, id(p)) for g, group in enumerate(self.param_groups) for p in group["params"]]
+        if every == self._order:
             return
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("the states must be made before a graph is captured: run an eager step")
+            raise RuntimeError("the states must be made, and tensors take their groups, before a graph is captured: run an eager step")
+        group_of = {i: g for g, i in every}
         have = {id(p) for s in self._sets for p in s.params}
         kinds: Dict[tuple, Tuple[list, list]] = {}
-        for g, p in every:
-            if id(p) in have:
-                continue
-            if not p.is_cuda or not p.is_contiguous() or p.dtype not in (torch.float16, torch.bfloat16, torch.float32):
-                raise RuntimeError("No suitable kernel: parameters must be contiguous fp16, bf16 or float32 tensors on a GPU")
-            ps, gs = kinds.setdefault((p.device, p.dtype), ([], []))
-            ps.append(p), gs.append(g)
+        for group in self.param_groups:
+            for p in group["params"]:
+                if id(p) in have:
+                    continue
+                if not p.is_cuda or not p.is_contiguous() or p.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+                    raise RuntimeError("No suitable kernel: parameters must be contiguous fp16, bf16 or float32 tensors on a GPU")
+                ps, gs = kinds.setdefault((p.device, p.dtype), ([], []))
+                ps.append(p), gs.append(group_of[id(p)])
+        for s in self._sets:  # (a group that was taken out, or moved up because another was)
+            s.regroup([group_of.get(id(p), -1) for p in s.params])
         self._sets += [_Set(ps, gs, self.state_bits, self.master) for ps, gs in kinds.values()]
+        self._order = every
 
     def update_rates(self) -> None:
         """Writes the groups' lr, betas, eps and weight decay to the device where they have changed (step does so itself; a captured
@@ -122,10 +134,11 @@ class AdamW(torch.optim.Optimizer):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("rates changed while a graph is captured: call update_rates before")
             tables = was[1] if was is not None else []
-            if not tables or tables[-1].size(0) != len(now):
+            if not tables or tables[-1].size(0) < len(now):
                 tables.append(torch.empty(len(now), 5, device=dev))
-            for table in tables:
-                kernel.put_words(table, struct.pack(f"{table.numel()}f", *[v for row in now[:table.size(0)] for v in row]))
+            for table in tables:  # (rows that no group has any more are zeros)
+                rows = [*now, *[(0.0,) * 5] * table.size(0)][:table.size(0)]
+                kernel.put_words(table, struct.pack(f"{table.numel()}f", *[v for row in rows for v in row]))
             self._rates[dev] = (now, tables)
 
     @torch.no_grad()

@@ -493,3 +493,40 @@ def test_copies_go_on_alone(bits, again):
     take_step(x, a, 4), take_step(y, b, 4)
     assert all(torch.equal(p, q) for p, q in zip(a, b))
     assert all(torch.equal(x.state_of(p)[n], y.state_of(q)[n]) for p, q in zip(a, b) for n in x.state_of(p))
+
+
+def test_groups_that_leave_and_join():
+    """An adapter's group is taken out and another's joins, in one step or two: the one that left stays as it is, gradient or not, the others keep their
+    rates, the new one learns, and one that comes back goes on."""
+    a = tensors(300, 500, 700)
+    new = lambda ps: AdamW([dict(params=[p], lr=r) for p, r in zip(ps, (1e-2, 2e-2))])
+    x = new(a)
+    take_step(x, a[:2], 1)
+    left = x.param_groups.pop(0)
+    x.add_param_group(dict(params=[a[2]], lr=4e-2))
+    before = [t.detach().clone() for t in a]
+    take_step(x, a, 2)
+    assert torch.equal(a[0], before[0]) and x.state_of(a[0])["step"] == 1
+    for p, b, lr in ((a[1], before[1], 2e-2), (a[2], before[2], 4e-2)):
+        b = b.clone().requires_grad_(True)
+        y = AdamW([b], lr=lr)
+        if p is a[1]:
+            g = torch.Generator().manual_seed(1)
+            torch.randn(300, generator=g)
+            c = tensors(300, 500, 700)[1]
+            y = AdamW([c], lr=lr)
+            c.grad = (torch.randn(500, generator=g) * 1e-2).to(BF16).cuda()
+            y.step()
+            b = c
+        b.grad = p.grad.clone()
+        y.step()
+        assert torch.equal(p, b)
+    del x.param_groups[0]
+    x.step()
+    x.param_groups.insert(0, left)
+    take_step(x, a[:1], 3)
+    assert [int(x.state_of(p)["step"]) for p in a] == [2, 2, 3]
+    del x.param_groups[:]
+    before = [t.detach().clone() for t in a]
+    x.step()
+    assert all(torch.equal(p, b) for p, b in zip(a, before))
