@@ -202,7 +202,7 @@ SMLM_API int smlm_vocab_loss_fwd(float* loss, float* lse, float* means, float* w
     LossSpace s{};
     if (kept && kept_bytes < loss_keep(kept, T, H, V, &s)) return SMLM_ERR_WORKSPACE;
     if (workspace_bytes < loss_carve(workspace, T, H, V, kept ? 4 : 0, &s)) return SMLM_ERR_WORKSPACE;
-    const LossScanArgs sa{s.rows, labels, loss, lse, nullptr, partition, nullptr, T, V, P, 0, kept != nullptr};
+    const LossScanArgs sa{s.rows, labels, loss, lse, nullptr, partition, nullptr, T, V, P, 0, kept != nullptr, 0};
     LOSS_TRY(launch(loss_scan_kernel<false>, dim3(1), dim3(kLossScanThreads), st, sa));
     const LossGatherArgs ga{s.rows, reinterpret_cast<const uint16_t*>(x), T, H, 0};
     LOSS_TRY(loss_gather(dtype == SMLM_DTYPE_F16, T, st, ga));
@@ -262,9 +262,10 @@ SMLM_API int smlm_vocab_loss_bwd(void* dx, void* dw, const float* grad, const fl
   hipStream_t st = (hipStream_t)stream;
   const bool f16 = dtype == SMLM_DTYPE_F16, few = loss_few(T, V);
   const int twice = loss_twice(T, (dx ? 1 : 0) | (dw ? 2 : 0));
-  if (!dw || !partition || twice) s.rows.rest = nullptr;  // (twice: nothing is lost that it would save)
+  const bool split = dw && partition && !twice;  // (twice: nothing is lost that it would save)
+  if (!f16 && !split) s.rows.rest = nullptr;
   if (!s.rows.rest && !twice) s.rows.y = nullptr;
-  const LossScanArgs sa{s.rows, labels, const_cast<float*>(loss), const_cast<float*>(lse), grad, partition, weight, T, V, P, f16, 1};
+  const LossScanArgs sa{s.rows, labels, const_cast<float*>(loss), const_cast<float*>(lse), grad, partition, weight, T, V, P, f16, 1, split};
   LOSS_TRY(launch(loss_scan_kernel<true>, dim3(1), dim3(kLossScanThreads), st, sa));
   const LossGatherArgs ga{s.rows, reinterpret_cast<const uint16_t*>(x), T, H, twice};
   LOSS_TRY(loss_gather(f16, twice ? 2 * kLossTwice : T, st, ga));

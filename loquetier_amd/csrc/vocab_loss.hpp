@@ -45,12 +45,12 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // What the labelled rows are numbered into; n = count[0].
 struct LossRows {
-  int32_t* count;    // [1]
+  int32_t* count;    // [2] n; whether any `rest` is not 1 (backward)
   int32_t* row;      // [T] row of the batch
   int32_t* label;    // [T]
   int32_t* number;   // [T] of a row of the batch, -1: none (backward)
   float* coef;       // [T] c relative to `unit`, or a power of two (backward)
-  float* rest;       // [T] what c is of coef, in [0.5, 1], or NULL: all 1 (backward)
+  float* rest;       // [T] what c is of coef, up to 1, or NULL: all 1 (backward)
   float* lse2;       // [T] lse in powers of two (backward)
   float* own;        // [T] exp(-loss) - 1 (backward)
   float* lost;       // [T] what rounding took from G at the label (backward)
@@ -61,7 +61,7 @@ struct LossRows {
   float* turn;       // [T] what the sums so far are multiplied with
   int32_t* moved;    // [T / 16] whether anything of sixteen rows' entries is to be turned
   uint16_t* x;       // [n, H] the rows side by side, unless n == T
-  uint16_t* y;       // [n, H], or [64, H] where G is held twice: the rows (times `rest`), for dw (backward; NULL: x will do)
+  uint16_t* y;       // [n, H], or [64, H] where G is held twice: the rows times `rest`, for dw (backward; NULL: x will do)
 };
 
 struct LossScanArgs {
@@ -72,8 +72,12 @@ struct LossScanArgs {
   const float* grad;      // [T], or [P] (backward)
   const int32_t* partition;  // [P + 1] or NULL
   const float* weight;       // [P] (backward)
-  int T, V, P, f16, number;  // number: rows' numbers are wanted
+  int T, V, P, f16, number, split;  // number: rows' numbers are wanted; split: coef is a power of two (backward)
 };
+// fp16's entries of G are multiples of 2^-24, and a coefficient far below the largest, which is 2^14, would leave its row's none.  From 2^-11 of the
+// largest down, G therefore takes 2^-11 of it and the rows the rest (rounded for dw; dx takes it in float): G's entries are off by half a step or
+// 2^-28 of c, the rows' elements in dw by half a step or 2^-36 of the largest c.
+constexpr float kLossLeast = 8.0f;
 
 // Index of the partition that row t lies in, -1: none.
 __device__ __forceinline__ int loss_partition(const int32_t* partition, int P, int t) {
@@ -152,17 +156,24 @@ __global__ __launch_bounds__(kLossScanThreads) void loss_scan_kernel(LossScanArg
     const bool turn = top > 0.0f;
     const float up = a.f16 ? 0x1p14f : 1.0f;  // (fp16: out of the subnormal numbers)
     if (threadIdx.x == 0) a.to.unit[0] = turn ? top / up : 1.0f;
+    bool any = false;
     for (int i = threadIdx.x; i < before; i += kLossScanThreads) {
       float c = a.to.coef[i];
       if (turn) c = c / top * up;  // (dividing first: neither quotient nor product leaves the floats)
       if (a.to.rest) {
         const float two = 2.0f * __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, c) & 0xff800000u);
-        const bool plain = !(fabsf(c) < INFINITY) || two == 0.0f;
-        a.to.rest[i] = plain ? 1.0f : c / two;
-        c = plain ? c : two;
+        float held = c;
+        if (a.f16 && fabsf(c) < kLossLeast) held = copysignf(kLossLeast, c);
+        else if (a.split && fabsf(c) < INFINITY && two != 0.0f) held = two;
+        const bool plain = !(fabsf(held) > fabsf(c));
+        a.to.rest[i] = plain ? 1.0f : c / held;
+        c = plain ? c : held;
+        any |= !plain;
       }
       a.to.coef[i] = c;
     }
+    any = __syncthreads_or(any);
+    if (threadIdx.x == 0) a.to.count[1] = any;
   }
 }
 
@@ -176,16 +187,20 @@ constexpr int kLossTwice = 32;
 // Of a partition's rows c is one number, and its rounding at their labels, where G is nearly -c, would be one error of all of them: in dw up to
 // eps / 2, where the output's own rounding is 0.41 of that in the mean square.  So coef is the power of two above c, and dw's other operand, the rows,
 // is multiplied with the rest, c / coef, and rounded: errors of random sign, none for the partition of the largest c.  dx takes the rest in float.
+// (Nothing is copied for it where every rest is 1.)
 struct LossGatherArgs {
   LossRows rows;
   const uint16_t* x;
   int T, H, twice;
 };
+// Whether dw takes the rows from y.
+__device__ __forceinline__ bool loss_y(const LossRows& r, int twice) { return r.y && (twice || uload(r.count, 1)); }
 // A wave a row.
 template <int DT>
 __global__ __launch_bounds__(256) void loss_gather_kernel(LossGatherArgs a) {
   const int n = uload(a.rows.count, 0), lane = threadIdx.x & 63, all = a.twice ? 2 * kLossTwice : n;
-  if (n == a.T && !a.rows.y) return;
+  const bool y = loss_y(a.rows, a.twice);
+  if (n == a.T && !y) return;
   for (int i = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6); i < all; i += (int)gridDim.x * 4) {
     const int at = a.twice ? i & (kLossTwice - 1) : i;
     const bool none = at >= n;
@@ -195,7 +210,7 @@ __global__ __launch_bounds__(256) void loss_gather_kernel(LossGatherArgs a) {
       u32x4 v = {0u, 0u, 0u, 0u};
       if (!none) v = ldg16(from + c);
       if (n != a.T && i < n) stg16(a.rows.x + (int64_t)i * a.H + c, v);
-      if (!a.rows.y) continue;
+      if (!y) continue;
       float f[8];
       unpack8<DT>(v, f);
 #pragma unroll
@@ -536,7 +551,7 @@ __global__ __launch_bounds__(256, 1) void loss_dw_kernel(LossTileArgs a) {
   f32x16 acc[IA][JB];
   loss_zero(acc);
   const int first_h = u.rows * S::kA, first_v = u.other * S::kB;
-  GemmTile<DT, WA, IA, true, WB, JB, true>::run(acc, lds, GemmOperand{a.rows.y ? a.rows.y : loss_x(a, n), a.H, n}, first_h,
+  GemmTile<DT, WA, IA, true, WB, JB, true>::run(acc, lds, GemmOperand{loss_y(a.rows, a.twice) ? a.rows.y : loss_x(a, n), a.H, n}, first_h,
                                             GemmOperand{a.g, a.ldg, n}, first_v, 0, n);
   const float unit = uload(a.rows.unit, 0);
 #pragma unroll

@@ -657,3 +657,38 @@ def test_more_partitions_than_a_launch_takes():
     first = torch.arange(P, device="cuda") % 4 == 3
     first &= torch.arange(P, device="cuda") // 4 < T
     assert torch.equal(means[first], rows) and not means[~first].any()
+
+
+@pytest.mark.parametrize("T", [20, 80, 300])
+@pytest.mark.parametrize("parted", [True, False])
+@pytest.mark.parametrize("apart", [13, 20, 26])
+@pytest.mark.parametrize("want_w", [True, False])
+def test_small_weights_beside_large_ones_in_fp16(T, parted, apart, want_w):
+    """Half of the rows weigh 2^-13 to 2^-26 of the others, with the vocabulary's gradient beside the rows', so G is made: entries are off by eps / 2
+    or 2^-28 of their own row's weight, and rows' gradients by sum |w| of that; in the vocabulary's gradient the rows are rounded once
+    more where they take the rest of the weight, by eps / 2 or 2^-36 of the largest weight's |x|."""
+    H, V, eps = 128, 5000, 2.0 ** -10
+    x, w, labels = make(T, H, V, FP16, T)
+    g = torch.full((T,), 2.0 ** 10, device="cuda")
+    half = T // 2
+    g[half:] *= 2.0 ** -apart
+    part = torch.tensor([0, half, T], dtype=torch.int32, device="cuda")
+    grad = torch.stack([g[0] * half, g[-1] * (T - half)]) if parted else g
+    a, b = x.clone().requires_grad_(True), w.clone().requires_grad_(want_w)
+    if want_w:
+        out = linear_cross_entropy.apply(a, b, labels, part if parted else None)
+        dx, dw = torch.autograd.grad(out, (a, b), grad)
+    else:  # (the same G, without what the forward keeps)
+        loss, lse, dx, means, weight = *(torch.empty(T, device="cuda") for _ in range(2)), torch.empty_like(x), *(torch.empty(2, device="cuda") for _ in range(2))
+        K.linear_cross_entropy(loss, lse, x, w, labels, *((part, means, weight) if parted else ()))
+        K.linear_cross_entropy_backward(dx, None, grad, loss, lse, x, w, labels, *((part, weight) if parted else ()))
+    _, _, want_x, want_dw, bx, bw = want(x, w, labels, g)
+    top = (x.double().norm(dim=1).max() * w.double().norm(dim=1).max()).item()
+    c, X, W = g.double().cpu(), x.double().cpu().abs(), w.double().cpu().abs()
+    off = (dx.double().cpu() - want_x).abs()
+    limit = bx[0] * eps / 2 + bx[1] * (2e-6 * top + 2e-6) + want_x.abs() * eps / 2 + c[:, None] * 2.0 ** -28 * W.sum(0) + 2.0 ** -25
+    assert (off <= limit).all(), (off / limit).max()
+    if want_w:
+        off = (dw.double().cpu() - want_dw).abs()
+        limit = bw[0] * eps + bw[1] * (2e-6 * top + 2e-6) + want_dw.abs() * eps / 2 + c @ X * 2.0 ** -28 + 2.0 ** 10 * T * 2.0 ** -36 + 2.0 ** -25
+        assert (off <= limit).all(), (off / limit).max()
