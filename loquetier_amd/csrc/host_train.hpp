@@ -246,9 +246,10 @@ PyObject* py_adamw_step(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
       (master && !is(*master, at::kFloat, 1)))
     Py_RETURN_FALSE;
   std::vector<void*> where(n), full;
+  std::vector<std::pair<uintptr_t, uintptr_t>> written;  // from, to
   std::vector<const void*> at_(n, nullptr);
   std::vector<int64_t> sizes(n);
-  full.reserve(n);
+  full.reserve(n), written.reserve(n);
   int64_t blocks = 0;
   at::ScalarType type{};
   for (Py_ssize_t i = 0; i < n; ++i) {
@@ -266,6 +267,7 @@ PyObject* py_adamw_step(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
     }
     where[i] = t.data_ptr(), sizes[i] = t.numel();
     if (sizes[i]) full.push_back(where[i]);
+    if (sizes[i] && at_[i]) written.emplace_back((uintptr_t)where[i], (uintptr_t)where[i] + t.nbytes());
     blocks += (sizes[i] + 255) / 256;
   }
   const bool f32 = type == at::kFloat;
@@ -275,6 +277,9 @@ PyObject* py_adamw_step(PyObject*, PyObject* const* p, Py_ssize_t nargs) {
     Py_RETURN_FALSE;
   std::sort(full.begin(), full.end());
   if (std::adjacent_find(full.begin(), full.end()) != full.end()) Py_RETURN_FALSE;
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); ++i)
+    if (written[i - 1].second > written[i].first) Py_RETURN_FALSE;
   size_t need = 0;
   check(lib.adamw_size((int)n, &need), "smlm_adamw_workspace_size");
   const Tensor mem = scratch(p[10], need, m);

@@ -1448,6 +1448,9 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
     full = [p for p, size in zip(where, sizes) if size]
     if len(set(full)) != len(full):
         raise RuntimeError("a tensor is named twice")
+    written = sorted((p, p + size * params[0].element_size()) for p, g, size in zip(where, at, sizes) if size and g)
+    if any(end > start for (_, end), (start, _) in zip(written, written[1:])):
+        raise RuntimeError("tensors that are written overlap")
     for t, name in ((exp_avg, "exp_avg"), (exp_avg_sq, "exp_avg_sq"), (master, "master")):
         if t is not None and t.size(0) != blocks * ADAMW_BLOCK:
             raise RuntimeError(f"{name} must have {blocks * ADAMW_BLOCK} entries")

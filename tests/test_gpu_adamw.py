@@ -530,3 +530,20 @@ def test_groups_that_leave_and_join():
     before = [t.detach().clone() for t in a]
     x.step()
     assert all(torch.equal(p, b) for p, b in zip(a, before))
+
+
+def test_tensors_that_overlap_are_refused():
+    """Two waves would update the same weight, one after the other or not.  Tensors side by side, and one without a gradient, are none of that."""
+    flat, g = torch.randn(600, device="cuda").to(BF16), torch.randn(600, device="cuda").to(BF16)
+    p = Problem([300, 300], BF16, 32, True)
+    for a, b, ok in ((flat[:300], flat[300:], True), (flat[:300], flat[296:596], False), (flat[200:500], flat[:300], False)):
+        p.params, p.grads = [a, b], [g[:300], g[300:]]
+        if ok:
+            p.run()
+            continue
+        before = flat.clone()
+        with pytest.raises(RuntimeError, match="overlap"):
+            p.run()
+        assert torch.equal(flat, before)
+        p.run([g[:300], None])
+        assert not torch.equal(flat, before)
