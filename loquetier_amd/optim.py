@@ -78,6 +78,7 @@ class AdamW(torch.optim.Optimizer):
         self.state_bits, self.master = state_bits, bool(master)
         self._sets: List[_Set] = []
         self._order: List[Tuple[int, int]] = []  # the tensors' groups and ids, as the sets have them
+        self._captured = False  # whether a step was
         # what was written, and the tables: the newest, and smaller ones that a captured step may read
         self._rates: Dict[torch.device, Tuple[tuple, List[torch.Tensor]]] = {}
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
@@ -88,7 +89,7 @@ class AdamW(torch.optim.Optimizer):
     def __setstate__(self, state: Dict[str, Any]) -> None:
         super().__setstate__(state)
         if "_sets" in state:  # (a copy, or what was pickled: the rates' tables are for the steps captured here)
-            self._rates, self._order = {}, []
+            self._rates, self._order, self._captured = {}, [], False
 
     def add_param_group(self, param_group: Dict[str, Any]) -> None:
         super().add_param_group(param_group)
@@ -116,6 +117,9 @@ class AdamW(torch.optim.Optimizer):
                     raise RuntimeError("No suitable kernel: parameters must be contiguous fp16, bf16 or float32 tensors on a GPU")
                 ps, gs = kinds.setdefault((p.device, p.dtype), ([], []))
                 ps.append(p), gs.append(group_of[id(p)])
+        rows = min((tables[0].size(0) for _, tables in self._rates.values()), default=0)
+        if self._captured and any(group_of.get(i, -1) >= rows for i in have):
+            raise RuntimeError("a captured step's table has no row for a group that others were put before: append them")
         for s in self._sets:  # (a group that was taken out, or moved up because another was)
             s.regroup([group_of.get(id(p), -1) for p in s.params])
         self._sets += [_Set(ps, gs, self.state_bits, self.master) for ps, gs in kinds.values()]
@@ -148,6 +152,7 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         self.update_rates()
+        self._captured = self._captured or bool(self._sets) and torch.cuda.is_current_stream_capturing()
         for s in self._sets:
             grads = [p.grad for p in s.params]
             if any(g is not None and not g.is_contiguous() for g in grads):

@@ -547,3 +547,47 @@ def test_tensors_that_overlap_are_refused():
         assert torch.equal(flat, before)
         p.run([g[:300], None])
         assert not torch.equal(flat, before)
+
+
+def test_groups_that_leave_and_join_beside_a_captured_step():
+    a, b = tensors(300, 500), tensors(300, 500)
+    x, y = (AdamW([dict(params=t[:1], lr=1e-2), dict(params=t[1:], lr=2e-2)]) for t in (a, b))
+    for t in a + b:
+        t.grad = torch.ones_like(t)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        x.step()
+        with torch.cuda.graph(graph, stream=s):
+            x.step()
+    torch.cuda.current_stream().wait_stream(s)
+    y.step()
+    same = lambda: all(torch.equal(p, q) for p, q in zip(a, b))
+
+    def replay():
+        x.update_rates()
+        graph.replay()
+        torch.cuda.synchronize()
+        y.step()
+    replay()
+    assert same()
+    left = [o.param_groups.pop(0) for o in (x, y)]  # (the other's group moves up)
+    before = a[0].detach().clone()
+    replay()
+    assert same() and torch.equal(a[0], before)
+    for o, g in zip((x, y), left):
+        o.param_groups.append(g)
+    replay()
+    assert same() and not torch.equal(a[0], before)
+    more = tensors(64)
+    x.add_param_group(dict(params=more))
+    x.update_rates()  # (a larger table; the captured step's is kept up)
+    replay()
+    assert same()
+    x.param_groups.insert(0, x.param_groups.pop())
+    with pytest.raises(RuntimeError, match="append"):
+        x.update_rates()
+    x.param_groups.append(x.param_groups.pop(0))
+    replay()
+    assert same()
