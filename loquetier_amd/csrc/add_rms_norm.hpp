@@ -10,8 +10,8 @@
 //
 // Bound by HBM: 4 bytes read and 4 written an element, 5 with the 8-bit form.  A row stays in registers from its sum to its last
 // output.  The backward is rms_norm.hpp's, to which the gradient that reaches h through the residual is added.  (4096 columns: 4096
-// rows bf16 23.2 us, 5.8 TB/s, backward 26.3, 5.1, and its fold 3.9; 2112 rows with e4m3 by 128 columns 16.7, 4.7; 256 rows
-// with e4m3 by row 4.3.)
+// rows bf16 23.2 us, 5.8 TB/s, backward 26.4, 5.1, and its fold 3.9; 2112 rows with e4m3 by 128 columns 17.3, 4.5 (16.6 with
+// products for quotients); 256 rows with e4m3 by row 4.4.)
 #pragma once
 #include "rms_norm.hpp"
 

@@ -15,7 +15,7 @@
 // A piece of the vocabulary at a time the exponentials are stored in 16 bits, each row's against its reference of the pieces
 // before, and multiplied with w.  Where the piece outgrows the reference (or there is none yet) a part is stored against its own,
 // and turned to the row's new one before the product, as the sums so far are: references are whole powers of two, so turning rounds
-// nothing.  The backward divides and multiplies with c.
+// nothing but what it takes down among fp16's subnormal numbers.  The backward divides and multiplies with c.
 //
 // With the gradient of w the backward makes the logits again, by piece, turns them into G in 16 bits, and multiplies that with w and x.
 //
@@ -25,11 +25,15 @@
 //
 // Rounding to 16 bits: half a step of each entry, as any product of 16-bit operands has it (of G at the label too, where dw is
 // wanted: what dx loses by it is given back in float).  fp16 entries are held 2^15 times as large: probabilities of a large vocabulary lie
-// below fp16's normal numbers.  G is held relative to the largest |c|, in fp16 as 2^14.
+// below fp16's normal numbers.  G is held relative to the largest |c|, in fp16 as 2^14 (and rows of far smaller |c| by their own: kLossLeast).
 //
-// Measured, us (4096 columns; PFLOP/s): 4099 rows of 128256 entries, bf16, logits with exponentials 4020 (1.07), dx 3920 (1.10), fold 65; 2458
-// labelled rows of 4096, 32000 entries, 636 (1.01), 702 (0.92), 30; 2048 rows of 32000, fp16, logits 499 (1.07), again for G 501,
-// dx 527 (1.02), dw 583 (0.92); 200 rows of 128256 the loss alone 254 to 270 (4.1 to 3.9 TB/s of w).  Power bounds the products: 1.75 with zeros.
+// Measured, us (4096 columns; PFLOP/s): 4099 rows of 128256 entries, bf16, logits with exponentials 3977 (1.08), dx 3919 (1.10), fold 65; 2458
+// labelled rows of 4096, 32000 entries, 618 (1.04), 708 (0.91), 30; 2048 rows of 32000, fp16, logits 493 (1.09), again for G 494,
+// dx 521 (1.03), dw 582 (0.92); 200 rows of 128256 the loss alone 274 (3.8 TB/s of w).
+// What bounds the products: a wave a SIMD and a tile a workgroup, so that a tile's first loads and everything after its last product stand alone, with
+// the matrix cores busy in 67 to 69 % of a compute unit's cycles (logits), 57 to 60 (dx) and 55 (dw).  The tiles of 256 rows take all 512 registers and
+// keep 68 to 264 bytes a lane of the logits' epilogue, 364 of dx's `add`, in scratch memory, outside of the loops: 501 tiles of the losses alone
+// write 34 MB where their parts are 2.  The card's power is the bound beyond: the tile alone does 1.23, with zeros 1.75.
 #pragma once
 #include "gemm_tile.hpp"
 #include "rms_norm.hpp"
@@ -333,7 +337,8 @@ __device__ __forceinline__ void loss_lds_free() {
 constexpr int kLossSums = 0, kLossSoft = 1, kLossGrad = 2;  // what becomes of the logits: sums alone, exponentials too, G
 
 // A reference of a part's own is above its maximum by less than one, or by the room that is left for later pieces: bf16 has exponents
-// enough for any (60 above), fp16 gets 2^4 at the price of entries below 2^-28 of the maximum losing bits.  bf16's first piece takes 1
+// enough for any (60 above), fp16 gets 2^4 at the price of bits of entries below 2^-24 of the maximum: that one is 2^10 to 2^11 against a new
+// reference, smaller entries are multiples of 2^-24 and off by 2^-35 of the maximum at most.  bf16's first piece takes 1
 // as every row's reference, where the part's maximum is within 2^+-60: a model's logits are, and nothing needs to be turned.  (Of 4099 rows
 // of 64128 entries, 0.5 GB: 200 us.)
 template <int DT>
