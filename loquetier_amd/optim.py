@@ -66,7 +66,7 @@ class AdamW(torch.optim.Optimizer):
     state_bits 32: averages in float; 8: in e4m3 with a float scale each for 256 weights.  master: float weights beside 16-bit ones,
     which are their rounding (small updates add up that a 16-bit weight would lose); a weight that somebody sets is taken over
     at the next step.  A tensor without a gradient stays as it is, its average's age too, so adapters may take steps by turns; one whose
-    group is taken out of `param_groups` stays too, and goes on if it comes back.
+    group is taken out of `param_groups` stays too, where it lies, and goes on if it comes back.
 
     Step counts live on the device, so `step` may be captured into a graph after one eager step; the groups' rates too: `step`
     writes those that have changed, between replays `update_rates` does.  Nothing waits for the GPU."""
@@ -77,7 +77,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("state_bits must be 8 or 32")
         self.state_bits, self.master = state_bits, bool(master)
         self._sets: List[_Set] = []
-        self._order: List[Tuple[int, int]] = []  # the tensors' groups and ids, as the sets have them
+        self._order: List[List[int]] = []  # the groups' tensors by id, as the sets have them
         self._captured = False  # whether a step was
         # what was written, and the tables: the newest, and smaller ones that a captured step may read
         self._rates: Dict[torch.device, Tuple[tuple, List[torch.Tensor]]] = {}
@@ -101,12 +101,12 @@ class AdamW(torch.optim.Optimizer):
 
     def _prepare(self) -> None:
         """States of the tensors that have none yet, and the groups of those that have."""
-        every = [(g, id(p)) for g, group in enumerate(self.param_groups) for p in group["params"]]
-        if every == self._order:
+        order = [list(map(id, group["params"])) for group in self.param_groups]
+        if order == self._order:
             return
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("the states must be made, and tensors take their groups, before a graph is captured: run an eager step")
-        group_of = {i: g for g, i in every}
+        group_of = {i: g for g, ids in enumerate(order) for i in ids}
         have = {id(p) for s in self._sets for p in s.params}
         kinds: Dict[tuple, Tuple[list, list]] = {}
         for group in self.param_groups:
@@ -118,12 +118,13 @@ class AdamW(torch.optim.Optimizer):
                 ps, gs = kinds.setdefault((p.device, p.dtype), ([], []))
                 ps.append(p), gs.append(group_of[id(p)])
         rows = min((tables[0].size(0) for _, tables in self._rates.values()), default=0)
-        if self._captured and any(group_of.get(i, -1) >= rows for i in have):
+        groups = [[group_of.get(id(p), -1) for p in s.params] for s in self._sets]
+        if self._captured and any(g != was and g >= rows for s, now in zip(self._sets, groups) for g, was in zip(now, s.groups)):
             raise RuntimeError("a captured step's table has no row for a group that others were put before: append them")
-        for s in self._sets:  # (a group that was taken out, or moved up because another was)
-            s.regroup([group_of.get(id(p), -1) for p in s.params])
+        for s, now in zip(self._sets, groups):  # (a group that was taken out, or moved up because another was)
+            s.regroup(now)
         self._sets += [_Set(ps, gs, self.state_bits, self.master) for ps, gs in kinds.values()]
-        self._order = every
+        self._order = order
 
     def update_rates(self) -> None:
         """Writes the groups' lr, betas, eps and weight decay to the device where they have changed (step does so itself; a captured

@@ -549,6 +549,27 @@ def test_tensors_that_overlap_are_refused():
         assert not torch.equal(flat, before)
 
 
+def test_groups_that_join_one_after_another_beside_a_captured_step():
+    a = tensors(300, 500, 64)
+    for t in a:
+        t.grad = torch.ones_like(t)
+    x = AdamW(a[:1])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        x.step()
+        with torch.cuda.graph(graph, stream=s):
+            x.step()
+    torch.cuda.current_stream().wait_stream(s)
+    for i in (1, 2):
+        x.add_param_group(dict(params=a[i:i + 1], lr=1e-2))
+        x.step()
+        graph.replay()
+        torch.cuda.synchronize()
+    assert [int(x.state_of(p)["step"]) for p in a] == [5, 2, 1]
+
+
 def test_groups_that_leave_and_join_beside_a_captured_step():
     a, b = tensors(300, 500), tensors(300, 500)
     x, y = (AdamW([dict(params=t[:1], lr=1e-2), dict(params=t[1:], lr=2e-2)]) for t in (a, b))
