@@ -616,7 +616,8 @@ SMLM_API int smlm_add_rms_norm_bwd(void* dh, void* dw, const void* g, const void
  *   lse[t] = log sum_v exp(x[t] . w[v]),  loss[t] = lse[t] - x[t] . w[labels[t]]     float [T]; both 0 without a label
  * With partition (int32 [P + 1], not decreasing, rows [partition[p], partition[p + 1]) of the batch) also, float [P],
  *   means[p] = the mean of its labelled rows' losses (0 where there are none), weight[p] = one over their number (0)
- * and rows outside every partition have no label.  H a multiple of 8.  Sums are taken in a fixed order.
+ * and rows outside every partition have no label.  H a multiple of 8, T up to 2^28 - 16.  Sums are taken in a fixed order.  Where the label's logit
+ * is +infinity or NaN, loss is NaN; where it is -infinity beside finite ones, loss is infinite and the gradients finite.
  * kept (16-byte aligned; NULL: not wanted) is filled with what smlm_vocab_loss_bwd_kept makes dx of: a product more here, none there.
  */
 SMLM_API int smlm_vocab_loss_workspace_size(int T, int H, int V, int what, size_t* bytes); /* what: 0 forward, 4 forward with kept; backward:
@@ -635,7 +636,7 @@ SMLM_API int smlm_vocab_loss_bwd_kept(void* dx, const float* grad, const void* k
 
 /*
  * dx and dw [V, H] (either may be NULL) without anything kept but loss and lse: the logits are made again, a piece of the vocabulary at a time;
- * rows that nothing hangs on cost nothing.
+ * rows that nothing hangs on cost nothing.  The entries of the logits' gradient are rounded to 16 bits, in fp16 to half a step or 2^-28 of their row's weight.
  */
 SMLM_API int smlm_vocab_loss_bwd(void* dx, void* dw, const float* grad, const float* loss, const float* lse, const void* x,
                                  const void* w, const int64_t* labels, const int32_t* partition, const float* weight, int P, void* workspace,
